@@ -109,6 +109,7 @@ int nwd_workspace_check(void* workspace, size_t ws_bytes, uint32_t* device_error
 
 #define NWD_DEVERR_PIPE_TIMEOUT 1u  /* an mbarrier wait hit its iteration limit */
 #define NWD_DEVERR_ROW_RANGE 2u     /* a row index fell outside the pool */
+#define NWD_DEVERR_TREE 4u          /* a parent, tree length, token or path entry out of range */
 
 /* Failure-detection self-test: launches one CTA whose bounded mbarrier wait
  * (the one every kernel here uses) is made to run out; after about 2 s the
@@ -418,6 +419,100 @@ int nwd_attn_prefill(const uint16_t* q, const uint16_t* k_pool, const uint16_t* 
                      uint32_t n_q, uint32_t start_pos, uint32_t n_heads, uint32_t n_kv_heads,
                      uint32_t head_dim, float scale, void* workspace, size_t ws_bytes,
                      void* stream);
+
+/* ------------------------------------------------------------------ */
+/* Speculative decoding: a tree of drafted tokens per step             */
+/* ------------------------------------------------------------------ */
+
+/* The reference decodes one token per step (engine/runtime.js:447-467).  These
+ * calls let a step carry a tree of drafted tokens per sequence: attention for
+ * all of its nodes over one read of the cache (nwd_attn_tree, with the nodes'
+ * K/V rows written first nwd_kv_append_attn_tree), the decision which of them
+ * stand (nwd_verify_tree), and the cache left as if only those had been
+ * decoded (nwd_kv_commit).
+ *
+ * A tree: parents [batch, n_nodes] (device int32), parents[b, i] < i, -1 for a
+ * root; n_nodes at most 64.  tree_len (device int32[batch], may be NULL: all):
+ * sequence b has tree_len[b] nodes, the rest are absent.  Node i's K/V row is
+ * pool row row_offset[b] + seq_len[b] + i: behind the context rows.
+ *
+ * err: a device word (may be NULL) that receives NWD_DEVERR_* bits; zero it
+ * once (any workspace's first word serves: nwd_workspace_check reads it).  A
+ * parent outside [-1, i) counts as -1, a tree_len outside [0, n_nodes] as the
+ * nearer bound (both NWD_DEVERR_TREE); a sequence whose rows leave the pool
+ * (NWD_DEVERR_ROW_RANGE) is treated as one without rows or nodes. */
+
+/* Workspace of the two attention calls on the current device, 256-byte aligned.
+ * It needs no initialisation and holds nothing between calls; calls that may
+ * overlap on the GPU need one each. */
+int nwd_attn_tree_workspace_size(uint32_t batch, uint32_t n_nodes, uint32_t n_heads,
+                                 uint32_t n_kv_heads, uint32_t head_dim, size_t* bytes);
+
+/* kernels/sparse_attn.wgsl:32-113 for every node of every tree: node i attends
+ * the context rows [0, seq_len[b]), its ancestors' rows and its own.
+ *   q, o          : [batch, n_nodes, n_heads, head_dim]; absent nodes' o = 0
+ *   k_pool, v_pool: [pool_rows, n_kv_heads, head_dim], the nodes' rows in place
+ *   row_offset    : device int64[batch]; seq_len: device int32[batch]
+ * head_dim 128, group 1..8, batch <= 4096.  Rows that a node does not attend
+ * never reach its output, whatever they hold. */
+int nwd_attn_tree(const uint16_t* q, const uint16_t* k_pool, const uint16_t* v_pool,
+                  uint64_t pool_rows, const int64_t* row_offset, const int32_t* seq_len,
+                  const int32_t* parents, const int32_t* tree_len, uint16_t* o, uint32_t batch,
+                  uint32_t n_nodes, uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim,
+                  float scale, void* workspace, size_t ws_bytes, uint32_t* err, void* stream);
+
+/* The same after writing the present nodes' rows k_new / v_new ([batch, n_nodes,
+ * n_kv_heads, head_dim]) into the pools (bit-exact).  Sequences of one call must
+ * not share the rows that they write. */
+int nwd_kv_append_attn_tree(const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
+                            uint16_t* k_pool, uint16_t* v_pool, uint64_t pool_rows,
+                            const int64_t* row_offset, const int32_t* pos, const int32_t* parents,
+                            const int32_t* tree_len, uint16_t* o, uint32_t batch, uint32_t n_nodes,
+                            uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,
+                            void* workspace, size_t ws_bytes, uint32_t* err, void* stream);
+
+/* Which drafted tokens stand, and the next token, from given uniform numbers
+ * (multi-round rejection sampling; the reference's counterpart is the argmax of
+ * one row, kernels/argmax_partial.wgsl).
+ *   tokens      : int32 [batch, n_nodes]; node 0 is the pending token, whose
+ *                 own token is not read
+ *   target_probs: f32 [batch, n_nodes, vocab], row i: the target's distribution
+ *                 behind node i
+ *   draft_probs : f32, the same shape, row i: what node i's children were drawn
+ *                 from, independently of one another; NULL: drafted tokens
+ *                 without probabilities (the likeliest ones, a table's)
+ *   u           : f32 [batch, n_nodes] in [0, 1), u[b, c] decides on node c
+ *   w           : f32 [batch] in [0, 1), for the next token
+ * From node 0 on, with r = target_probs[i]: children c of node i in index
+ * order; c is accepted if u[c] * q_i(t_c) < r(t_c) and the walk goes on there;
+ * else r = max(r - q_i, 0) / its sum (r = target_probs[i] again if nothing is
+ * left).  With draft_probs NULL: accepted if u[c] < r(t_c), else r(t_c) = 0,
+ * renormalised.  Without an accepted child the walk ends and the next token is
+ * the lowest x whose running sum of r exceeds w * sum(r).
+ *   path        : int32 [batch, n_nodes], the accepted nodes from node 0 on,
+ *                 then -1; n_accepted: int32 [batch] (node 0 counts)
+ *   next_token  : int32 [batch]; -1 if the row holds no positive number
+ * Probabilities that are not above zero (NaN too) count as zero.  A sequence
+ * without nodes gets n_accepted 0 and next_token -1.  A token outside
+ * [0, vocab) is never accepted (NWD_DEVERR_TREE). */
+int nwd_verify_tree(const int32_t* tokens, const int32_t* parents, const int32_t* tree_len,
+                    const float* target_probs, const float* draft_probs, const float* u,
+                    const float* w, int32_t* path, int32_t* n_accepted, int32_t* next_token,
+                    uint32_t batch, uint32_t n_nodes, uint32_t vocab, uint32_t* err, void* stream);
+
+/* Moves the accepted nodes' rows behind the context: pool row row_offset[b] +
+ * pos[b] + path[b, j] to row_offset[b] + pos[b] + j for j < n_accepted[b], in
+ * each of n_pools (at most 16) pools [pool_rows, n_kv, hd] of fp16 (K and V of
+ * several layers; `pools` is a host array of device pointers).  path
+ * [batch, n_nodes] as nwd_verify_tree writes it: ascending within n_accepted.
+ * Bit-exact; other rows stay.  A sequence whose path does not ascend within
+ * [0, n_nodes) (NWD_DEVERR_TREE) or whose rows leave the pool
+ * (NWD_DEVERR_ROW_RANGE) is left as it is.  Pools, and the sequences' rows in
+ * them, must not overlap. */
+int nwd_kv_commit(uint16_t* const* pools, uint32_t n_pools, uint64_t pool_rows,
+                  const int64_t* row_offset, const int32_t* pos, const int32_t* path,
+                  const int32_t* n_accepted, uint32_t batch, uint32_t n_nodes, uint32_t n_kv,
+                  uint32_t hd, uint32_t* err, void* stream);
 
 /* ------------------------------------------------------------------ */
 /* Synthetic inputs                                                    */

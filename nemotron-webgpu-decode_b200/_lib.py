@@ -25,6 +25,7 @@ NWD_ERR_DEVICE = 8
 
 NWD_DEVERR_PIPE_TIMEOUT = 1
 NWD_DEVERR_ROW_RANGE = 2
+NWD_DEVERR_TREE = 4
 
 
 class NwdError(RuntimeError):
@@ -83,6 +84,14 @@ SIGNATURES = {
                                           _P, _sz, _P]),
     "nwd_attn_prefill": (ctypes.c_int, [_P, _P, _P, _u64, _P, _P, _u32, _u32, _u32, _u32, _u32,
                                         _u32, _f32, _P, _sz, _P]),
+    "nwd_attn_tree_workspace_size": (ctypes.c_int, [_u32] * 5 + [ctypes.POINTER(_sz)]),
+    "nwd_attn_tree": (ctypes.c_int, [_P, _P, _P, _u64, _P, _P, _P, _P, _P, _u32, _u32, _u32, _u32,
+                                     _u32, _f32, _P, _sz, _P, _P]),
+    "nwd_kv_append_attn_tree": (ctypes.c_int, [_P, _P, _P, _P, _P, _u64, _P, _P, _P, _P, _P, _u32,
+                                               _u32, _u32, _u32, _u32, _f32, _P, _sz, _P, _P]),
+    "nwd_verify_tree": (ctypes.c_int, [_P] * 10 + [_u32] * 3 + [_P, _P]),
+    "nwd_kv_commit": (ctypes.c_int, [_P, _u32, _u64, _P, _P, _P, _P, _u32, _u32, _u32, _u32, _P,
+                                     _P]),
     "nwd_mgpu_unique_id": (ctypes.c_int, [_P]),
     "nwd_mgpu_init": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_int, ctypes.c_int, _u32, _u32,
                                      ctypes.POINTER(_P)]),

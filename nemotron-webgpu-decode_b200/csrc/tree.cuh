@@ -1,0 +1,67 @@
+// Trees of drafted tokens, as the speculative-decoding kernels read them.
+//
+// A tree of n <= 64 nodes is parents[0..n): parents[i] < i, or -1 for a root.
+// Nodes at or past tree_len[b] are absent.  A parent outside [-1, i) is
+// recorded as NWD_DEVERR_TREE and read as -1, so every walk towards the root
+// descends strictly and ends.
+#pragma once
+
+#include <stdint.h>
+
+#include "nwd.h"
+
+namespace nwd {
+
+constexpr uint32_t TREE_MAX_NODES = 64;  // one 64-bit mask per node
+
+// Node i's parent, or -1.
+static __device__ __forceinline__ int tree_parent(const int32_t* parents, int i, uint32_t* err) {
+  const int p = parents[i];
+  if (p >= -1 && p < i) return p;
+  if (err) atomicOr(err, NWD_DEVERR_TREE);
+  return -1;
+}
+
+// Bit j: node i sees node j (its ancestors and itself).
+static __device__ __forceinline__ uint64_t tree_mask(const int32_t* parents, int i, uint32_t* err) {
+  uint64_t m = 0;
+  for (; i >= 0; i = tree_parent(parents, i, err)) m |= 1ull << i;
+  return m;
+}
+
+// Present nodes of sequence b: tree_len[b] (nullptr: all), held to [0, n].
+static __device__ __forceinline__ uint32_t tree_nodes(const int32_t* tree_len, uint32_t b,
+                                                      uint32_t n, uint32_t* err) {
+  if (!tree_len) return n;
+  const int32_t l = tree_len[b];
+  if (l >= 0 && (uint32_t)l <= n) return (uint32_t)l;
+  if (err) atomicOr(err, NWD_DEVERR_TREE);
+  return l < 0 ? 0u : n;
+}
+
+// The rows of a sequence: ctx context rows from pool row row0, then its nodes'.
+// A sequence whose rows leave the pool is recorded as NWD_DEVERR_ROW_RANGE and
+// has no rows and no nodes.
+struct TreeSeq {
+  int64_t row0;
+  uint32_t ctx, nodes;
+};
+static __device__ __forceinline__ TreeSeq tree_seq(const int64_t* row_offset,
+                                                   const int32_t* seq_len, const int32_t* tree_len,
+                                                   uint64_t pool_rows, uint32_t b, uint32_t n,
+                                                   uint32_t* err) {
+  TreeSeq s;
+  s.row0 = row_offset[b];
+  const int32_t ctx = seq_len[b];
+  s.nodes = tree_nodes(tree_len, b, n, err);
+  s.ctx = (uint32_t)ctx;
+  if (s.row0 < 0 || ctx < 0 || (uint64_t)s.row0 > pool_rows ||
+      (uint64_t)ctx + s.nodes > pool_rows - (uint64_t)s.row0) {
+    if (err) atomicOr(err, NWD_DEVERR_ROW_RANGE);
+    s.row0 = 0;
+    s.ctx = s.nodes = 0;
+  }
+  return s;
+}
+
+}  // namespace nwd

@@ -185,6 +185,7 @@ class BatchedDecodeAttention:
         self.row_offset = offs.to(self.device)
         self.lengths = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
         self.workspace = ops.Workspace(self.batch, heads, kv_heads, head_dim, self.device)
+        self.scratch = ops.Scratch(self.device)  # device errors of the speculative calls
 
     def step(self, q, k_new, v_new, out=None, stream=None) -> torch.Tensor:
         """Every sequence appends one row and attends over its rows (fused launch)."""
@@ -198,6 +199,25 @@ class BatchedDecodeAttention:
         self.lengths += 1
         return out
 
+    def tree_step(self, q, k_new, v_new, parents, tree_len=None, out=None,
+                  stream=None) -> torch.Tensor:
+        """A speculative step: the trees' K/V rows go behind every sequence's rows and each
+        node attends the rows, its ancestors and itself.  q [B, N, heads, hd], k_new / v_new
+        [B, N, kv_heads, hd], parents [B, N] (:func:`ops.attention_tree`).  The lengths stay
+        until :meth:`commit`."""
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.float16, device=self.device)
+        return ops.kv_append_attention_tree(q, k_new, v_new, self.k_pool, self.v_pool,
+                                            self.row_offset, self.lengths, parents, out,
+                                            self.heads, self.kv_heads, self.head_dim,
+                                            tree_len=tree_len, scale=self.scale,
+                                            scratch=self.scratch, stream=stream)
+
+    def commit(self, path, n_accepted, stream=None) -> None:
+        """Keeps the accepted nodes of the last :meth:`tree_step` (:func:`ops.verify_tree`'s
+        path and n_accepted): their rows follow the context and the lengths grow by them."""
+        commit_layers([self], path, n_accepted, stream=stream)
+
     def attend(self, q, out=None, stream=None) -> torch.Tensor:
         if out is None:
             out = torch.empty(self.batch, self.heads, self.head_dim, dtype=torch.float16,
@@ -205,3 +225,22 @@ class BatchedDecodeAttention:
         return ops.attention_batched(q, self.k_pool, self.v_pool, self.row_offset, self.lengths,
                                      out, self.heads, self.kv_heads, self.head_dim,
                                      scale=self.scale, workspace=self.workspace, stream=stream)
+
+
+def commit_layers(layers, path, n_accepted, stream=None) -> None:
+    """:meth:`BatchedDecodeAttention.commit` for the layers of one model: the same sequences
+    and lengths in each (every layer has run the step's trees), all their pools moved in one
+    launch per eight layers."""
+    layers = list(layers)
+    if not layers:
+        return
+    first = layers[0]
+    pools = [p for layer in layers for p in (layer.k_pool, layer.v_pool)]
+
+    def run(raw):
+        ops.kv_commit(pools, first.row_offset, first.lengths, path, n_accepted,
+                      scratch=first.scratch, stream=stream)
+        for layer in layers:
+            layer.lengths += n_accepted
+
+    ops._on(first.lengths.device, stream, run)

@@ -371,6 +371,216 @@ def q4_qkv_append(h: torch.Tensor, wq: Q4Weights, wk: Q4Weights, wv: Q4Weights,
     return q_out
 
 
+# ---------------------------------------------------------------- speculative decoding
+
+def _same_device(device, named) -> None:
+    for name, t in named:
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
+
+
+def _shaped(t, dtype, shape, name) -> int:
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return _ptr(t, dtype, name)
+
+
+class TreeWorkspace:
+    """Partials of the tree-attention calls of one shape.  Needs no initialisation and
+    keeps nothing between calls; calls that may overlap need one each (without one, a
+    call allocates its own from PyTorch's allocator, on its stream)."""
+
+    def __init__(self, batch: int, n_nodes: int, n_heads: int, n_kv_heads: int,
+                 head_dim: int = 128, device=None):
+        device = torch.device(device if device is not None else "cuda")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.device = device
+        self.nbytes = _tree_ws_bytes(device.index, batch, n_nodes, n_heads, n_kv_heads, head_dim)
+        self._buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
+        self.ptr = self._buf.data_ptr()
+
+
+_tree_ws_sizes: dict = {}
+
+
+def _tree_ws_bytes(device: int, *shape) -> int:
+    """nwd_attn_tree_workspace_size of a shape (a pure function of shape and device)."""
+    key = (device,) + shape
+    n = _tree_ws_sizes.get(key)
+    if n is None:
+        v = ctypes.c_size_t(0)
+        with torch.cuda.device(device):
+            call("nwd_attn_tree_workspace_size", *shape, ctypes.byref(v))
+        n = _tree_ws_sizes[key] = int(v.value)
+    return n
+
+
+def _on(device, stream, fn):
+    """fn(raw stream) with `device` current and, for a given stream, PyTorch's allocations
+    on it: what the call allocates belongs to the stream that uses it."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _on(device, stream, fn)
+    if stream is None:
+        return fn(torch.cuda.current_stream(device).cuda_stream)
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    with torch.cuda.stream(stream):
+        return fn(stream.cuda_stream)
+
+
+def _attention_tree(name, q, new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads,
+                    n_kv_heads, head_dim, tree_len, scale, workspace, scratch, stream):
+    dev = q.device
+    _same_device(dev, (("k_pool", k_pool), ("v_pool", v_pool), ("row_offset", row_offset),
+                       ("seq_len", seq_len), ("parents", parents), ("tree_len", tree_len), ("o", o)))
+    if parents.dim() != 2:
+        raise ValueError(f"parents must be [batch, n_nodes], got {tuple(parents.shape)}")
+    batch, n = parents.shape
+    row = n_kv_heads * head_dim
+    qo = (batch, n, n_heads, head_dim)
+    qp = _shaped(q, torch.float16, qo, "q")
+    op = _shaped(o, torch.float16, qo, "o")
+    if row == 0 or k_pool.numel() % row or v_pool.numel() != k_pool.numel():
+        raise ValueError("k_pool and v_pool must hold the same whole number of rows")
+    args = [qp]
+    if new is not None:
+        _same_device(dev, (("k_new", new[0]), ("v_new", new[1])))
+        kv = (batch, n, n_kv_heads, head_dim)
+        args += [_shaped(new[0], torch.float16, kv, "k_new"),
+                 _shaped(new[1], torch.float16, kv, "v_new")]
+    args += [_h(k_pool, "k_pool"), _h(v_pool, "v_pool"), k_pool.numel() // row,
+             _shaped(row_offset, torch.int64, (batch,), "row_offset"),
+             _shaped(seq_len, torch.int32, (batch,), "seq_len" if new is None else "pos"),
+             _ptr(parents, torch.int32, "parents"),
+             None if tree_len is None else _shaped(tree_len, torch.int32, (batch,), "tree_len"),
+             op, batch, n, n_heads, n_kv_heads, head_dim, float(scale)]
+    err = None
+    if scratch is not None:
+        err = scratch.ptr
+
+    def run(raw):
+        ws, buf = workspace, None
+        if ws is None:
+            nbytes = _tree_ws_bytes(dev.index, batch, n, n_heads, n_kv_heads, head_dim)
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            call(name, *args, buf.data_ptr(), nbytes, err, raw)
+        else:
+            call(name, *args, ws.ptr, ws.nbytes, err, raw)
+        return o
+
+    return _on(dev, stream, run)
+
+
+def attention_tree(q, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads: int,
+                   n_kv_heads: int, head_dim: int = 128, tree_len=None, scale: float = 0.0,
+                   workspace: TreeWorkspace | None = None, scratch: Scratch | None = None,
+                   stream=None) -> torch.Tensor:
+    """Attention for a tree of drafted tokens per sequence, over one read of the cache:
+    q/o [B, N, n_heads, hd] fp16; node i of sequence b (pool row row_offset[b] + seq_len[b]
+    + i, already written) attends the seq_len[b] context rows, its ancestors and itself.
+
+    parents [B, N] int32: parents[b, i] < i, -1 for a root; N <= 64.  tree_len [B] int32:
+    nodes at or past it are absent (their o is zero).  Device errors (a parent or length out
+    of range, rows outside the pool) go to `scratch` (:meth:`Scratch.check`) when given."""
+    return _attention_tree("nwd_attn_tree", q, None, k_pool, v_pool, row_offset, seq_len, parents,
+                           o, n_heads, n_kv_heads, head_dim, tree_len, scale, workspace, scratch,
+                           stream)
+
+
+def kv_append_attention_tree(q, k_new, v_new, k_pool, v_pool, row_offset, pos, parents, o,
+                             n_heads: int, n_kv_heads: int, head_dim: int = 128, tree_len=None,
+                             scale: float = 0.0, workspace: TreeWorkspace | None = None,
+                             scratch: Scratch | None = None, stream=None) -> torch.Tensor:
+    """:func:`attention_tree` after writing the present nodes' rows k_new / v_new
+    [B, N, n_kv, hd] to pool rows row_offset[b] + pos[b] + i (pos: rows before the tree)."""
+    return _attention_tree("nwd_kv_append_attn_tree", q, (k_new, v_new), k_pool, v_pool,
+                           row_offset, pos, parents, o, n_heads, n_kv_heads, head_dim, tree_len,
+                           scale, workspace, scratch, stream)
+
+
+def verify_tree(tokens, parents, target_probs, u, w, draft_probs=None, tree_len=None, out=None,
+                scratch: Scratch | None = None, stream=None):
+    """Which drafted tokens stand (multi-round rejection sampling from given uniforms):
+    (path [B, N] int32: accepted nodes from node 0 on, then -1; n_accepted [B] int32;
+    next_token [B] int32).
+
+    tokens / parents [B, N] int32, node 0 the pending token; target_probs [B, N, V] f32 (row
+    i: the target behind node i); draft_probs of the same shape (row i: what node i's
+    children were drawn from) or None for drafts without probabilities; u [B, N], w [B] f32
+    uniforms in [0, 1).  `out`: the three outputs, to be written in place."""
+    dev = target_probs.device
+    _same_device(dev, (("tokens", tokens), ("parents", parents), ("u", u), ("w", w),
+                       ("draft_probs", draft_probs), ("tree_len", tree_len)))
+    if target_probs.dim() != 3:
+        raise ValueError("target_probs must be [batch, n_nodes, vocab], got "
+                         f"{tuple(target_probs.shape)}")
+    shape = target_probs.shape
+    batch, n, vocab = shape
+    bn, b1 = (batch, n), (batch,)
+    args = [_shaped(tokens, torch.int32, bn, "tokens"), _shaped(parents, torch.int32, bn, "parents"),
+            None if tree_len is None else _shaped(tree_len, torch.int32, b1, "tree_len"),
+            _ptr(target_probs, torch.float32, "target_probs"),
+            None if draft_probs is None else _shaped(draft_probs, torch.float32, shape,
+                                                     "draft_probs"),
+            _shaped(u, torch.float32, bn, "u"), _shaped(w, torch.float32, b1, "w")]
+    err = None if scratch is None else scratch.ptr
+
+    def run(raw):
+        res = out
+        if res is None:
+            res = (torch.empty(bn, dtype=torch.int32, device=dev),
+                   torch.empty(b1, dtype=torch.int32, device=dev),
+                   torch.empty(b1, dtype=torch.int32, device=dev))
+        else:
+            _same_device(dev, (("path", res[0]), ("n_accepted", res[1]), ("next_token", res[2])))
+        call("nwd_verify_tree", *args, _shaped(res[0], torch.int32, bn, "path"),
+             _shaped(res[1], torch.int32, b1, "n_accepted"),
+             _shaped(res[2], torch.int32, b1, "next_token"), batch, n, vocab, err, raw)
+        return tuple(res)
+
+    return _on(dev, stream, run)
+
+
+def kv_commit(pools, row_offset, pos, path, n_accepted, scratch: Scratch | None = None,
+              stream=None) -> None:
+    """Leaves the cache as if only the accepted nodes had been decoded: pool row
+    row_offset[b] + pos[b] + path[b, j] moves to row_offset[b] + pos[b] + j for j <
+    n_accepted[b], in every pool of `pools` (K and V of several layers, each [rows, n_kv, hd]
+    fp16, 16 per launch).  path / n_accepted as :func:`verify_tree` returns them; the
+    caller's lengths grow by n_accepted."""
+    pools = list(pools)
+    if path.dim() != 2:
+        raise ValueError(f"path must be [batch, n_nodes], got {tuple(path.shape)}")
+    batch, n = path.shape
+    dev = path.device
+    _same_device(dev, (("row_offset", row_offset), ("pos", pos), ("n_accepted", n_accepted)))
+    args = (_shaped(row_offset, torch.int64, (batch,), "row_offset"),
+            _shaped(pos, torch.int32, (batch,), "pos"), _ptr(path, torch.int32, "path"),
+            _shaped(n_accepted, torch.int32, (batch,), "n_accepted"))
+    if not pools:
+        return
+    shape = pools[0].shape
+    if len(shape) != 3:
+        raise ValueError(f"pools must be [rows, n_kv, hd], got {tuple(shape)}")
+    ptrs = []
+    for i, t in enumerate(pools):
+        _same_device(dev, ((f"pool {i}", t),))
+        ptrs.append(_shaped(t, torch.float16, shape, f"pool {i}"))
+    if len(set(ptrs)) != len(ptrs):
+        raise ValueError("pools must differ from one another")
+    err = None if scratch is None else scratch.ptr
+
+    def run(raw):
+        for i in range(0, len(ptrs), 16):
+            part = ptrs[i:i + 16]
+            call("nwd_kv_commit", (ctypes.c_void_p * len(part))(*part), len(part), shape[0], *args,
+                 batch, n, shape[1], shape[2], err, raw)
+
+    _on(dev, stream, run)
+
+
 def selftest_wait_timeout(workspace: "Workspace", stream=None) -> int:
     """Make one of the library's bounded device waits run out (about 2 s) and return the
     workspace's device error word afterwards (NWD_DEVERR_PIPE_TIMEOUT expected); the
@@ -416,5 +626,6 @@ __all__ = [
     "kv_append_batched", "attention", "kv_append_attention", "attention_batched",
     "kv_append_attention_batched", "attention_partial", "merge", "fill_normal", "Scratch",
     "kv_append_rows", "attention_prefill", "packed_partials", "merge_packed", "Q4Weights",
-    "q4_gemv", "q4_qkv_append",
+    "q4_gemv", "q4_qkv_append", "TreeWorkspace", "attention_tree", "kv_append_attention_tree",
+    "verify_tree", "kv_commit",
 ]
