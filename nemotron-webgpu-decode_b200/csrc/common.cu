@@ -75,6 +75,41 @@ int current_device_info(DeviceInfo* out) {
   return NWD_OK;
 }
 
+// The driver's tensor-map encoder, looked up once.
+static int load_encoder() {
+  std::call_once(g_encode_once, [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    g_encode_err = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000,
+                                                    cudaEnableDefault, &q);
+    if (g_encode_err == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  });
+  if (!g_encode)
+    return fail(NWD_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable (%s)",
+                cudaGetErrorString(g_encode_err));
+  return NWD_OK;
+}
+
+int tree_q_tensor_map(CUtensorMap* out, const void* base, uint64_t nodes, uint32_t n_kv,
+                      uint32_t group, uint32_t box_nodes) {
+  int st = load_encoder();
+  if (st) return st;
+  const cuuint64_t hd = 128;
+  cuuint64_t dims[5] = {64, 2, group, n_kv, nodes};
+  cuuint64_t strides[4] = {128, hd * 2, hd * 2 * group, hd * 2 * group * n_kv};
+  cuuint32_t box[5] = {64, 1, group, 1, box_nodes};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = g_encode(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(base), dims,
+                        strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(NWD_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d) for base %p nodes %llu group %u",
+                (int)r, base, (unsigned long long)nodes, group);
+  return NWD_OK;
+}
+
 int kv_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, uint32_t n_kv, uint32_t hd,
                   uint32_t box_rows, uint32_t box_chunks) {
   int dev = 0;
@@ -88,18 +123,8 @@ int kv_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, uint32_t n_
       return NWD_OK;
     }
   }
-  std::call_once(g_encode_once, [] {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    g_encode_err = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000,
-                                                    cudaEnableDefault, &q);
-    if (g_encode_err == cudaSuccess && q == cudaDriverEntryPointSuccess)
-      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-  });
-  if (!g_encode) {
-    return fail(NWD_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable (%s)",
-                cudaGetErrorString(g_encode_err));
-  }
+  int st = load_encoder();
+  if (st) return st;
   if (hd % 64 != 0) return fail(NWD_ERR_UNSUPPORTED, "head_dim %u is not a multiple of 64", hd);
   if (rows == 0 || rows > (1ull << 31))
     return fail(NWD_ERR_INVALID, "cache rows %llu outside [1, 2^31]", (unsigned long long)rows);

@@ -33,6 +33,12 @@ int current_device_info(DeviceInfo* out);
 int kv_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, uint32_t n_kv, uint32_t hd,
                   uint32_t box_rows, uint32_t box_chunks = 0);
 
+// Encodes the 5-D tensor map of a tree's queries [nodes, n_kv, group, 128] of
+// fp16: dims {64, 2, group, n_kv, nodes}, box {64, 1, group, 1, box_nodes},
+// 128-byte swizzle: box_nodes * group rows of one 64-wide column chunk.
+int tree_q_tensor_map(CUtensorMap* out, const void* base, uint64_t nodes, uint32_t n_kv,
+                      uint32_t group, uint32_t box_nodes);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---- decode of one short sequence (decode_short.cu) ----

@@ -1,4 +1,5 @@
-// Attention for a tree of drafted tokens over the KV pool.
+// Attention for a tree of drafted tokens over the KV pool, on the
+// 5th-generation tensor cores (tcgen05.mma, accumulators in tensor memory).
 //
 // Node i of sequence b sits at pool row row_offset[b] + seq_len[b] + i and
 // attends the seq_len[b] context rows, its ancestors' rows and its own:
@@ -7,77 +8,886 @@
 // chain of n nodes computes what n of its steps would, a tree several such
 // chains that share their beginnings, over one read of the cache.
 //
-// One warp per (sequence, node, head): the lanes hold 4 of the 128 dims each,
-// a row's score is a warp sum, the softmax runs online in f32.
+// Tiles.  The n_nodes * group query rows of a kv head (node-major) are cut
+// into tiles of whole nodes, at most 128 rows: the M of an MMA.  A unit is a
+// (sequence, kv head) with one or two of its tiles, a block 128 cache rows.
+// The blocks of all units form one line that is cut into an equal range per
+// persistent CTA (one per SM); a unit that a cut divides leaves one partial
+// (m, l, O) per CTA in the workspace, which merge_kernel joins in order.
+//
+// A CTA's 12 warps:
+//   warps 0, 2, 3  TMA producers: K blocks into 3 stages, each unit's Q tiles
+//                  into 2, V blocks into 2 (each 128 x 128 fp16 as two
+//                  64-column chunks, 128-byte swizzle: the K-major operand
+//                  layout).  Separate warps, so none waits behind another's
+//                  buffers.  Warp 2 also owns the tensor memory.
+//   warp 1         MMA issuer (one thread): a turn is S = Q K^T of one (block,
+//                  tile) and O += P V after its softmax.  Turns alternate
+//                  between the two softmax groups, S two turns ahead of P V,
+//                  so one group's softmax runs beside the other's MMAs.
+//   warps 4-7, 8-11  the softmax groups, a thread per query row, each with its
+//                  own score and output accumulators (S0 S1 O0 O1: all 512
+//                  columns).  A unit of two tiles gives each group a tile and
+//                  both use every K/V block; a unit of one tile gives the
+//                  groups alternate blocks and joins their (m, l, O) at its
+//                  end, which keeps both busy when there are few query rows.
+//
+// Softmax in the log2 domain with a lazily moved maximum (O is rescaled in
+// tensor memory only when a row's maximum grows by more than 2^8).  P is
+// rounded to fp16 once, as P V's operand: 2^-11 of a weight, at random over
+// the rows, so about the size of the output's own rounding; its largest value
+// is put near 2^15 (P_BIAS) so that weights down to 2^-29 of the largest keep
+// all their bits, which a long flat tail behind one large score needs.  Sums
+// and accumulators are f32.
+//
+// Rows a node does not attend never reach its output: scores are selected to
+// -inf before the maximum, V rows behind the tree are zeroed in shared memory
+// (0 x NaN would be NaN), and NaN or infinities in the V rows of the tree are
+// zeroed there too and added at the end to the nodes that see them.
+//
+// All waits are bounded: on expiry the kernel records NWD_DEVERR_PIPE_TIMEOUT,
+// lets its copies and MMAs land, frees its tensor memory and returns.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstring>
 
 #include "nwd_common.h"
+#include "ptx.cuh"
+#include "tc.cuh"
 #include "tree.cuh"
 
 namespace {
 
+using namespace nwd::ptx;
+using namespace nwd::tc;
 using nwd::TreeSeq;
 
 constexpr uint32_t HD = 128;
+constexpr uint32_t BM = 128;            // query rows per tile
+constexpr uint32_t BN = 128;            // cache rows per block
+constexpr int THREADS = 384;
+constexpr uint32_t CHUNK = 128 * 128;   // 128 rows x 64 fp16
+constexpr uint32_t TILE = 2 * CHUNK;    // 128 x 128 fp16: 32 KiB
+constexpr uint32_t NQ = 2, NK = 3, NV = 2;  // stages
+constexpr uint32_t MAX_GROUPS32 = 128;  // batch / 32
+constexpr uint32_t MIN_BLOCKS = 1;      // least blocks per CTA range
 
-struct TreeParams {
-  const __half* q;
-  const __half* k;
+constexpr uint32_t O_Q = 0;
+constexpr uint32_t O_K = O_Q + NQ * TILE;
+constexpr uint32_t O_V = O_K + NK * TILE;
+constexpr uint32_t O_ML = O_V + NV * TILE;        // [2 groups][128] (m, l); the plan's sums before
+constexpr uint32_t O_BAR = O_ML + 2 * BM * 8;
+constexpr int B_QFULL = 0, B_QEMPTY = B_QFULL + NQ, B_KFULL = B_QEMPTY + NQ,
+              B_KEMPTY = B_KFULL + NK, B_VFULL = B_KEMPTY + NK, B_VEMPTY = B_VFULL + NV,
+              B_VTMA = B_VEMPTY + NV,
+              // by softmax group
+    B_SFULL = B_VTMA + 1, B_PFULL = B_SFULL + 2, B_OFULL = B_PFULL + 2, B_OEMPTY = B_OFULL + 2,
+              B_ML = B_OEMPTY + 2, B_DRAIN = B_ML + 2, NBAR = B_DRAIN + 1;
+constexpr uint32_t O_PLAN = O_BAR + NBAR * 8;     // Plan
+constexpr uint32_t O_VBAD = O_PLAN + 48;          // [NV] u64: tree rows with NaN or inf in V
+constexpr uint32_t O_GBAD = O_VBAD + NV * 8;      // [2] u64: the same, gathered per group
+constexpr uint32_t O_MISC = O_GBAD + 16;          // tensor memory base, abort flag
+constexpr uint32_t SMEM_USED = O_MISC + 16;
+// dynamic shared memory starts 1024-byte aligned (there is no static shared
+// memory in this kernel); the kernel checks it
+constexpr uint32_t SMEM_BYTES = SMEM_USED;
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
+static_assert(MAX_GROUPS32 * 8 <= 2 * BM * 8, "the plan's sums fit the (m, l) area");
+
+constexpr uint32_t TMEM_COLS = 512;  // S0 S1 O0 O1, 128 columns each
+constexpr uint32_t TMEM_O = 256;
+constexpr float RESCALE_LOG2 = 8.f;
+constexpr float P_BIAS = 7.f;  // P = 2^(s - m + 7) <= 2^15, m within 2^8 of the maximum
+constexpr uint32_t IDESC_S = idesc_f16(BM, BN, false);
+constexpr uint32_t IDESC_O = idesc_f16(BM, HD, true);
+
+struct TParams {
   const __half* v;
   __half* o;
   const int64_t* row_offset;
   const int32_t* seq_len;
   const int32_t* parents;
   const int32_t* tree_len;
-  uint32_t* err;
+  uint32_t* err;      // the caller's error word, or the workspace's
+  uint8_t* ws;
   uint64_t pool_rows;
   uint32_t batch, n_nodes, n_heads, n_kv, group;
-  float scale;
+  uint32_t tile_nodes, n_tiles, unit_tiles, n_units;  // n_units: per sequence
+  float scale_log2;
 };
 
-__device__ __forceinline__ float4 load4(const __half* p) {
-  const uint2 u = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-  return make_float4(a.x, a.y, b.x, b.y);
+struct Plan {
+  uint64_t left;  // blocks of this CTA's range
+  uint32_t b, u, blk;
+  uint32_t pad[5];
+};
+static_assert(sizeof(Plan) <= 48, "plan");
+
+// ---- workspace: [0, 256) an error word nobody reads (when the caller gives
+// none), MergeDesc per CTA, then per CTA two slots (the piece its range begins
+// with, the piece it ends with) of unit_tiles tiles: (m, l) [tile][128], then
+// O [tile][32 column quads][128 rows][4] f32.
+struct MergeDesc {
+  uint32_t valid, b, u, first;  // the unit's pieces are CTAs first .. this one
+};
+constexpr uint32_t MAX_CTAS = 240;
+constexpr size_t WS_DESC = 256;
+constexpr size_t WS_ML = WS_DESC + MAX_CTAS * sizeof(MergeDesc);
+__host__ __device__ inline size_t ws_o(uint32_t ctas, uint32_t unit_tiles) {
+  return WS_ML + (size_t)ctas * 2 * unit_tiles * BM * 8;
+}
+__host__ __device__ inline size_t ws_total(uint32_t ctas, uint32_t unit_tiles) {
+  return ws_o(ctas, unit_tiles) + (size_t)ctas * 2 * unit_tiles * BM * HD * 4;
+}
+static_assert(WS_ML % 256 == 0, "alignment");
+
+__device__ __forceinline__ TreeSeq load_seq(const TParams& p, uint32_t b, uint32_t* err) {
+  return nwd::tree_seq(p.row_offset, p.seq_len, p.tree_len, p.pool_rows, b, p.n_nodes, err);
+}
+// A unit has at least one block, so that every output row is written.
+__device__ __forceinline__ uint32_t seq_blocks(const TreeSeq& s) {
+  return max(1u, (s.ctx + s.nodes + BN - 1) / BN);
 }
 
-__global__ void tree_attn_kernel(const TreeParams p) {
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t hkv = blockIdx.x % p.n_kv, i = blockIdx.x / p.n_kv, b = blockIdx.y;
-  const uint32_t h = hkv * p.group + warp;
-  const TreeSeq s = nwd::tree_seq(p.row_offset, p.seq_len, p.tree_len, p.pool_rows, b, p.n_nodes,
-                                  p.err);
-  const uint64_t sees =
-      i < s.nodes ? nwd::tree_mask(p.parents + (uint64_t)b * p.n_nodes, (int)i, p.err) : 0;
-  const uint64_t at = (((uint64_t)b * p.n_nodes + i) * p.n_heads + h) * HD + lane * 4;
-  const float4 q = load4(p.q + at);
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const uint32_t rows = i < s.nodes ? s.ctx + i + 1 : 0;
-  for (uint32_t t = 0; t < rows; t++) {
-    if (t >= s.ctx && !((sees >> (t - s.ctx)) & 1)) continue;
-    const uint64_t r = (((uint64_t)s.row0 + t) * p.n_kv + hkv) * HD + lane * 4;
-    const float4 k = load4(p.k + r);
-    float d = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
-#pragma unroll
-    for (int x = 16; x; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
-    d *= p.scale;
-    const float mn = fmaxf(m, d), alpha = m == -INFINITY ? 0.f : expf(m - mn), w = expf(d - mn);
-    const float4 v = load4(p.v + r);
-    l = l * alpha + w;
-    acc.x = acc.x * alpha + w * v.x;
-    acc.y = acc.y * alpha + w * v.y;
-    acc.z = acc.z * alpha + w * v.z;
-    acc.w = acc.w * alpha + w * v.w;
-    m = mn;
+// The pieces of a CTA's range: blocks [blk, blk + nb) of unit u of sequence b.
+struct Pieces {
+  uint64_t left;
+  uint32_t b, u, blk, nb, nblk;
+  TreeSeq s;
+  __device__ __forceinline__ void load(const TParams& p) {
+    s = load_seq(p, b, nullptr);
+    nblk = seq_blocks(s);
   }
-  const float inv = rows ? 1.f / l : 0.f;
-  __half2* out = reinterpret_cast<__half2*>(p.o + at);
-  out[0] = __floats2half2_rn(acc.x * inv, acc.y * inv);
-  out[1] = __floats2half2_rn(acc.z * inv, acc.w * inv);
+  __device__ __forceinline__ bool begin(const TParams& p, const Plan& plan) {
+    left = plan.left;
+    b = plan.b;
+    u = plan.u;
+    blk = plan.blk;
+    if (left == 0) return false;
+    load(p);
+    nb = (uint32_t)min((uint64_t)(nblk - blk), left);
+    return true;
+  }
+  __device__ __forceinline__ bool next(const TParams& p) {
+    left -= nb;
+    if (left == 0) return false;
+    blk = 0;
+    if (++u == p.n_units) {
+      u = 0;
+      b++;
+      load(p);
+    }
+    nb = (uint32_t)min((uint64_t)nblk, left);
+    return true;
+  }
+};
+// A unit's kv head, first tile and number of tiles.
+struct Unit {
+  uint32_t hkv, tile0, tiles;
+};
+__device__ __forceinline__ Unit unit_of(const TParams& p, uint32_t u) {
+  const uint32_t per_head = (p.n_tiles + p.unit_tiles - 1) / p.unit_tiles;
+  Unit r;
+  r.hkv = u / per_head;
+  r.tile0 = (u % per_head) * p.unit_tiles;
+  r.tiles = min(p.unit_tiles, p.n_tiles - r.tile0);
+  return r;
+}
+
+// Position in a ring of N stages.
+template <uint32_t N>
+struct Ring {
+  uint32_t i = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == N) {
+      i = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// This CTA's range of the line of blocks.  Called by all threads; `sums` is
+// shared scratch.  per = the range length, the same in every CTA.
+__device__ void make_plan(const TParams& p, uint64_t* sums, Plan* plan, MergeDesc* desc) {
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t groups = (p.batch + 31) / 32;
+  auto blocks_of = [&](uint32_t b) {
+    return b < p.batch ? seq_blocks(load_seq(p, b, p.err)) : 0u;
+  };
+  for (uint32_t g = warp; g < groups; g += THREADS / 32) {
+    const uint32_t n = __reduce_add_sync(0xffffffffu, blocks_of(g * 32 + lane));
+    if (lane == 0) sums[g] = n;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    // lane l holds groups 4 l .. 4 l + 3
+    uint64_t mine = 0;
+    for (uint32_t g = lane * 4; g < min(groups, lane * 4 + 4); g++) mine += sums[g];
+    uint64_t incl = mine;
+#pragma unroll
+    for (int i = 1; i < 32; i <<= 1) {
+      const uint64_t y = __shfl_up_sync(0xffffffffu, incl, i);
+      if ((int)lane >= i) incl += y;
+    }
+    const uint64_t total = __shfl_sync(0xffffffffu, incl, 31) * p.n_units;
+    const uint64_t per = max((total + gridDim.x - 1) / gridDim.x, (uint64_t)MIN_BLOCKS);
+    const uint64_t x0 = min(total, (uint64_t)blockIdx.x * per), x1 = min(total, x0 + per);
+    MergeDesc d{0, 0, 0, 0};
+    Plan pl{};
+    pl.left = x1 - x0;
+    if (x1 > x0) {
+      const uint64_t y = x0 / p.n_units;  // in blocks of a single unit per sequence
+      uint64_t base = incl - mine;
+      const uint32_t owner =
+          __ffs(__ballot_sync(0xffffffffu, base <= y && y < incl)) - 1;
+      uint32_t g = lane * 4;
+      if (lane == owner)
+        while (y >= base + sums[g]) base += sums[g++];
+      g = __shfl_sync(0xffffffffu, g, owner);
+      base = __shfl_sync(0xffffffffu, base, owner);
+      const uint32_t n = blocks_of(g * 32 + lane);
+      uint32_t upto = n;
+#pragma unroll
+      for (int i = 1; i < 32; i <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, i);
+        if ((int)lane >= i) upto += v;
+      }
+      const uint64_t lo = base + upto - n;
+      const uint32_t at = __ffs(__ballot_sync(0xffffffffu, lo <= y && y < lo + n)) - 1;
+      if (lane == at) {
+        const uint64_t r = x0 - lo * p.n_units;
+        pl.b = g * 32 + lane;
+        pl.u = (uint32_t)(r / n);
+        pl.blk = (uint32_t)(r % n);
+        const uint64_t ends = x0 - pl.blk + n;  // of the unit, on the line
+        if (pl.blk > 0 && ends <= x1)
+          d = MergeDesc{1, pl.b, pl.u, (uint32_t)((x0 - pl.blk) / per)};
+        *plan = pl;
+        desc[blockIdx.x] = d;
+      }
+    } else if (lane == 0) {
+      *plan = pl;
+      desc[blockIdx.x] = d;
+    }
+  }
+  __syncthreads();
+}
+
+// Stores 4 columns (from column c) of a partial's row.
+__device__ __forceinline__ void store_part(float* slot, uint32_t row, uint32_t c, const float* v) {
+  *reinterpret_cast<float4*>(slot + ((size_t)(c >> 2) * BM + row) * 4) =
+      make_float4(v[0], v[1], v[2], v[3]);
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+    tree_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                const __grid_constant__ CUtensorMap tmv, const __grid_constant__ TParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sb = smem_u32(smem);
+  const uint32_t bar = sb + O_BAR;  // + 8 * index
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + O_MISC);
+  volatile int32_t* abort_flag = reinterpret_cast<int32_t*>(smem + O_MISC + 4);
+  volatile uint64_t* vbad = reinterpret_cast<uint64_t*>(smem + O_VBAD);
+  volatile uint64_t* gbad = reinterpret_cast<uint64_t*>(smem + O_GBAD);
+  const Plan& plan = *reinterpret_cast<const Plan*>(smem + O_PLAN);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t* const err = p.err;
+
+  nwd::pdl_trigger();
+  if (tid == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < NBAR; i++) {
+      uint32_t count = 1;
+      if (i >= B_PFULL && i < B_PFULL + 2) count = BM;
+      if (i >= B_OEMPTY && i < B_OEMPTY + 2) count = 2 * BM;
+      if (i >= B_ML && i < B_ML + 2) count = BM;
+      mbar_init(bar + 8 * i, count);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  nwd::pdl_wait();
+  make_plan(p, reinterpret_cast<uint64_t*>(smem + O_ML),
+            reinterpret_cast<Plan*>(smem + O_PLAN),
+            reinterpret_cast<MergeDesc*>(p.ws + WS_DESC));
+  if (tid == 0 && (sb & 1023u)) {  // the swizzled tiles would not line up: no work
+    reinterpret_cast<Plan*>(smem + O_PLAN)->left = 0;
+    atomicOr(err, NWD_DEVERR_PIPE_TIMEOUT);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // Registers per thread: 56 for the first warpgroup, 224 for the softmax
+  // groups: 128 * (56 + 2 * 224) = 64512, the 384 * 168 of the launch.
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
+    if (warp == 0) {
+      // ======================= K =======================
+      const uint64_t policy = p.n_units == p.n_kv ? evict_first_policy() : evict_last_policy();
+      uint32_t issued[NK] = {};
+      Ring<NK> r;
+      Pieces w;
+      bool ok = true;
+      for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
+        const int hkv = (int)unit_of(p, w.u).hkv;
+        for (uint32_t j = 0; j < w.nb; j++) {
+          if (!warp_wait(bar + 8 * (B_KEMPTY + r.i), r.phase ^ 1u, abort_flag, err)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            const uint32_t fb = bar + 8 * (B_KFULL + r.i), dst = sb + O_K + r.i * TILE;
+            const int row = (int)(w.s.row0 + (int64_t)(w.blk + j) * BN);
+            mbar_arrive_tx(fb, TILE);
+            tma_load_4d(dst, &tmk, fb, 0, 0, hkv, row, policy);
+            tma_load_4d(dst + CHUNK, &tmk, fb, 0, 1, hkv, row, policy);
+          }
+          __syncwarp();
+#pragma unroll
+          for (uint32_t i = 0; i < NK; i++) issued[i] += r.i == i;
+          r.next();
+        }
+      }
+      if (!ok) {  // let the copies in flight land before the CTA can exit
+        const uint64_t t0 = globaltimer();
+#pragma unroll
+        for (uint32_t i = 0; i < NK; i++)
+          if (issued[i])
+            while (!mbar_try_wait(bar + 8 * (B_KFULL + i), (issued[i] - 1) & 1) &&
+                   globaltimer() - t0 < WAIT_LIMIT_NS) {
+            }
+      }
+    } else if (warp == 2) {
+      // ======================= Q =======================
+      const uint64_t policy = evict_first_policy();
+      const uint32_t bytes = 2 * p.tile_nodes * p.group * 128;
+      uint32_t issued[NQ] = {};
+      Ring<NQ> r;
+      Pieces w;
+      bool ok = true;
+      for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
+        const Unit un = unit_of(p, w.u);
+        for (uint32_t t = 0; t < un.tiles; t++) {
+          if (!warp_wait(bar + 8 * (B_QEMPTY + r.i), r.phase ^ 1u, abort_flag, err)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            const uint32_t fb = bar + 8 * (B_QFULL + r.i), dst = sb + O_Q + r.i * TILE;
+            const int node = (int)(w.b * p.n_nodes + (un.tile0 + t) * p.tile_nodes);
+            mbar_arrive_tx(fb, bytes);
+            tma_load_5d(dst, &tmq, fb, 0, 0, 0, (int)un.hkv, node, policy);
+            tma_load_5d(dst + CHUNK, &tmq, fb, 0, 1, 0, (int)un.hkv, node, policy);
+          }
+          __syncwarp();
+#pragma unroll
+          for (uint32_t i = 0; i < NQ; i++) issued[i] += r.i == i;
+          r.next();
+        }
+      }
+      if (!ok) {
+        const uint64_t t0 = globaltimer();
+#pragma unroll
+        for (uint32_t i = 0; i < NQ; i++)
+          if (issued[i])
+            while (!mbar_try_wait(bar + 8 * (B_QFULL + i), (issued[i] - 1) & 1) &&
+                   globaltimer() - t0 < WAIT_LIMIT_NS) {
+            }
+      }
+    } else if (warp == 3) {
+      // ======================= V =======================
+      const uint64_t policy = p.n_units == p.n_kv ? evict_first_policy() : evict_last_policy();
+      uint32_t issued[NV] = {}, tails = 0;
+      Ring<NV> r;
+      Pieces w;
+      bool ok = true;
+      for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
+        const int hkv = (int)unit_of(p, w.u).hkv;
+        for (uint32_t j = 0; j < w.nb; j++) {
+          if (!warp_wait(bar + 8 * (B_VEMPTY + r.i), r.phase ^ 1u, abort_flag, err)) {
+            ok = false;
+            break;
+          }
+          const uint32_t key0 = (w.blk + j) * BN, rows = w.s.ctx + w.s.nodes;
+          // a block with rows of the tree, or behind it, completes on VTMA;
+          // this warp makes it fit to multiply and releases the stage
+          const bool tail = key0 + BN > w.s.ctx;
+          const uint32_t fb = bar + 8 * (tail ? B_VTMA : B_VFULL + (int)r.i);
+          if (lane == 0) {
+            const uint32_t dst = sb + O_V + r.i * TILE;
+            const int row = (int)(w.s.row0 + key0);
+            mbar_arrive_tx(fb, TILE);
+            tma_load_4d(dst, &tmv, fb, 0, 0, hkv, row, policy);
+            tma_load_4d(dst + CHUNK, &tmv, fb, 0, 1, hkv, row, policy);
+          }
+          __syncwarp();
+          if (tail) {
+            tails++;
+            if (!warp_wait(fb, (tails - 1) & 1, abort_flag, err)) {
+              ok = false;
+              break;
+            }
+            const uint32_t t0 = w.s.ctx > key0 ? w.s.ctx - key0 : 0;
+            const uint32_t t1 = rows > key0 ? min(rows - key0, BN) : 0;
+            uint4* st = reinterpret_cast<uint4*>(smem + O_V + r.i * TILE);
+            // the tree's rows: 8 uint4 of a row per chunk (a swizzled row
+            // stays within its 128 bytes)
+            uint64_t bad = 0;
+            for (uint32_t i = t0 * 8 + lane; i < t1 * 8; i += 32) {
+#pragma unroll
+              for (uint32_t c = 0; c < 2; c++) {
+                uint4* at = st + c * (CHUNK / 16) + i;
+                uint4 x = *at;
+                uint32_t* e = &x.x;
+                bool hit = false;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                  const bool lo = (e[k] & 0x7c00u) == 0x7c00u;
+                  const bool hi = (e[k] & 0x7c000000u) == 0x7c000000u;
+                  hit |= lo | hi;
+                  if (lo) e[k] &= 0xffff0000u;
+                  if (hi) e[k] &= 0x0000ffffu;
+                }
+                if (hit) {
+                  *at = x;
+                  bad |= 1ull << (key0 + i / 8 - w.s.ctx);
+                }
+              }
+            }
+            const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+            for (uint32_t i = max(t1, t0) * 8 + lane; i < BN * 8; i += 32) {
+              st[i] = z;
+              st[CHUNK / 16 + i] = z;
+            }
+            const uint32_t blo = __reduce_or_sync(0xffffffffu, (uint32_t)bad);
+            const uint32_t bhi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32));
+            if (lane == 0) vbad[r.i] = (uint64_t)bhi << 32 | blo;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar + 8 * (B_VFULL + r.i));
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < NV; i++) issued[i] += r.i == i;
+          r.next();
+        }
+      }
+      if (!ok) {
+        const uint64_t t0 = globaltimer();
+#pragma unroll
+        for (uint32_t i = 0; i < NV; i++)
+          if (issued[i])
+            while (!mbar_try_wait(bar + 8 * (B_VFULL + i), (issued[i] - 1) & 1) &&
+                   globaltimer() - t0 < WAIT_LIMIT_NS) {
+            }
+        if (tails)
+          while (!mbar_try_wait(bar + 8 * B_VTMA, (tails - 1) & 1) &&
+                 globaltimer() - t0 < WAIT_LIMIT_NS) {
+          }
+      }
+    } else {
+      // ======================= MMA issuer =======================
+      // Turn x (block j, tile t of a piece; group x & 1): S(x), S(x+1), then
+      // for each x: P V(x), S(x+2).  S(x+2) overwrites the scores that P V(x)
+      // reads as P: the MMAs of one thread run in order.
+      if (lane == 0) {
+        Pieces ws, wp;
+        Unit us{}, up{};
+        uint32_t js = 0, ts = 0, jp = 0, tp = 0, xs = 0, xp = 0;
+        Ring<NQ> rq, rq_piece;
+        Ring<NK> rk;
+        Ring<NV> rv;
+        uint32_t p_phase[2] = {0, 0}, o_units[2] = {0, 0};
+        bool have_s = ws.begin(p, plan), have_p = wp.begin(p, plan);
+        if (have_s) us = up = unit_of(p, ws.u);
+        auto issue_s = [&]() -> bool {
+          const uint32_t g = xs & 1;
+          if (ts == 0) {
+            if (js == 0) rq_piece = rq;
+            rq = rq_piece;  // tile 0's buffer
+          }
+          if (js == 0 && !mbar_wait(bar + 8 * (B_QFULL + rq.i), rq.phase, abort_flag, err))
+            return false;
+          if (!mbar_wait(bar + 8 * (B_KFULL + rk.i), rk.phase, abort_flag, err)) return false;
+          tc_fence_after();
+          const uint64_t da = sdesc(sb + O_Q + rq.i * TILE, 16, 1024);
+          const uint64_t db = sdesc(sb + O_K + rk.i * TILE, 16, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 8; kk++) {
+            const uint32_t off = ((uint32_t)(kk >> 2) * CHUNK + (uint32_t)(kk & 3) * 32) >> 4;
+            umma(tmem + g * BN, da + off, db + off, IDESC_S, kk > 0);
+          }
+          umma_commit(bar + 8 * (B_SFULL + g));
+          if (js + 1 == ws.nb) umma_commit(bar + 8 * (B_QEMPTY + rq.i));
+          rq.next();
+          xs++;
+          if (++ts == us.tiles) {
+            umma_commit(bar + 8 * (B_KEMPTY + rk.i));
+            rk.next();
+            ts = 0;
+            if (++js == ws.nb) {
+              js = 0;
+              have_s = ws.next(p);
+              if (have_s) us = unit_of(p, ws.u);
+            }
+          }
+          return true;
+        };
+        bool ok = true;
+        for (int i = 0; i < 2 && ok && have_s; i++) ok = issue_s();
+        while (ok && have_p) {
+          const uint32_t g = xp & 1;
+          // the group's first and last turns of the piece
+          const bool first = up.tiles == 2 ? jp == 0 : jp < 2;
+          const bool last = up.tiles == 2 ? jp + 1 == wp.nb : jp + 2 >= wp.nb;
+          if ((first && !mbar_wait(bar + 8 * (B_OEMPTY + g), (o_units[g] & 1) ^ 1, abort_flag, err)) ||
+              !mbar_wait(bar + 8 * (B_PFULL + g), p_phase[g], abort_flag, err) ||
+              !mbar_wait(bar + 8 * (B_VFULL + rv.i), rv.phase, abort_flag, err))
+            break;
+          tc_fence_after();
+          // P: key pairs in the first 64 score columns; V MN-major (head_dim
+          // contiguous), its 64-column chunks 16 KiB apart, 16 keys 2 KiB
+          const uint64_t dv = sdesc(sb + O_V + rv.i * TILE, CHUNK, 1024);
+#pragma unroll
+          for (int kk = 0; kk < 8; kk++)
+            umma_ts(tmem + TMEM_O + g * HD, tmem + g * BN + (uint32_t)kk * 8u,
+                    dv + (((uint32_t)kk * 16 * 128) >> 4), IDESC_O, (!first || kk > 0) ? 1u : 0u);
+          if (last) {
+            umma_commit(bar + 8 * (B_OFULL + g));
+            o_units[g]++;
+          }
+          p_phase[g] ^= 1u;
+          xp++;
+          if (++tp == up.tiles) {
+            umma_commit(bar + 8 * (B_VEMPTY + rv.i));
+            rv.next();
+            tp = 0;
+            if (++jp == wp.nb) {
+              jp = 0;
+              have_p = wp.next(p);
+              if (have_p) up = unit_of(p, wp.u);
+            }
+          }
+          if (have_s) ok = issue_s();
+        }
+        // every MMA this thread issued has completed before the tensor
+        // memory is released
+        umma_commit(bar + 8 * B_DRAIN);
+        const uint64_t t0 = globaltimer();
+        while (!mbar_try_wait(bar + 8 * B_DRAIN, 0) && globaltimer() - t0 < WAIT_LIMIT_NS) {
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;" ::: "memory");
+    // ======================= softmax groups =======================
+    const uint32_t g = (uint32_t)(warp - 4) >> 2;
+    const uint32_t quad = (uint32_t)warp & 3u;
+    const uint32_t r = quad * 32u + (uint32_t)lane;  // row of the tile = tensor memory lane
+    const uint32_t lanes = quad * 32u << 16;
+    const uint32_t tmem_s = tmem + g * BN + lanes, tmem_o = tmem + TMEM_O + lanes;
+    float2* ml = reinterpret_cast<float2*>(smem + O_ML);
+    const uint32_t q_node = r / p.group, q_head = r % p.group;
+    uint32_t s_phase = 0, x0 = 0;      // x0: turns before this piece
+    uint32_t o_units[2] = {0, 0};      // pieces that group 0 / 1 had turns in
+    uint32_t ml_units[2] = {0, 0};     // of those, pieces of one tile
+    Ring<NV> rv;
+    bool ok = true;
+    Pieces w;
+    for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
+      const Unit un = unit_of(p, w.u);
+      const bool two = un.tiles == 2;
+      const uint32_t mine = (g - x0) & 1;  // two tiles: my tile; one: my first block
+      const uint32_t tile = un.tile0 + (two ? mine : 0);
+      const uint32_t tile_nodes = min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes);
+      const uint32_t node = tile * p.tile_nodes + q_node;
+      const bool row_used = q_node < tile_nodes;
+      const bool warp_used = quad * 32u < tile_nodes * p.group;
+      // which rows of the tree this row sees: none if its node is absent
+      const bool has_tail = (w.blk + w.nb) * BN > w.s.ctx;
+      uint64_t sees = 0;
+      if (has_tail && row_used && node < w.s.nodes)
+        sees = nwd::tree_mask(p.parents + (size_t)w.b * p.n_nodes, (int)node, err);
+      float m = -INFINITY, l = 0.f;
+      uint64_t bad = 0;
+      for (uint32_t j = 0; j < w.nb; j++) {
+        const bool my_turn = two || (j & 1) == mine;
+        const uint32_t key0 = (w.blk + j) * BN;
+        const bool tail = key0 + BN > w.s.ctx;
+        if (!my_turn) {
+          rv.next();
+          continue;
+        }
+        if (!warp_wait(bar + 8 * (B_SFULL + g), s_phase, abort_flag, err)) {
+          ok = false;
+          break;
+        }
+        s_phase ^= 1u;
+        tc_fence_after();
+        if (warp_used) {
+          float s[128];
+#pragma unroll
+          for (int c = 0; c < 4; c++) tmem_ld32(tmem_s + c * 32, s + c * 32);
+          tmem_ld_wait();
+          if (tail) {
+            // bit c of word i: this row attends cache row key0 + 32 i + c
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int64_t at = (int64_t)key0 + 32 * i - (int64_t)w.s.ctx;  // in the tree
+              uint32_t ok32;
+              if (at <= -32) ok32 = 0xffffffffu;
+              else if (at < 0) ok32 = (uint32_t)(sees << -at) | ((1u << -at) - 1u);
+              else ok32 = at < 64 ? (uint32_t)(sees >> at) : 0u;
+#pragma unroll
+              for (int c = 0; c < 32; c++)
+                if (!((ok32 >> c) & 1u)) s[32 * i + c] = -INFINITY;
+            }
+          }
+          float mv[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) mv[i] = s[i];
+#pragma unroll
+          for (int c = 8; c < 128; c++) mv[c & 7] = fmaxf(mv[c & 7], s[c]);
+#pragma unroll
+          for (int i = 0; i < 4; i++) mv[i] = fmaxf(mv[i], mv[i + 4]);
+          const float mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * p.scale_log2;
+          const bool up = mx > m + RESCALE_LOG2;
+          if (__any_sync(0xffffffffu, up)) {
+            const float alpha = up ? ex2f(m - mx) : 1.f;  // 0 while m is -inf
+            if (two ? j > 0 : j > 1) {
+              // S of this turn is done, so P V of the group's last turn,
+              // issued before it, is too
+#pragma unroll
+              for (int c = 0; c < 4; c++) {
+                float ov[32];
+                tmem_ld32(tmem_o + g * HD + c * 32, ov);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; i++) ov[i] *= alpha;
+                tmem_st32(tmem_o + g * HD + c * 32, ov);
+              }
+            }
+            l *= alpha;
+            if (up) m = mx;
+          }
+          const float nb = m == -INFINITY ? 0.f : P_BIAS - m;
+          float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            float pk[32];
+#pragma unroll
+            for (int c = 0; c < 32; c++) {
+              const float p0 = ex2f(fmaf(s[64 * h + 2 * c], p.scale_log2, nb));
+              const float p1 = ex2f(fmaf(s[64 * h + 2 * c + 1], p.scale_log2, nb));
+              rs[c & 3] += p0 + p1;
+              const __half2 hh = __floats2half2_rn(p0, p1);
+              pk[c] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&hh));
+            }
+            tmem_st32(tmem_s + 32 * h, pk);
+          }
+          l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+          tmem_st_wait();
+        }
+        if (tail) {  // V rows with NaN or infinities, found by the V producer
+          if (!warp_wait(bar + 8 * (B_VFULL + rv.i), rv.phase, abort_flag, err)) {
+            ok = false;
+            break;
+          }
+          bad |= vbad[rv.i];
+        }
+        rv.next();
+        tc_fence_before();
+        mbar_arrive(bar + 8 * (B_PFULL + g));
+      }
+      if (!ok) break;
+
+      // ---- the piece's end: O of the tile (two), or of both groups' halves
+      const bool direct = w.blk == 0 && w.nb == w.nblk;
+      const uint32_t slot_at = ((blockIdx.x * 2 + (w.blk > 0 ? 0 : 1)) * p.unit_tiles +
+                                (two ? mine : 0)) * BM;
+      float2* slot_ml = reinterpret_cast<float2*>(p.ws + WS_ML) + slot_at;
+      float* slot_o =
+          reinterpret_cast<float*>(p.ws + ws_o(gridDim.x, p.unit_tiles)) + (size_t)slot_at * HD;
+      const bool absent = node >= w.s.nodes;
+      __half* orow = p.o + (((size_t)w.b * p.n_nodes + node) * p.n_heads + un.hkv * p.group +
+                            q_head) * HD;
+      const __half* vrow = p.v + (((size_t)w.s.row0 + w.s.ctx) * p.n_kv + un.hkv) * HD;
+      // adds what the V producer took out of the rows that this one sees
+      auto restore = [&](float* ov, uint32_t col, uint64_t rows) {
+        for (uint64_t x = rows & sees; x; x &= x - 1) {
+          const __half* src = vrow + (size_t)(__ffsll((long long)x) - 1) * p.n_kv * HD + col;
+#pragma unroll
+          for (int i = 0; i < 32; i++) {
+            const float e = __half2float(src[i]);
+            if (!isfinite(e)) ov[i] += e;
+          }
+        }
+      };
+      auto put = [&](float* ov, uint32_t col, float inv) {
+        if (direct) {
+          uint4* dst = reinterpret_cast<uint4*>(orow + col);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const __half2 x = __floats2half2_rn(ov[8 * i + 2 * k] * inv,
+                                                  ov[8 * i + 2 * k + 1] * inv);
+              h[k] = absent ? 0u : *reinterpret_cast<const uint32_t*>(&x);
+            }
+            dst[i] = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) store_part(slot_o, r, col + i, ov + i);
+        }
+      };
+      if (two) {
+        if (!warp_wait(bar + 8 * (B_OFULL + g), o_units[g] & 1, abort_flag, err)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (warp_used) {
+          const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            float ov[32];
+            tmem_ld32(tmem_o + g * HD + c * 32, ov);
+            tmem_ld_wait();
+            if (row_used) {
+              if (bad) restore(ov, c * 32, bad);
+              put(ov, c * 32, inv);
+            }
+          }
+          if (!direct && row_used) slot_ml[r] = make_float2(m, l);
+        }
+        tc_fence_before();
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 2;" ::"r"(bar + 8 * (B_OEMPTY + g))
+                     : "memory");
+        o_units[0]++;
+        o_units[1]++;
+      } else {
+        // group of block 0: x0 & 1; the other has turns from two blocks on
+        const bool had[2] = {w.nb > 1 || (x0 & 1) == 0, w.nb > 1 || (x0 & 1) == 1};
+        if (had[g]) {
+          ml[g * BM + r] = make_float2(m, l);
+          if (r == 0) gbad[g] = bad;
+          mbar_arrive(bar + 8 * (B_ML + g));
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 2; i++)
+          if (ok && had[i])
+            ok = warp_wait(bar + 8 * (B_ML + i), ml_units[i] & 1, abort_flag, err) &&
+                 warp_wait(bar + 8 * (B_OFULL + i), o_units[i] & 1, abort_flag, err);
+        if (!ok) break;
+        tc_fence_after();
+        if (warp_used) {
+          const float2 a0 = had[0] ? ml[r] : make_float2(-INFINITY, 0.f);
+          const float2 a1 = had[1] ? ml[BM + r] : make_float2(-INFINITY, 0.f);
+          const uint64_t both = (had[0] ? gbad[0] : 0) | (had[1] ? gbad[1] : 0);
+          const float M = fmaxf(a0.x, a1.x);
+          // a group without weights counts for nothing (l may be NaN)
+          const float w0 = a0.y != 0.f ? ex2f(a0.x - M) : 0.f;
+          const float w1 = a1.y != 0.f ? ex2f(a1.x - M) : 0.f;
+          const float L = (a0.y != 0.f ? a0.y * w0 : 0.f) + (a1.y != 0.f ? a1.y * w1 : 0.f);
+          const float inv = L != 0.f ? 1.f / L : 0.f;
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            const uint32_t col = g * 64 + c * 32;  // each group half of the columns
+            float ov[32], o1[32];
+            tmem_ld32(tmem_o + col, ov);
+            tmem_ld32(tmem_o + HD + col, o1);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+              ov[i] = (a0.y != 0.f ? ov[i] * w0 : 0.f) + (a1.y != 0.f ? o1[i] * w1 : 0.f);
+            if (row_used) {
+              if (both) restore(ov, col, both);
+              put(ov, col, inv);
+            }
+          }
+          if (!direct && row_used && g == 0) slot_ml[r] = make_float2(M, L);
+        }
+        tc_fence_before();
+#pragma unroll
+        for (uint32_t i = 0; i < 2; i++)
+          if (had[i]) {
+            mbar_arrive(bar + 8 * (B_OEMPTY + i));
+            o_units[i]++;
+            ml_units[i]++;
+          }
+      }
+      x0 += w.nb * un.tiles;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(TMEM_COLS)
+                 : "memory");
+}
+
+// Joins the partials of the unit that ends in CTA blockIdx.x's range, in CTA
+// order (deterministic): M = max m, O = sum O_c 2^(m_c - M) / sum l_c 2^(m_c - M).
+// A block has 8 rows: thread (row, column quad).
+constexpr uint32_t MERGE_ROWS = 8;
+__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TParams p) {
+  nwd::pdl_trigger();
+  nwd::pdl_wait();
+  const uint32_t c = blockIdx.x, last = c;
+  const MergeDesc d = reinterpret_cast<const MergeDesc*>(p.ws + WS_DESC)[c];
+  if (!d.valid) return;
+  const Unit un = unit_of(p, d.u);
+  const uint32_t t = blockIdx.y / (BM / MERGE_ROWS);
+  const uint32_t row = blockIdx.y % (BM / MERGE_ROWS) * MERGE_ROWS + (threadIdx.x & 7);
+  const uint32_t quad = threadIdx.x >> 3;
+  if (t >= un.tiles) return;
+  const uint32_t tile = un.tile0 + t, node = tile * p.tile_nodes + row / p.group;
+  if (row >= min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes) * p.group) return;
+  const float2* ml = reinterpret_cast<const float2*>(p.ws + WS_ML);
+  const float4* po = reinterpret_cast<const float4*>(p.ws + ws_o(gridDim.x, p.unit_tiles));
+  // the unit's first piece is the one its CTA ended with, the others begin theirs
+  auto slot = [&](uint32_t i) {
+    return ((i * 2 + (i == d.first ? 1 : 0)) * p.unit_tiles + t) * BM;
+  };
+  float M = -INFINITY;
+  for (uint32_t i = d.first; i <= last; i++) M = fmaxf(M, ml[slot(i) + row].x);
+  float L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (uint32_t i = d.first; i <= last; i++) {
+    const float2 a = ml[slot(i) + row];
+    const float4 x = po[(size_t)slot(i) * (HD / 4) + quad * BM + row];
+    if (a.y != 0.f) {
+      const float w = ex2f(a.x - M);
+      L += a.y * w;
+      o.x += x.x * w;
+      o.y += x.y * w;
+      o.z += x.z * w;
+      o.w += x.w * w;
+    }
+  }
+  const TreeSeq s = load_seq(p, d.b, nullptr);
+  const float inv = L != 0.f && node < s.nodes ? 1.f / L : 0.f;
+  const bool none = node >= s.nodes;
+  __half2 h[2] = {__floats2half2_rn(none ? 0.f : o.x * inv, none ? 0.f : o.y * inv),
+                  __floats2half2_rn(none ? 0.f : o.z * inv, none ? 0.f : o.w * inv)};
+  *reinterpret_cast<uint2*>(p.o + (((size_t)d.b * p.n_nodes + node) * p.n_heads +
+                                   un.hkv * p.group + row % p.group) * HD + quad * 4) =
+      *reinterpret_cast<const uint2*>(h);
 }
 
 // The nodes' K / V rows [batch, n_nodes, n_kv, hd] into pool rows
@@ -87,6 +897,8 @@ __global__ void tree_append_kernel(const uint4* __restrict__ k_new, const uint4*
                                    const int64_t* row_offset, const int32_t* pos,
                                    const int32_t* tree_len, uint64_t pool_rows, uint32_t n_nodes,
                                    uint32_t row_vec, uint32_t* err) {
+  nwd::pdl_trigger();
+  nwd::pdl_wait();
   const uint32_t b = blockIdx.y;
   const TreeSeq s = nwd::tree_seq(row_offset, pos, tree_len, pool_rows, b, n_nodes, err);
   const uint64_t dst = ((uint64_t)s.row0 + s.ctx) * row_vec, src = (uint64_t)b * n_nodes * row_vec;
@@ -111,6 +923,7 @@ int check_tree(const char* who, const void* q, const void* k_pool, const void* v
                 head_dim, n_heads / n_kv);
   if (n_nodes > TREE_MAX_NODES)
     return fail(NWD_ERR_UNSUPPORTED, "%s: %u nodes (at most %u)", who, n_nodes, TREE_MAX_NODES);
+  if (n_heads > 16384) return fail(NWD_ERR_UNSUPPORTED, "%s: %u heads (at most 16384)", who, n_heads);
   if (batch > 4096) return fail(NWD_ERR_UNSUPPORTED, "%s: batch %u (at most 4096)", who, batch);
   if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(o))
     return fail(NWD_ERR_INVALID, "%s: tensors must be 16-byte aligned", who);
@@ -120,6 +933,96 @@ int check_tree(const char* who, const void* q, const void* k_pool, const void* v
     return fail(NWD_ERR_INVALID, "%s: pool rows %llu outside [1, 2^31]", who,
                 (unsigned long long)pool_rows);
   return NWD_OK;
+}
+
+// How a shape's query rows are tiled: whole nodes per tile, tiles per unit.
+struct Tiling {
+  uint32_t tile_nodes, n_tiles, unit_tiles;
+};
+Tiling tiling(uint32_t n_nodes, uint32_t group) {
+  Tiling t;
+  t.n_tiles = (n_nodes * group + BM - 1) / BM;
+  while ((n_nodes + t.n_tiles - 1) / t.n_tiles * group > BM) t.n_tiles++;
+  t.tile_nodes = (n_nodes + t.n_tiles - 1) / t.n_tiles;
+  t.n_tiles = (n_nodes + t.tile_nodes - 1) / t.tile_nodes;
+  t.unit_tiles = t.n_tiles > 1 ? 2 : 1;
+  return t;
+}
+
+// Checks the workspace, then launches the append (when there are new rows),
+// the attention and the join of its partials.
+int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const uint16_t* v_pool,
+             uint64_t pool_rows, const int64_t* row_offset, const int32_t* seq_len,
+             const int32_t* parents, const int32_t* tree_len, uint16_t* o, uint32_t batch,
+             uint32_t n_nodes, uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, float scale,
+             void* workspace, size_t ws_bytes, uint32_t* err, void* stream,
+             const uint16_t* k_new = nullptr, const uint16_t* v_new = nullptr) {
+  using namespace nwd;
+  const uint32_t group = n_heads / n_kv;
+  const Tiling t = tiling(n_nodes, group);
+  if (!workspace || ((uintptr_t)workspace & 255u))
+    return fail(NWD_ERR_WORKSPACE, "%s: the workspace is NULL or not 256-byte aligned", who);
+  if (ws_bytes < ws_total(1, t.unit_tiles))
+    return fail(NWD_ERR_WORKSPACE, "%s: a workspace of %zu bytes is too small", who, ws_bytes);
+  DeviceInfo di;
+  int st = current_device_info(&di);
+  if (st) return st;
+  if (di.sm_count > (int)MAX_CTAS)
+    return fail(NWD_ERR_UNSUPPORTED, "%s: %d SMs (at most %u)", who, di.sm_count, MAX_CTAS);
+  const size_t need = ws_total((uint32_t)di.sm_count, t.unit_tiles);
+  if (ws_bytes < need)
+    return fail(NWD_ERR_WORKSPACE, "%s: needs a workspace of >= %zu bytes, got %zu", who, need,
+                ws_bytes);
+  static bool smem_set[64] = {};
+  if (!smem_set[di.device]) {
+    cudaError_t e = cudaFuncSetAttribute(tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)SMEM_BYTES);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(tree_kernel)");
+    smem_set[di.device] = true;
+  }
+  CUtensorMap tq, tk, tv;
+  if ((st = tree_q_tensor_map(&tq, q, (uint64_t)batch * n_nodes, n_kv, group, t.tile_nodes)) ||
+      (st = kv_tensor_map(&tk, k_pool, pool_rows, n_kv, head_dim, BN, 1)) ||
+      (st = kv_tensor_map(&tv, v_pool, pool_rows, n_kv, head_dim, BN, 1)))
+    return st;
+  TParams p{};
+  p.v = reinterpret_cast<const __half*>(v_pool);
+  p.o = reinterpret_cast<__half*>(o);
+  p.row_offset = row_offset;
+  p.seq_len = seq_len;
+  p.parents = parents;
+  p.tree_len = tree_len;
+  p.ws = reinterpret_cast<uint8_t*>(workspace);
+  p.err = err ? err : reinterpret_cast<uint32_t*>(workspace);
+  p.pool_rows = pool_rows;
+  p.batch = batch;
+  p.n_nodes = n_nodes;
+  p.n_heads = n_heads;
+  p.n_kv = n_kv;
+  p.group = group;
+  p.tile_nodes = t.tile_nodes;
+  p.n_tiles = t.n_tiles;
+  p.unit_tiles = t.unit_tiles;
+  p.n_units = n_kv * ((t.n_tiles + t.unit_tiles - 1) / t.unit_tiles);
+  p.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f;
+  cudaStream_t s = (cudaStream_t)stream;
+  cudaError_t e = cudaSuccess;
+  if (k_new) {
+    const uint32_t row_vec = n_kv * head_dim / 8;
+    e = launch_pdl(tree_append_kernel, dim3((n_nodes * row_vec + 255) / 256, batch), dim3(256), 0, s,
+                   reinterpret_cast<const uint4*>(k_new), reinterpret_cast<const uint4*>(v_new),
+                   reinterpret_cast<uint4*>(const_cast<uint16_t*>(k_pool)),
+                   reinterpret_cast<uint4*>(const_cast<uint16_t*>(v_pool)), row_offset, seq_len,
+                   tree_len, pool_rows, n_nodes, row_vec, p.err);
+    if (e != cudaSuccess) return cuda_fail(e, who);
+  }
+  const uint32_t ctas = (uint32_t)di.sm_count;
+  e = launch_pdl(tree_kernel, dim3(ctas), dim3(THREADS), SMEM_BYTES, s, tq, tk, tv, p);
+  if (e == cudaSuccess)
+    e = launch_pdl(tree_merge_kernel, dim3(ctas, t.unit_tiles * (BM / MERGE_ROWS)), dim3(256), 0, s,
+                   p);
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return ok();
 }
 
 }  // namespace
@@ -136,7 +1039,11 @@ int nwd_attn_tree_workspace_size(uint32_t batch, uint32_t n_nodes, uint32_t n_he
   int st = check_tree(who, p, p, p, p, p, p, p, 1, batch, n_nodes, n_heads, n_kv_heads, head_dim,
                       0.f);
   if (st) return st;
-  *bytes = 256;
+  DeviceInfo di;
+  st = current_device_info(&di);
+  if (st) return st;
+  const Tiling t = tiling(n_nodes ? n_nodes : 1, n_heads / n_kv_heads);
+  *bytes = ws_total((uint32_t)di.sm_count, t.unit_tiles);
   return ok();
 }
 
@@ -149,30 +1056,10 @@ int nwd_attn_tree(const uint16_t* q, const uint16_t* k_pool, const uint16_t* v_p
   int st = check_tree(who, q, k_pool, v_pool, row_offset, seq_len, parents, o, pool_rows, batch,
                       n_nodes, n_heads, n_kv_heads, head_dim, scale);
   if (st) return st;
-  if (!workspace || ws_bytes < 256 || ((uintptr_t)workspace & 255u))
-    return fail(NWD_ERR_WORKSPACE, "%s: needs a 256-byte aligned workspace of >= 256 bytes", who);
   if (batch == 0 || n_nodes == 0) return ok();
-  TreeParams p{};
-  p.q = reinterpret_cast<const __half*>(q);
-  p.k = reinterpret_cast<const __half*>(k_pool);
-  p.v = reinterpret_cast<const __half*>(v_pool);
-  p.o = reinterpret_cast<__half*>(o);
-  p.row_offset = row_offset;
-  p.seq_len = seq_len;
-  p.parents = parents;
-  p.tree_len = tree_len;
-  p.err = err;
-  p.pool_rows = pool_rows;
-  p.batch = batch;
-  p.n_nodes = n_nodes;
-  p.n_heads = n_heads;
-  p.n_kv = n_kv_heads;
-  p.group = n_heads / n_kv_heads;
-  p.scale = scale != 0.f ? scale : 1.0f / sqrtf((float)head_dim);
-  tree_attn_kernel<<<dim3(n_kv_heads * n_nodes, batch), 32 * p.group, 0, (cudaStream_t)stream>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, who);
-  return ok();
+  return run_tree(who, q, k_pool, v_pool, pool_rows, row_offset, seq_len, parents, tree_len, o,
+                  batch, n_nodes, n_heads, n_kv_heads, head_dim, scale, workspace, ws_bytes, err,
+                  stream);
 }
 
 int nwd_kv_append_attn_tree(const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
@@ -188,20 +1075,10 @@ int nwd_kv_append_attn_tree(const uint16_t* q, const uint16_t* k_new, const uint
   if (!k_new || !v_new) return fail(NWD_ERR_INVALID, "%s: null pointer", who);
   if (!aligned16(k_new) || !aligned16(v_new))
     return fail(NWD_ERR_INVALID, "%s: tensors must be 16-byte aligned", who);
-  if (!workspace || ws_bytes < 256 || ((uintptr_t)workspace & 255u))
-    return fail(NWD_ERR_WORKSPACE, "%s: needs a 256-byte aligned workspace of >= 256 bytes", who);
   if (batch == 0 || n_nodes == 0) return ok();
-  const uint32_t row_vec = n_kv_heads * head_dim / 8;
-  const uint32_t bx = (n_nodes * row_vec + 255) / 256;
-  tree_append_kernel<<<dim3(bx, batch), 256, 0, (cudaStream_t)stream>>>(
-      reinterpret_cast<const uint4*>(k_new), reinterpret_cast<const uint4*>(v_new),
-      reinterpret_cast<uint4*>(k_pool), reinterpret_cast<uint4*>(v_pool), row_offset, pos,
-      tree_len, pool_rows, n_nodes, row_vec, err);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, who);
-  return nwd_attn_tree(q, k_pool, v_pool, pool_rows, row_offset, pos, parents, tree_len, o, batch,
-                       n_nodes, n_heads, n_kv_heads, head_dim, scale, workspace, ws_bytes, err,
-                       stream);
+  return run_tree(who, q, k_pool, v_pool, pool_rows, row_offset, pos, parents, tree_len, o, batch,
+                  n_nodes, n_heads, n_kv_heads, head_dim, scale, workspace, ws_bytes, err, stream,
+                  k_new, v_new);
 }
 
 }  // extern "C"
