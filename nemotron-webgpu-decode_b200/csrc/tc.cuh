@@ -10,7 +10,7 @@ namespace tc {
 // Shared-memory matrix descriptor: start address, leading / stride byte
 // offsets (all >> 4), descriptor version 1 (bits 46-47), 128-byte swizzle
 // (layout type 2 in bits 61-63).
-static __device__ __forceinline__ uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+static __host__ __device__ constexpr uint64_t sdesc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
   return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
          ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
 }

@@ -16,21 +16,23 @@
 // (m, l, O) per CTA in the workspace, which merge_kernel joins in order.
 //
 // A CTA's 12 warps:
-//   warps 0, 2, 3  TMA producers: K blocks into 3 stages, each unit's Q tiles
-//                  into 2, V blocks into 2 (each 128 x 128 fp16 as two
-//                  64-column chunks, 128-byte swizzle: the K-major operand
-//                  layout).  Separate warps, so none waits behind another's
-//                  buffers.  Warp 2 also owns the tensor memory.
-//   warp 1         MMA issuer (one thread): a turn is S = Q K^T of one (block,
-//                  tile) and O += P V after its softmax.  Turns alternate
-//                  between the two softmax groups, S two turns ahead of P V,
-//                  so one group's softmax runs beside the other's MMAs.
+//   warps 0, 3  TMA producers: K blocks into 3 stages; V blocks into 2 and each
+//               unit's Q tiles into 2 (each 128 x 128 fp16 as two 64-column
+//               chunks, 128-byte swizzle: the K-major operand layout).  Warp 0
+//               also owns the tensor memory.
+//   warps 1, 2  MMA issuers, one thread each, one per softmax group.  A turn
+//               is S = Q K^T of one (block, tile) and O += P V after its
+//               softmax; an issuer goes P V, S of its group's next turn, and
+//               so on, so one group's MMAs run beside the other's softmax.
+//               (One issuer for both spent as long between the MMAs, in waits
+//               and bookkeeping of a single thread, as in them: 2600 cycles a
+//               turn.)
 //   warps 4-7, 8-11  the softmax groups, a thread per query row, each with its
-//                  own score and output accumulators (S0 S1 O0 O1: all 512
-//                  columns).  A unit of two tiles gives each group a tile and
-//                  both use every K/V block; a unit of one tile gives the
-//                  groups alternate blocks and joins their (m, l, O) at its
-//                  end, which keeps both busy when there are few query rows.
+//               own score and output accumulators (S0 S1 O0 O1: all 512
+//               columns).  A unit of two tiles gives each group a tile and
+//               both use every K/V block; a unit of one tile gives the
+//               groups alternate blocks and joins their (m, l, O) at its
+//               end, which keeps both busy when there are few query rows.
 //
 // Softmax in the log2 domain with a lazily moved maximum (O is rescaled in
 // tensor memory only when a row's maximum grows by more than 2^8).  P is
@@ -200,11 +202,67 @@ __device__ __forceinline__ Unit unit_of(const TParams& p, uint32_t u) {
 template <uint32_t N>
 struct Ring {
   uint32_t i = 0, phase = 0;
-  __device__ __forceinline__ void next() {
-    if (++i == N) {
-      i = 0;
+  // n <= N
+  __device__ __forceinline__ void step(uint32_t n) {
+    i += n;
+    if (i >= N) {
+      i -= N;
       phase ^= 1u;
     }
+  }
+  __device__ __forceinline__ void next() { step(1); }
+  __device__ __forceinline__ void add(uint32_t n) {
+    i += n;
+    phase ^= (i / N) & 1u;
+    i %= N;
+  }
+};
+
+// The turns of one softmax group, with the ring position of their blocks (K or
+// V, N stages) and of their Q tile.  x0: turns before the piece.
+template <uint32_t N>
+struct Own {
+  Pieces w;
+  bool two, first;
+  uint32_t x0, j;
+  Ring<N> r, r0;    // of block j, of the piece's first block
+  Ring<NQ> q, q0;
+  // the piece's first turn of group g, or the next piece's that has one
+  __device__ __forceinline__ bool settle(const TParams& p, uint32_t g) {
+    for (;;) {
+      two = unit_of(p, w.u).tiles == 2;
+      const uint32_t mine = (g - x0) & 1;  // two tiles: the tile; one: the first block
+      j = two ? 0 : mine;
+      if (j < w.nb) {
+        first = true;
+        r = r0;
+        r.step(j);
+        q = q0;
+        if (two) q.step(mine);
+        return true;
+      }
+      if (!leave(p)) return false;
+    }
+  }
+  __device__ __forceinline__ bool leave(const TParams& p) {
+    r0.add(w.nb);
+    q0.step(two ? 2 : 1);
+    x0 += two ? 2 * w.nb : w.nb;
+    return w.next(p);
+  }
+  __device__ __forceinline__ bool begin(const TParams& p, const Plan& plan, uint32_t g) {
+    x0 = 0;
+    return w.begin(p, plan) && settle(p, g);
+  }
+  __device__ __forceinline__ bool last() const { return j + (two ? 1 : 2) >= w.nb; }
+  __device__ __forceinline__ bool next(const TParams& p, uint32_t g) {
+    const uint32_t n = two ? 1 : 2;
+    if ((j += n) < w.nb) {
+      first = false;
+      r.step(n);
+      return true;
+    }
+    return leave(p) && settle(p, g);
   }
 };
 
@@ -303,11 +361,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (i >= B_PFULL && i < B_PFULL + 2) count = BM;
       if (i >= B_OEMPTY && i < B_OEMPTY + 2) count = 2 * BM;
       if (i >= B_ML && i < B_ML + 2) count = BM;
+      // a stage is released by both issuers, or twice by its only user
+      if ((i >= B_QEMPTY && i < B_QEMPTY + (int)NQ) || (i >= B_KEMPTY && i < B_KEMPTY + (int)NK) ||
+          (i >= B_VEMPTY && i < B_VEMPTY + (int)NV) || i == B_DRAIN)
+        count = 2;
       mbar_init(bar + 8 * i, count);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 2) {
+  if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_slot)),
                  "r"(TMEM_COLS)
@@ -367,51 +429,41 @@ __global__ void __launch_bounds__(THREADS, 1)
                    globaltimer() - t0 < WAIT_LIMIT_NS) {
             }
       }
-    } else if (warp == 2) {
-      // ======================= Q =======================
-      const uint64_t policy = evict_first_policy();
-      const uint32_t bytes = 2 * p.tile_nodes * p.group * 128;
-      uint32_t issued[NQ] = {};
-      Ring<NQ> r;
-      Pieces w;
+    } else if (warp == 3) {
+      // ======================= V and Q =======================
+      // The next piece's Q goes out with the last V block of a piece (before
+      // this warp waits for that block, if it is a tail): its buffers fill as
+      // soon as the S that read them are done.
+      const uint64_t policy = p.n_units == p.n_kv ? evict_first_policy() : evict_last_policy();
+      const uint64_t q_policy = evict_first_policy();
+      const uint32_t q_bytes = 2 * p.tile_nodes * p.group * 128;
+      uint32_t issued[NV] = {}, q_issued[NQ] = {}, tails = 0;
+      Ring<NV> r;
+      Ring<NQ> rq;
+      Pieces w, wq;
       bool ok = true;
-      for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
-        const Unit un = unit_of(p, w.u);
+      bool more_q = wq.begin(p, plan);
+      auto load_q = [&]() -> bool {
+        const Unit un = unit_of(p, wq.u);
         for (uint32_t t = 0; t < un.tiles; t++) {
-          if (!warp_wait(bar + 8 * (B_QEMPTY + r.i), r.phase ^ 1u, abort_flag, err)) {
-            ok = false;
-            break;
-          }
+          if (!warp_wait(bar + 8 * (B_QEMPTY + rq.i), rq.phase ^ 1u, abort_flag, err)) return false;
           if (lane == 0) {
-            const uint32_t fb = bar + 8 * (B_QFULL + r.i), dst = sb + O_Q + r.i * TILE;
-            const int node = (int)(w.b * p.n_nodes + (un.tile0 + t) * p.tile_nodes);
-            mbar_arrive_tx(fb, bytes);
-            tma_load_5d(dst, &tmq, fb, 0, 0, 0, (int)un.hkv, node, policy);
-            tma_load_5d(dst + CHUNK, &tmq, fb, 0, 1, 0, (int)un.hkv, node, policy);
+            const uint32_t fb = bar + 8 * (B_QFULL + rq.i), dst = sb + O_Q + rq.i * TILE;
+            const int node = (int)(wq.b * p.n_nodes + (un.tile0 + t) * p.tile_nodes);
+            mbar_arrive_tx(fb, q_bytes);
+            tma_load_5d(dst, &tmq, fb, 0, 0, 0, (int)un.hkv, node, q_policy);
+            tma_load_5d(dst + CHUNK, &tmq, fb, 0, 1, 0, (int)un.hkv, node, q_policy);
           }
           __syncwarp();
 #pragma unroll
-          for (uint32_t i = 0; i < NQ; i++) issued[i] += r.i == i;
-          r.next();
+          for (uint32_t i = 0; i < NQ; i++) q_issued[i] += rq.i == i;
+          rq.next();
         }
-      }
-      if (!ok) {
-        const uint64_t t0 = globaltimer();
-#pragma unroll
-        for (uint32_t i = 0; i < NQ; i++)
-          if (issued[i])
-            while (!mbar_try_wait(bar + 8 * (B_QFULL + i), (issued[i] - 1) & 1) &&
-                   globaltimer() - t0 < WAIT_LIMIT_NS) {
-            }
-      }
-    } else if (warp == 3) {
-      // ======================= V =======================
-      const uint64_t policy = p.n_units == p.n_kv ? evict_first_policy() : evict_last_policy();
-      uint32_t issued[NV] = {}, tails = 0;
-      Ring<NV> r;
-      Pieces w;
-      bool ok = true;
-      for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
+        more_q = wq.next(p);
+        return true;
+      };
+      if (more_q) ok = load_q();
+      for (bool more = ok && w.begin(p, plan); more && ok; more = w.next(p)) {
         const int hkv = (int)unit_of(p, w.u).hkv;
         for (uint32_t j = 0; j < w.nb; j++) {
           if (!warp_wait(bar + 8 * (B_VEMPTY + r.i), r.phase ^ 1u, abort_flag, err)) {
@@ -431,8 +483,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             tma_load_4d(dst + CHUNK, &tmv, fb, 0, 1, hkv, row, policy);
           }
           __syncwarp();
+#pragma unroll
+          for (uint32_t i = 0; i < NV; i++) issued[i] += !tail && r.i == i;
+          tails += tail;
+          if (j + 1 == w.nb && more_q && !load_q()) {
+            ok = false;
+            break;
+          }
           if (tail) {
-            tails++;
             if (!warp_wait(fb, (tails - 1) & 1, abort_flag, err)) {
               ok = false;
               break;
@@ -475,9 +533,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(bar + 8 * (B_VFULL + r.i));
-          }
 #pragma unroll
-          for (uint32_t i = 0; i < NV; i++) issued[i] += r.i == i;
+            for (uint32_t i = 0; i < NV; i++) issued[i] += r.i == i;
+          }
           r.next();
         }
       }
@@ -489,95 +547,78 @@ __global__ void __launch_bounds__(THREADS, 1)
             while (!mbar_try_wait(bar + 8 * (B_VFULL + i), (issued[i] - 1) & 1) &&
                    globaltimer() - t0 < WAIT_LIMIT_NS) {
             }
+#pragma unroll
+        for (uint32_t i = 0; i < NQ; i++)
+          if (q_issued[i])
+            while (!mbar_try_wait(bar + 8 * (B_QFULL + i), (q_issued[i] - 1) & 1) &&
+                   globaltimer() - t0 < WAIT_LIMIT_NS) {
+            }
         if (tails)
           while (!mbar_try_wait(bar + 8 * B_VTMA, (tails - 1) & 1) &&
                  globaltimer() - t0 < WAIT_LIMIT_NS) {
           }
       }
     } else {
-      // ======================= MMA issuer =======================
-      // Turn x (block j, tile t of a piece; group x & 1): S(x), S(x+1), then
-      // for each x: P V(x), S(x+2).  S(x+2) overwrites the scores that P V(x)
-      // reads as P: the MMAs of one thread run in order.
+      // ======================= MMA issuers =======================
+      // S of the group's next turn overwrites the scores that P V reads as P:
+      // the MMAs of one thread run in order.
       if (lane == 0) {
-        Pieces ws, wp;
-        Unit us{}, up{};
-        uint32_t js = 0, ts = 0, jp = 0, tp = 0, xs = 0, xp = 0;
-        Ring<NQ> rq, rq_piece;
-        Ring<NK> rk;
-        Ring<NV> rv;
-        uint32_t p_phase[2] = {0, 0}, o_units[2] = {0, 0};
-        bool have_s = ws.begin(p, plan), have_p = wp.begin(p, plan);
-        if (have_s) us = up = unit_of(p, ws.u);
+        const uint32_t g = (uint32_t)warp - 1;
+        const uint32_t tmem_s = tmem + g * BN, tmem_o = tmem + TMEM_O + g * HD;
+        const uint32_t sfull = bar + 8 * (B_SFULL + g), pfull = bar + 8 * (B_PFULL + g);
+        Own<NK> ts;  // the next S
+        Own<NV> tv;  // the next P V
+        bool have_s = ts.begin(p, plan, g), have_v = tv.begin(p, plan, g);
+        uint32_t p_phase = 0, o_units = 0;
         auto issue_s = [&]() -> bool {
-          const uint32_t g = xs & 1;
-          if (ts == 0) {
-            if (js == 0) rq_piece = rq;
-            rq = rq_piece;  // tile 0's buffer
-          }
-          if (js == 0 && !mbar_wait(bar + 8 * (B_QFULL + rq.i), rq.phase, abort_flag, err))
+          if (ts.first && !mbar_wait(bar + 8 * (B_QFULL + ts.q.i), ts.q.phase, abort_flag, err))
             return false;
-          if (!mbar_wait(bar + 8 * (B_KFULL + rk.i), rk.phase, abort_flag, err)) return false;
+          if (!mbar_wait(bar + 8 * (B_KFULL + ts.r.i), ts.r.phase, abort_flag, err)) return false;
           tc_fence_after();
-          const uint64_t da = sdesc(sb + O_Q + rq.i * TILE, 16, 1024);
-          const uint64_t db = sdesc(sb + O_K + rk.i * TILE, 16, 1024);
+          const uint32_t da = (sb + O_Q + ts.q.i * TILE) >> 4, db = (sb + O_K + ts.r.i * TILE) >> 4;
+          constexpr uint64_t top = sdesc(0, 16, 1024);
 #pragma unroll
           for (int kk = 0; kk < 8; kk++) {
             const uint32_t off = ((uint32_t)(kk >> 2) * CHUNK + (uint32_t)(kk & 3) * 32) >> 4;
-            umma(tmem + g * BN, da + off, db + off, IDESC_S, kk > 0);
+            umma(tmem_s, top | (da + off), top | (db + off), IDESC_S, kk > 0);
           }
-          umma_commit(bar + 8 * (B_SFULL + g));
-          if (js + 1 == ws.nb) umma_commit(bar + 8 * (B_QEMPTY + rq.i));
-          rq.next();
-          xs++;
-          if (++ts == us.tiles) {
-            umma_commit(bar + 8 * (B_KEMPTY + rk.i));
-            rk.next();
-            ts = 0;
-            if (++js == ws.nb) {
-              js = 0;
-              have_s = ws.next(p);
-              if (have_s) us = unit_of(p, ws.u);
-            }
+          umma_commit(sfull);
+          const uint32_t kempty = bar + 8 * (B_KEMPTY + ts.r.i);
+          umma_commit(kempty);
+          if (!ts.two) mbar_arrive(kempty);
+          if (ts.last()) {
+            const uint32_t qempty = bar + 8 * (B_QEMPTY + ts.q.i);
+            umma_commit(qempty);
+            if (ts.two || ts.w.nb == 1) mbar_arrive(qempty);
           }
+          have_s = ts.next(p, g);
           return true;
         };
-        bool ok = true;
-        for (int i = 0; i < 2 && ok && have_s; i++) ok = issue_s();
-        while (ok && have_p) {
-          const uint32_t g = xp & 1;
-          // the group's first and last turns of the piece
-          const bool first = up.tiles == 2 ? jp == 0 : jp < 2;
-          const bool last = up.tiles == 2 ? jp + 1 == wp.nb : jp + 2 >= wp.nb;
-          if ((first && !mbar_wait(bar + 8 * (B_OEMPTY + g), (o_units[g] & 1) ^ 1, abort_flag, err)) ||
-              !mbar_wait(bar + 8 * (B_PFULL + g), p_phase[g], abort_flag, err) ||
-              !mbar_wait(bar + 8 * (B_VFULL + rv.i), rv.phase, abort_flag, err))
+        bool ok = !have_s || issue_s();
+        while (ok && have_v) {
+          if ((tv.first && !mbar_wait(bar + 8 * (B_OEMPTY + g), (o_units & 1) ^ 1, abort_flag, err)) ||
+              !mbar_wait(bar + 8 * (B_VFULL + tv.r.i), tv.r.phase, abort_flag, err) ||
+              !mbar_wait(pfull, p_phase, abort_flag, err))
             break;
           tc_fence_after();
           // P: key pairs in the first 64 score columns; V MN-major (head_dim
           // contiguous), its 64-column chunks 16 KiB apart, 16 keys 2 KiB
-          const uint64_t dv = sdesc(sb + O_V + rv.i * TILE, CHUNK, 1024);
+          const uint32_t dv = (sb + O_V + tv.r.i * TILE) >> 4;
+          constexpr uint64_t top = sdesc(0, CHUNK, 1024);
+          umma_ts(tmem_o, tmem_s, top | dv, IDESC_O, !tv.first);
 #pragma unroll
-          for (int kk = 0; kk < 8; kk++)
-            umma_ts(tmem + TMEM_O + g * HD, tmem + g * BN + (uint32_t)kk * 8u,
-                    dv + (((uint32_t)kk * 16 * 128) >> 4), IDESC_O, (!first || kk > 0) ? 1u : 0u);
-          if (last) {
+          for (uint32_t kk = 1; kk < 8; kk++)
+            umma_ts(tmem_o, tmem_s + kk * 8u, top | (dv + ((kk * 16 * 128) >> 4)), IDESC_O, 1u);
+          const uint32_t vempty = bar + 8 * (B_VEMPTY + tv.r.i);
+          umma_commit(vempty);
+          if (!tv.two) mbar_arrive(vempty);
+          if (tv.last()) {
             umma_commit(bar + 8 * (B_OFULL + g));
-            o_units[g]++;
+            o_units++;
           }
-          p_phase[g] ^= 1u;
-          xp++;
-          if (++tp == up.tiles) {
-            umma_commit(bar + 8 * (B_VEMPTY + rv.i));
-            rv.next();
-            tp = 0;
-            if (++jp == wp.nb) {
-              jp = 0;
-              have_p = wp.next(p);
-              if (have_p) up = unit_of(p, wp.u);
-            }
-          }
+          p_phase ^= 1u;
           if (have_s) ok = issue_s();
+          have_v = tv.next(p, g);
         }
         // every MMA this thread issued has completed before the tensor
         // memory is released
@@ -834,7 +875,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 2)
+  if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(TMEM_COLS)
                  : "memory");

@@ -3,7 +3,7 @@
 
 * the split: the CTAs' pieces cover every unit's blocks once, every unit that a cut divides
   has exactly one joining CTA, whose piece list is the unit's, and no partial slot is used twice;
-* the protocol: MMA issuer, producers and the two softmax groups, with mbarriers that only
+* the protocol: the MMA issuers, producers and the two softmax groups, with mbarriers that only
   know the parity of their phase, run under random timing to the end, each turn's softmax
   reads the scores of its own block, and no accumulator or stage is overwritten in use.
 """
@@ -92,11 +92,14 @@ def protocol(plan, seed, NQ=2, NK=3, NV=2):
     def bar(name, i, count=1):
         return bars.setdefault((name, i), Bar(count))
 
+    for name, n in (("QE", NQ), ("KE", NK), ("VE", NV)):
+        for i in range(n):
+            bar(name, i, 2)
     for g in range(2):
         bar("P", g, 2), bar("OE", g, 4), bar("ML", g, 2)  # two threads stand for a group's 128
     q, k, v = [None] * NQ, [None] * NK, [None] * NV
     s_buf, o_buf, log = [None, None], [None, None], []
-    mma = []  # issued, not yet run: (function) in order
+    mmas = [[], []]  # issued by the group's issuer, not yet run, in order
 
     def wait(b, parity):
         while not b.passed(parity):
@@ -113,53 +116,55 @@ def protocol(plan, seed, NQ=2, NK=3, NV=2):
             if i == slots:
                 i, ph = 0, ph ^ 1
 
-    def issuer():
-        turns = [(n, j, t, tiles, nb) for n, (nb, tiles) in enumerate(plan) for j in range(nb)
-                 for t in range(tiles)]
-        st = dict(q=0, qp=0, qpiece=(0, 0), k=0, kp=0, x=0)
+    def turns_of(g):
+        """(piece, block, tile, first, last, Q tile index, block index) of the group's turns."""
+        x0, q0, n0, out = 0, 0, 0, []
+        for n, (nb, tiles) in enumerate(plan):
+            mine = (g - x0) & 1
+            js = range(nb) if tiles == 2 else range(mine, nb, 2)
+            for j in js:
+                out.append((n, j, mine if tiles == 2 else 0, j == js[0], j == js[-1],
+                            q0 + (mine if tiles == 2 else 0), n0 + j))
+            x0, q0, n0 = x0 + nb * tiles, q0 + tiles, n0 + nb
+        return out
 
-        def issue_s():
-            n, j, t, tiles, nb = turns[st["x"]]
-            g = st["x"] & 1
-            if t == 0:
-                if j == 0:
-                    st["qpiece"] = (st["q"], st["qp"])
-                st["q"], st["qp"] = st["qpiece"]
-            if j == 0:
-                yield from wait(bar("QF", st["q"]), st["qp"])
-            yield from wait(bar("KF", st["k"]), st["kp"])
-            qi, ki = st["q"], st["k"]
+    def issuer(g):
+        turns = turns_of(g)
+        mma = mmas[g]
+
+        def release(name, i, twice):
+            mma.append(lambda: bar(name, i, 2).arrive())
+            if twice:
+                bar(name, i, 2).arrive()
+
+        def issue_s(turn):
+            n, j, t, first, last, qn, kn = turn
+            nb, tiles = plan[n]
+            qi, ki = qn % NQ, kn % NK
+            if first:
+                yield from wait(bar("QF", qi), qn // NQ & 1)
+            yield from wait(bar("KF", ki), kn // NK & 1)
 
             def run():
                 assert q[qi] == (n, t) and k[ki] == (n, j)
                 s_buf[g] = ("S", n, j, t)
             mma.append(run)
             mma.append(lambda: bar("S", g).arrive())
-            if j + 1 == nb:
-                mma.append(lambda: bar("QE", qi).arrive())
-            st["q"] += 1
-            if st["q"] == NQ:
-                st["q"], st["qp"] = 0, st["qp"] ^ 1
-            st["x"] += 1
-            if t + 1 == tiles:
-                mma.append(lambda: bar("KE", ki).arrive())
-                st["k"] += 1
-                if st["k"] == NK:
-                    st["k"], st["kp"] = 0, st["kp"] ^ 1
+            release("KE", ki, tiles == 1)
+            if last:
+                release("QE", qi, tiles == 2 or nb == 1)
 
-        for _ in range(min(2, len(turns))):
-            yield from issue_s()
-        vi, vp, pp, ou = 0, 0, [0, 0], [0, 0]
-        for x, (n, j, t, tiles, nb) in enumerate(turns):
-            g = x & 1
-            first = j == 0 if tiles == 2 else j < 2
-            last = j + 1 == nb if tiles == 2 else j + 2 >= nb
+        pp = ou = 0
+        if turns:
+            yield from issue_s(turns[0])
+        for x, (n, j, t, first, last, _, vn) in enumerate(turns):
+            vi = vn % NV
             if first:
-                yield from wait(bar("OE", g), (ou[g] & 1) ^ 1)
-            yield from wait(bar("P", g), pp[g])
-            yield from wait(bar("VF", vi), vp)
+                yield from wait(bar("OE", g), (ou & 1) ^ 1)
+            yield from wait(bar("VF", vi), vn // NV & 1)
+            yield from wait(bar("P", g), pp)
 
-            def run(g=g, n=n, j=j, t=t, vi=vi, first=first):
+            def run(n=n, j=j, t=t, vi=vi, first=first):
                 assert s_buf[g] == ("P", n, j, t) and v[vi] == (n, j)
                 if first:
                     assert o_buf[g] is None, "accumulator not read yet"
@@ -168,17 +173,13 @@ def protocol(plan, seed, NQ=2, NK=3, NV=2):
                 o_buf[g][1].append((j, t))
                 log.append((n, j, t))
             mma.append(run)
+            release("VE", vi, plan[n][1] == 1)
             if last:
-                mma.append(lambda g=g: bar("OF", g).arrive())
-                ou[g] += 1
-            pp[g] ^= 1
-            if t + 1 == tiles:
-                mma.append(lambda vi=vi: bar("VE", vi).arrive())
-                vi += 1
-                if vi == NV:
-                    vi, vp = 0, vp ^ 1
-            if st["x"] < len(turns):
-                yield from issue_s()
+                mma.append(lambda: bar("OF", g).arrive())
+                ou += 1
+            pp ^= 1
+            if x + 1 < len(turns):
+                yield from issue_s(turns[x + 1])
 
     read = {}
 
@@ -230,13 +231,40 @@ def protocol(plan, seed, NQ=2, NK=3, NV=2):
 
     def tensor_core():
         while True:
+            mma = rnd.choice(mmas)
             if mma:
                 mma.pop(0)()
             yield
 
     kv = [(n, j) for n, (nb, _) in enumerate(plan) for j in range(nb)]
-    roles = [issuer(), load("K", NK, k, kv), load("V", NV, v, kv),
-             load("Q", NQ, q, [(n, t) for n, (_, tiles) in enumerate(plan) for t in range(tiles)])]
+    def v_and_q():
+        """V blocks; the next piece's Q with a piece's last block, before that block is waited
+        for (a tail: every last block here)."""
+        qs = [[(n, t) for t in range(tiles)] for n, (_, tiles) in enumerate(plan)]
+        state = dict(q=0, v=0)
+
+        def load_q():
+            for item in qs.pop(0):
+                i = state["q"] % NQ
+                yield from wait(bar("QE", i), (state["q"] // NQ & 1) ^ 1)
+                q[i] = item
+                yield
+                bar("QF", i).arrive()
+                state["q"] += 1
+
+        yield from load_q()
+        for n, (nb, _) in enumerate(plan):
+            for j in range(nb):
+                i = state["v"] % NV
+                yield from wait(bar("VE", i), (state["v"] // NV & 1) ^ 1)
+                v[i] = (n, j)
+                if j + 1 == nb and qs:
+                    yield from load_q()
+                yield
+                bar("VF", i).arrive()
+                state["v"] += 1
+
+    roles = [issuer(0), issuer(1), load("K", NK, k, kv), v_and_q()]
     roles += [softmax(g, th) for g in range(2) for th in range(2)]
     tc = tensor_core()
     idle = 0
@@ -251,8 +279,8 @@ def protocol(plan, seed, NQ=2, NK=3, NV=2):
                 roles.pop(i)
         idle += 1
         assert idle < 400 * (len(kv) + 10) * 40, "no end in sight"
-    assert log == [(n, j, t) for n, (nb, tiles) in enumerate(plan) for j in range(nb)
-                   for t in range(tiles)]
+    assert sorted(log) == [(n, j, t) for n, (nb, tiles) in enumerate(plan) for j in range(nb)
+                           for t in range(tiles)]
 
 
 @pytest.mark.parametrize("seed", range(40))
