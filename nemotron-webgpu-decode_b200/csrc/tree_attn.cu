@@ -10,26 +10,23 @@
 //
 // Tiles.  The n_nodes * group query rows of a kv head (node-major) are cut
 // into tiles of whole nodes, at most 128 rows: the M of an MMA.  A unit is a
-// (sequence, kv head) with one or two of its tiles, a block 128 cache rows.
+// (sequence, kv head) with one or two of its tiles, a block 64 cache rows.
 // The blocks of all units form one line that is cut into an equal range per
 // persistent CTA (one per SM); a unit that a cut divides leaves one partial
 // (m, l, O) per CTA in the workspace, which merge_kernel joins in order.
 //
 // A CTA's 12 warps:
-//   warps 0, 3  TMA producers: K blocks into 3 stages; V blocks into 2 and each
-//               unit's Q tiles into 2 (each 128 x 128 fp16 as two 64-column
-//               chunks, 128-byte swizzle: the K-major operand layout).  Warp 0
-//               also owns the tensor memory.
+//   warps 0, 3  TMA producers: K blocks into 5 stages; V blocks into 5 and each
+//               unit's Q tiles into 2 (as 64-column chunks, 128-byte swizzle:
+//               the K-major operand layout).  Warp 0 also owns the tensor
+//               memory.
 //   warps 1, 2  MMA issuers, one thread each, one per softmax group.  A turn
 //               is S = Q K^T of one (block, tile) and O += P V after its
-//               softmax; an issuer goes P V, S of its group's next turn, and
-//               so on, so one group's MMAs run beside the other's softmax.
-//               (One issuer for both spent as long between the MMAs, in waits
-//               and bookkeeping of a single thread, as in them: 2600 cycles a
-//               turn.)
+//               softmax; S runs two turns ahead into the other of the group's
+//               two score buffers, so the softmax of a turn never waits for
+//               the P V of the one before it.
 //   warps 4-7, 8-11  the softmax groups, a thread per query row, each with its
-//               own score and output accumulators (S0 S1 O0 O1: all 512
-//               columns).  A unit of two tiles gives each group a tile and
+//               own score buffers and output accumulator (all 512 columns).  A unit of two tiles gives each group a tile and
 //               both use every K/V block; a unit of one tile gives the
 //               groups alternate blocks and joins their (m, l, O) at its
 //               end, which keeps both busy when there are few query rows.
@@ -68,26 +65,29 @@ using nwd::TreeSeq;
 
 constexpr uint32_t HD = 128;
 constexpr uint32_t BM = 128;            // query rows per tile
-constexpr uint32_t BN = 128;            // cache rows per block
+constexpr uint32_t BN = 64;             // cache rows per block
 constexpr int THREADS = 384;
-constexpr uint32_t CHUNK = 128 * 128;   // 128 rows x 64 fp16
-constexpr uint32_t TILE = 2 * CHUNK;    // 128 x 128 fp16: 32 KiB
-constexpr uint32_t NQ = 2, NK = 3, NV = 2;  // stages
+constexpr uint32_t Q_CHUNK = BM * 128;  // rows x 64 fp16
+constexpr uint32_t Q_TILE = 2 * Q_CHUNK;
+constexpr uint32_t CHUNK = BN * 128;
+constexpr uint32_t TILE = 2 * CHUNK;    // a K or V block: 16 KiB
+constexpr uint32_t NQ = 2, NK = 5, NV = 5;  // stages
 constexpr uint32_t MAX_GROUPS32 = 128;  // batch / 32
 constexpr uint32_t MIN_BLOCKS = 1;      // least blocks per CTA range
 
 constexpr uint32_t O_Q = 0;
-constexpr uint32_t O_K = O_Q + NQ * TILE;
+constexpr uint32_t O_K = O_Q + NQ * Q_TILE;
 constexpr uint32_t O_V = O_K + NK * TILE;
 constexpr uint32_t O_ML = O_V + NV * TILE;        // [2 groups][128] (m, l); the plan's sums before
 constexpr uint32_t O_BAR = O_ML + 2 * BM * 8;
 constexpr int B_QFULL = 0, B_QEMPTY = B_QFULL + NQ, B_KFULL = B_QEMPTY + NQ,
               B_KEMPTY = B_KFULL + NK, B_VFULL = B_KEMPTY + NK, B_VEMPTY = B_VFULL + NV,
               B_VTMA = B_VEMPTY + NV,
+              // by 2 * softmax group + score buffer
+    B_SFULL = B_VTMA + 1, B_PFULL = B_SFULL + 4, B_PVDONE = B_PFULL + 4,
               // by softmax group
-    B_SFULL = B_VTMA + 1, B_PFULL = B_SFULL + 2, B_OFULL = B_PFULL + 2, B_OEMPTY = B_OFULL + 2,
-              B_ML = B_OEMPTY + 2, B_DRAIN = B_ML + 2, NBAR = B_DRAIN + 1;
-constexpr uint32_t O_PLAN = O_BAR + NBAR * 8;     // Plan
+    B_OEMPTY = B_PVDONE + 4, B_ML = B_OEMPTY + 2, B_DRAIN = B_ML + 2, NBAR = B_DRAIN + 1;
+constexpr uint32_t O_PLAN = (O_BAR + NBAR * 8 + 15) / 16 * 16;  // Plan
 constexpr uint32_t O_VBAD = O_PLAN + 48;          // [NV] u64: tree rows with NaN or inf in V
 constexpr uint32_t O_GBAD = O_VBAD + NV * 8;      // [2] u64: the same, gathered per group
 constexpr uint32_t O_MISC = O_GBAD + 16;          // tensor memory base, abort flag
@@ -98,7 +98,7 @@ constexpr uint32_t SMEM_BYTES = SMEM_USED;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 static_assert(MAX_GROUPS32 * 8 <= 2 * BM * 8, "the plan's sums fit the (m, l) area");
 
-constexpr uint32_t TMEM_COLS = 512;  // S0 S1 O0 O1, 128 columns each
+constexpr uint32_t TMEM_COLS = 512;  // 2 groups x 2 score buffers of 64, then O0 O1 of 128
 constexpr uint32_t TMEM_O = 256;
 constexpr float RESCALE_LOG2 = 8.f;
 constexpr float P_BIAS = 7.f;  // P = 2^(s - m + 7) <= 2^15, m within 2^8 of the maximum
@@ -202,31 +202,22 @@ __device__ __forceinline__ Unit unit_of(const TParams& p, uint32_t u) {
 template <uint32_t N>
 struct Ring {
   uint32_t i = 0, phase = 0;
-  // n <= N
-  __device__ __forceinline__ void step(uint32_t n) {
-    i += n;
-    if (i >= N) {
-      i -= N;
+  __device__ __forceinline__ void next() {
+    if (++i == N) {
+      i = 0;
       phase ^= 1u;
     }
   }
-  __device__ __forceinline__ void next() { step(1); }
-  __device__ __forceinline__ void add(uint32_t n) {
-    i += n;
-    phase ^= (i / N) & 1u;
-    i %= N;
-  }
 };
 
-// The turns of one softmax group, with the ring position of their blocks (K or
-// V, N stages) and of their Q tile.  x0: turns before the piece.
-template <uint32_t N>
+// The turns of one softmax group: the index (in this CTA) of a turn's block
+// and of its Q tile.  x0: turns of both groups before the piece.
 struct Own {
   Pieces w;
   bool two, first;
   uint32_t x0, j;
-  Ring<N> r, r0;    // of block j, of the piece's first block
-  Ring<NQ> q, q0;
+  uint32_t n, n0;  // index of block j, of the piece's first block
+  uint32_t q, q0;  // index of the group's tile, of the piece's first tile
   // the piece's first turn of group g, or the next piece's that has one
   __device__ __forceinline__ bool settle(const TParams& p, uint32_t g) {
     for (;;) {
@@ -235,34 +226,58 @@ struct Own {
       j = two ? 0 : mine;
       if (j < w.nb) {
         first = true;
-        r = r0;
-        r.step(j);
-        q = q0;
-        if (two) q.step(mine);
+        n = n0 + j;
+        q = q0 + (two ? mine : 0);
         return true;
       }
       if (!leave(p)) return false;
     }
   }
   __device__ __forceinline__ bool leave(const TParams& p) {
-    r0.add(w.nb);
-    q0.step(two ? 2 : 1);
+    n0 += w.nb;
+    q0 += two ? 2 : 1;
     x0 += two ? 2 * w.nb : w.nb;
     return w.next(p);
   }
   __device__ __forceinline__ bool begin(const TParams& p, const Plan& plan, uint32_t g) {
-    x0 = 0;
+    x0 = n0 = q0 = 0;
     return w.begin(p, plan) && settle(p, g);
   }
   __device__ __forceinline__ bool last() const { return j + (two ? 1 : 2) >= w.nb; }
   __device__ __forceinline__ bool next(const TParams& p, uint32_t g) {
-    const uint32_t n = two ? 1 : 2;
-    if ((j += n) < w.nb) {
+    const uint32_t step = two ? 1 : 2;
+    if ((j += step) < w.nb) {
       first = false;
-      r.step(n);
+      n += step;
       return true;
     }
     return leave(p) && settle(p, g);
+  }
+};
+
+// An issuer's way through the stages of a ring.  Both issuers wait for every
+// copy, in order, and release it, the ones that only the other group uses
+// too: a parity wait cannot tell a phase from the one two before or after it,
+// so nobody may fall, or run, two uses of a stage behind the others.
+template <uint32_t N>
+struct Walker {
+  uint32_t i = 0, phase = 0, n = 0;
+  __device__ __forceinline__ void next() {
+    n++;
+    if (++i == N) {
+      i = 0;
+      phase ^= 1u;
+    }
+  }
+  // waits for copy `to`; the ones before it are released as they land
+  __device__ __forceinline__ bool reach(uint32_t to, uint32_t full, uint32_t empty,
+                                        volatile int32_t* abort_flag, uint32_t* err) {
+    while (n != to) {
+      if (!mbar_wait(full + 8 * i, phase, abort_flag, err)) return false;
+      mbar_arrive(empty + 8 * i);
+      next();
+    }
+    return mbar_wait(full + 8 * i, phase, abort_flag, err);
   }
 };
 
@@ -358,10 +373,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     *abort_flag = 0;
     for (int i = 0; i < NBAR; i++) {
       uint32_t count = 1;
-      if (i >= B_PFULL && i < B_PFULL + 2) count = BM;
+      if (i >= B_PFULL && i < B_PFULL + 4) count = BM;
       if (i >= B_OEMPTY && i < B_OEMPTY + 2) count = 2 * BM;
       if (i >= B_ML && i < B_ML + 2) count = BM;
-      // a stage is released by both issuers, or twice by its only user
+      // a stage is released by both issuers
       if ((i >= B_QEMPTY && i < B_QEMPTY + (int)NQ) || (i >= B_KEMPTY && i < B_KEMPTY + (int)NK) ||
           (i >= B_VEMPTY && i < B_VEMPTY + (int)NV) || i == B_DRAIN)
         count = 2;
@@ -448,11 +463,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (uint32_t t = 0; t < un.tiles; t++) {
           if (!warp_wait(bar + 8 * (B_QEMPTY + rq.i), rq.phase ^ 1u, abort_flag, err)) return false;
           if (lane == 0) {
-            const uint32_t fb = bar + 8 * (B_QFULL + rq.i), dst = sb + O_Q + rq.i * TILE;
+            const uint32_t fb = bar + 8 * (B_QFULL + rq.i), dst = sb + O_Q + rq.i * Q_TILE;
             const int node = (int)(wq.b * p.n_nodes + (un.tile0 + t) * p.tile_nodes);
             mbar_arrive_tx(fb, q_bytes);
             tma_load_5d(dst, &tmq, fb, 0, 0, 0, (int)un.hkv, node, q_policy);
-            tma_load_5d(dst + CHUNK, &tmq, fb, 0, 1, 0, (int)un.hkv, node, q_policy);
+            tma_load_5d(dst + Q_CHUNK, &tmq, fb, 0, 1, 0, (int)un.hkv, node, q_policy);
           }
           __syncwarp();
 #pragma unroll
@@ -560,63 +575,64 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     } else {
       // ======================= MMA issuers =======================
-      // S of the group's next turn overwrites the scores that P V reads as P:
-      // the MMAs of one thread run in order.
+      // S(x), S(x+1), then for each of the group's turns x: P V(x), S(x+2).
+      // S(x+2) overwrites the scores that P V(x) reads as P: the MMAs of one
+      // thread run in order.
       if (lane == 0) {
         const uint32_t g = (uint32_t)warp - 1;
-        const uint32_t tmem_s = tmem + g * BN, tmem_o = tmem + TMEM_O + g * HD;
-        const uint32_t sfull = bar + 8 * (B_SFULL + g), pfull = bar + 8 * (B_PFULL + g);
-        Own<NK> ts;  // the next S
-        Own<NV> tv;  // the next P V
+        const uint32_t tmem_s = tmem + g * 2 * BN, tmem_o = tmem + TMEM_O + g * HD;
+        Own ts, tv;  // the next S, the next P V
+        Walker<NQ> q;
+        Walker<NK> k;
+        Walker<NV> v;
         bool have_s = ts.begin(p, plan, g), have_v = tv.begin(p, plan, g);
-        uint32_t p_phase = 0, o_units = 0;
+        uint32_t s_buf = 0, p_buf = 0, p_phase = 0, o_units = 0, q_slot = 0;
         auto issue_s = [&]() -> bool {
-          if (ts.first && !mbar_wait(bar + 8 * (B_QFULL + ts.q.i), ts.q.phase, abort_flag, err))
-            return false;
-          if (!mbar_wait(bar + 8 * (B_KFULL + ts.r.i), ts.r.phase, abort_flag, err)) return false;
+          if (ts.first) {
+            if (!q.reach(ts.q, bar + 8 * B_QFULL, bar + 8 * B_QEMPTY, abort_flag, err)) return false;
+            q_slot = q.i;
+            q.next();
+          }
+          if (!k.reach(ts.n, bar + 8 * B_KFULL, bar + 8 * B_KEMPTY, abort_flag, err)) return false;
           tc_fence_after();
-          const uint32_t da = (sb + O_Q + ts.q.i * TILE) >> 4, db = (sb + O_K + ts.r.i * TILE) >> 4;
+          const uint32_t da = (sb + O_Q + q_slot * Q_TILE) >> 4, db = (sb + O_K + k.i * TILE) >> 4;
           constexpr uint64_t top = sdesc(0, 16, 1024);
 #pragma unroll
-          for (int kk = 0; kk < 8; kk++) {
-            const uint32_t off = ((uint32_t)(kk >> 2) * CHUNK + (uint32_t)(kk & 3) * 32) >> 4;
-            umma(tmem_s, top | (da + off), top | (db + off), IDESC_S, kk > 0);
-          }
-          umma_commit(sfull);
-          const uint32_t kempty = bar + 8 * (B_KEMPTY + ts.r.i);
-          umma_commit(kempty);
-          if (!ts.two) mbar_arrive(kempty);
-          if (ts.last()) {
-            const uint32_t qempty = bar + 8 * (B_QEMPTY + ts.q.i);
-            umma_commit(qempty);
-            if (ts.two || ts.w.nb == 1) mbar_arrive(qempty);
-          }
+          for (uint32_t kk = 0; kk < 8; kk++)
+            umma(tmem_s + s_buf * BN, top | (da + (((kk >> 2) * Q_CHUNK + (kk & 3) * 32) >> 4)),
+                 top | (db + (((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4)), IDESC_S, kk > 0);
+          umma_commit(bar + 8 * (B_SFULL + 2 * g + s_buf));
+          umma_commit(bar + 8 * (B_KEMPTY + k.i));
+          k.next();
+          if (ts.last()) umma_commit(bar + 8 * (B_QEMPTY + q_slot));
+          s_buf ^= 1u;
           have_s = ts.next(p, g);
           return true;
         };
-        bool ok = !have_s || issue_s();
+        bool ok = true;
+        for (int i = 0; i < 2 && ok && have_s; i++) ok = issue_s();
         while (ok && have_v) {
           if ((tv.first && !mbar_wait(bar + 8 * (B_OEMPTY + g), (o_units & 1) ^ 1, abort_flag, err)) ||
-              !mbar_wait(bar + 8 * (B_VFULL + tv.r.i), tv.r.phase, abort_flag, err) ||
-              !mbar_wait(pfull, p_phase, abort_flag, err))
+              !v.reach(tv.n, bar + 8 * B_VFULL, bar + 8 * B_VEMPTY, abort_flag, err) ||
+              !mbar_wait(bar + 8 * (B_PFULL + 2 * g + p_buf), p_phase, abort_flag, err))
             break;
           tc_fence_after();
-          // P: key pairs in the first 64 score columns; V MN-major (head_dim
-          // contiguous), its 64-column chunks 16 KiB apart, 16 keys 2 KiB
-          const uint32_t dv = (sb + O_V + tv.r.i * TILE) >> 4;
+          // P: key pairs in the buffer's first 32 columns; V MN-major
+          // (head_dim contiguous), its 64-column chunks 8 KiB apart, 16 keys
+          // 2 KiB
+          const uint32_t dv = (sb + O_V + v.i * TILE) >> 4;
           constexpr uint64_t top = sdesc(0, CHUNK, 1024);
-          umma_ts(tmem_o, tmem_s, top | dv, IDESC_O, !tv.first);
+          umma_ts(tmem_o, tmem_s + p_buf * BN, top | dv, IDESC_O, !tv.first);
 #pragma unroll
-          for (uint32_t kk = 1; kk < 8; kk++)
-            umma_ts(tmem_o, tmem_s + kk * 8u, top | (dv + ((kk * 16 * 128) >> 4)), IDESC_O, 1u);
-          const uint32_t vempty = bar + 8 * (B_VEMPTY + tv.r.i);
-          umma_commit(vempty);
-          if (!tv.two) mbar_arrive(vempty);
-          if (tv.last()) {
-            umma_commit(bar + 8 * (B_OFULL + g));
-            o_units++;
-          }
-          p_phase ^= 1u;
+          for (uint32_t kk = 1; kk < BN / 16; kk++)
+            umma_ts(tmem_o, tmem_s + p_buf * BN + kk * 8u, top | (dv + ((kk * 16 * 128) >> 4)),
+                    IDESC_O, 1u);
+          umma_commit(bar + 8 * (B_PVDONE + 2 * g + p_buf));
+          umma_commit(bar + 8 * (B_VEMPTY + v.i));
+          v.next();
+          o_units += tv.last();
+          p_phase ^= p_buf;
+          p_buf ^= 1u;
           if (have_s) ok = issue_s();
           have_v = tv.next(p, g);
         }
@@ -636,12 +652,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t quad = (uint32_t)warp & 3u;
     const uint32_t r = quad * 32u + (uint32_t)lane;  // row of the tile = tensor memory lane
     const uint32_t lanes = quad * 32u << 16;
-    const uint32_t tmem_s = tmem + g * BN + lanes, tmem_o = tmem + TMEM_O + lanes;
+    const uint32_t tmem_o = tmem + TMEM_O + lanes;
     float2* ml = reinterpret_cast<float2*>(smem + O_ML);
     const uint32_t q_node = r / p.group, q_head = r % p.group;
-    uint32_t s_phase = 0, x0 = 0;      // x0: turns before this piece
-    uint32_t o_units[2] = {0, 0};      // pieces that group 0 / 1 had turns in
-    uint32_t ml_units[2] = {0, 0};     // of those, pieces of one tile
+    uint32_t x0 = 0;                   // turns before this piece, of both groups
+    uint32_t turns[2] = {0, 0};        // of each group
+    uint32_t ml_units[2] = {0, 0};     // pieces of one tile that a group had turns in
+    // a group's turn i uses its score buffer i & 1, for the (i >> 1)th time
+    auto turn_done = [&](uint32_t of, uint32_t i) {  // its P V has completed
+      return warp_wait(bar + 8 * (B_PVDONE + 2 * of + (i & 1)), (i >> 1) & 1, abort_flag, err);
+    };
     Ring<NV> rv;
     bool ok = true;
     Pieces w;
@@ -669,21 +689,22 @@ __global__ void __launch_bounds__(THREADS, 1)
           rv.next();
           continue;
         }
-        if (!warp_wait(bar + 8 * (B_SFULL + g), s_phase, abort_flag, err)) {
+        const uint32_t turn = turns[g]++, buf = turn & 1;
+        const uint32_t tmem_s = tmem + (2 * g + buf) * BN + lanes;
+        if (!warp_wait(bar + 8 * (B_SFULL + 2 * g + buf), (turn >> 1) & 1, abort_flag, err)) {
           ok = false;
           break;
         }
-        s_phase ^= 1u;
         tc_fence_after();
         if (warp_used) {
-          float s[128];
+          float s[BN];
 #pragma unroll
-          for (int c = 0; c < 4; c++) tmem_ld32(tmem_s + c * 32, s + c * 32);
+          for (int c = 0; c < 2; c++) tmem_ld32(tmem_s + c * 32, s + c * 32);
           tmem_ld_wait();
           if (tail) {
             // bit c of word i: this row attends cache row key0 + 32 i + c
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < 2; i++) {
               const int64_t at = (int64_t)key0 + 32 * i - (int64_t)w.s.ctx;  // in the tree
               uint32_t ok32;
               if (at <= -32) ok32 = 0xffffffffu;
@@ -698,7 +719,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 8; i++) mv[i] = s[i];
 #pragma unroll
-          for (int c = 8; c < 128; c++) mv[c & 7] = fmaxf(mv[c & 7], s[c]);
+          for (int c = 8; c < (int)BN; c++) mv[c & 7] = fmaxf(mv[c & 7], s[c]);
 #pragma unroll
           for (int i = 0; i < 4; i++) mv[i] = fmaxf(mv[i], mv[i + 4]);
           const float mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * p.scale_log2;
@@ -706,8 +727,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (__any_sync(0xffffffffu, up)) {
             const float alpha = up ? ex2f(m - mx) : 1.f;  // 0 while m is -inf
             if (two ? j > 0 : j > 1) {
-              // S of this turn is done, so P V of the group's last turn,
-              // issued before it, is too
+              // O is rescaled once the P V of the group's last turn is in it
+              if (!turn_done(g, turn - 1)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
 #pragma unroll
               for (int c = 0; c < 4; c++) {
                 float ov[32];
@@ -723,19 +748,16 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           const float nb = m == -INFINITY ? 0.f : P_BIAS - m;
           float rs[4] = {0.f, 0.f, 0.f, 0.f};
+          float pk[32];
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            float pk[32];
-#pragma unroll
-            for (int c = 0; c < 32; c++) {
-              const float p0 = ex2f(fmaf(s[64 * h + 2 * c], p.scale_log2, nb));
-              const float p1 = ex2f(fmaf(s[64 * h + 2 * c + 1], p.scale_log2, nb));
-              rs[c & 3] += p0 + p1;
-              const __half2 hh = __floats2half2_rn(p0, p1);
-              pk[c] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&hh));
-            }
-            tmem_st32(tmem_s + 32 * h, pk);
+          for (int c = 0; c < 32; c++) {
+            const float p0 = ex2f(fmaf(s[2 * c], p.scale_log2, nb));
+            const float p1 = ex2f(fmaf(s[2 * c + 1], p.scale_log2, nb));
+            rs[c & 3] += p0 + p1;
+            const __half2 hh = __floats2half2_rn(p0, p1);
+            pk[c] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&hh));
           }
+          tmem_st32(tmem_s, pk);
           l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
           tmem_st_wait();
         }
@@ -748,7 +770,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         rv.next();
         tc_fence_before();
-        mbar_arrive(bar + 8 * (B_PFULL + g));
+        mbar_arrive(bar + 8 * (B_PFULL + 2 * g + buf));
       }
       if (!ok) break;
 
@@ -794,7 +816,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       };
       if (two) {
-        if (!warp_wait(bar + 8 * (B_OFULL + g), o_units[g] & 1, abort_flag, err)) {
+        turns[g ^ 1] += w.nb;
+        if (!turn_done(g, turns[g] - 1)) {
           ok = false;
           break;
         }
@@ -816,12 +839,18 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_before();
         asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 2;" ::"r"(bar + 8 * (B_OEMPTY + g))
                      : "memory");
-        o_units[0]++;
-        o_units[1]++;
       } else {
         // group of block 0: x0 & 1; the other has turns from two blocks on
         const bool had[2] = {w.nb > 1 || (x0 & 1) == 0, w.nb > 1 || (x0 & 1) == 1};
+        // the other group's turns: blocks (mine ^ 1), (mine ^ 1) + 2, ..
+        turns[g ^ 1] += (w.nb + mine) / 2;
+        // (m, l) are handed over once the group's O is complete: that needs the
+        // O before it released, by threads that have read the (m, l) before
         if (had[g]) {
+          if (!turn_done(g, turns[g] - 1)) {
+            ok = false;
+            break;
+          }
           ml[g * BM + r] = make_float2(m, l);
           if (r == 0) gbad[g] = bad;
           mbar_arrive(bar + 8 * (B_ML + g));
@@ -830,7 +859,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (uint32_t i = 0; i < 2; i++)
           if (ok && had[i])
             ok = warp_wait(bar + 8 * (B_ML + i), ml_units[i] & 1, abort_flag, err) &&
-                 warp_wait(bar + 8 * (B_OFULL + i), o_units[i] & 1, abort_flag, err);
+                 turn_done(i, turns[i] - 1);
         if (!ok) break;
         tc_fence_after();
         if (warp_used) {
@@ -865,7 +894,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (uint32_t i = 0; i < 2; i++)
           if (had[i]) {
             mbar_arrive(bar + 8 * (B_OEMPTY + i));
-            o_units[i]++;
             ml_units[i]++;
           }
       }
