@@ -154,7 +154,9 @@ def check(status: int) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args))
+    status = getattr(_lib or load(), name)(*args)
+    if status != NWD_OK:
+        check(status)
 
 
 def version() -> str:

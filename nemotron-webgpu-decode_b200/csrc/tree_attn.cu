@@ -15,21 +15,25 @@
 // persistent CTA (one per SM); a unit that a cut divides leaves one partial
 // (m, l, O) per CTA in the workspace, which merge_kernel joins in order.
 //
-// A CTA's 12 warps:
-//   warps 0, 3  TMA producers: K blocks into 5 stages; V blocks into 5 and each
-//               unit's Q tiles into 2 (as 64-column chunks, 128-byte swizzle:
-//               the K-major operand layout).  Warp 0 also owns the tensor
-//               memory.
-//   warps 1, 2  MMA issuers, one thread each, one per softmax group.  A turn
-//               is S = Q K^T of one (block, tile) and O += P V after its
-//               softmax; S runs two turns ahead into the other of the group's
-//               two score buffers, so the softmax of a turn never waits for
-//               the P V of the one before it.
-//   warps 4-7, 8-11  the softmax groups, a thread per query row, each with its
-//               own score buffers and output accumulator (all 512 columns).  A unit of two tiles gives each group a tile and
-//               both use every K/V block; a unit of one tile gives the
-//               groups alternate blocks and joins their (m, l, O) at its
-//               end, which keeps both busy when there are few query rows.
+// A CTA's 16 warps:
+//   warps 0, 1    TMA producers: K blocks into 5 stages; V blocks into 5 and
+//                 each unit's Q tiles into 2 (as 64-column chunks, 128-byte
+//                 swizzle: the K-major operand layout).  Warp 0 also owns the
+//                 tensor memory; warps 2, 3 are idle.
+//   warps 4 - 7   MMA issuers: S of softmax group 0, of group 1, P V of group
+//                 0, of group 1.  A turn is S = Q K^T of one (block, tile) and
+//                 O += P V after its softmax; S runs two turns ahead into the
+//                 other of the group's two score buffers, so the softmax of a
+//                 turn does not wait for the P V of the one before it.  An
+//                 issuer's waits, descriptors and commits are a chain of some
+//                 hundred dependent instructions per turn, longer than the
+//                 MMAs that it issues: hence four.
+//   warps 8-11, 12-15  the softmax groups, a thread per query row, each with
+//                 its own score buffers and output accumulator (all 512
+//                 columns).  A unit of two tiles gives each group a tile and
+//                 both use every K/V block; a unit of one tile gives the
+//                 groups alternate blocks and joins their (m, l, O) at its
+//                 end, which keeps both busy when there are few query rows.
 //
 // Softmax in the log2 domain with a lazily moved maximum (O is rescaled in
 // tensor memory only when a row's maximum grows by more than 2^8).  P is
@@ -66,7 +70,7 @@ using nwd::TreeSeq;
 constexpr uint32_t HD = 128;
 constexpr uint32_t BM = 128;            // query rows per tile
 constexpr uint32_t BN = 64;             // cache rows per block
-constexpr int THREADS = 384;
+constexpr int THREADS = 512;
 constexpr uint32_t Q_CHUNK = BM * 128;  // rows x 64 fp16
 constexpr uint32_t Q_TILE = 2 * Q_CHUNK;
 constexpr uint32_t CHUNK = BN * 128;
@@ -153,6 +157,18 @@ __device__ __forceinline__ uint32_t seq_blocks(const TreeSeq& s) {
   return max(1u, (s.ctx + s.nodes + BN - 1) / BN);
 }
 
+// A value that is the same in all lanes of a warp, in a way that the compiler
+// sees: it then stays in uniform registers, which the MMA instructions take
+// their operands from.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) {
+  return __reduce_max_sync(0xffffffffu, x);
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+
 // The pieces of a CTA's range: blocks [blk, blk + nb) of unit u of sequence b.
 struct Pieces {
   uint64_t left;
@@ -160,13 +176,13 @@ struct Pieces {
   TreeSeq s;
   __device__ __forceinline__ void load(const TParams& p) {
     s = load_seq(p, b, nullptr);
-    nblk = seq_blocks(s);
+    nblk = uniform(seq_blocks(s));
   }
   __device__ __forceinline__ bool begin(const TParams& p, const Plan& plan) {
-    left = plan.left;
-    b = plan.b;
-    u = plan.u;
-    blk = plan.blk;
+    left = (uint64_t)uniform((uint32_t)(plan.left >> 32)) << 32 | uniform((uint32_t)plan.left);
+    b = uniform(plan.b);
+    u = uniform(plan.u);
+    blk = uniform(plan.blk);
     if (left == 0) return false;
     load(p);
     nb = (uint32_t)min((uint64_t)(nblk - blk), left);
@@ -255,7 +271,7 @@ struct Own {
   }
 };
 
-// An issuer's way through the stages of a ring.  Both issuers wait for every
+// An issuer's way through the stages of a ring.  Both groups' issuers wait for every
 // copy, in order, and release it, the ones that only the other group uses
 // too: a parity wait cannot tell a phase from the one two before or after it,
 // so nobody may fall, or run, two uses of a stage behind the others.
@@ -273,13 +289,19 @@ struct Walker {
   __device__ __forceinline__ bool reach(uint32_t to, uint32_t full, uint32_t empty,
                                         volatile int32_t* abort_flag, uint32_t* err) {
     while (n != to) {
-      if (!mbar_wait(full + 8 * i, phase, abort_flag, err)) return false;
-      mbar_arrive(empty + 8 * i);
+      if (!warp_wait(full + 8 * i, phase, abort_flag, err)) return false;
+      if (elect_one()) mbar_arrive(empty + 8 * i);
       next();
     }
-    return mbar_wait(full + 8 * i, phase, abort_flag, err);
+    return warp_wait(full + 8 * i, phase, abort_flag, err);
   }
 };
+
+// a / b, by the 32-bit division where both fit it (nearly always: the 64-bit
+// one takes about half a microsecond of the plan each time).
+__device__ __forceinline__ uint64_t div_small(uint64_t a, uint64_t b) {
+  return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 
 // This CTA's range of the line of blocks.  Called by all threads; `sums` is
 // shared scratch.  per = the range length, the same in every CTA.
@@ -305,13 +327,13 @@ __device__ void make_plan(const TParams& p, uint64_t* sums, Plan* plan, MergeDes
       if ((int)lane >= i) incl += y;
     }
     const uint64_t total = __shfl_sync(0xffffffffu, incl, 31) * p.n_units;
-    const uint64_t per = max((total + gridDim.x - 1) / gridDim.x, (uint64_t)MIN_BLOCKS);
+    const uint64_t per = max(div_small(total + gridDim.x - 1, gridDim.x), (uint64_t)MIN_BLOCKS);
     const uint64_t x0 = min(total, (uint64_t)blockIdx.x * per), x1 = min(total, x0 + per);
     MergeDesc d{0, 0, 0, 0};
     Plan pl{};
     pl.left = x1 - x0;
     if (x1 > x0) {
-      const uint64_t y = x0 / p.n_units;  // in blocks of a single unit per sequence
+      const uint64_t y = div_small(x0, p.n_units);  // in blocks of a single unit per sequence
       uint64_t base = incl - mine;
       const uint32_t owner =
           __ffs(__ballot_sync(0xffffffffu, base <= y && y < incl)) - 1;
@@ -332,11 +354,11 @@ __device__ void make_plan(const TParams& p, uint64_t* sums, Plan* plan, MergeDes
       if (lane == at) {
         const uint64_t r = x0 - lo * p.n_units;
         pl.b = g * 32 + lane;
-        pl.u = (uint32_t)(r / n);
-        pl.blk = (uint32_t)(r % n);
+        pl.u = (uint32_t)div_small(r, n);
+        pl.blk = (uint32_t)(r - (uint64_t)pl.u * n);
         const uint64_t ends = x0 - pl.blk + n;  // of the unit, on the line
         if (pl.blk > 0 && ends <= x1)
-          d = MergeDesc{1, pl.b, pl.u, (uint32_t)((x0 - pl.blk) / per)};
+          d = MergeDesc{1, pl.b, pl.u, (uint32_t)div_small(x0 - pl.blk, per)};
         *plan = pl;
         desc[blockIdx.x] = d;
       }
@@ -348,6 +370,22 @@ __device__ void make_plan(const TParams& p, uint64_t* sums, Plan* plan, MergeDes
   __syncthreads();
 }
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 // Stores 4 columns (from column c) of a partial's row.
 __device__ __forceinline__ void store_part(float* slot, uint32_t row, uint32_t c, const float* v) {
   *reinterpret_cast<float4*>(slot + ((size_t)(c >> 2) * BM + row) * 4) =
@@ -376,10 +414,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (i >= B_PFULL && i < B_PFULL + 4) count = BM;
       if (i >= B_OEMPTY && i < B_OEMPTY + 2) count = 2 * BM;
       if (i >= B_ML && i < B_ML + 2) count = BM;
-      // a stage is released by both issuers
+      // a stage is released by both groups' issuers
       if ((i >= B_QEMPTY && i < B_QEMPTY + (int)NQ) || (i >= B_KEMPTY && i < B_KEMPTY + (int)NK) ||
-          (i >= B_VEMPTY && i < B_VEMPTY + (int)NV) || i == B_DRAIN)
+          (i >= B_VEMPTY && i < B_VEMPTY + (int)NV))
         count = 2;
+      if (i == B_DRAIN) count = 4;
       mbar_init(bar + 8 * i, count);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -390,6 +429,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                  "r"(TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmq)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmk)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmv)) : "memory");
   }
   nwd::pdl_wait();
   make_plan(p, reinterpret_cast<uint64_t*>(smem + O_ML),
@@ -404,9 +448,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Registers per thread: 56 for the first warpgroup, 224 for the softmax
-  // groups: 128 * (56 + 2 * 224) = 64512, the 384 * 168 of the launch.
-  if (warp < 4) {
+  // Registers per thread: 56 for the first two warpgroups, 200 for the softmax
+  // groups: 128 * 2 * (56 + 200) = 65536, the 512 * 128 of the launch.
+  if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
     if (warp == 0) {
       // ======================= K =======================
@@ -444,7 +488,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                    globaltimer() - t0 < WAIT_LIMIT_NS) {
             }
       }
-    } else if (warp == 3) {
+    } else if (warp == 1) {
       // ======================= V and Q =======================
       // The next piece's Q goes out with the last V block of a piece (before
       // this warp waits for that block, if it is a tail): its buffers fill as
@@ -573,48 +617,59 @@ __global__ void __launch_bounds__(THREADS, 1)
                  globaltimer() - t0 < WAIT_LIMIT_NS) {
           }
       }
-    } else {
+    } else if (warp >= 4) {
       // ======================= MMA issuers =======================
-      // S(x), S(x+1), then for each of the group's turns x: P V(x), S(x+2).
-      // S(x+2) overwrites the scores that P V(x) reads as P: the MMAs of one
-      // thread run in order.
-      if (lane == 0) {
-        const uint32_t g = (uint32_t)warp - 1;
-        const uint32_t tmem_s = tmem + g * 2 * BN, tmem_o = tmem + TMEM_O + g * HD;
-        Own ts, tv;  // the next S, the next P V
+      // The whole warp walks its group's turns x, one lane issues.
+      const uint32_t role = uniform((uint32_t)warp - 4);
+      const uint32_t g = role & 1;
+      const bool leader = elect_one();
+      const uint32_t tm = uniform(tmem);
+      const uint32_t tmem_s = tm + g * 2 * BN;
+      Own t;
+      bool have = t.begin(p, plan, g);
+      uint32_t buf = 0, phase = 0;  // of the group's score buffers
+      if (role < 2) {
+        // ---- S(x), once P V(x - 2) has read the P in its buffer
         Walker<NQ> q;
         Walker<NK> k;
-        Walker<NV> v;
-        bool have_s = ts.begin(p, plan, g), have_v = tv.begin(p, plan, g);
-        uint32_t s_buf = 0, p_buf = 0, p_phase = 0, o_units = 0, q_slot = 0;
-        auto issue_s = [&]() -> bool {
-          if (ts.first) {
-            if (!q.reach(ts.q, bar + 8 * B_QFULL, bar + 8 * B_QEMPTY, abort_flag, err)) return false;
+        uint32_t q_slot = 0;
+        while (have) {
+          if (t.first) {
+            if (!q.reach(t.q, bar + 8 * B_QFULL, bar + 8 * B_QEMPTY, abort_flag, err)) break;
             q_slot = q.i;
             q.next();
           }
-          if (!k.reach(ts.n, bar + 8 * B_KFULL, bar + 8 * B_KEMPTY, abort_flag, err)) return false;
+          if (!k.reach(t.n, bar + 8 * B_KFULL, bar + 8 * B_KEMPTY, abort_flag, err) ||
+              !warp_wait(bar + 8 * (B_PVDONE + 2 * g + buf), phase ^ 1u, abort_flag, err))
+            break;
           tc_fence_after();
           const uint32_t da = (sb + O_Q + q_slot * Q_TILE) >> 4, db = (sb + O_K + k.i * TILE) >> 4;
           constexpr uint64_t top = sdesc(0, 16, 1024);
+          if (leader) {
 #pragma unroll
-          for (uint32_t kk = 0; kk < 8; kk++)
-            umma(tmem_s + s_buf * BN, top | (da + (((kk >> 2) * Q_CHUNK + (kk & 3) * 32) >> 4)),
-                 top | (db + (((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4)), IDESC_S, kk > 0);
-          umma_commit(bar + 8 * (B_SFULL + 2 * g + s_buf));
-          umma_commit(bar + 8 * (B_KEMPTY + k.i));
+            for (uint32_t kk = 0; kk < 8; kk++)
+              umma(tmem_s + buf * BN, top | (da + (((kk >> 2) * Q_CHUNK + (kk & 3) * 32) >> 4)),
+                   top | (db + (((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4)), IDESC_S, kk > 0);
+            umma_commit(bar + 8 * (B_SFULL + 2 * g + buf));
+            umma_commit(bar + 8 * (B_KEMPTY + k.i));
+            if (t.last()) umma_commit(bar + 8 * (B_QEMPTY + q_slot));
+          }
+          __syncwarp();
           k.next();
-          if (ts.last()) umma_commit(bar + 8 * (B_QEMPTY + q_slot));
-          s_buf ^= 1u;
-          have_s = ts.next(p, g);
-          return true;
-        };
-        bool ok = true;
-        for (int i = 0; i < 2 && ok && have_s; i++) ok = issue_s();
-        while (ok && have_v) {
-          if ((tv.first && !mbar_wait(bar + 8 * (B_OEMPTY + g), (o_units & 1) ^ 1, abort_flag, err)) ||
-              !v.reach(tv.n, bar + 8 * B_VFULL, bar + 8 * B_VEMPTY, abort_flag, err) ||
-              !mbar_wait(bar + 8 * (B_PFULL + 2 * g + p_buf), p_phase, abort_flag, err))
+          phase ^= buf;
+          buf ^= 1u;
+          have = t.next(p, g);
+        }
+      } else {
+        // ---- P V(x)
+        const uint32_t tmem_o = tm + TMEM_O + g * HD;
+        Walker<NV> v;
+        uint32_t o_units = 0;
+        while (have) {
+          if ((t.first &&
+               !warp_wait(bar + 8 * (B_OEMPTY + g), (o_units & 1) ^ 1, abort_flag, err)) ||
+              !v.reach(t.n, bar + 8 * B_VFULL, bar + 8 * B_VEMPTY, abort_flag, err) ||
+              !warp_wait(bar + 8 * (B_PFULL + 2 * g + buf), phase, abort_flag, err))
             break;
           tc_fence_after();
           // P: key pairs in the buffer's first 32 columns; V MN-major
@@ -622,33 +677,36 @@ __global__ void __launch_bounds__(THREADS, 1)
           // 2 KiB
           const uint32_t dv = (sb + O_V + v.i * TILE) >> 4;
           constexpr uint64_t top = sdesc(0, CHUNK, 1024);
-          umma_ts(tmem_o, tmem_s + p_buf * BN, top | dv, IDESC_O, !tv.first);
+          if (leader) {
+            umma_ts(tmem_o, tmem_s + buf * BN, top | dv, IDESC_O, !t.first);
 #pragma unroll
-          for (uint32_t kk = 1; kk < BN / 16; kk++)
-            umma_ts(tmem_o, tmem_s + p_buf * BN + kk * 8u, top | (dv + ((kk * 16 * 128) >> 4)),
-                    IDESC_O, 1u);
-          umma_commit(bar + 8 * (B_PVDONE + 2 * g + p_buf));
-          umma_commit(bar + 8 * (B_VEMPTY + v.i));
+            for (uint32_t kk = 1; kk < BN / 16; kk++)
+              umma_ts(tmem_o, tmem_s + buf * BN + kk * 8u, top | (dv + ((kk * 16 * 128) >> 4)),
+                      IDESC_O, 1u);
+            umma_commit(bar + 8 * (B_PVDONE + 2 * g + buf));
+            umma_commit(bar + 8 * (B_VEMPTY + v.i));
+          }
+          __syncwarp();
           v.next();
-          o_units += tv.last();
-          p_phase ^= p_buf;
-          p_buf ^= 1u;
-          if (have_s) ok = issue_s();
-          have_v = tv.next(p, g);
+          o_units += t.last();
+          phase ^= buf;
+          buf ^= 1u;
+          have = t.next(p, g);
         }
-        // every MMA this thread issued has completed before the tensor
-        // memory is released
-        umma_commit(bar + 8 * B_DRAIN);
-        const uint64_t t0 = globaltimer();
-        while (!mbar_try_wait(bar + 8 * B_DRAIN, 0) && globaltimer() - t0 < WAIT_LIMIT_NS) {
-        }
+      }
+      // every MMA this warp issued has completed before the tensor memory is
+      // released
+      if (leader) umma_commit(bar + 8 * B_DRAIN);
+      __syncwarp();
+      const uint64_t t0 = globaltimer();
+      while (!mbar_try_wait(bar + 8 * B_DRAIN, 0) && globaltimer() - t0 < WAIT_LIMIT_NS) {
       }
       __syncwarp();
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;" ::: "memory");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;" ::: "memory");
     // ======================= softmax groups =======================
-    const uint32_t g = (uint32_t)(warp - 4) >> 2;
+    const uint32_t g = (uint32_t)(warp - 8) >> 2;
     const uint32_t quad = (uint32_t)warp & 3u;
     const uint32_t r = quad * 32u + (uint32_t)lane;  // row of the tile = tensor memory lane
     const uint32_t lanes = quad * 32u << 16;
@@ -662,7 +720,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto turn_done = [&](uint32_t of, uint32_t i) {  // its P V has completed
       return warp_wait(bar + 8 * (B_PVDONE + 2 * of + (i & 1)), (i >> 1) & 1, abort_flag, err);
     };
-    Ring<NV> rv;
+    uint32_t n0 = 0;                   // blocks before this piece
     bool ok = true;
     Pieces w;
     for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
@@ -681,16 +739,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         sees = nwd::tree_mask(p.parents + (size_t)w.b * p.n_nodes, (int)node, err);
       float m = -INFINITY, l = 0.f;
       uint64_t bad = 0;
-      for (uint32_t j = 0; j < w.nb; j++) {
-        const bool my_turn = two || (j & 1) == mine;
-        const uint32_t key0 = (w.blk + j) * BN;
-        const bool tail = key0 + BN > w.s.ctx;
-        if (!my_turn) {
-          rv.next();
-          continue;
-        }
+      const uint32_t step = two ? 1 : 2;
+      uint32_t j = two ? 0 : mine;
+      const uint32_t first_turn = turns[g];
+      for (; j < w.nb; j += step) {
         const uint32_t turn = turns[g]++, buf = turn & 1;
         const uint32_t tmem_s = tmem + (2 * g + buf) * BN + lanes;
+        const uint32_t key0 = (w.blk + j) * BN;
+        const bool tail = key0 + BN > w.s.ctx;
         if (!warp_wait(bar + 8 * (B_SFULL + 2 * g + buf), (turn >> 1) & 1, abort_flag, err)) {
           ok = false;
           break;
@@ -698,8 +754,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_after();
         if (warp_used) {
           float s[BN];
-#pragma unroll
-          for (int c = 0; c < 2; c++) tmem_ld32(tmem_s + c * 32, s + c * 32);
+          tmem_ld32(tmem_s, s);
+          tmem_ld32(tmem_s + 32, s + 32);
           tmem_ld_wait();
           if (tail) {
             // bit c of word i: this row attends cache row key0 + 32 i + c
@@ -715,63 +771,70 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (!((ok32 >> c) & 1u)) s[32 * i + c] = -INFINITY;
             }
           }
-          float mv[8];
-#pragma unroll
-          for (int i = 0; i < 8; i++) mv[i] = s[i];
-#pragma unroll
-          for (int c = 8; c < (int)BN; c++) mv[c & 7] = fmaxf(mv[c & 7], s[c]);
-#pragma unroll
-          for (int i = 0; i < 4; i++) mv[i] = fmaxf(mv[i], mv[i + 4]);
-          const float mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * p.scale_log2;
-          const bool up = mx > m + RESCALE_LOG2;
-          if (__any_sync(0xffffffffu, up)) {
-            const float alpha = up ? ex2f(m - mx) : 1.f;  // 0 while m is -inf
-            if (two ? j > 0 : j > 1) {
-              // O is rescaled once the P V of the group's last turn is in it
-              if (!turn_done(g, turn - 1)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-#pragma unroll
-              for (int c = 0; c < 4; c++) {
-                float ov[32];
-                tmem_ld32(tmem_o + g * HD + c * 32, ov);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 32; i++) ov[i] *= alpha;
-                tmem_st32(tmem_o + g * HD + c * 32, ov);
-              }
-            }
-            l *= alpha;
-            if (up) m = mx;
-          }
-          const float nb = m == -INFINITY ? 0.f : P_BIAS - m;
-          float rs[4] = {0.f, 0.f, 0.f, 0.f};
+          // The exponentials are taken against the maximum so far, beside the
+          // search for this block's: only where that lies 2^8 above it (the
+          // first blocks, as a rule) is O rescaled and are they taken again.
           float pk[32];
+          float2 sum, sum1;
+          bool again;
+          do {
+            const float nb = m == -INFINITY ? 0.f : P_BIAS - m;
+            const float2 sc = make_float2(p.scale_log2, p.scale_log2), nb2 = make_float2(nb, nb);
+            sum = sum1 = make_float2(0.f, 0.f);
+            float mv[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 32; c++) {
-            const float p0 = ex2f(fmaf(s[2 * c], p.scale_log2, nb));
-            const float p1 = ex2f(fmaf(s[2 * c + 1], p.scale_log2, nb));
-            rs[c & 3] += p0 + p1;
-            const __half2 hh = __floats2half2_rn(p0, p1);
-            pk[c] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&hh));
-          }
+            for (int c = 0; c < 32; c++) {
+              const float2 x = fma2(make_float2(s[2 * c], s[2 * c + 1]), sc, nb2);
+              const float2 e = make_float2(ex2f(x.x), ex2f(x.y));
+              mv[c & 3] = fmaxf(mv[c & 3], fmaxf(s[2 * c], s[2 * c + 1]));
+              if (c & 1) sum1 = add2(sum1, e);
+              else sum = add2(sum, e);
+              const __half2 hh = __floats2half2_rn(e.x, e.y);
+              pk[c] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&hh));
+            }
+            const float mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * p.scale_log2;
+            const bool up = mx > m + RESCALE_LOG2;
+            again = __any_sync(0xffffffffu, up);
+            if (again) {
+              const float alpha = up ? ex2f(m - mx) : 1.f;  // 0 while m is -inf
+              if (turn != first_turn) {
+                // O is rescaled once the P V of the group's last turn is in it
+                if (!turn_done(g, turn - 1)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+#pragma unroll 1
+                for (int c = 0; c < 8; c++) {
+                  float ov[16];
+                  tmem_ld16(tmem_o + g * HD + c * 16, ov);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int i = 0; i < 16; i++) ov[i] *= alpha;
+                  tmem_st16(tmem_o + g * HD + c * 16, ov);
+                }
+              }
+              l *= alpha;
+              if (up) m = mx;
+            }
+          } while (again);
+          if (!ok) break;
           tmem_st32(tmem_s, pk);
-          l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+          l += (sum.x + sum.y) + (sum1.x + sum1.y);
           tmem_st_wait();
         }
         if (tail) {  // V rows with NaN or infinities, found by the V producer
-          if (!warp_wait(bar + 8 * (B_VFULL + rv.i), rv.phase, abort_flag, err)) {
+          const uint32_t n = n0 + j;
+          if (!warp_wait(bar + 8 * (B_VFULL + n % NV), (n / NV) & 1, abort_flag, err)) {
             ok = false;
             break;
           }
-          bad |= vbad[rv.i];
+          bad |= vbad[n % NV];
         }
-        rv.next();
         tc_fence_before();
         mbar_arrive(bar + 8 * (B_PFULL + 2 * g + buf));
       }
+      n0 += w.nb;
       if (!ok) break;
 
       // ---- the piece's end: O of the tile (two), or of both groups' halves
@@ -911,49 +974,78 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 // Joins the partials of the unit that ends in CTA blockIdx.x's range, in CTA
 // order (deterministic): M = max m, O = sum O_c 2^(m_c - M) / sum l_c 2^(m_c - M).
-// A block has 8 rows: thread (row, column quad).
+// A block has 8 rows of a tile, a thread one row's column quad.  The rows'
+// (m, l) of all pieces are fetched at once and become weights in shared
+// memory; the O terms are then independent loads, 8 in flight per thread.
 constexpr uint32_t MERGE_ROWS = 8;
 __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ TParams p) {
+  __shared__ float2 w[(MAX_CTAS + 1) * MERGE_ROWS];  // (m, l), then (weight, weighted l); last 1 / L
   nwd::pdl_trigger();
   nwd::pdl_wait();
-  const uint32_t c = blockIdx.x, last = c;
-  const MergeDesc d = reinterpret_cast<const MergeDesc*>(p.ws + WS_DESC)[c];
+  const MergeDesc d = reinterpret_cast<const MergeDesc*>(p.ws + WS_DESC)[blockIdx.x];
   if (!d.valid) return;
+  const uint32_t first = d.first, n = blockIdx.x - d.first + 1;
   const Unit un = unit_of(p, d.u);
   const uint32_t t = blockIdx.y / (BM / MERGE_ROWS);
-  const uint32_t row = blockIdx.y % (BM / MERGE_ROWS) * MERGE_ROWS + (threadIdx.x & 7);
-  const uint32_t quad = threadIdx.x >> 3;
-  if (t >= un.tiles) return;
-  const uint32_t tile = un.tile0 + t, node = tile * p.tile_nodes + row / p.group;
-  if (row >= min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes) * p.group) return;
+  const uint32_t row0 = blockIdx.y % (BM / MERGE_ROWS) * MERGE_ROWS;
+  const uint32_t tile = un.tile0 + t;
+  const uint32_t rows = tile < p.n_tiles
+                            ? min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes) * p.group
+                            : 0;
+  if (t >= un.tiles || row0 >= rows) return;
+  const TreeSeq s = load_seq(p, d.b, nullptr);
   const float2* ml = reinterpret_cast<const float2*>(p.ws + WS_ML);
   const float4* po = reinterpret_cast<const float4*>(p.ws + ws_o(gridDim.x, p.unit_tiles));
   // the unit's first piece is the one its CTA ended with, the others begin theirs
   auto slot = [&](uint32_t i) {
-    return ((i * 2 + (i == d.first ? 1 : 0)) * p.unit_tiles + t) * BM;
+    return (((first + i) * 2 + (i == 0 ? 1 : 0)) * p.unit_tiles + t) * BM;
   };
-  float M = -INFINITY;
-  for (uint32_t i = d.first; i <= last; i++) M = fmaxf(M, ml[slot(i) + row].x);
-  float L = 0.f;
+  for (uint32_t i = threadIdx.x; i < n * MERGE_ROWS; i += 256)
+    w[i] = ml[slot(i / MERGE_ROWS) + row0 + i % MERGE_ROWS];
+  __syncthreads();
+  if (threadIdx.x < MERGE_ROWS * 32) {  // a warp per row
+    const uint32_t r = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float M = -INFINITY, L = 0.f;
+    for (uint32_t i = lane; i < n; i += 32) M = fmaxf(M, w[i * MERGE_ROWS + r].x);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    for (uint32_t i = lane; i < n; i += 32) {
+      const float2 a = w[i * MERGE_ROWS + r];
+      // a piece without weights counts for nothing (l may be NaN)
+      const float e = a.y != 0.f ? ex2f(a.x - M) : 0.f;
+      const float l = a.y != 0.f ? a.y * e : 0.f;
+      w[i * MERGE_ROWS + r] = make_float2(e, l);
+      L += l;
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+    if (lane == 0) w[n * MERGE_ROWS + r].x = L != 0.f ? 1.f / L : 0.f;
+  }
+  __syncthreads();
+  const uint32_t r = threadIdx.x & 7, row = row0 + r, quad = threadIdx.x >> 3;
+  const uint32_t node = tile * p.tile_nodes + row / p.group;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (uint32_t i = d.first; i <= last; i++) {
-    const float2 a = ml[slot(i) + row];
-    const float4 x = po[(size_t)slot(i) * (HD / 4) + quad * BM + row];
-    if (a.y != 0.f) {
-      const float w = ex2f(a.x - M);
-      L += a.y * w;
-      o.x += x.x * w;
-      o.y += x.y * w;
-      o.z += x.z * w;
-      o.w += x.w * w;
+  for (uint32_t i0 = 0; i0 < n; i0 += 8) {
+    float4 x[8];
+#pragma unroll
+    for (uint32_t k = 0; k < 8; k++)
+      if (i0 + k < n) x[k] = __ldcg(po + (size_t)slot(i0 + k) * (HD / 4) + quad * BM + row);
+#pragma unroll
+    for (uint32_t k = 0; k < 8; k++) {
+      const float e = i0 + k < n ? w[(i0 + k) * MERGE_ROWS + r].x : 0.f;
+      if (e != 0.f) {
+        o.x += x[k].x * e;
+        o.y += x[k].y * e;
+        o.z += x[k].z * e;
+        o.w += x[k].w * e;
+      }
     }
   }
-  const TreeSeq s = load_seq(p, d.b, nullptr);
-  const float inv = L != 0.f && node < s.nodes ? 1.f / L : 0.f;
+  if (row >= rows) return;
+  const float inv = w[n * MERGE_ROWS + r].x;
   const bool none = node >= s.nodes;
-  __half2 h[2] = {__floats2half2_rn(none ? 0.f : o.x * inv, none ? 0.f : o.y * inv),
-                  __floats2half2_rn(none ? 0.f : o.z * inv, none ? 0.f : o.w * inv)};
+  const __half2 h[2] = {__floats2half2_rn(none ? 0.f : o.x * inv, none ? 0.f : o.y * inv),
+                        __floats2half2_rn(none ? 0.f : o.z * inv, none ? 0.f : o.w * inv)};
   *reinterpret_cast<uint2*>(p.o + (((size_t)d.b * p.n_nodes + node) * p.n_heads +
                                    un.hkv * p.group + row % p.group) * HD + quad * 4) =
       *reinterpret_cast<const uint2*>(h);

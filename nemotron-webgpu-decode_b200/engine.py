@@ -239,7 +239,7 @@ def commit_layers(layers, path, n_accepted, stream=None) -> None:
 
     def run(raw):
         ops.kv_commit(pools, first.row_offset, first.lengths, path, n_accepted,
-                      scratch=first.scratch, stream=stream)
+                      scratch=first.scratch)
         for layer in layers:
             layer.lengths += n_accepted
 

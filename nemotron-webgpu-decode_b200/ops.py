@@ -373,16 +373,18 @@ def q4_qkv_append(h: torch.Tensor, wq: Q4Weights, wk: Q4Weights, wv: Q4Weights,
 
 # ---------------------------------------------------------------- speculative decoding
 
-def _same_device(device, named) -> None:
-    for name, t in named:
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not on {device}")
-
-
-def _shaped(t, dtype, shape, name) -> int:
-    if t.shape != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    return _ptr(t, dtype, name)
+def _dev_ptr(t, dtype, shape, device, name) -> int:
+    """The pointer of a contiguous tensor of this type, shape and (CUDA) device."""
+    try:
+        if (t.dtype is dtype and t.shape == shape and t.device == device
+                and device.type == "cuda" and t.is_contiguous()):
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _ptr(t, dtype, name)
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
 class TreeWorkspace:
@@ -416,61 +418,56 @@ def _tree_ws_bytes(device: int, *shape) -> int:
     return n
 
 
-def _on(device, stream, fn):
-    """fn(raw stream) with `device` current and, for a given stream, PyTorch's allocations
-    on it: what the call allocates belongs to the stream that uses it."""
+def _on(device, stream, fn, *args):
+    """fn(raw stream, *args) with `device` current and, for a given stream, PyTorch's
+    allocations on it: what the call allocates belongs to the stream that uses it."""
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _on(device, stream, fn)
+            return _on(device, stream, fn, *args)
     if stream is None:
-        return fn(torch.cuda.current_stream(device).cuda_stream)
+        return fn(torch._C._cuda_getCurrentRawStream(device.index), *args)
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
     with torch.cuda.stream(stream):
-        return fn(stream.cuda_stream)
+        return fn(stream.cuda_stream, *args)
+
+
+def _run_tree(raw, name, args, shape, workspace, scratch, device):
+    err = None if scratch is None else scratch.ptr
+    if workspace is not None:
+        call(name, *args, workspace.ptr, workspace.nbytes, err, raw)
+        return
+    nbytes = _tree_ws_bytes(device.index, *shape)
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    call(name, *args, buf.data_ptr(), nbytes, err, raw)
 
 
 def _attention_tree(name, q, new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads,
                     n_kv_heads, head_dim, tree_len, scale, workspace, scratch, stream):
-    dev = q.device
-    _same_device(dev, (("k_pool", k_pool), ("v_pool", v_pool), ("row_offset", row_offset),
-                       ("seq_len", seq_len), ("parents", parents), ("tree_len", tree_len), ("o", o)))
+    dev, f16, i32 = q.device, torch.float16, torch.int32
     if parents.dim() != 2:
         raise ValueError(f"parents must be [batch, n_nodes], got {tuple(parents.shape)}")
-    batch, n = parents.shape
-    row = n_kv_heads * head_dim
-    qo = (batch, n, n_heads, head_dim)
-    qp = _shaped(q, torch.float16, qo, "q")
-    op = _shaped(o, torch.float16, qo, "o")
-    if row == 0 or k_pool.numel() % row or v_pool.numel() != k_pool.numel():
-        raise ValueError("k_pool and v_pool must hold the same whole number of rows")
-    args = [qp]
+    bn = parents.shape
+    batch, n = bn
+    row, qo, b1 = n_kv_heads * head_dim, (batch, n, n_heads, head_dim), (batch,)
+    args = [_dev_ptr(q, f16, qo, dev, "q")]
     if new is not None:
-        _same_device(dev, (("k_new", new[0]), ("v_new", new[1])))
         kv = (batch, n, n_kv_heads, head_dim)
-        args += [_shaped(new[0], torch.float16, kv, "k_new"),
-                 _shaped(new[1], torch.float16, kv, "v_new")]
-    args += [_h(k_pool, "k_pool"), _h(v_pool, "v_pool"), k_pool.numel() // row,
-             _shaped(row_offset, torch.int64, (batch,), "row_offset"),
-             _shaped(seq_len, torch.int32, (batch,), "seq_len" if new is None else "pos"),
-             _ptr(parents, torch.int32, "parents"),
-             None if tree_len is None else _shaped(tree_len, torch.int32, (batch,), "tree_len"),
-             op, batch, n, n_heads, n_kv_heads, head_dim, float(scale)]
-    err = None
-    if scratch is not None:
-        err = scratch.ptr
-
-    def run(raw):
-        ws, buf = workspace, None
-        if ws is None:
-            nbytes = _tree_ws_bytes(dev.index, batch, n, n_heads, n_kv_heads, head_dim)
-            buf = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            call(name, *args, buf.data_ptr(), nbytes, err, raw)
-        else:
-            call(name, *args, ws.ptr, ws.nbytes, err, raw)
-        return o
-
-    return _on(dev, stream, run)
+        args += [_dev_ptr(new[0], f16, kv, dev, "k_new"), _dev_ptr(new[1], f16, kv, dev, "v_new")]
+    pool = k_pool.shape
+    rows = k_pool.numel() // row if row else 0
+    if rows * row != k_pool.numel() or v_pool.numel() != rows * row:
+        raise ValueError("k_pool and v_pool must hold the same whole number of rows")
+    args += [_dev_ptr(k_pool, f16, pool, dev, "k_pool"),
+             _dev_ptr(v_pool, f16, v_pool.shape, dev, "v_pool"), rows,
+             _dev_ptr(row_offset, torch.int64, b1, dev, "row_offset"),
+             _dev_ptr(seq_len, i32, b1, dev, "seq_len" if new is None else "pos"),
+             _dev_ptr(parents, i32, bn, dev, "parents"),
+             None if tree_len is None else _dev_ptr(tree_len, i32, b1, dev, "tree_len"),
+             _dev_ptr(o, f16, qo, dev, "o"), batch, n, n_heads, n_kv_heads, head_dim, scale]
+    _on(dev, stream, _run_tree, name, args, (batch, n, n_heads, n_kv_heads, head_dim), workspace,
+        scratch, dev)
+    return o
 
 
 def attention_tree(q, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads: int,
@@ -510,37 +507,33 @@ def verify_tree(tokens, parents, target_probs, u, w, draft_probs=None, tree_len=
     i: the target behind node i); draft_probs of the same shape (row i: what node i's
     children were drawn from) or None for drafts without probabilities; u [B, N], w [B] f32
     uniforms in [0, 1).  `out`: the three outputs, to be written in place."""
-    dev = target_probs.device
-    _same_device(dev, (("tokens", tokens), ("parents", parents), ("u", u), ("w", w),
-                       ("draft_probs", draft_probs), ("tree_len", tree_len)))
+    dev, i32, f32 = target_probs.device, torch.int32, torch.float32
     if target_probs.dim() != 3:
         raise ValueError("target_probs must be [batch, n_nodes, vocab], got "
                          f"{tuple(target_probs.shape)}")
     shape = target_probs.shape
     batch, n, vocab = shape
     bn, b1 = (batch, n), (batch,)
-    args = [_shaped(tokens, torch.int32, bn, "tokens"), _shaped(parents, torch.int32, bn, "parents"),
-            None if tree_len is None else _shaped(tree_len, torch.int32, b1, "tree_len"),
-            _ptr(target_probs, torch.float32, "target_probs"),
-            None if draft_probs is None else _shaped(draft_probs, torch.float32, shape,
-                                                     "draft_probs"),
-            _shaped(u, torch.float32, bn, "u"), _shaped(w, torch.float32, b1, "w")]
-    err = None if scratch is None else scratch.ptr
+    args = (_dev_ptr(tokens, i32, bn, dev, "tokens"), _dev_ptr(parents, i32, bn, dev, "parents"),
+            None if tree_len is None else _dev_ptr(tree_len, i32, b1, dev, "tree_len"),
+            _dev_ptr(target_probs, f32, shape, dev, "target_probs"),
+            None if draft_probs is None else _dev_ptr(draft_probs, f32, shape, dev, "draft_probs"),
+            _dev_ptr(u, f32, bn, dev, "u"), _dev_ptr(w, f32, b1, dev, "w"))
+    if out is not None:
+        path, n_accepted, next_token = out
+        _dev_ptr(path, i32, bn, dev, "path")
+        _dev_ptr(n_accepted, i32, b1, dev, "n_accepted")
+        _dev_ptr(next_token, i32, b1, dev, "next_token")
+        out = (path, n_accepted, next_token)
+    return _on(dev, stream, _run_verify, args, bn, vocab, out, scratch, tokens)
 
-    def run(raw):
-        res = out
-        if res is None:
-            res = (torch.empty(bn, dtype=torch.int32, device=dev),
-                   torch.empty(b1, dtype=torch.int32, device=dev),
-                   torch.empty(b1, dtype=torch.int32, device=dev))
-        else:
-            _same_device(dev, (("path", res[0]), ("n_accepted", res[1]), ("next_token", res[2])))
-        call("nwd_verify_tree", *args, _shaped(res[0], torch.int32, bn, "path"),
-             _shaped(res[1], torch.int32, b1, "n_accepted"),
-             _shaped(res[2], torch.int32, b1, "next_token"), batch, n, vocab, err, raw)
-        return tuple(res)
 
-    return _on(dev, stream, run)
+def _run_verify(raw, args, bn, vocab, out, scratch, tokens):
+    if out is None:
+        out = tokens.new_empty(bn), tokens.new_empty(bn[0]), tokens.new_empty(bn[0])
+    call("nwd_verify_tree", *args, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), *bn,
+         vocab, None if scratch is None else scratch.ptr, raw)
+    return out
 
 
 def kv_commit(pools, row_offset, pos, path, n_accepted, scratch: Scratch | None = None,
@@ -550,35 +543,31 @@ def kv_commit(pools, row_offset, pos, path, n_accepted, scratch: Scratch | None 
     n_accepted[b], in every pool of `pools` (K and V of several layers, each [rows, n_kv, hd]
     fp16, 16 per launch).  path / n_accepted as :func:`verify_tree` returns them; the
     caller's lengths grow by n_accepted."""
-    pools = list(pools)
     if path.dim() != 2:
         raise ValueError(f"path must be [batch, n_nodes], got {tuple(path.shape)}")
-    batch, n = path.shape
-    dev = path.device
-    _same_device(dev, (("row_offset", row_offset), ("pos", pos), ("n_accepted", n_accepted)))
-    args = (_shaped(row_offset, torch.int64, (batch,), "row_offset"),
-            _shaped(pos, torch.int32, (batch,), "pos"), _ptr(path, torch.int32, "path"),
-            _shaped(n_accepted, torch.int32, (batch,), "n_accepted"))
+    bn = path.shape
+    dev, i32, b1 = path.device, torch.int32, (bn[0],)
+    args = (_dev_ptr(row_offset, torch.int64, b1, dev, "row_offset"),
+            _dev_ptr(pos, i32, b1, dev, "pos"), _dev_ptr(path, i32, bn, dev, "path"),
+            _dev_ptr(n_accepted, i32, b1, dev, "n_accepted"), *bn)
+    pools = list(pools)
     if not pools:
         return
     shape = pools[0].shape
     if len(shape) != 3:
         raise ValueError(f"pools must be [rows, n_kv, hd], got {tuple(shape)}")
-    ptrs = []
-    for i, t in enumerate(pools):
-        _same_device(dev, ((f"pool {i}", t),))
-        ptrs.append(_shaped(t, torch.float16, shape, f"pool {i}"))
+    ptrs = [_dev_ptr(t, torch.float16, shape, dev, "pool") for t in pools]
     if len(set(ptrs)) != len(ptrs):
         raise ValueError("pools must differ from one another")
+    _on(dev, stream, _run_commit, ptrs, shape, args, scratch)
+
+
+def _run_commit(raw, ptrs, shape, args, scratch):
     err = None if scratch is None else scratch.ptr
-
-    def run(raw):
-        for i in range(0, len(ptrs), 16):
-            part = ptrs[i:i + 16]
-            call("nwd_kv_commit", (ctypes.c_void_p * len(part))(*part), len(part), shape[0], *args,
-                 batch, n, shape[1], shape[2], err, raw)
-
-    _on(dev, stream, run)
+    for i in range(0, len(ptrs), 16):
+        part = ptrs[i:i + 16]
+        call("nwd_kv_commit", (ctypes.c_void_p * len(part))(*part), len(part), shape[0], *args,
+             shape[1], shape[2], err, raw)
 
 
 def selftest_wait_timeout(workspace: "Workspace", stream=None) -> int:

@@ -99,7 +99,7 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
         bar("P", 2 * g, 2), bar("P", 2 * g + 1, 2), bar("OE", g, 4), bar("ML", g, 2)  # two threads stand for a group's 128
     q, k, v = [None] * NQ, [None] * NK, [None] * NV
     s_buf, o_buf, log = [None] * 4, [None, None], []
-    mmas = [[], []]  # issued by the group's issuer, not yet run, in order
+    mmas = [[], [], [], []]  # issued by an issuer, not yet run, in order
 
     def wait(b, parity):
         while not b.passed(parity):
@@ -140,9 +140,9 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
             x0, q0, n0 = x0 + nb * tiles, q0 + tiles, n0 + nb
         return out
 
-    def issuer(g):
+    def issuer(g, kind):
         turns = turns_of(g)
-        mma = mmas[g]
+        mma = mmas[2 * g + (kind == "PV")]
         seen = dict(Q=0, K=0, V=0)
 
         def see(name, slots, upto):
@@ -156,52 +156,45 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
                     bar(name + "E", i).arrive()
                 seen[name] += 1
 
-        def release(name, i):
-            mma.append(bar(name, i).arrive)
-
-        def issue_s(y):
-            n, j, t, first, last, qn, kn = turns[y]
-            buf = 2 * g + (y & 1)
-            nb, tiles = plan[n]
-            qi, ki = qn % NQ, kn % NK
-            if first:
-                yield from see("Q", NQ, qn)
-            yield from see("K", NK, kn)
-
-            def run():
-                assert q[qi] == (n, t) and k[ki] == (n, j)
-                s_buf[buf] = ("S", n, j, t)
-            mma.append(run)
-            mma.append(lambda: bar("S", buf).arrive())
-            release("KE", ki)
-            if last:
-                release("QE", qi)
-
         ou = 0
-        for y in range(min(2, len(turns))):
-            yield from issue_s(y)
-        for x, (n, j, t, first, last, _, vn) in enumerate(turns):
-            vi = vn % NV
-            if first:
-                yield from wait(bar("OE", g), (ou & 1) ^ 1)
-            yield from see("V", NV, vn)
+        for x, (n, j, t, first, last, qn, kn) in enumerate(turns):
             buf = 2 * g + (x & 1)
-            yield from wait(bar("P", buf), x >> 1 & 1)
-
-            def run(n=n, j=j, t=t, vi=vi, first=first, buf=buf):
-                assert s_buf[buf] == ("P", n, j, t) and v[vi] == (n, j)
+            if kind == "S":
+                qi, ki = qn % NQ, kn % NK
                 if first:
-                    assert o_buf[g] is None, "accumulator not read yet"
-                    o_buf[g] = (n, [])
-                assert o_buf[g][0] == n
-                o_buf[g][1].append((j, t))
-                log.append((n, j, t))
-            mma.append(run)
-            mma.append(lambda buf=buf: bar("PV", buf).arrive())
-            release("VE", vi)
-            ou += last
-            if x + 2 < len(turns):
-                yield from issue_s(x + 2)
+                    yield from see("Q", NQ, qn)
+                yield from see("K", NK, kn)
+                yield from wait(bar("PV", buf), (x >> 1 & 1) ^ 1)
+
+                def run(n=n, j=j, t=t, qi=qi, ki=ki, buf=buf):
+                    assert q[qi] == (n, t) and k[ki] == (n, j)
+                    assert s_buf[buf] in (None, "free")
+                    s_buf[buf] = ("S", n, j, t)
+                mma.append(run)
+                mma.append(bar("S", buf).arrive)
+                mma.append(bar("KE", ki).arrive)
+                if last:
+                    mma.append(bar("QE", qi).arrive)
+            else:
+                vi = kn % NV
+                if first:
+                    yield from wait(bar("OE", g), (ou & 1) ^ 1)
+                yield from see("V", NV, kn)
+                yield from wait(bar("P", buf), x >> 1 & 1)
+
+                def run(n=n, j=j, t=t, vi=vi, first=first, buf=buf):
+                    assert s_buf[buf] == ("P", n, j, t) and v[vi] == (n, j)
+                    s_buf[buf] = "free"
+                    if first:
+                        assert o_buf[g] is None, "accumulator not read yet"
+                        o_buf[g] = (n, [])
+                    assert o_buf[g][0] == n
+                    o_buf[g][1].append((j, t))
+                    log.append((n, j, t))
+                mma.append(run)
+                mma.append(bar("PV", buf).arrive)
+                mma.append(bar("VE", vi).arrive)
+                ou += last
 
     read = {}
 
@@ -295,7 +288,8 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
                     bar("VF", i).arrive()
                 state["v"] += 1
 
-    roles = [issuer(0), issuer(1), load("K", NK, k, kv), v_and_q()]
+    roles = [issuer(g, kind) for g in range(2) for kind in ("S", "PV")]
+    roles += [load("K", NK, k, kv), v_and_q()]
     roles += [softmax(g, th) for g in range(2) for th in range(2)]
     tc, cp = tensor_core(), copies()
     idle = 0
