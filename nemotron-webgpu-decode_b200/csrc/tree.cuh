@@ -46,22 +46,35 @@ struct TreeSeq {
   int64_t row0;
   uint32_t ctx, nodes;
 };
-static __device__ __forceinline__ TreeSeq tree_seq(const int64_t* row_offset,
+struct TreeRaw {
+  int64_t row_offset;
+  int32_t seq_len, tree_len;
+};
+static __device__ __forceinline__ TreeRaw tree_raw(const int64_t* row_offset,
                                                    const int32_t* seq_len, const int32_t* tree_len,
-                                                   uint64_t pool_rows, uint32_t b, uint32_t n,
-                                                   uint32_t* err) {
+                                                   uint32_t b, uint32_t n) {
+  return TreeRaw{row_offset[b], seq_len[b], tree_len ? tree_len[b] : (int32_t)n};
+}
+static __device__ __forceinline__ TreeSeq tree_seq(const TreeRaw& raw, uint64_t pool_rows,
+                                                   uint32_t n, uint32_t* err) {
   TreeSeq s;
-  s.row0 = row_offset[b];
-  const int32_t ctx = seq_len[b];
-  s.nodes = tree_nodes(tree_len, b, n, err);
-  s.ctx = (uint32_t)ctx;
-  if (s.row0 < 0 || ctx < 0 || (uint64_t)s.row0 > pool_rows ||
-      (uint64_t)ctx + s.nodes > pool_rows - (uint64_t)s.row0) {
+  s.row0 = raw.row_offset;
+  s.ctx = (uint32_t)raw.seq_len;
+  s.nodes = min((uint32_t)max(raw.tree_len, 0), n);
+  if ((uint32_t)raw.tree_len > n && err) atomicOr(err, NWD_DEVERR_TREE);
+  if (s.row0 < 0 || raw.seq_len < 0 || (uint64_t)s.row0 > pool_rows ||
+      (uint64_t)s.ctx + s.nodes > pool_rows - (uint64_t)s.row0) {
     if (err) atomicOr(err, NWD_DEVERR_ROW_RANGE);
     s.row0 = 0;
     s.ctx = s.nodes = 0;
   }
   return s;
+}
+static __device__ __forceinline__ TreeSeq tree_seq(const int64_t* row_offset,
+                                                   const int32_t* seq_len, const int32_t* tree_len,
+                                                   uint64_t pool_rows, uint32_t b, uint32_t n,
+                                                   uint32_t* err) {
+  return tree_seq(tree_raw(row_offset, seq_len, tree_len, b, n), pool_rows, n, err);
 }
 
 }  // namespace nwd

@@ -15,25 +15,30 @@
 // persistent CTA (one per SM); a unit that a cut divides leaves one partial
 // (m, l, O) per CTA in the workspace, which merge_kernel joins in order.
 //
-// A CTA's 16 warps:
+// A CTA's 20 warps:
 //   warps 0, 1    TMA producers: K blocks into 5 stages; V blocks into 5 and
 //                 each unit's Q tiles into 2 (as 64-column chunks, 128-byte
 //                 swizzle: the K-major operand layout).  Warp 0 also owns the
-//                 tensor memory; warps 2, 3 are idle.
+//                 tensor memory.
+//   warps 2, 3    make V blocks with rows of the tree, or behind it, fit to
+//                 multiply (below).
 //   warps 4 - 7   MMA issuers: S of softmax group 0, of group 1, P V of group
 //                 0, of group 1.  A turn is S = Q K^T of one (block, tile) and
 //                 O += P V after its softmax; S runs two turns ahead into the
 //                 other of the group's two score buffers, so the softmax of a
-//                 turn does not wait for the P V of the one before it.  An
-//                 issuer's waits, descriptors and commits are a chain of some
-//                 hundred dependent instructions per turn, longer than the
-//                 MMAs that it issues: hence four.
+//                 turn does not wait for the P V of the one before it.
 //   warps 8-11, 12-15  the softmax groups, a thread per query row, each with
 //                 its own score buffers and output accumulator (all 512
 //                 columns).  A unit of two tiles gives each group a tile and
 //                 both use every K/V block; a unit of one tile gives the
-//                 groups alternate blocks and joins their (m, l, O) at its
-//                 end, which keeps both busy when there are few query rows.
+//                 groups alternate blocks, which keeps both busy when there
+//                 are few query rows.
+//   warps 16-19   the epilogue: a unit's O out of tensor memory, joined over
+//                 the two groups where they shared its tile, normalised and
+//                 stored (or left as a partial), while the softmax groups are
+//                 at the next unit.  (With the epilogue in the softmax warps a
+//                 unit's end cost 5-6 us of a loop that takes 0.6 us per
+//                 block.)
 //
 // Softmax in the log2 domain with a lazily moved maximum (O is rescaled in
 // tensor memory only when a row's maximum grows by more than 2^8).  P is
@@ -70,14 +75,16 @@ using nwd::TreeSeq;
 constexpr uint32_t HD = 128;
 constexpr uint32_t BM = 128;            // query rows per tile
 constexpr uint32_t BN = 64;             // cache rows per block
-constexpr int THREADS = 512;
+constexpr int THREADS = 640;
+constexpr int LAUNCH_REGS = 96;         // what __launch_bounds__ gives 640 threads
 constexpr uint32_t Q_CHUNK = BM * 128;  // rows x 64 fp16
 constexpr uint32_t Q_TILE = 2 * Q_CHUNK;
 constexpr uint32_t CHUNK = BN * 128;
 constexpr uint32_t TILE = 2 * CHUNK;    // a K or V block: 16 KiB
 constexpr uint32_t NQ = 2, NK = 5, NV = 5;  // stages
 constexpr uint32_t MAX_GROUPS32 = 128;  // batch / 32
-constexpr uint32_t MIN_BLOCKS = 1;      // least blocks per CTA range
+// what a block costs in a unit of one tile, of two (in the same unit of time)
+constexpr uint32_t COST1 = 1, COST2 = 2;
 
 constexpr uint32_t O_Q = 0;
 constexpr uint32_t O_K = O_Q + NQ * Q_TILE;
@@ -88,12 +95,12 @@ constexpr int B_QFULL = 0, B_QEMPTY = B_QFULL + NQ, B_KFULL = B_QEMPTY + NQ,
               B_KEMPTY = B_KFULL + NK, B_VFULL = B_KEMPTY + NK, B_VEMPTY = B_VFULL + NV,
               B_VTMA = B_VEMPTY + NV,
               // by 2 * softmax group + score buffer
-    B_SFULL = B_VTMA + 1, B_PFULL = B_SFULL + 4, B_PVDONE = B_PFULL + 4,
+    B_SFULL = B_VTMA + NV, B_PFULL = B_SFULL + 4, B_PVDONE = B_PFULL + 4,
               // by softmax group
     B_OEMPTY = B_PVDONE + 4, B_ML = B_OEMPTY + 2, B_DRAIN = B_ML + 2, NBAR = B_DRAIN + 1;
 constexpr uint32_t O_PLAN = (O_BAR + NBAR * 8 + 15) / 16 * 16;  // Plan
-constexpr uint32_t O_VBAD = O_PLAN + 48;          // [NV] u64: tree rows with NaN or inf in V
-constexpr uint32_t O_GBAD = O_VBAD + NV * 8;      // [2] u64: the same, gathered per group
+constexpr uint32_t O_VBAD = O_PLAN + 48;          // [NV][2] u64: tree rows with NaN or inf in V
+constexpr uint32_t O_GBAD = O_VBAD + NV * 16;      // [2] u64: the same, gathered per group
 constexpr uint32_t O_MISC = O_GBAD + 16;          // tensor memory base, abort flag
 constexpr uint32_t SMEM_USED = O_MISC + 16;
 // dynamic shared memory starts 1024-byte aligned (there is no static shared
@@ -121,11 +128,13 @@ struct TParams {
   uint64_t pool_rows;
   uint32_t batch, n_nodes, n_heads, n_kv, group;
   uint32_t tile_nodes, n_tiles, unit_tiles, n_units;  // n_units: per sequence
+  uint32_t min_cost;                 // least cost of a CTA's range
+  uint32_t cost1, cost2, head_cost;  // of a block of a unit of one tile, of two, of all of a head's
   float scale_log2;
 };
 
 struct Plan {
-  uint64_t left;  // blocks of this CTA's range
+  int64_t left;  // of this CTA's range, from the first piece on
   uint32_t b, u, blk;
   uint32_t pad[5];
 };
@@ -169,38 +178,6 @@ __device__ __forceinline__ bool elect_one() {
   return is != 0;
 }
 
-// The pieces of a CTA's range: blocks [blk, blk + nb) of unit u of sequence b.
-struct Pieces {
-  uint64_t left;
-  uint32_t b, u, blk, nb, nblk;
-  TreeSeq s;
-  __device__ __forceinline__ void load(const TParams& p) {
-    s = load_seq(p, b, nullptr);
-    nblk = uniform(seq_blocks(s));
-  }
-  __device__ __forceinline__ bool begin(const TParams& p, const Plan& plan) {
-    left = (uint64_t)uniform((uint32_t)(plan.left >> 32)) << 32 | uniform((uint32_t)plan.left);
-    b = uniform(plan.b);
-    u = uniform(plan.u);
-    blk = uniform(plan.blk);
-    if (left == 0) return false;
-    load(p);
-    nb = (uint32_t)min((uint64_t)(nblk - blk), left);
-    return true;
-  }
-  __device__ __forceinline__ bool next(const TParams& p) {
-    left -= nb;
-    if (left == 0) return false;
-    blk = 0;
-    if (++u == p.n_units) {
-      u = 0;
-      b++;
-      load(p);
-    }
-    nb = (uint32_t)min((uint64_t)nblk, left);
-    return true;
-  }
-};
 // A unit's kv head, first tile and number of tiles.
 struct Unit {
   uint32_t hkv, tile0, tiles;
@@ -214,6 +191,52 @@ __device__ __forceinline__ Unit unit_of(const TParams& p, uint32_t u) {
   return r;
 }
 
+// The pieces of a CTA's range: blocks [blk, blk + nb) of unit u of sequence b.
+// The line that is cut into ranges is as long as the blocks' costs; a cut
+// inside a block gives the block to the CTA before the cut.
+struct Pieces {
+  int64_t left;
+  uint32_t b, u, blk, nb, nblk, cost;
+  TreeSeq s;
+  Unit un;
+  nwd::TreeRaw ahead;  // sequence b + 1's entries, on their way since sequence b was entered
+  __device__ __forceinline__ void load(const TParams& p) {
+    s = nwd::tree_seq(ahead, p.pool_rows, p.n_nodes, nullptr);
+    nblk = uniform(seq_blocks(s));
+    if (b + 1 < p.batch) ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, b + 1, p.n_nodes);
+  }
+  __device__ __forceinline__ void enter(const TParams& p) {
+    un = unit_of(p, u);
+    cost = un.tiles == 2 ? p.cost2 : p.cost1;
+    const uint64_t most = (uint64_t)(nblk - blk) * cost;
+    nb = (uint64_t)left >= most ? nblk - blk : ((uint32_t)left + cost - 1) / cost;
+  }
+  __device__ __forceinline__ bool begin(const TParams& p, const Plan& plan) {
+    left = (int64_t)((uint64_t)uniform((uint32_t)((uint64_t)plan.left >> 32)) << 32 |
+                     uniform((uint32_t)plan.left));
+    b = uniform(plan.b);
+    u = uniform(plan.u);
+    blk = uniform(plan.blk);
+    if (left <= 0) return false;
+    ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, b, p.n_nodes);
+    load(p);
+    enter(p);
+    return true;
+  }
+  __device__ __forceinline__ bool next(const TParams& p) {
+    left -= (int64_t)nb * cost;
+    if (left <= 0) return false;
+    blk = 0;
+    if (++u == p.n_units) {
+      u = 0;
+      b++;
+      load(p);
+    }
+    enter(p);
+    return true;
+  }
+};
+
 // Position in a ring of N stages.
 template <uint32_t N>
 struct Ring {
@@ -223,6 +246,11 @@ struct Ring {
       i = 0;
       phase ^= 1u;
     }
+  }
+  __device__ __forceinline__ void add(uint32_t n) {
+    i += n;
+    phase ^= (i / N) & 1u;
+    i %= N;
   }
 };
 
@@ -237,7 +265,7 @@ struct Own {
   // the piece's first turn of group g, or the next piece's that has one
   __device__ __forceinline__ bool settle(const TParams& p, uint32_t g) {
     for (;;) {
-      two = unit_of(p, w.u).tiles == 2;
+      two = w.un.tiles == 2;
       const uint32_t mine = (g - x0) & 1;  // two tiles: the tile; one: the first block
       j = two ? 0 : mine;
       if (j < w.nb) {
@@ -326,14 +354,14 @@ __device__ void make_plan(const TParams& p, uint64_t* sums, Plan* plan, MergeDes
       const uint64_t y = __shfl_up_sync(0xffffffffu, incl, i);
       if ((int)lane >= i) incl += y;
     }
-    const uint64_t total = __shfl_sync(0xffffffffu, incl, 31) * p.n_units;
-    const uint64_t per = max(div_small(total + gridDim.x - 1, gridDim.x), (uint64_t)MIN_BLOCKS);
+    const uint32_t seq_cost = p.n_kv * p.head_cost;  // of a sequence per block of its length
+    const uint64_t total = __shfl_sync(0xffffffffu, incl, 31) * seq_cost;
+    const uint64_t per = max(div_small(total + gridDim.x - 1, gridDim.x), (uint64_t)p.min_cost);
     const uint64_t x0 = min(total, (uint64_t)blockIdx.x * per), x1 = min(total, x0 + per);
     MergeDesc d{0, 0, 0, 0};
     Plan pl{};
-    pl.left = x1 - x0;
     if (x1 > x0) {
-      const uint64_t y = div_small(x0, p.n_units);  // in blocks of a single unit per sequence
+      const uint64_t y = div_small(x0, seq_cost);  // in blocks of sequence length
       uint64_t base = incl - mine;
       const uint32_t owner =
           __ffs(__ballot_sync(0xffffffffu, base <= y && y < incl)) - 1;
@@ -352,13 +380,29 @@ __device__ void make_plan(const TParams& p, uint64_t* sums, Plan* plan, MergeDes
       const uint64_t lo = base + upto - n;
       const uint32_t at = __ffs(__ballot_sync(0xffffffffu, lo <= y && y < lo + n)) - 1;
       if (lane == at) {
-        const uint64_t r = x0 - lo * p.n_units;
+        // the unit of this sequence that x0 falls into, and where it starts
+        const uint64_t of_head = (uint64_t)n * p.head_cost, of_pair = (uint64_t)n * p.cost2;
+        uint64_t r = x0 - lo * seq_cost;
+        const uint32_t head = (uint32_t)div_small(r, of_head), per_head = p.n_units / p.n_kv;
+        r -= head * of_head;
+        const uint32_t k = min((uint32_t)div_small(r, of_pair), per_head - 1);
+        r -= k * of_pair;
+        const uint64_t start = x0 - r;  // of the unit, on the line
         pl.b = g * 32 + lane;
-        pl.u = (uint32_t)div_small(r, n);
-        pl.blk = (uint32_t)(r - (uint64_t)pl.u * n);
-        const uint64_t ends = x0 - pl.blk + n;  // of the unit, on the line
-        if (pl.blk > 0 && ends <= x1)
-          d = MergeDesc{1, pl.b, pl.u, (uint32_t)div_small(x0 - pl.blk, per)};
+        pl.u = head * per_head + k;
+        const uint32_t cost = unit_of(p, pl.u).tiles == 2 ? p.cost2 : p.cost1;
+        pl.blk = (uint32_t)div_small(r + cost - 1, cost);
+        pl.left = (int64_t)(x1 - start) - (int64_t)((uint64_t)pl.blk * cost);
+        if (pl.blk < n) {
+          if (pl.blk > 0 && pl.left > 0 && pl.blk + div_small(pl.left + cost - 1, cost) >= n)
+            d = MergeDesc{1, pl.b, pl.u, (uint32_t)div_small(start, per)};
+        } else {  // the unit's last block is the CTA's before: on to the next unit
+          pl.blk = 0;
+          if (++pl.u == p.n_units) {
+            pl.u = 0;
+            pl.b++;
+          }
+        }
         *plan = pl;
         desc[blockIdx.x] = d;
       }
@@ -386,6 +430,53 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
+// The rows of the tree that `node` sees (its ancestors and itself), from the
+// parents of all nodes: lane i has those of nodes i and i + 32.  The lanes walk
+// up in doubling steps, so a chain takes as many as the logarithm of its depth.
+__device__ uint64_t tree_masks(int2 par, uint32_t n, uint32_t node, uint32_t* err) {
+  const int lane = (int)(threadIdx.x & 31);
+  uint64_t seen[2];
+  int up[2] = {par.x, par.y};
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const int i = lane + 32 * k;
+    if (up[k] < -1 || up[k] >= i) {
+      if (i < (int)n) atomicOr(err, NWD_DEVERR_TREE);
+      up[k] = -1;
+    }
+    seen[k] = 1ull << i;
+  }
+  while (__any_sync(0xffffffffu, up[0] >= 0 || up[1] >= 0)) {
+    uint64_t more[2];
+    int far[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int from = up[k] & 31;
+      const uint64_t lo = __shfl_sync(0xffffffffu, seen[0], from);
+      const uint64_t hi = __shfl_sync(0xffffffffu, seen[1], from);
+      const int flo = __shfl_sync(0xffffffffu, up[0], from);
+      const int fhi = __shfl_sync(0xffffffffu, up[1], from);
+      more[k] = up[k] < 0 ? 0 : up[k] < 32 ? lo : hi;
+      far[k] = up[k] < 0 ? -1 : up[k] < 32 ? flo : fhi;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      seen[k] |= more[k];
+      up[k] = far[k];
+    }
+  }
+  const uint64_t lo = __shfl_sync(0xffffffffu, seen[0], (int)(node & 31));
+  const uint64_t hi = __shfl_sync(0xffffffffu, seen[1], (int)(node & 31));
+  return node < 32 ? lo : hi;
+}
+
+// 32 bytes, a whole sector, at a 32-byte aligned address.
+__device__ __forceinline__ void store32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // Stores 4 columns (from column c) of a partial's row.
 __device__ __forceinline__ void store_part(float* slot, uint32_t row, uint32_t c, const float* v) {
   *reinterpret_cast<float4*>(slot + ((size_t)(c >> 2) * BM + row) * 4) =
@@ -412,12 +503,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < NBAR; i++) {
       uint32_t count = 1;
       if (i >= B_PFULL && i < B_PFULL + 4) count = BM;
-      if (i >= B_OEMPTY && i < B_OEMPTY + 2) count = 2 * BM;
+      if (i >= B_OEMPTY && i < B_OEMPTY + 2) count = BM;
       if (i >= B_ML && i < B_ML + 2) count = BM;
       // a stage is released by both groups' issuers
       if ((i >= B_QEMPTY && i < B_QEMPTY + (int)NQ) || (i >= B_KEMPTY && i < B_KEMPTY + (int)NK) ||
           (i >= B_VEMPTY && i < B_VEMPTY + (int)NV))
         count = 2;
+      // a V block by its producer, twice, or by the two warps that mend a tail
+      if (i >= B_VFULL && i < B_VFULL + (int)NV) count = 2;
       if (i == B_DRAIN) count = 4;
       mbar_init(bar + 8 * i, count);
     }
@@ -448,10 +541,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Registers per thread: 56 for the first two warpgroups, 200 for the softmax
-  // groups: 128 * 2 * (56 + 200) = 65536, the 512 * 128 of the launch.
+  // Registers per thread: 48 for the first two warpgroups, 152 for the softmax
+  // groups, 80 for the epilogue: 128 * (2 * 48 + 2 * 152 + 80) = 61440, the
+  // 640 * 96 of the launch.
   if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;" ::: "memory");
     if (warp == 0) {
       // ======================= K =======================
       const uint64_t policy = p.n_units == p.n_kv ? evict_first_policy() : evict_last_policy();
@@ -460,7 +554,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       Pieces w;
       bool ok = true;
       for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
-        const int hkv = (int)unit_of(p, w.u).hkv;
+        const int hkv = (int)w.un.hkv;
         for (uint32_t j = 0; j < w.nb; j++) {
           if (!warp_wait(bar + 8 * (B_KEMPTY + r.i), r.phase ^ 1u, abort_flag, err)) {
             ok = false;
@@ -490,132 +584,161 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     } else if (warp == 1) {
       // ======================= V and Q =======================
-      // The next piece's Q goes out with the last V block of a piece (before
-      // this warp waits for that block, if it is a tail): its buffers fill as
-      // soon as the S that read them are done.
+      // The next piece's Q goes out as soon as its buffers are free, looked
+      // for with every V block; with the piece's last one it is waited for.
       const uint64_t policy = p.n_units == p.n_kv ? evict_first_policy() : evict_last_policy();
       const uint64_t q_policy = evict_first_policy();
       const uint32_t q_bytes = 2 * p.tile_nodes * p.group * 128;
-      uint32_t issued[NV] = {}, q_issued[NQ] = {}, tails = 0;
+      uint32_t issued[NV] = {}, tails[NV] = {}, q_issued[NQ] = {};
       Ring<NV> r;
       Ring<NQ> rq;
       Pieces w, wq;
       bool ok = true;
       bool more_q = wq.begin(p, plan);
-      auto load_q = [&]() -> bool {
-        const Unit un = unit_of(p, wq.u);
-        for (uint32_t t = 0; t < un.tiles; t++) {
-          if (!warp_wait(bar + 8 * (B_QEMPTY + rq.i), rq.phase ^ 1u, abort_flag, err)) return false;
+      uint32_t q_tile = 0;  // next tile of wq's piece to load
+      auto load_q = [&](bool block) -> bool {
+        while (q_tile < wq.un.tiles) {
+          const uint32_t empty = bar + 8 * (B_QEMPTY + rq.i);
+          if (block) {
+            if (!warp_wait(empty, rq.phase ^ 1u, abort_flag, err)) return false;
+          } else if (!__all_sync(0xffffffffu, mbar_test_wait(empty, rq.phase ^ 1u))) {
+            return true;
+          }
           if (lane == 0) {
             const uint32_t fb = bar + 8 * (B_QFULL + rq.i), dst = sb + O_Q + rq.i * Q_TILE;
-            const int node = (int)(wq.b * p.n_nodes + (un.tile0 + t) * p.tile_nodes);
+            const int node = (int)(wq.b * p.n_nodes + (wq.un.tile0 + q_tile) * p.tile_nodes);
             mbar_arrive_tx(fb, q_bytes);
-            tma_load_5d(dst, &tmq, fb, 0, 0, 0, (int)un.hkv, node, q_policy);
-            tma_load_5d(dst + Q_CHUNK, &tmq, fb, 0, 1, 0, (int)un.hkv, node, q_policy);
+            tma_load_5d(dst, &tmq, fb, 0, 0, 0, (int)wq.un.hkv, node, q_policy);
+            tma_load_5d(dst + Q_CHUNK, &tmq, fb, 0, 1, 0, (int)wq.un.hkv, node, q_policy);
           }
           __syncwarp();
 #pragma unroll
           for (uint32_t i = 0; i < NQ; i++) q_issued[i] += rq.i == i;
           rq.next();
+          q_tile++;
         }
-        more_q = wq.next(p);
         return true;
       };
-      if (more_q) ok = load_q();
+      auto next_q = [&]() {  // on to the piece whose Q comes next
+        more_q = wq.next(p);
+        q_tile = 0;
+      };
+      if (more_q) {
+        ok = load_q(true);
+        next_q();
+      }
       for (bool more = ok && w.begin(p, plan); more && ok; more = w.next(p)) {
-        const int hkv = (int)unit_of(p, w.u).hkv;
+        const int hkv = (int)w.un.hkv;
         for (uint32_t j = 0; j < w.nb; j++) {
           if (!warp_wait(bar + 8 * (B_VEMPTY + r.i), r.phase ^ 1u, abort_flag, err)) {
             ok = false;
             break;
           }
-          const uint32_t key0 = (w.blk + j) * BN, rows = w.s.ctx + w.s.nodes;
-          // a block with rows of the tree, or behind it, completes on VTMA;
-          // this warp makes it fit to multiply and releases the stage
+          const uint32_t key0 = (w.blk + j) * BN;
+          // a block with rows of the tree, or behind it, completes on VTMA:
+          // warps 2 and 3 release it to its users
           const bool tail = key0 + BN > w.s.ctx;
-          const uint32_t fb = bar + 8 * (tail ? B_VTMA : B_VFULL + (int)r.i);
           if (lane == 0) {
+            const uint32_t fb = bar + 8 * ((tail ? B_VTMA : B_VFULL) + (int)r.i);
             const uint32_t dst = sb + O_V + r.i * TILE;
             const int row = (int)(w.s.row0 + key0);
+            if (!tail) mbar_arrive(fb);
             mbar_arrive_tx(fb, TILE);
             tma_load_4d(dst, &tmv, fb, 0, 0, hkv, row, policy);
             tma_load_4d(dst + CHUNK, &tmv, fb, 0, 1, hkv, row, policy);
           }
           __syncwarp();
 #pragma unroll
-          for (uint32_t i = 0; i < NV; i++) issued[i] += !tail && r.i == i;
-          tails += tail;
-          if (j + 1 == w.nb && more_q && !load_q()) {
+          for (uint32_t i = 0; i < NV; i++) {
+            issued[i] += !tail && r.i == i;
+            tails[i] += tail && r.i == i;
+          }
+          r.next();
+          if (more_q && !load_q(j + 1 == w.nb)) {
             ok = false;
             break;
           }
-          if (tail) {
-            if (!warp_wait(fb, (tails - 1) & 1, abort_flag, err)) {
-              ok = false;
-              break;
-            }
-            const uint32_t t0 = w.s.ctx > key0 ? w.s.ctx - key0 : 0;
-            const uint32_t t1 = rows > key0 ? min(rows - key0, BN) : 0;
-            uint4* st = reinterpret_cast<uint4*>(smem + O_V + r.i * TILE);
-            // the tree's rows: 8 uint4 of a row per chunk (a swizzled row
-            // stays within its 128 bytes)
-            uint64_t bad = 0;
-            for (uint32_t i = t0 * 8 + lane; i < t1 * 8; i += 32) {
-#pragma unroll
-              for (uint32_t c = 0; c < 2; c++) {
-                uint4* at = st + c * (CHUNK / 16) + i;
-                uint4 x = *at;
-                uint32_t* e = &x.x;
-                bool hit = false;
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                  const bool lo = (e[k] & 0x7c00u) == 0x7c00u;
-                  const bool hi = (e[k] & 0x7c000000u) == 0x7c000000u;
-                  hit |= lo | hi;
-                  if (lo) e[k] &= 0xffff0000u;
-                  if (hi) e[k] &= 0x0000ffffu;
-                }
-                if (hit) {
-                  *at = x;
-                  bad |= 1ull << (key0 + i / 8 - w.s.ctx);
-                }
-              }
-            }
-            const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-            for (uint32_t i = max(t1, t0) * 8 + lane; i < BN * 8; i += 32) {
-              st[i] = z;
-              st[CHUNK / 16 + i] = z;
-            }
-            const uint32_t blo = __reduce_or_sync(0xffffffffu, (uint32_t)bad);
-            const uint32_t bhi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32));
-            if (lane == 0) vbad[r.i] = (uint64_t)bhi << 32 | blo;
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar + 8 * (B_VFULL + r.i));
-#pragma unroll
-            for (uint32_t i = 0; i < NV; i++) issued[i] += r.i == i;
-          }
-          r.next();
         }
+        if (ok && more_q) next_q();
       }
       if (!ok) {
         const uint64_t t0 = globaltimer();
 #pragma unroll
-        for (uint32_t i = 0; i < NV; i++)
-          if (issued[i])
-            while (!mbar_try_wait(bar + 8 * (B_VFULL + i), (issued[i] - 1) & 1) &&
+        for (uint32_t i = 0; i < NV; i++) {
+          // (a block's last completion on VFULL may be warp 2's and 3's, of a tail)
+          if (issued[i] + tails[i])
+            while (!mbar_try_wait(bar + 8 * (B_VFULL + i), (issued[i] + tails[i] - 1) & 1) &&
                    globaltimer() - t0 < WAIT_LIMIT_NS) {
             }
+          if (tails[i])
+            while (!mbar_try_wait(bar + 8 * (B_VTMA + i), (tails[i] - 1) & 1) &&
+                   globaltimer() - t0 < WAIT_LIMIT_NS) {
+            }
+        }
 #pragma unroll
         for (uint32_t i = 0; i < NQ; i++)
           if (q_issued[i])
             while (!mbar_try_wait(bar + 8 * (B_QFULL + i), (q_issued[i] - 1) & 1) &&
                    globaltimer() - t0 < WAIT_LIMIT_NS) {
             }
-        if (tails)
-          while (!mbar_try_wait(bar + 8 * B_VTMA, (tails - 1) & 1) &&
-                 globaltimer() - t0 < WAIT_LIMIT_NS) {
+      }
+    } else if (warp < 4) {
+      // ======================= V blocks with rows of the tree =======================
+      // Rows behind the tree become zeros (0 x NaN would be NaN), NaN and
+      // infinities in the tree's rows too; which rows had some is noted.  Warp
+      // 2 has a block's first 64 columns, warp 3 the others.
+      const uint32_t half = (uint32_t)warp - 2;
+      uint32_t phases = 0;  // of VTMA, bit i: stage i
+      Ring<NV> r;
+      Pieces w;
+      bool ok = true;
+      for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
+        // the blocks before the tree's first row are not this warp's
+        const uint32_t from = w.s.ctx / BN, skip = from > w.blk ? min(from - w.blk, w.nb) : 0;
+        r.add(skip);
+        for (uint32_t j = skip; j < w.nb; j++, r.next()) {
+          const uint32_t key0 = (w.blk + j) * BN, rows = w.s.ctx + w.s.nodes;
+          if (!warp_wait(bar + 8 * (B_VTMA + r.i), (phases >> r.i) & 1u, abort_flag, err)) {
+            ok = false;
+            break;
           }
+          phases ^= 1u << r.i;
+          const uint32_t t0 = w.s.ctx > key0 ? w.s.ctx - key0 : 0;
+          const uint32_t t1 = max(rows > key0 ? min(rows - key0, BN) : 0u, t0);
+          // 8 uint4 of a row per chunk (a swizzled row stays within its 128
+          // bytes): lane l has those of rows l / 8, l / 8 + 4, ..
+          uint4* st = reinterpret_cast<uint4*>(smem + O_V + r.i * TILE + half * CHUNK) + lane;
+          uint64_t bad = 0;
+#pragma unroll 1
+          for (uint32_t i0 = 0; i0 < BN / 4; i0 += 4) {
+            uint4 x[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) x[i] = st[(i0 + i) * 32];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+              const uint32_t row = (i0 + i) * 4 + (uint32_t)lane / 8;
+              if (row < t0) continue;
+              uint32_t* e = &x[i].x;
+              bool hit = row >= t1;
+#pragma unroll
+              for (int k = 0; k < 4; k++) {
+                const bool lo = (e[k] & 0x7c00u) == 0x7c00u || row >= t1;
+                const bool hi = (e[k] & 0x7c000000u) == 0x7c000000u || row >= t1;
+                hit |= lo | hi;
+                if (lo) e[k] &= 0xffff0000u;
+                if (hi) e[k] &= 0x0000ffffu;
+              }
+              if (hit) st[(i0 + i) * 32] = x[i];
+              if (hit && row < t1) bad |= 1ull << (key0 + row - w.s.ctx);
+            }
+          }
+          const uint32_t blo = __reduce_or_sync(0xffffffffu, (uint32_t)bad);
+          const uint32_t bhi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32));
+          if (lane == 0) vbad[2 * r.i + half] = (uint64_t)bhi << 32 | blo;
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar + 8 * (B_VFULL + r.i));
+        }
       }
     } else if (warp >= 4) {
       // ======================= MMA issuers =======================
@@ -703,8 +826,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       __syncwarp();
     }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;" ::: "memory");
+  } else if (warp < 16) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 152;" ::: "memory");
     // ======================= softmax groups =======================
     const uint32_t g = (uint32_t)(warp - 8) >> 2;
     const uint32_t quad = (uint32_t)warp & 3u;
@@ -712,19 +835,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lanes = quad * 32u << 16;
     const uint32_t tmem_o = tmem + TMEM_O + lanes;
     float2* ml = reinterpret_cast<float2*>(smem + O_ML);
-    const uint32_t q_node = r / p.group, q_head = r % p.group;
-    uint32_t x0 = 0;                   // turns before this piece, of both groups
-    uint32_t turns[2] = {0, 0};        // of each group
-    uint32_t ml_units[2] = {0, 0};     // pieces of one tile that a group had turns in
-    // a group's turn i uses its score buffer i & 1, for the (i >> 1)th time
-    auto turn_done = [&](uint32_t of, uint32_t i) {  // its P V has completed
-      return warp_wait(bar + 8 * (B_PVDONE + 2 * of + (i & 1)), (i >> 1) & 1, abort_flag, err);
-    };
-    uint32_t n0 = 0;                   // blocks before this piece
+    const uint32_t q_node = r / p.group;
+    uint32_t x0 = 0;       // turns before this piece, of both groups
+    uint32_t my_turns = 0, my_units = 0;
+    uint32_t n0 = 0;       // blocks before this piece
     bool ok = true;
     Pieces w;
     for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
-      const Unit un = unit_of(p, w.u);
+      const Unit un = w.un;
       const bool two = un.tiles == 2;
       const uint32_t mine = (g - x0) & 1;  // two tiles: my tile; one: my first block
       const uint32_t tile = un.tile0 + (two ? mine : 0);
@@ -732,18 +850,23 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t node = tile * p.tile_nodes + q_node;
       const bool row_used = q_node < tile_nodes;
       const bool warp_used = quad * 32u < tile_nodes * p.group;
-      // which rows of the tree this row sees: none if its node is absent
-      const bool has_tail = (w.blk + w.nb) * BN > w.s.ctx;
+      // which rows of the tree this row sees (none if its node is absent):
+      // found at the first block that has some, from parents fetched now
+      int2 par = make_int2(-1, -1);
+      if ((w.blk + w.nb) * BN > w.s.ctx) {
+        const int32_t* src = p.parents + (size_t)w.b * p.n_nodes;
+        if ((uint32_t)lane < p.n_nodes) par.x = src[lane];
+        if ((uint32_t)lane + 32 < p.n_nodes) par.y = src[lane + 32];
+      }
+      bool have_mask = false;
       uint64_t sees = 0;
-      if (has_tail && row_used && node < w.s.nodes)
-        sees = nwd::tree_mask(p.parents + (size_t)w.b * p.n_nodes, (int)node, err);
       float m = -INFINITY, l = 0.f;
       uint64_t bad = 0;
       const uint32_t step = two ? 1 : 2;
       uint32_t j = two ? 0 : mine;
-      const uint32_t first_turn = turns[g];
+      const uint32_t first_turn = my_turns;
       for (; j < w.nb; j += step) {
-        const uint32_t turn = turns[g]++, buf = turn & 1;
+        const uint32_t turn = my_turns++, buf = turn & 1;
         const uint32_t tmem_s = tmem + (2 * g + buf) * BN + lanes;
         const uint32_t key0 = (w.blk + j) * BN;
         const bool tail = key0 + BN > w.s.ctx;
@@ -758,6 +881,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           tmem_ld32(tmem_s + 32, s + 32);
           tmem_ld_wait();
           if (tail) {
+            if (!have_mask) {
+              have_mask = true;
+              const uint64_t all = tree_masks(par, p.n_nodes, node, err);
+              sees = row_used && node < w.s.nodes ? all : 0;
+            }
             // bit c of word i: this row attends cache row key0 + 32 i + c
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -799,7 +927,9 @@ __global__ void __launch_bounds__(THREADS, 1)
               const float alpha = up ? ex2f(m - mx) : 1.f;  // 0 while m is -inf
               if (turn != first_turn) {
                 // O is rescaled once the P V of the group's last turn is in it
-                if (!turn_done(g, turn - 1)) {
+                const uint32_t last = turn - 1;
+                if (!warp_wait(bar + 8 * (B_PVDONE + 2 * g + (last & 1)), (last >> 1) & 1,
+                               abort_flag, err)) {
                   ok = false;
                   break;
                 }
@@ -823,142 +953,172 @@ __global__ void __launch_bounds__(THREADS, 1)
           l += (sum.x + sum.y) + (sum1.x + sum1.y);
           tmem_st_wait();
         }
-        if (tail) {  // V rows with NaN or infinities, found by the V producer
+        if (tail && quad == 0) {  // V rows with NaN or infinities, noted by warps 2 and 3
           const uint32_t n = n0 + j;
           if (!warp_wait(bar + 8 * (B_VFULL + n % NV), (n / NV) & 1, abort_flag, err)) {
             ok = false;
             break;
           }
-          bad |= vbad[n % NV];
+          bad |= vbad[2 * (n % NV)] | vbad[2 * (n % NV) + 1];
         }
         tc_fence_before();
         mbar_arrive(bar + 8 * (B_PFULL + 2 * g + buf));
       }
-      n0 += w.nb;
       if (!ok) break;
-
-      // ---- the piece's end: O of the tile (two), or of both groups' halves
+      n0 += w.nb;
+      x0 += w.nb * un.tiles;
+      if (my_turns != first_turn) {
+        // (m, l) to the epilogue, once it has read the last ones
+        if (!warp_wait(bar + 8 * (B_OEMPTY + g), (my_units & 1) ^ 1, abort_flag, err)) break;
+        my_units++;
+        ml[g * BM + r] = make_float2(m, l);
+        if (r == 0) gbad[g] = bad;
+        mbar_arrive(bar + 8 * (B_ML + g));
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;" ::: "memory");
+    // ======================= epilogue =======================
+    const uint32_t quad = (uint32_t)warp & 3u;
+    const uint32_t r = quad * 32u + (uint32_t)lane;
+    const uint32_t tmem_o = tmem + TMEM_O + (quad * 32u << 16);
+    const float2* ml = reinterpret_cast<const float2*>(smem + O_ML);
+    const uint32_t q_node = r / p.group, q_head = r % p.group;
+    uint32_t x0 = 0;
+    uint32_t turns[2] = {0, 0}, units[2] = {0, 0};  // of each group
+    const bool wide = (reinterpret_cast<uintptr_t>(p.o) & 31u) == 0;  // whole sectors per store
+    // group i's part of the piece is complete: its (m, l), and its last P V
+    auto complete = [&](uint32_t i) -> bool {
+      const uint32_t last = turns[i] - 1;
+      return warp_wait(bar + 8 * (B_ML + i), units[i] & 1, abort_flag, err) &&
+             warp_wait(bar + 8 * (B_PVDONE + 2 * i + (last & 1)), (last >> 1) & 1, abort_flag, err);
+    };
+    auto release = [&](uint32_t i) {
+      mbar_arrive(bar + 8 * (B_OEMPTY + i));
+      units[i]++;
+    };
+    bool ok = true;
+    Pieces w;
+    for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
+      const Unit un = w.un;
+      const bool two = un.tiles == 2;
       const bool direct = w.blk == 0 && w.nb == w.nblk;
-      const uint32_t slot_at = ((blockIdx.x * 2 + (w.blk > 0 ? 0 : 1)) * p.unit_tiles +
-                                (two ? mine : 0)) * BM;
-      float2* slot_ml = reinterpret_cast<float2*>(p.ws + WS_ML) + slot_at;
-      float* slot_o =
-          reinterpret_cast<float*>(p.ws + ws_o(gridDim.x, p.unit_tiles)) + (size_t)slot_at * HD;
-      const bool absent = node >= w.s.nodes;
-      __half* orow = p.o + (((size_t)w.b * p.n_nodes + node) * p.n_heads + un.hkv * p.group +
-                            q_head) * HD;
-      const __half* vrow = p.v + (((size_t)w.s.row0 + w.s.ctx) * p.n_kv + un.hkv) * HD;
-      // adds what the V producer took out of the rows that this one sees
-      auto restore = [&](float* ov, uint32_t col, uint64_t rows) {
-        for (uint64_t x = rows & sees; x; x &= x - 1) {
-          const __half* src = vrow + (size_t)(__ffsll((long long)x) - 1) * p.n_kv * HD + col;
+      // a row's outputs, from column `col`: 32 columns
+      auto put = [&](uint32_t t, uint32_t col, float* ov, float inv, uint64_t bad) {
+        const uint32_t tile = un.tile0 + t;
+        const uint32_t node = tile * p.tile_nodes + q_node;
+        if (q_node >= min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes)) return;
+        const bool absent = node >= w.s.nodes;
+        if (bad && !absent) {
+          // what was taken out of the V rows that this row sees
+          const uint64_t sees =
+              nwd::tree_mask(p.parents + (size_t)w.b * p.n_nodes, (int)node, nullptr);
+          const __half* v = p.v + (((size_t)w.s.row0 + w.s.ctx) * p.n_kv + un.hkv) * HD + col;
+          for (uint64_t x = bad & sees; x; x &= x - 1) {
+            const __half* src = v + (size_t)(__ffsll((long long)x) - 1) * p.n_kv * HD;
 #pragma unroll
-          for (int i = 0; i < 32; i++) {
-            const float e = __half2float(src[i]);
-            if (!isfinite(e)) ov[i] += e;
+            for (int i = 0; i < 32; i++) {
+              const float e = __half2float(src[i]);
+              if (!isfinite(e)) ov[i] += e;
+            }
           }
         }
-      };
-      auto put = [&](float* ov, uint32_t col, float inv) {
         if (direct) {
-          uint4* dst = reinterpret_cast<uint4*>(orow + col);
+          __half* dst = p.o + (((size_t)w.b * p.n_nodes + node) * p.n_heads + un.hkv * p.group +
+                               q_head) * HD + col;
+          uint32_t h[16];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            uint32_t h[4];
+          for (int k = 0; k < 16; k++) {
+            const __half2 x = __floats2half2_rn(ov[2 * k] * inv, ov[2 * k + 1] * inv);
+            h[k] = absent ? 0u : *reinterpret_cast<const uint32_t*>(&x);
+          }
+          if (wide) {
+            store32(dst, h);
+            store32(dst + 16, h + 8);
+          } else {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const __half2 x = __floats2half2_rn(ov[8 * i + 2 * k] * inv,
-                                                  ov[8 * i + 2 * k + 1] * inv);
-              h[k] = absent ? 0u : *reinterpret_cast<const uint32_t*>(&x);
-            }
-            dst[i] = make_uint4(h[0], h[1], h[2], h[3]);
+            for (int i = 0; i < 4; i++)
+              reinterpret_cast<uint4*>(dst)[i] =
+                  make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
           }
         } else {
+          float* slot = reinterpret_cast<float*>(p.ws + ws_o(gridDim.x, p.unit_tiles)) +
+                        (size_t)((blockIdx.x * 2 + (w.blk > 0 ? 0 : 1)) * p.unit_tiles + t) * BM * HD;
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) store_part(slot_o, r, col + i, ov + i);
+          for (int i = 0; i < 32; i += 4) store_part(slot, r, col + i, ov + i);
         }
       };
+      auto put_ml = [&](uint32_t t, float m, float l) {
+        if (!direct)
+          reinterpret_cast<float2*>(p.ws + WS_ML)[((blockIdx.x * 2 + (w.blk > 0 ? 0 : 1)) *
+                                                       p.unit_tiles + t) * BM + r] =
+              make_float2(m, l);
+      };
       if (two) {
-        turns[g ^ 1] += w.nb;
-        if (!turn_done(g, turns[g] - 1)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        if (warp_used) {
-          const float inv = l != 0.f ? 1.f / l : 0.f;
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
-            float ov[32];
-            tmem_ld32(tmem_o + g * HD + c * 32, ov);
-            tmem_ld_wait();
-            if (row_used) {
-              if (bad) restore(ov, c * 32, bad);
-              put(ov, c * 32, inv);
-            }
-          }
-          if (!direct && row_used) slot_ml[r] = make_float2(m, l);
-        }
-        tc_fence_before();
-        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 2;" ::"r"(bar + 8 * (B_OEMPTY + g))
-                     : "memory");
-      } else {
-        // group of block 0: x0 & 1; the other has turns from two blocks on
-        const bool had[2] = {w.nb > 1 || (x0 & 1) == 0, w.nb > 1 || (x0 & 1) == 1};
-        // the other group's turns: blocks (mine ^ 1), (mine ^ 1) + 2, ..
-        turns[g ^ 1] += (w.nb + mine) / 2;
-        // (m, l) are handed over once the group's O is complete: that needs the
-        // O before it released, by threads that have read the (m, l) before
-        if (had[g]) {
-          if (!turn_done(g, turns[g] - 1)) {
+        turns[0] += w.nb;
+        turns[1] += w.nb;
+#pragma unroll 1
+        for (uint32_t i = 0; i < 2 && ok; i++) {
+          if (!complete(i)) {
             ok = false;
             break;
           }
-          ml[g * BM + r] = make_float2(m, l);
-          if (r == 0) gbad[g] = bad;
-          mbar_arrive(bar + 8 * (B_ML + g));
+          tc_fence_after();
+          const uint32_t t = (i - x0) & 1;  // the group's tile
+          const float2 a = ml[i * BM + r];
+          const uint64_t bad = gbad[i];
+          const float inv = a.y != 0.f ? 1.f / a.y : 0.f;
+#pragma unroll 1
+          for (uint32_t c = 0; c < HD; c += 32) {
+            float ov[32];
+            tmem_ld32(tmem_o + i * HD + c, ov);
+            tmem_ld_wait();
+            put(t, c, ov, inv, bad);
+          }
+          put_ml(t, a.x, a.y);
+          tc_fence_before();
+          release(i);
         }
-#pragma unroll
-        for (uint32_t i = 0; i < 2; i++)
-          if (ok && had[i])
-            ok = warp_wait(bar + 8 * (B_ML + i), ml_units[i] & 1, abort_flag, err) &&
-                 turn_done(i, turns[i] - 1);
+      } else {
+        const uint32_t lead = x0 & 1;  // the group of the first block
+        turns[lead] += (w.nb + 1) / 2;
+        turns[lead ^ 1] += w.nb / 2;
+        const bool both = w.nb > 1;
+        ok = complete(lead) && (!both || complete(lead ^ 1));
         if (!ok) break;
         tc_fence_after();
-        if (warp_used) {
-          const float2 a0 = had[0] ? ml[r] : make_float2(-INFINITY, 0.f);
-          const float2 a1 = had[1] ? ml[BM + r] : make_float2(-INFINITY, 0.f);
-          const uint64_t both = (had[0] ? gbad[0] : 0) | (had[1] ? gbad[1] : 0);
-          const float M = fmaxf(a0.x, a1.x);
-          // a group without weights counts for nothing (l may be NaN)
-          const float w0 = a0.y != 0.f ? ex2f(a0.x - M) : 0.f;
-          const float w1 = a1.y != 0.f ? ex2f(a1.x - M) : 0.f;
-          const float L = (a0.y != 0.f ? a0.y * w0 : 0.f) + (a1.y != 0.f ? a1.y * w1 : 0.f);
-          const float inv = L != 0.f ? 1.f / L : 0.f;
+        const float2 a = ml[lead * BM + r];
+        const float2 b = both ? ml[(lead ^ 1) * BM + r] : make_float2(-INFINITY, 0.f);
+        const uint64_t bad = gbad[lead] | (both ? gbad[lead ^ 1] : 0);
+        // a group without weights counts for nothing (l may be NaN)
+        const float M = fmaxf(a.x, b.x);
+        const float wa = a.y != 0.f ? ex2f(a.x - M) : 0.f, wb = b.y != 0.f ? ex2f(b.x - M) : 0.f;
+        const float L = (a.y != 0.f ? a.y * wa : 0.f) + (b.y != 0.f ? b.y * wb : 0.f);
+        const float inv = L != 0.f ? 1.f / L : 0.f;
+#pragma unroll 1
+        for (uint32_t c = 0; c < HD; c += 32) {
+          float ov[32], o1[16];
+          tmem_ld32(tmem_o + lead * HD + c, ov);
+          tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
-            const uint32_t col = g * 64 + c * 32;  // each group half of the columns
-            float ov[32], o1[32];
-            tmem_ld32(tmem_o + col, ov);
-            tmem_ld32(tmem_o + HD + col, o1);
-            tmem_ld_wait();
+          for (int i = 0; i < 32; i++) ov[i] = a.y != 0.f ? ov[i] * wa : 0.f;
+          if (both) {
 #pragma unroll
-            for (int i = 0; i < 32; i++)
-              ov[i] = (a0.y != 0.f ? ov[i] * w0 : 0.f) + (a1.y != 0.f ? o1[i] * w1 : 0.f);
-            if (row_used) {
-              if (both) restore(ov, col, both);
-              put(ov, col, inv);
+            for (int h = 0; h < 2; h++) {
+              tmem_ld16(tmem_o + (lead ^ 1) * HD + c + 16 * h, o1);
+              tmem_ld_wait();
+              if (b.y != 0.f) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) ov[16 * h + i] += o1[i] * wb;
+              }
             }
           }
-          if (!direct && row_used && g == 0) slot_ml[r] = make_float2(M, L);
+          put(0, c, ov, inv, bad);
         }
+        put_ml(0, M, L);
         tc_fence_before();
-#pragma unroll
-        for (uint32_t i = 0; i < 2; i++)
-          if (had[i]) {
-            mbar_arrive(bar + 8 * (B_OEMPTY + i));
-            ml_units[i]++;
-          }
+        release(lead);
+        if (both) release(lead ^ 1);
       }
       x0 += w.nb * un.tiles;
     }
@@ -1139,6 +1299,14 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
     cudaError_t e = cudaFuncSetAttribute(tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)SMEM_BYTES);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(tree_kernel)");
+    // setmaxnreg's shares add up to the registers of the launch: fewer would
+    // leave the softmax groups waiting for theirs
+    cudaFuncAttributes at;
+    e = cudaFuncGetAttributes(&at, tree_kernel);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(tree_kernel)");
+    if (at.numRegs < LAUNCH_REGS)
+      return fail(NWD_ERR_UNSUPPORTED, "%s: built with %d registers per thread, not %d", who,
+                  at.numRegs, LAUNCH_REGS);
     smem_set[di.device] = true;
   }
   CUtensorMap tq, tk, tv;
@@ -1165,6 +1333,10 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
   p.n_tiles = t.n_tiles;
   p.unit_tiles = t.unit_tiles;
   p.n_units = n_kv * ((t.n_tiles + t.unit_tiles - 1) / t.unit_tiles);
+  p.cost1 = COST1;
+  p.cost2 = COST2;
+  p.head_cost = t.n_tiles / 2 * p.cost2 + (t.n_tiles & 1) * p.cost1;
+  p.min_cost = p.cost2;
   p.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f;
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e = cudaSuccess;

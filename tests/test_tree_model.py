@@ -16,35 +16,68 @@ import pytest
 BN = 64
 
 
-def pieces(blocks, n_units, ctas, min_blocks=1):
-    """Per CTA the list of (b, u, blk, nb), and the joins (cta -> (b, u, first))."""
-    line = [(b, u, n) for b, n in enumerate(blocks) for u in range(n_units)]
-    total = sum(n for _, _, n in line)
-    per = max(-(-total // ctas), min_blocks)
+def unit_tiles(u, n_tiles):
+    per_head = -(-n_tiles // 2)
+    return 2 if (u % per_head) * 2 + 1 < n_tiles else 1
+
+
+def pieces(blocks, n_kv, n_tiles, ctas, cost1, cost2):
+    """Per CTA the list of (b, u, blk, nb) and its join (b, u, first), as the kernel finds them."""
+    per_head = -(-n_tiles // 2)
+    n_units, head_cost = n_kv * per_head, n_tiles // 2 * cost2 + n_tiles % 2 * cost1
+    seq_cost = n_kv * head_cost
+    total = sum(blocks) * seq_cost
+    per = max(-(-total // ctas), cost2)
+    cost_of = lambda u: cost2 if unit_tiles(u, n_tiles) == 2 else cost1  # noqa: E731
     out, joins = [], {}
     for c in range(ctas):
         x0, x1 = min(total, c * per), min(total, c * per + per)
-        mine, at = [], 0
-        for b, u, n in line:
-            lo, hi = max(x0, at), min(x1, at + n)
-            if lo < hi:
-                mine.append((b, u, lo - at, hi - lo))
-                if lo > at and hi == at + n:
-                    joins[c] = (b, u, at // per)
-            at += n
+        mine = []
         out.append(mine)
-    return out, joins
+        if x0 >= x1:
+            continue
+        y, lo, b = x0 // seq_cost, 0, 0
+        while not lo <= y < lo + blocks[b]:
+            lo += blocks[b]
+            b += 1
+        n = blocks[b]
+        r = x0 - lo * seq_cost
+        head, r = divmod(r, n * head_cost)
+        k = min(r // (n * cost2), per_head - 1)
+        r -= k * n * cost2
+        start, u = x0 - r, head * per_head + k
+        cost = cost_of(u)
+        blk = -(-r // cost)
+        left = x1 - start - blk * cost
+        if blk < n:
+            if blk > 0 and left > 0 and blk + -(-left // cost) >= n:
+                joins[c] = (b, u, start // per)
+        else:
+            blk, u = 0, u + 1
+            if u == n_units:
+                u, b = 0, b + 1
+        while left > 0:
+            n, cost = blocks[b], cost_of(u)
+            nb = n - blk if left >= (n - blk) * cost else -(-left // cost)
+            mine.append((b, u, blk, nb))
+            left -= nb * cost
+            blk, u = 0, u + 1
+            if u == n_units:
+                u, b = 0, b + 1
+    return out, joins, n_units
 
 
-@pytest.mark.parametrize("seed", range(12))
+@pytest.mark.parametrize("seed", range(60))
 def test_split_covers_every_unit(seed):
     r = random.Random(seed)
     blocks = [r.choice([1, 1, 2, 5, 33, r.randint(1, 400)]) for _ in range(r.choice([1, 2, 7, 64]))]
-    n_units, ctas = r.choice([1, 2, 8, 16]), r.choice([1, 7, 148])
-    got, joins = pieces(blocks, n_units, ctas, r.choice([1, 3]))
+    cost1 = r.choice([1, 1, 2, 3])
+    got, joins, n_units = pieces(blocks, r.choice([1, 2, 8]), r.choice([1, 2, 3, 4]),
+                                 r.choice([1, 7, 148]), cost1, r.randint(cost1, 2 * cost1))
     seen, slots = {}, set()
     for c, mine in enumerate(got):
         for b, u, blk, nb in mine:
+            assert nb > 0
             seen.setdefault((b, u), []).append((blk, nb, c))
             if not (blk == 0 and nb == blocks[b]):
                 slot = (c, 0 if blk > 0 else 1)
@@ -96,7 +129,7 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
         for i in range(n):
             bar(name, i, 2)
     for g in range(2):
-        bar("P", 2 * g, 2), bar("P", 2 * g + 1, 2), bar("OE", g, 4), bar("ML", g, 2)  # two threads stand for a group's 128
+        bar("P", 2 * g, 2), bar("P", 2 * g + 1, 2), bar("OE", g, 2), bar("ML", g, 2)  # two threads stand for a group's 128
     q, k, v = [None] * NQ, [None] * NK, [None] * NV
     s_buf, o_buf, log = [None] * 4, [None, None], []
     mmas = [[], [], [], []]  # issued by an issuer, not yet run, in order
@@ -196,60 +229,61 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
                 mma.append(bar("VE", vi).arrive)
                 ou += last
 
-    read = {}
+    read, handed = {}, [[None, None], [None, None]]  # [group][thread]
 
     def softmax(g, th):
-        x0, turns, mu = 0, [0, 0], [0, 0]
-
-        def turn_done(of, i):
-            yield from wait(bar("PV", 2 * of + (i & 1)), i >> 1 & 1)
-
+        x0, turn, units = 0, 0, 0
         for n, (nb, tiles) in enumerate(plan):
-            mine = (g - x0) & 1
-            for j in range(nb):
-                if tiles == 1 and (j & 1) != mine:
-                    continue
-                x, buf = turns[g], 2 * g + (turns[g] & 1)
-                turns[g] += 1
+            mine, first = (g - x0) & 1, turn
+            for j in range(nb) if tiles == 2 else range(mine, nb, 2):
+                x, buf = turn, 2 * g + (turn & 1)
+                turn += 1
                 yield from wait(bar("S", buf), x >> 1 & 1)
                 want = (n, j, mine if tiles == 2 else 0)
                 assert s_buf[buf] in (("S",) + want, ("P",) + want)
                 yield
-                if j > (tiles == 1) and rnd.random() < 0.3:  # the maximum moved: rescale O
-                    yield from turn_done(g, x - 1)
+                if x != first and rnd.random() < 0.3:  # the maximum moved: rescale O
+                    yield from wait(bar("PV", 2 * g + (x - 1 & 1)), x - 1 >> 1 & 1)
                     assert o_buf[g][0] == n and o_buf[g][1][-1][0] == j - 3 + tiles
                 s_buf[buf] = ("P",) + want
                 bar("P", buf).arrive()
-            if tiles == 2:
-                turns[g ^ 1] += nb
-                yield from turn_done(g, turns[g] - 1)
-                assert o_buf[g] == (n, [(j, mine) for j in range(nb)])
-                read.setdefault((n, g), set()).add((g, th))
+            x0 += nb * tiles
+            if turn != first:
+                yield from wait(bar("OE", g), (units & 1) ^ 1)
+                units += 1
+                assert handed[g][th] is None
+                handed[g][th] = n
+                bar("ML", g).arrive()
+
+    def epilogue(th):
+        x0, turns, units = 0, [0, 0], [0, 0]
+
+        def complete(i):
+            yield from wait(bar("ML", i), units[i] & 1)
+            last = turns[i] - 1
+            yield from wait(bar("PV", 2 * i + (last & 1)), last >> 1 & 1)
+
+        for n, (nb, tiles) in enumerate(plan):
+            lead = x0 & 1
+            own = {0: nb, 1: nb} if tiles == 2 else {lead: (nb + 1) // 2, lead ^ 1: nb // 2}
+            groups = [i for i in (own if tiles == 2 else (lead, lead ^ 1)) if own[i]]
+            for i in groups:
+                turns[i] += own[i]
+            for part in [[i] for i in groups] if tiles == 2 else [groups]:
+                for i in part:
+                    yield from complete(i)
+                for i in part:
+                    js = [(j, (i - x0) & 1) for j in range(nb)] if tiles == 2 else \
+                        [(j, 0) for j in range(nb) if (x0 + j) & 1 == i]
+                    assert o_buf[i] == (n, js) and handed[i][th] == n
                 yield
-                if len(read[(n, g)]) == 2:
-                    o_buf[g] = None
-                bar("OE", g).arrive(2)
-            else:
-                had = [nb > 1 or (x0 & 1) == i for i in range(2)]
-                turns[g ^ 1] += (nb + mine) // 2
-                if had[g]:
-                    yield from turn_done(g, turns[g] - 1)
-                    bar("ML", g).arrive()
-                for i in range(2):
-                    if had[i]:
-                        yield from wait(bar("ML", i), mu[i] & 1)
-                        yield from turn_done(i, turns[i] - 1)
-                for i in range(2):
-                    if had[i]:
-                        assert o_buf[i] == (n, [(j, 0) for j in range(nb) if (x0 + j) & 1 == i])
-                        read.setdefault((n, i), set()).add((g, th))
-                yield
-                for i in range(2):
-                    if had[i]:
-                        if len(read[(n, i)]) == 4:
-                            o_buf[i] = None
-                        bar("OE", i).arrive()
-                        mu[i] += 1
+                for i in part:
+                    handed[i][th] = None
+                    read.setdefault((n, i), set()).add(th)
+                    if len(read[(n, i)]) == 2:
+                        o_buf[i] = None
+                    bar("OE", i).arrive()
+                    units[i] += 1
             x0 += nb * tiles
 
     def tensor_core():
@@ -264,32 +298,44 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
         """V blocks; the next piece's Q with a piece's last block, before that block is waited
         for (a tail: every last block here)."""
         qs = [[(n, t) for t in range(tiles)] for n, (_, tiles) in enumerate(plan)]
-        state = dict(q=0, v=0, t=0)
+        state = dict(q=0, v=0)
 
-        def load_q():
-            for item in qs.pop(0):
-                i = state["q"] % NQ
-                yield from wait(bar("QE", i), (state["q"] // NQ & 1) ^ 1)
-                copy(q, i, item, bar("QF", i))
+        def load_q(block=True):
+            while qs[0]:
+                i, parity = state["q"] % NQ, (state["q"] // NQ & 1) ^ 1
+                if not block and not bar("QE", i).passed(parity):
+                    return
+                yield from wait(bar("QE", i), parity)
+                copy(q, i, qs[0].pop(0), bar("QF", i))
                 state["q"] += 1
 
         yield from load_q()
+        qs.pop(0)
         for n, (nb, _) in enumerate(plan):
             for j in range(nb):
                 i = state["v"] % NV
                 yield from wait(bar("VE", i), (state["v"] // NV & 1) ^ 1)
-                tail = j + 2 >= nb  # waited for, made fit and released by this warp
-                copy(v, i, (n, j), bar("VT", 0) if tail else bar("VF", i))
-                if j + 1 == nb and qs:
-                    yield from load_q()
-                if tail:
-                    yield from wait(bar("VT", 0), state["t"] & 1)
-                    state["t"] += 1
-                    bar("VF", i).arrive()
+                tail = j + 2 >= nb  # made fit and released by another warp
+                copy(v, i, (n, j), bar("VT", i) if tail else bar("VF", i))
                 state["v"] += 1
+                if qs:
+                    yield from load_q(j + 1 == nb)
+            if qs:
+                qs.pop(0)
+
+    def tails():
+        phases, i = [0] * NV, 0
+        for n, (nb, _) in enumerate(plan):
+            for j in range(nb):
+                if j + 2 >= nb:
+                    yield from wait(bar("VT", i), phases[i])
+                    phases[i] ^= 1
+                    yield
+                    bar("VF", i).arrive()
+                i = (i + 1) % NV
 
     roles = [issuer(g, kind) for g in range(2) for kind in ("S", "PV")]
-    roles += [load("K", NK, k, kv), v_and_q()]
+    roles += [load("K", NK, k, kv), v_and_q(), tails()] + [epilogue(th) for th in range(2)]
     roles += [softmax(g, th) for g in range(2) for th in range(2)]
     tc, cp = tensor_core(), copies()
     idle = 0
