@@ -20,8 +20,13 @@
 //                 each unit's Q tiles into 2 (as 64-column chunks, 128-byte
 //                 swizzle: the K-major operand layout).  Warp 0 also owns the
 //                 tensor memory.
-//   warps 2, 3    make V blocks with rows of the tree, or behind it, fit to
+//   warp 2        makes V blocks with rows of the tree, or behind it, fit to
 //                 multiply (below).
+//   warp 3        plans: finds this CTA's range and hands its pieces (blocks of
+//                 one unit) to the other warps through a ring of descriptors.
+//                 (Nine roles that each walked the sequences for themselves
+//                 made the kernel larger than the instruction cache, and a
+//                 unit's end cost 5 to 9 us.)
 //   warps 4 - 7   MMA issuers: S of softmax group 0, of group 1, P V of group
 //                 0, of group 1.  A turn is S = Q K^T of one (block, tile) and
 //                 O += P V after its softmax; S runs two turns ahead into the
@@ -36,9 +41,7 @@
 //   warps 16-19   the epilogue: a unit's O out of tensor memory, joined over
 //                 the two groups where they shared its tile, normalised and
 //                 stored (or left as a partial), while the softmax groups are
-//                 at the next unit.  (With the epilogue in the softmax warps a
-//                 unit's end cost 5-6 us of a loop that takes 0.6 us per
-//                 block.)
+//                 at the next unit.
 //
 // Softmax in the log2 domain with a lazily moved maximum (O is rescaled in
 // tensor memory only when a row's maximum grows by more than 2^8).  P is
@@ -82,14 +85,15 @@ constexpr uint32_t Q_TILE = 2 * Q_CHUNK;
 constexpr uint32_t CHUNK = BN * 128;
 constexpr uint32_t TILE = 2 * CHUNK;    // a K or V block: 16 KiB
 constexpr uint32_t NQ = 2, NK = 5, NV = 5;  // stages
-constexpr uint32_t MAX_GROUPS32 = 128;  // batch / 32
+constexpr uint32_t NP = 4;              // piece descriptors
+constexpr uint32_t PIECE_USERS = 19;    // warps that read them: all but the planner
 // what a block costs in a unit of one tile, of two (in the same unit of time)
 constexpr uint32_t COST1 = 1, COST2 = 2;
 
 constexpr uint32_t O_Q = 0;
 constexpr uint32_t O_K = O_Q + NQ * Q_TILE;
 constexpr uint32_t O_V = O_K + NK * TILE;
-constexpr uint32_t O_ML = O_V + NV * TILE;        // [2 groups][128] (m, l); the plan's sums before
+constexpr uint32_t O_ML = O_V + NV * TILE;        // [2 groups][128] (m, l)
 constexpr uint32_t O_BAR = O_ML + 2 * BM * 8;
 constexpr int B_QFULL = 0, B_QEMPTY = B_QFULL + NQ, B_KFULL = B_QEMPTY + NQ,
               B_KEMPTY = B_KFULL + NK, B_VFULL = B_KEMPTY + NK, B_VEMPTY = B_VFULL + NV,
@@ -97,17 +101,17 @@ constexpr int B_QFULL = 0, B_QEMPTY = B_QFULL + NQ, B_KFULL = B_QEMPTY + NQ,
               // by 2 * softmax group + score buffer
     B_SFULL = B_VTMA + NV, B_PFULL = B_SFULL + 4, B_PVDONE = B_PFULL + 4,
               // by softmax group
-    B_OEMPTY = B_PVDONE + 4, B_ML = B_OEMPTY + 2, B_DRAIN = B_ML + 2, NBAR = B_DRAIN + 1;
-constexpr uint32_t O_PLAN = (O_BAR + NBAR * 8 + 15) / 16 * 16;  // Plan
-constexpr uint32_t O_VBAD = O_PLAN + 48;          // [NV][2] u64: tree rows with NaN or inf in V
-constexpr uint32_t O_GBAD = O_VBAD + NV * 16;      // [2] u64: the same, gathered per group
+    B_OEMPTY = B_PVDONE + 4, B_ML = B_OEMPTY + 2, B_DRAIN = B_ML + 2,
+              B_PCFULL = B_DRAIN + 1, B_PCEMPTY = B_PCFULL + NP, NBAR = B_PCEMPTY + NP;
+constexpr uint32_t O_PIECE = (O_BAR + NBAR * 8 + 15) / 16 * 16;  // [NP] Piece
+constexpr uint32_t O_VBAD = O_PIECE + NP * 64;    // [NV] u64: tree rows with NaN or inf in V
+constexpr uint32_t O_GBAD = O_VBAD + NV * 8;      // [2] u64: the same, gathered per group
 constexpr uint32_t O_MISC = O_GBAD + 16;          // tensor memory base, abort flag
 constexpr uint32_t SMEM_USED = O_MISC + 16;
 // dynamic shared memory starts 1024-byte aligned (there is no static shared
 // memory in this kernel); the kernel checks it
 constexpr uint32_t SMEM_BYTES = SMEM_USED;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
-static_assert(MAX_GROUPS32 * 8 <= 2 * BM * 8, "the plan's sums fit the (m, l) area");
 
 constexpr uint32_t TMEM_COLS = 512;  // 2 groups x 2 score buffers of 64, then O0 O1 of 128
 constexpr uint32_t TMEM_O = 256;
@@ -133,12 +137,16 @@ struct TParams {
   float scale_log2;
 };
 
-struct Plan {
-  int64_t left;  // of this CTA's range, from the first piece on
-  uint32_t b, u, blk;
-  uint32_t pad[5];
+// Blocks [blk, blk + nb) of a unit: what the roles do with it.
+struct __align__(16) Piece {
+  uint32_t row0, ctx, nodes, b;  // the sequence: first pool row, context rows, nodes
+  uint32_t blk, nb, hkv, tile0;
+  uint32_t tiles;                // 1 or 2; 0: no more pieces
+  uint32_t whole;                // the unit is this piece: its outputs are final
+  uint32_t x0, n0, q0;           // turns, blocks and Q tiles of this CTA before it
+  uint32_t pad[3];
 };
-static_assert(sizeof(Plan) <= 48, "plan");
+static_assert(sizeof(Piece) == 64, "piece");
 
 // ---- workspace: [0, 256) an error word nobody reads (when the caller gives
 // none), MergeDesc per CTA, then per CTA two slots (the piece its range begins
@@ -191,52 +199,6 @@ __device__ __forceinline__ Unit unit_of(const TParams& p, uint32_t u) {
   return r;
 }
 
-// The pieces of a CTA's range: blocks [blk, blk + nb) of unit u of sequence b.
-// The line that is cut into ranges is as long as the blocks' costs; a cut
-// inside a block gives the block to the CTA before the cut.
-struct Pieces {
-  int64_t left;
-  uint32_t b, u, blk, nb, nblk, cost;
-  TreeSeq s;
-  Unit un;
-  nwd::TreeRaw ahead;  // sequence b + 1's entries, on their way since sequence b was entered
-  __device__ __forceinline__ void load(const TParams& p) {
-    s = nwd::tree_seq(ahead, p.pool_rows, p.n_nodes, nullptr);
-    nblk = uniform(seq_blocks(s));
-    if (b + 1 < p.batch) ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, b + 1, p.n_nodes);
-  }
-  __device__ __forceinline__ void enter(const TParams& p) {
-    un = unit_of(p, u);
-    cost = un.tiles == 2 ? p.cost2 : p.cost1;
-    const uint64_t most = (uint64_t)(nblk - blk) * cost;
-    nb = (uint64_t)left >= most ? nblk - blk : ((uint32_t)left + cost - 1) / cost;
-  }
-  __device__ __forceinline__ bool begin(const TParams& p, const Plan& plan) {
-    left = (int64_t)((uint64_t)uniform((uint32_t)((uint64_t)plan.left >> 32)) << 32 |
-                     uniform((uint32_t)plan.left));
-    b = uniform(plan.b);
-    u = uniform(plan.u);
-    blk = uniform(plan.blk);
-    if (left <= 0) return false;
-    ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, b, p.n_nodes);
-    load(p);
-    enter(p);
-    return true;
-  }
-  __device__ __forceinline__ bool next(const TParams& p) {
-    left -= (int64_t)nb * cost;
-    if (left <= 0) return false;
-    blk = 0;
-    if (++u == p.n_units) {
-      u = 0;
-      b++;
-      load(p);
-    }
-    enter(p);
-    return true;
-  }
-};
-
 // Position in a ring of N stages.
 template <uint32_t N>
 struct Ring {
@@ -254,164 +216,211 @@ struct Ring {
   }
 };
 
-// The turns of one softmax group: the index (in this CTA) of a turn's block
-// and of its Q tile.  x0: turns of both groups before the piece.
-struct Own {
-  Pieces w;
-  bool two, first;
-  uint32_t x0, j;
-  uint32_t n, n0;  // index of block j, of the piece's first block
-  uint32_t q, q0;  // index of the group's tile, of the piece's first tile
-  // the piece's first turn of group g, or the next piece's that has one
-  __device__ __forceinline__ bool settle(const TParams& p, uint32_t g) {
-    for (;;) {
-      two = w.un.tiles == 2;
-      const uint32_t mine = (g - x0) & 1;  // two tiles: the tile; one: the first block
-      j = two ? 0 : mine;
-      if (j < w.nb) {
-        first = true;
-        n = n0 + j;
-        q = q0 + (two ? mine : 0);
-        return true;
-      }
-      if (!leave(p)) return false;
+// What every warp of a CTA knows.
+struct Ctx {
+  uint8_t* smem;
+  uint32_t sb, bar;  // shared memory, its barriers
+  volatile int32_t* abort_flag;
+  uint32_t* err;
+  __device__ __forceinline__ bool wait(int b, uint32_t parity) const {
+    return warp_wait(bar + 8 * b, parity, abort_flag, err);
+  }
+  __device__ __forceinline__ void arrive(int b) const { mbar_arrive(bar + 8 * b); }
+};
+
+// A warp's way through the piece descriptors.
+struct PieceIn {
+  Ring<NP> r;
+  // the next piece; false: there is none (or the CTA is aborting, then !ok)
+  __device__ __forceinline__ bool get(const Ctx& c, Piece& d, bool& ok) {
+    if (!c.wait(B_PCFULL + (int)r.i, r.phase)) {
+      ok = false;
+      return false;
     }
-  }
-  __device__ __forceinline__ bool leave(const TParams& p) {
-    n0 += w.nb;
-    q0 += two ? 2 : 1;
-    x0 += two ? 2 * w.nb : w.nb;
-    return w.next(p);
-  }
-  __device__ __forceinline__ bool begin(const TParams& p, const Plan& plan, uint32_t g) {
-    x0 = n0 = q0 = 0;
-    return w.begin(p, plan) && settle(p, g);
-  }
-  __device__ __forceinline__ bool last() const { return j + (two ? 1 : 2) >= w.nb; }
-  __device__ __forceinline__ bool next(const TParams& p, uint32_t g) {
-    const uint32_t step = two ? 1 : 2;
-    if ((j += step) < w.nb) {
-      first = false;
-      n += step;
-      return true;
-    }
-    return leave(p) && settle(p, g);
+    d = reinterpret_cast<const Piece*>(c.smem + O_PIECE)[r.i];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) c.arrive(B_PCEMPTY + (int)r.i);
+    r.next();
+    return d.tiles != 0;
   }
 };
 
-// An issuer's way through the stages of a ring.  Both groups' issuers wait for every
-// copy, in order, and release it, the ones that only the other group uses
-// too: a parity wait cannot tell a phase from the one two before or after it,
-// so nobody may fall, or run, two uses of a stage behind the others.
+// An issuer's way through the stages of a ring.  Both groups' issuers wait for
+// every copy, in order, and release it, the ones that only the other group
+// uses too: a parity wait cannot tell a phase from the one two before or after
+// it, so nobody may fall, or run, two uses of a stage behind the others.
 template <uint32_t N>
 struct Walker {
-  uint32_t i = 0, phase = 0, n = 0;
+  Ring<N> r;
+  uint32_t n = 0;
   __device__ __forceinline__ void next() {
     n++;
-    if (++i == N) {
-      i = 0;
-      phase ^= 1u;
-    }
+    r.next();
   }
   // waits for copy `to`; the ones before it are released as they land
-  __device__ __forceinline__ bool reach(uint32_t to, uint32_t full, uint32_t empty,
-                                        volatile int32_t* abort_flag, uint32_t* err) {
-    while (n != to) {
-      if (!warp_wait(full + 8 * i, phase, abort_flag, err)) return false;
-      if (elect_one()) mbar_arrive(empty + 8 * i);
+  __device__ __forceinline__ bool reach(const Ctx& c, uint32_t to, int full, int empty) {
+    for (;;) {
+      if (!c.wait(full + (int)r.i, r.phase)) return false;
+      if (n == to) return true;
+      if (elect_one()) c.arrive(empty + (int)r.i);
       next();
     }
-    return warp_wait(full + 8 * i, phase, abort_flag, err);
   }
 };
 
-// a / b, by the 32-bit division where both fit it (nearly always: the 64-bit
-// one takes about half a microsecond of the plan each time).
+// a / b, by the 32-bit division where both fit it (nearly always), else bit by
+// bit: the compiler's 64-bit division is some hundred instructions wherever it
+// stands, and this kernel's code has to fit the instruction cache.
 __device__ __forceinline__ uint64_t div_small(uint64_t a, uint64_t b) {
-  return ((a | b) >> 32) == 0 ? (uint64_t)((uint32_t)a / (uint32_t)b) : a / b;
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  uint64_t q = 0, r = 0;
+#pragma unroll 1
+  for (int i = 63; i >= 0; i--) {
+    r = r << 1 | ((a >> i) & 1);
+    q <<= 1;
+    if (r >= b) {
+      r -= b;
+      q |= 1;
+    }
+  }
+  return q;
 }
 
-// This CTA's range of the line of blocks.  Called by all threads; `sums` is
-// shared scratch.  per = the range length, the same in every CTA.
-__device__ void make_plan(const TParams& p, uint64_t* sums, Plan* plan, MergeDesc* desc) {
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t groups = (p.batch + 31) / 32;
-  auto blocks_of = [&](uint32_t b) {
-    return b < p.batch ? seq_blocks(load_seq(p, b, p.err)) : 0u;
+// The planner (one warp): this CTA's range, its join, and its pieces.
+//
+// The line that is cut into equal ranges is as long as the blocks' costs; a
+// cut inside a block gives the block to the CTA before the cut.
+__device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
+  const uint32_t lane = threadIdx.x & 31;
+  const uint32_t groups = (p.batch + 31) / 32, per_head = p.n_units / p.n_kv;
+  const uint32_t seq_cost = p.n_kv * p.head_cost;  // of a sequence per block of its length
+  auto cost_of = [&](uint32_t tiles) { return tiles == 2 ? p.cost2 : p.cost1; };
+  // blocks of 32 sequences at a time; lane l keeps group l's
+  auto group_blocks = [&](uint32_t g, uint32_t* err) -> uint32_t {
+    const uint32_t i = g * 32 + lane;
+    return i < p.batch ? seq_blocks(load_seq(p, i, err)) : 0u;
   };
-  for (uint32_t g = warp; g < groups; g += THREADS / 32) {
-    const uint32_t n = __reduce_add_sync(0xffffffffu, blocks_of(g * 32 + lane));
-    if (lane == 0) sums[g] = n;
+  uint32_t kept = 0;
+  uint64_t total = 0;
+#pragma unroll 2
+  for (uint32_t g = 0; g < groups; g++) {
+    const uint32_t sum = __reduce_add_sync(0xffffffffu, group_blocks(g, p.err));
+    if (lane == g) kept = sum;
+    total += sum;
   }
-  __syncthreads();
-  if (warp == 0) {
-    // lane l holds groups 4 l .. 4 l + 3
-    uint64_t mine = 0;
-    for (uint32_t g = lane * 4; g < min(groups, lane * 4 + 4); g++) mine += sums[g];
-    uint64_t incl = mine;
+  total *= seq_cost;
+  const uint64_t per = max(div_small(total + gridDim.x - 1, gridDim.x), (uint64_t)p.min_cost);
+  const uint64_t x0 = min(total, (uint64_t)blockIdx.x * per), x1 = min(total, x0 + per);
+  MergeDesc join{0, 0, 0, 0};
+  int64_t left = 0;
+  uint32_t b = 0, u = 0, blk = 0;
+  TreeSeq s{};
+  uint32_t nblk = 0;
+  if (x1 > x0) {
+    // the sequence that x0 falls into: its group, then its lane
+    const uint64_t y = div_small(x0, seq_cost);  // in blocks of sequence length
+    uint64_t base = 0, upto64 = kept;
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) {
-      const uint64_t y = __shfl_up_sync(0xffffffffu, incl, i);
-      if ((int)lane >= i) incl += y;
+      const uint64_t v = __shfl_up_sync(0xffffffffu, upto64, i);
+      if ((int)lane >= i) upto64 += v;
     }
-    const uint32_t seq_cost = p.n_kv * p.head_cost;  // of a sequence per block of its length
-    const uint64_t total = __shfl_sync(0xffffffffu, incl, 31) * seq_cost;
-    const uint64_t per = max(div_small(total + gridDim.x - 1, gridDim.x), (uint64_t)p.min_cost);
-    const uint64_t x0 = min(total, (uint64_t)blockIdx.x * per), x1 = min(total, x0 + per);
-    MergeDesc d{0, 0, 0, 0};
-    Plan pl{};
-    if (x1 > x0) {
-      const uint64_t y = div_small(x0, seq_cost);  // in blocks of sequence length
-      uint64_t base = incl - mine;
-      const uint32_t owner =
-          __ffs(__ballot_sync(0xffffffffu, base <= y && y < incl)) - 1;
-      uint32_t g = lane * 4;
-      if (lane == owner)
-        while (y >= base + sums[g]) base += sums[g++];
-      g = __shfl_sync(0xffffffffu, g, owner);
-      base = __shfl_sync(0xffffffffu, base, owner);
-      const uint32_t n = blocks_of(g * 32 + lane);
-      uint32_t upto = n;
+    uint32_t group;
+    const uint32_t hit = __ballot_sync(0xffffffffu, y < upto64);
+    if (hit) {
+      group = (uint32_t)__ffs(hit) - 1;
+      base = __shfl_sync(0xffffffffu, upto64 - kept, (int)group);
+    } else {  // past the first 1024 sequences
+      base = __shfl_sync(0xffffffffu, upto64, 31);
+      for (group = 32;; group++) {
+        const uint32_t sum = __reduce_add_sync(0xffffffffu, group_blocks(group, nullptr));
+        if (y < base + sum) break;
+        base += sum;
+      }
+    }
+    b = group * 32 + lane;
+    if (b < p.batch) s = load_seq(p, b, nullptr);
+    nblk = b < p.batch ? seq_blocks(s) : 0u;
+    uint32_t upto = nblk;
 #pragma unroll
-      for (int i = 1; i < 32; i <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, i);
-        if ((int)lane >= i) upto += v;
-      }
-      const uint64_t lo = base + upto - n;
-      const uint32_t at = __ffs(__ballot_sync(0xffffffffu, lo <= y && y < lo + n)) - 1;
-      if (lane == at) {
-        // the unit of this sequence that x0 falls into, and where it starts
-        const uint64_t of_head = (uint64_t)n * p.head_cost, of_pair = (uint64_t)n * p.cost2;
-        uint64_t r = x0 - lo * seq_cost;
-        const uint32_t head = (uint32_t)div_small(r, of_head), per_head = p.n_units / p.n_kv;
-        r -= head * of_head;
-        const uint32_t k = min((uint32_t)div_small(r, of_pair), per_head - 1);
-        r -= k * of_pair;
-        const uint64_t start = x0 - r;  // of the unit, on the line
-        pl.b = g * 32 + lane;
-        pl.u = head * per_head + k;
-        const uint32_t cost = unit_of(p, pl.u).tiles == 2 ? p.cost2 : p.cost1;
-        pl.blk = (uint32_t)div_small(r + cost - 1, cost);
-        pl.left = (int64_t)(x1 - start) - (int64_t)((uint64_t)pl.blk * cost);
-        if (pl.blk < n) {
-          if (pl.blk > 0 && pl.left > 0 && pl.blk + div_small(pl.left + cost - 1, cost) >= n)
-            d = MergeDesc{1, pl.b, pl.u, (uint32_t)div_small(start, per)};
-        } else {  // the unit's last block is the CTA's before: on to the next unit
-          pl.blk = 0;
-          if (++pl.u == p.n_units) {
-            pl.u = 0;
-            pl.b++;
-          }
-        }
-        *plan = pl;
-        desc[blockIdx.x] = d;
-      }
-    } else if (lane == 0) {
-      *plan = pl;
-      desc[blockIdx.x] = d;
+    for (int i = 1; i < 32; i <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, i);
+      if ((int)lane >= i) upto += v;
     }
+    const int at = __ffs(__ballot_sync(0xffffffffu, y < base + upto)) - 1;
+    base += __shfl_sync(0xffffffffu, upto - nblk, at);
+    b = group * 32 + (uint32_t)at;
+    nblk = __shfl_sync(0xffffffffu, nblk, at);
+    s.row0 = __shfl_sync(0xffffffffu, s.row0, at);
+    s.ctx = __shfl_sync(0xffffffffu, s.ctx, at);
+    s.nodes = __shfl_sync(0xffffffffu, s.nodes, at);
+    // the unit of this sequence that x0 falls into, and where it starts
+    const uint64_t of_head = (uint64_t)nblk * p.head_cost, of_pair = (uint64_t)nblk * p.cost2;
+    uint64_t r = x0 - base * seq_cost;
+    const uint32_t head = (uint32_t)div_small(r, of_head);
+    r -= head * of_head;
+    const uint32_t k = min((uint32_t)div_small(r, of_pair), per_head - 1);
+    r -= k * of_pair;
+    const uint64_t start = x0 - r;  // of the unit, on the line
+    u = head * per_head + k;
+    const uint32_t cost = cost_of(unit_of(p, u).tiles);
+    blk = (uint32_t)div_small(r + cost - 1, cost);
+    left = (int64_t)(x1 - start) - (int64_t)((uint64_t)blk * cost);
+    if (blk > 0 && blk < nblk && left > 0 && blk + div_small(left + cost - 1, cost) >= nblk)
+      join = MergeDesc{1, b, u, (uint32_t)div_small(start, per)};
   }
-  __syncthreads();
+  if (lane == 0) reinterpret_cast<MergeDesc*>(p.ws + WS_DESC)[blockIdx.x] = join;
+
+  Ring<NP> r;
+  uint32_t turns = 0, blocks = 0, tiles = 0;
+  nwd::TreeRaw ahead{};
+  if (left > 0 && b + 1 < p.batch)
+    ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, b + 1, p.n_nodes);
+  for (;;) {
+    Piece d{};
+    if (left > 0 && blk == nblk) {  // on to the next unit (at the start: its last block is the
+      blk = 0;                      // CTA's before)
+      if (++u == p.n_units) {
+        u = 0;
+        b++;
+        s = nwd::tree_seq(ahead, p.pool_rows, p.n_nodes, nullptr);
+        nblk = seq_blocks(s);
+        if (b + 1 < p.batch)
+          ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, b + 1, p.n_nodes);
+      }
+    }
+    if (left > 0) {
+      const Unit un = unit_of(p, u);
+      const uint32_t cost = cost_of(un.tiles);
+      const uint64_t most = (uint64_t)(nblk - blk) * cost;
+      d.nb = (uint64_t)left >= most ? nblk - blk : ((uint32_t)left + cost - 1) / cost;
+      d.row0 = (uint32_t)s.row0;
+      d.ctx = s.ctx;
+      d.nodes = s.nodes;
+      d.b = b;
+      d.blk = blk;
+      d.hkv = un.hkv;
+      d.tile0 = un.tile0;
+      d.tiles = un.tiles;
+      d.whole = d.nb == nblk;
+      d.x0 = turns;
+      d.n0 = blocks;
+      d.q0 = tiles;
+      turns += d.nb * un.tiles;
+      blocks += d.nb;
+      tiles += un.tiles;
+      left -= (int64_t)d.nb * cost;
+      blk += d.nb;
+    }
+    if (!c.wait(B_PCEMPTY + (int)r.i, r.phase ^ 1u)) break;
+    if (lane == 0) {
+      reinterpret_cast<Piece*>(c.smem + O_PIECE)[r.i] = d;
+      c.arrive(B_PCFULL + (int)r.i);
+    }
+    __syncwarp();
+    r.next();
+    if (d.tiles == 0) break;
+  }
 }
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -477,42 +486,46 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* v) {
                : "memory");
 }
 
-// Stores 4 columns (from column c) of a partial's row.
-__device__ __forceinline__ void store_part(float* slot, uint32_t row, uint32_t c, const float* v) {
-  *reinterpret_cast<float4*>(slot + ((size_t)(c >> 2) * BM + row) * 4) =
-      make_float4(v[0], v[1], v[2], v[3]);
+// Before a CTA that gives up can exit: waits, within the limit, for a phase, and
+// for the last of `issued` copies into each stage of a ring.
+__device__ __forceinline__ void land_one(const Ctx& c, int b, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(c.bar + 8 * b, parity) && globaltimer() - t0 < WAIT_LIMIT_NS) {
+  }
+}
+template <uint32_t N>
+__device__ __forceinline__ void land(const Ctx& c, int full, uint32_t issued) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < N; i++) {
+    const uint32_t uses = (issued + N - 1 - i) / N;
+    if (uses) land_one(c, full + (int)i, (uses - 1) & 1);
+  }
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
     tree_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                 const __grid_constant__ CUtensorMap tmv, const __grid_constant__ TParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  const uint32_t sb = smem_u32(smem);
-  const uint32_t bar = sb + O_BAR;  // + 8 * index
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + O_MISC);
-  volatile int32_t* abort_flag = reinterpret_cast<int32_t*>(smem + O_MISC + 4);
   volatile uint64_t* vbad = reinterpret_cast<uint64_t*>(smem + O_VBAD);
   volatile uint64_t* gbad = reinterpret_cast<uint64_t*>(smem + O_GBAD);
-  const Plan& plan = *reinterpret_cast<const Plan*>(smem + O_PLAN);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint32_t* const err = p.err;
+  const Ctx c{smem, smem_u32(smem), smem_u32(smem) + O_BAR,
+              reinterpret_cast<int32_t*>(smem + O_MISC + 4), p.err};
 
   nwd::pdl_trigger();
-  if (tid == 0) {
-    *abort_flag = 0;
-    for (int i = 0; i < NBAR; i++) {
+  if (warp == 1) {
+    if (lane == 0) *c.abort_flag = 0;
+    for (int i = lane; i < NBAR; i += 32) {
       uint32_t count = 1;
-      if (i >= B_PFULL && i < B_PFULL + 4) count = BM;
-      if (i >= B_OEMPTY && i < B_OEMPTY + 2) count = BM;
-      if (i >= B_ML && i < B_ML + 2) count = BM;
       // a stage is released by both groups' issuers
-      if ((i >= B_QEMPTY && i < B_QEMPTY + (int)NQ) || (i >= B_KEMPTY && i < B_KEMPTY + (int)NK) ||
-          (i >= B_VEMPTY && i < B_VEMPTY + (int)NV))
+      if ((i >= B_QEMPTY && i < B_KFULL) || (i >= B_KEMPTY && i < B_VFULL) ||
+          (i >= B_VEMPTY && i < B_VTMA))
         count = 2;
-      // a V block by its producer, twice, or by the two warps that mend a tail
-      if (i >= B_VFULL && i < B_VFULL + (int)NV) count = 2;
+      if ((i >= B_PFULL && i < B_PVDONE) || (i >= B_OEMPTY && i < B_DRAIN)) count = BM;
       if (i == B_DRAIN) count = 4;
-      mbar_init(bar + 8 * i, count);
+      if (i >= B_PCEMPTY) count = PIECE_USERS;
+      mbar_init(c.bar + 8 * i, count);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -523,224 +536,181 @@ __global__ void __launch_bounds__(THREADS, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (tid == 32) {
+  if (tid == 64) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmq)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmk)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmv)) : "memory");
   }
-  nwd::pdl_wait();
-  make_plan(p, reinterpret_cast<uint64_t*>(smem + O_ML),
-            reinterpret_cast<Plan*>(smem + O_PLAN),
-            reinterpret_cast<MergeDesc*>(p.ws + WS_DESC));
-  if (tid == 0 && (sb & 1023u)) {  // the swizzled tiles would not line up: no work
-    reinterpret_cast<Plan*>(smem + O_PLAN)->left = 0;
-    atomicOr(err, NWD_DEVERR_PIPE_TIMEOUT);
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  nwd::pdl_wait();
+  if (c.sb & 1023u) {  // the swizzled tiles would not line up: no work
+    *c.abort_flag = 1;
+    if (tid == 0) atomicOr(p.err, NWD_DEVERR_PIPE_TIMEOUT);
+  }
   const uint32_t tmem = *tmem_slot;
+  PieceIn in;
+  Piece d;
+  bool ok = true;
 
   // Registers per thread: 48 for the first two warpgroups, 152 for the softmax
   // groups, 80 for the epilogue: 128 * (2 * 48 + 2 * 152 + 80) = 61440, the
   // 640 * 96 of the launch.
   if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;" ::: "memory");
+    // K and V are read once, unless a head's query rows are several units
+    const uint64_t policy = p.n_units == p.n_kv ? evict_first_policy() : evict_last_policy();
     if (warp == 0) {
       // ======================= K =======================
-      const uint64_t policy = p.n_units == p.n_kv ? evict_first_policy() : evict_last_policy();
-      uint32_t issued[NK] = {};
       Ring<NK> r;
-      Pieces w;
-      bool ok = true;
-      for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
-        const int hkv = (int)w.un.hkv;
-        for (uint32_t j = 0; j < w.nb; j++) {
-          if (!warp_wait(bar + 8 * (B_KEMPTY + r.i), r.phase ^ 1u, abort_flag, err)) {
-            ok = false;
-            break;
-          }
+      uint32_t issued = 0;
+      while (ok && in.get(c, d, ok)) {
+        int row = (int)(d.row0 + d.blk * BN);
+#pragma unroll 1
+        for (uint32_t j = 0; j < d.nb; j++, row += BN) {
+          ok = c.wait(B_KEMPTY + (int)r.i, r.phase ^ 1u);
+          if (!ok) break;
           if (lane == 0) {
-            const uint32_t fb = bar + 8 * (B_KFULL + r.i), dst = sb + O_K + r.i * TILE;
-            const int row = (int)(w.s.row0 + (int64_t)(w.blk + j) * BN);
+            const uint32_t fb = c.bar + 8 * (B_KFULL + r.i), dst = c.sb + O_K + r.i * TILE;
             mbar_arrive_tx(fb, TILE);
-            tma_load_4d(dst, &tmk, fb, 0, 0, hkv, row, policy);
-            tma_load_4d(dst + CHUNK, &tmk, fb, 0, 1, hkv, row, policy);
+            tma_load_4d(dst, &tmk, fb, 0, 0, (int)d.hkv, row, policy);
+            tma_load_4d(dst + CHUNK, &tmk, fb, 0, 1, (int)d.hkv, row, policy);
           }
           __syncwarp();
-#pragma unroll
-          for (uint32_t i = 0; i < NK; i++) issued[i] += r.i == i;
           r.next();
+          issued++;
         }
       }
-      if (!ok) {  // let the copies in flight land before the CTA can exit
-        const uint64_t t0 = globaltimer();
-#pragma unroll
-        for (uint32_t i = 0; i < NK; i++)
-          if (issued[i])
-            while (!mbar_try_wait(bar + 8 * (B_KFULL + i), (issued[i] - 1) & 1) &&
-                   globaltimer() - t0 < WAIT_LIMIT_NS) {
-            }
-      }
+      if (!ok) land<NK>(c, B_KFULL, issued);
     } else if (warp == 1) {
       // ======================= V and Q =======================
       // The next piece's Q goes out as soon as its buffers are free, looked
       // for with every V block; with the piece's last one it is waited for.
-      const uint64_t policy = p.n_units == p.n_kv ? evict_first_policy() : evict_last_policy();
       const uint64_t q_policy = evict_first_policy();
       const uint32_t q_bytes = 2 * p.tile_nodes * p.group * 128;
-      uint32_t issued[NV] = {}, tails[NV] = {}, q_issued[NQ] = {};
       Ring<NV> r;
       Ring<NQ> rq;
-      Pieces w, wq;
-      bool ok = true;
-      bool more_q = wq.begin(p, plan);
-      uint32_t q_tile = 0;  // next tile of wq's piece to load
-      auto load_q = [&](bool block) -> bool {
-        while (q_tile < wq.un.tiles) {
-          const uint32_t empty = bar + 8 * (B_QEMPTY + rq.i);
-          if (block) {
-            if (!warp_wait(empty, rq.phase ^ 1u, abort_flag, err)) return false;
-          } else if (!__all_sync(0xffffffffu, mbar_test_wait(empty, rq.phase ^ 1u))) {
-            return true;
+      uint32_t issued = 0, q_issued = 0, tails = 0, q_tile = 0;
+      auto load_q = [&](const Piece& e, bool block) -> bool {
+        while (q_tile < e.tiles) {
+          const int empty = B_QEMPTY + (int)rq.i;
+          if (!__all_sync(0xffffffffu, mbar_test_wait(c.bar + 8 * empty, rq.phase ^ 1u))) {
+            if (!block) return true;
+            if (!c.wait(empty, rq.phase ^ 1u)) return false;
           }
           if (lane == 0) {
-            const uint32_t fb = bar + 8 * (B_QFULL + rq.i), dst = sb + O_Q + rq.i * Q_TILE;
-            const int node = (int)(wq.b * p.n_nodes + (wq.un.tile0 + q_tile) * p.tile_nodes);
+            const uint32_t fb = c.bar + 8 * (B_QFULL + rq.i), dst = c.sb + O_Q + rq.i * Q_TILE;
+            const int node = (int)(e.b * p.n_nodes + (e.tile0 + q_tile) * p.tile_nodes);
             mbar_arrive_tx(fb, q_bytes);
-            tma_load_5d(dst, &tmq, fb, 0, 0, 0, (int)wq.un.hkv, node, q_policy);
-            tma_load_5d(dst + Q_CHUNK, &tmq, fb, 0, 1, 0, (int)wq.un.hkv, node, q_policy);
+            tma_load_5d(dst, &tmq, fb, 0, 0, 0, (int)e.hkv, node, q_policy);
+            tma_load_5d(dst + Q_CHUNK, &tmq, fb, 0, 1, 0, (int)e.hkv, node, q_policy);
           }
           __syncwarp();
-#pragma unroll
-          for (uint32_t i = 0; i < NQ; i++) q_issued[i] += rq.i == i;
           rq.next();
+          q_issued++;
           q_tile++;
         }
         return true;
       };
-      auto next_q = [&]() {  // on to the piece whose Q comes next
-        more_q = wq.next(p);
+      Piece e;  // the piece after d
+      bool more = in.get(c, e, ok);
+      d.nb = 0;
+      while (ok) {
+        // d's blocks, with e's Q (at first only e's Q)
+        int row = (int)(d.row0 + d.blk * BN);
+        uint32_t j = 0;
+#pragma unroll 1
+        do {
+          if (j < d.nb) {
+            ok = c.wait(B_VEMPTY + (int)r.i, r.phase ^ 1u);
+            if (!ok) break;
+            // a block with rows of the tree, or behind it, completes on VTMA:
+            // warp 2 releases it to its users
+            const bool tail = (d.blk + j + 1) * BN > d.ctx;
+            if (lane == 0) {
+              const uint32_t fb = c.bar + 8 * ((tail ? B_VTMA : B_VFULL) + (int)r.i);
+              const uint32_t dst = c.sb + O_V + r.i * TILE;
+              mbar_arrive_tx(fb, TILE);
+              tma_load_4d(dst, &tmv, fb, 0, 0, (int)d.hkv, row, policy);
+              tma_load_4d(dst + CHUNK, &tmv, fb, 0, 1, (int)d.hkv, row, policy);
+            }
+            __syncwarp();
+            if (tail) tails ^= 1u << r.i;
+            r.next();
+            issued++;
+            row += BN;
+          }
+          j++;
+          if (more) ok = load_q(e, j >= d.nb);
+        } while (ok && j < d.nb);
+        if (!ok || !more) break;
+        d = e;
+        more = in.get(c, e, ok);
         q_tile = 0;
-      };
-      if (more_q) {
-        ok = load_q(true);
-        next_q();
-      }
-      for (bool more = ok && w.begin(p, plan); more && ok; more = w.next(p)) {
-        const int hkv = (int)w.un.hkv;
-        for (uint32_t j = 0; j < w.nb; j++) {
-          if (!warp_wait(bar + 8 * (B_VEMPTY + r.i), r.phase ^ 1u, abort_flag, err)) {
-            ok = false;
-            break;
-          }
-          const uint32_t key0 = (w.blk + j) * BN;
-          // a block with rows of the tree, or behind it, completes on VTMA:
-          // warps 2 and 3 release it to its users
-          const bool tail = key0 + BN > w.s.ctx;
-          if (lane == 0) {
-            const uint32_t fb = bar + 8 * ((tail ? B_VTMA : B_VFULL) + (int)r.i);
-            const uint32_t dst = sb + O_V + r.i * TILE;
-            const int row = (int)(w.s.row0 + key0);
-            if (!tail) mbar_arrive(fb);
-            mbar_arrive_tx(fb, TILE);
-            tma_load_4d(dst, &tmv, fb, 0, 0, hkv, row, policy);
-            tma_load_4d(dst + CHUNK, &tmv, fb, 0, 1, hkv, row, policy);
-          }
-          __syncwarp();
-#pragma unroll
-          for (uint32_t i = 0; i < NV; i++) {
-            issued[i] += !tail && r.i == i;
-            tails[i] += tail && r.i == i;
-          }
-          r.next();
-          if (more_q && !load_q(j + 1 == w.nb)) {
-            ok = false;
-            break;
-          }
-        }
-        if (ok && more_q) next_q();
       }
       if (!ok) {
-        const uint64_t t0 = globaltimer();
-#pragma unroll
-        for (uint32_t i = 0; i < NV; i++) {
-          // (a block's last completion on VFULL may be warp 2's and 3's, of a tail)
-          if (issued[i] + tails[i])
-            while (!mbar_try_wait(bar + 8 * (B_VFULL + i), (issued[i] + tails[i] - 1) & 1) &&
-                   globaltimer() - t0 < WAIT_LIMIT_NS) {
-            }
-          if (tails[i])
-            while (!mbar_try_wait(bar + 8 * (B_VTMA + i), (tails[i] - 1) & 1) &&
-                   globaltimer() - t0 < WAIT_LIMIT_NS) {
-            }
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < NQ; i++)
-          if (q_issued[i])
-            while (!mbar_try_wait(bar + 8 * (B_QFULL + i), (q_issued[i] - 1) & 1) &&
-                   globaltimer() - t0 < WAIT_LIMIT_NS) {
-            }
+        // (a block's last completion on VFULL may be warp 2's, of a tail)
+        land<NV>(c, B_VFULL, issued);
+        land<NQ>(c, B_QFULL, q_issued);
+        for (uint32_t i = 0; i < NV; i++) land_one(c, B_VTMA + (int)i, ((tails >> i) & 1u) ^ 1u);
       }
-    } else if (warp < 4) {
+    } else if (warp == 2) {
       // ======================= V blocks with rows of the tree =======================
       // Rows behind the tree become zeros (0 x NaN would be NaN), NaN and
-      // infinities in the tree's rows too; which rows had some is noted.  Warp
-      // 2 has a block's first 64 columns, warp 3 the others.
-      const uint32_t half = (uint32_t)warp - 2;
+      // infinities in the tree's rows too; which rows had some is noted.
       uint32_t phases = 0;  // of VTMA, bit i: stage i
       Ring<NV> r;
-      Pieces w;
-      bool ok = true;
-      for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
+      while (ok && in.get(c, d, ok)) {
         // the blocks before the tree's first row are not this warp's
-        const uint32_t from = w.s.ctx / BN, skip = from > w.blk ? min(from - w.blk, w.nb) : 0;
+        const uint32_t from = d.ctx / BN, skip = from > d.blk ? min(from - d.blk, d.nb) : 0;
         r.add(skip);
-        for (uint32_t j = skip; j < w.nb; j++, r.next()) {
-          const uint32_t key0 = (w.blk + j) * BN, rows = w.s.ctx + w.s.nodes;
-          if (!warp_wait(bar + 8 * (B_VTMA + r.i), (phases >> r.i) & 1u, abort_flag, err)) {
-            ok = false;
-            break;
-          }
+#pragma unroll 1
+        for (uint32_t j = skip; j < d.nb; j++, r.next()) {
+          ok = c.wait(B_VTMA + (int)r.i, (phases >> r.i) & 1u);
+          if (!ok) break;
           phases ^= 1u << r.i;
-          const uint32_t t0 = w.s.ctx > key0 ? w.s.ctx - key0 : 0;
+          const uint32_t key0 = (d.blk + j) * BN, rows = d.ctx + d.nodes;
+          const uint32_t t0 = d.ctx > key0 ? d.ctx - key0 : 0;
           const uint32_t t1 = max(rows > key0 ? min(rows - key0, BN) : 0u, t0);
           // 8 uint4 of a row per chunk (a swizzled row stays within its 128
           // bytes): lane l has those of rows l / 8, l / 8 + 4, ..
-          uint4* st = reinterpret_cast<uint4*>(smem + O_V + r.i * TILE + half * CHUNK) + lane;
+          uint4* st = reinterpret_cast<uint4*>(smem + O_V + r.i * TILE) + lane;
           uint64_t bad = 0;
 #pragma unroll 1
-          for (uint32_t i0 = 0; i0 < BN / 4; i0 += 4) {
-            uint4 x[4];
+          for (uint32_t i = t0 / 4; i < BN / 4; i++) {
+            const uint32_t row = i * 4 + (uint32_t)lane / 8;
+            uint4 x[2] = {st[i * 32], st[CHUNK / 16 + i * 32]};
+            if (row < t0) continue;
 #pragma unroll
-            for (uint32_t i = 0; i < 4; i++) x[i] = st[(i0 + i) * 32];
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-              const uint32_t row = (i0 + i) * 4 + (uint32_t)lane / 8;
-              if (row < t0) continue;
-              uint32_t* e = &x[i].x;
+            for (int h = 0; h < 2; h++) {
+              uint32_t* w = &x[h].x;
               bool hit = row >= t1;
 #pragma unroll
               for (int k = 0; k < 4; k++) {
-                const bool lo = (e[k] & 0x7c00u) == 0x7c00u || row >= t1;
-                const bool hi = (e[k] & 0x7c000000u) == 0x7c000000u || row >= t1;
+                const bool lo = (w[k] & 0x7c00u) == 0x7c00u || row >= t1;
+                const bool hi = (w[k] & 0x7c000000u) == 0x7c000000u || row >= t1;
                 hit |= lo | hi;
-                if (lo) e[k] &= 0xffff0000u;
-                if (hi) e[k] &= 0x0000ffffu;
+                if (lo) w[k] &= 0xffff0000u;
+                if (hi) w[k] &= 0x0000ffffu;
               }
-              if (hit) st[(i0 + i) * 32] = x[i];
-              if (hit && row < t1) bad |= 1ull << (key0 + row - w.s.ctx);
+              if (hit) {
+                st[h * (CHUNK / 16) + i * 32] = x[h];
+                if (row < t1) bad |= 1ull << (key0 + row - d.ctx);
+              }
             }
           }
           const uint32_t blo = __reduce_or_sync(0xffffffffu, (uint32_t)bad);
           const uint32_t bhi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32));
-          if (lane == 0) vbad[2 * r.i + half] = (uint64_t)bhi << 32 | blo;
+          if (lane == 0) vbad[r.i] = (uint64_t)bhi << 32 | blo;
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar + 8 * (B_VFULL + r.i));
+          if (lane == 0) c.arrive(B_VFULL + (int)r.i);
         }
       }
-    } else if (warp >= 4) {
+    } else if (warp == 3) {
+      plan(p, c);
+    } else {
       // ======================= MMA issuers =======================
       // The whole warp walks its group's turns x, one lane issues.
       const uint32_t role = uniform((uint32_t)warp - 4);
@@ -748,83 +718,92 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool leader = elect_one();
       const uint32_t tm = uniform(tmem);
       const uint32_t tmem_s = tm + g * 2 * BN;
-      Own t;
-      bool have = t.begin(p, plan, g);
       uint32_t buf = 0, phase = 0;  // of the group's score buffers
       if (role < 2) {
         // ---- S(x), once P V(x - 2) has read the P in its buffer
         Walker<NQ> q;
         Walker<NK> k;
-        uint32_t q_slot = 0;
-        while (have) {
-          if (t.first) {
-            if (!q.reach(t.q, bar + 8 * B_QFULL, bar + 8 * B_QEMPTY, abort_flag, err)) break;
-            q_slot = q.i;
-            q.next();
-          }
-          if (!k.reach(t.n, bar + 8 * B_KFULL, bar + 8 * B_KEMPTY, abort_flag, err) ||
-              !warp_wait(bar + 8 * (B_PVDONE + 2 * g + buf), phase ^ 1u, abort_flag, err))
-            break;
-          tc_fence_after();
-          const uint32_t da = (sb + O_Q + q_slot * Q_TILE) >> 4, db = (sb + O_K + k.i * TILE) >> 4;
-          constexpr uint64_t top = sdesc(0, 16, 1024);
-          if (leader) {
+        while (ok && in.get(c, d, ok)) {
+          const bool two = uniform(d.tiles) == 2;
+          const uint32_t mine = uniform((g - d.x0) & 1);  // two tiles: the tile; one: the first block
+          const uint32_t step = two ? 1 : 2, nb = uniform(d.nb);
+          uint32_t j = two ? 0 : mine;
+          if (j >= nb) continue;
+          ok = q.reach(c, uniform(d.q0) + (two ? mine : 0), B_QFULL, B_QEMPTY);
+          if (!ok) break;
+          const uint32_t da = (c.sb + O_Q + q.r.i * Q_TILE) >> 4;
+          const uint32_t n0 = uniform(d.n0);
+#pragma unroll 1
+          for (; j < nb; j += step) {
+            ok = k.reach(c, n0 + j, B_KFULL, B_KEMPTY) &&
+                 c.wait(B_PVDONE + (int)(2 * g + buf), phase ^ 1u);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t db = (c.sb + O_K + k.r.i * TILE) >> 4;
+            constexpr uint64_t top = sdesc(0, 16, 1024);
+            if (leader) {
 #pragma unroll
-            for (uint32_t kk = 0; kk < 8; kk++)
-              umma(tmem_s + buf * BN, top | (da + (((kk >> 2) * Q_CHUNK + (kk & 3) * 32) >> 4)),
-                   top | (db + (((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4)), IDESC_S, kk > 0);
-            umma_commit(bar + 8 * (B_SFULL + 2 * g + buf));
-            umma_commit(bar + 8 * (B_KEMPTY + k.i));
-            if (t.last()) umma_commit(bar + 8 * (B_QEMPTY + q_slot));
+              for (uint32_t kk = 0; kk < 8; kk++)
+                umma(tmem_s + buf * BN, top | (da + (((kk >> 2) * Q_CHUNK + (kk & 3) * 32) >> 4)),
+                     top | (db + (((kk >> 2) * CHUNK + (kk & 3) * 32) >> 4)), IDESC_S, kk > 0);
+              umma_commit(c.bar + 8 * (B_SFULL + 2 * g + buf));
+              umma_commit(c.bar + 8 * (B_KEMPTY + k.r.i));
+            }
+            __syncwarp();
+            k.next();
+            phase ^= buf;
+            buf ^= 1u;
           }
+          if (leader) umma_commit(c.bar + 8 * (B_QEMPTY + q.r.i));
           __syncwarp();
-          k.next();
-          phase ^= buf;
-          buf ^= 1u;
-          have = t.next(p, g);
+          q.next();
         }
       } else {
         // ---- P V(x)
         const uint32_t tmem_o = tm + TMEM_O + g * HD;
         Walker<NV> v;
-        uint32_t o_units = 0;
-        while (have) {
-          if ((t.first &&
-               !warp_wait(bar + 8 * (B_OEMPTY + g), (o_units & 1) ^ 1, abort_flag, err)) ||
-              !v.reach(t.n, bar + 8 * B_VFULL, bar + 8 * B_VEMPTY, abort_flag, err) ||
-              !warp_wait(bar + 8 * (B_PFULL + 2 * g + buf), phase, abort_flag, err))
-            break;
-          tc_fence_after();
-          // P: key pairs in the buffer's first 32 columns; V MN-major
-          // (head_dim contiguous), its 64-column chunks 8 KiB apart, 16 keys
-          // 2 KiB
-          const uint32_t dv = (sb + O_V + v.i * TILE) >> 4;
-          constexpr uint64_t top = sdesc(0, CHUNK, 1024);
-          if (leader) {
-            umma_ts(tmem_o, tmem_s + buf * BN, top | dv, IDESC_O, !t.first);
+        uint32_t o_phase = 1;
+        while (ok && in.get(c, d, ok)) {
+          const bool two = uniform(d.tiles) == 2;
+          const uint32_t mine = uniform((g - d.x0) & 1);
+          const uint32_t step = two ? 1 : 2, nb = uniform(d.nb), n0 = uniform(d.n0);
+          uint32_t j = two ? 0 : mine;
+          if (j >= nb) continue;
+          ok = c.wait(B_OEMPTY + (int)g, o_phase);
+          o_phase ^= 1u;
+          uint32_t add = 0;
+#pragma unroll 1
+          for (; ok && j < nb; j += step) {
+            ok = v.reach(c, n0 + j, B_VFULL, B_VEMPTY) && c.wait(B_PFULL + (int)(2 * g + buf), phase);
+            if (!ok) break;
+            tc_fence_after();
+            // P: key pairs in the buffer's first 32 columns; V MN-major
+            // (head_dim contiguous), its 64-column chunks 8 KiB apart, 16
+            // keys 2 KiB
+            const uint32_t dv = (c.sb + O_V + v.r.i * TILE) >> 4;
+            constexpr uint64_t top = sdesc(0, CHUNK, 1024);
+            if (leader) {
+              umma_ts(tmem_o, tmem_s + buf * BN, top | dv, IDESC_O, add);
 #pragma unroll
-            for (uint32_t kk = 1; kk < BN / 16; kk++)
-              umma_ts(tmem_o, tmem_s + buf * BN + kk * 8u, top | (dv + ((kk * 16 * 128) >> 4)),
-                      IDESC_O, 1u);
-            umma_commit(bar + 8 * (B_PVDONE + 2 * g + buf));
-            umma_commit(bar + 8 * (B_VEMPTY + v.i));
+              for (uint32_t kk = 1; kk < BN / 16; kk++)
+                umma_ts(tmem_o, tmem_s + buf * BN + kk * 8u, top | (dv + ((kk * 16 * 128) >> 4)),
+                        IDESC_O, 1u);
+              umma_commit(c.bar + 8 * (B_PVDONE + 2 * g + buf));
+              umma_commit(c.bar + 8 * (B_VEMPTY + v.r.i));
+            }
+            __syncwarp();
+            add = 1;
+            v.next();
+            phase ^= buf;
+            buf ^= 1u;
           }
-          __syncwarp();
-          v.next();
-          o_units += t.last();
-          phase ^= buf;
-          buf ^= 1u;
-          have = t.next(p, g);
         }
       }
       // every MMA this warp issued has completed before the tensor memory is
       // released
-      if (leader) umma_commit(bar + 8 * B_DRAIN);
+      if (leader) umma_commit(c.bar + 8 * B_DRAIN);
       __syncwarp();
-      const uint64_t t0 = globaltimer();
-      while (!mbar_try_wait(bar + 8 * B_DRAIN, 0) && globaltimer() - t0 < WAIT_LIMIT_NS) {
-      }
-      __syncwarp();
+      land_one(c, B_DRAIN, 0);
     }
   } else if (warp < 16) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 152;" ::: "memory");
@@ -833,19 +812,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t quad = (uint32_t)warp & 3u;
     const uint32_t r = quad * 32u + (uint32_t)lane;  // row of the tile = tensor memory lane
     const uint32_t lanes = quad * 32u << 16;
-    const uint32_t tmem_o = tmem + TMEM_O + lanes;
-    float2* ml = reinterpret_cast<float2*>(smem + O_ML);
+    const uint32_t tmem_o = tmem + TMEM_O + g * HD + lanes;
     const uint32_t q_node = r / p.group;
-    uint32_t x0 = 0;       // turns before this piece, of both groups
-    uint32_t my_turns = 0, my_units = 0;
-    uint32_t n0 = 0;       // blocks before this piece
-    bool ok = true;
-    Pieces w;
-    for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
-      const Unit un = w.un;
-      const bool two = un.tiles == 2;
-      const uint32_t mine = (g - x0) & 1;  // two tiles: my tile; one: my first block
-      const uint32_t tile = un.tile0 + (two ? mine : 0);
+    uint32_t turn = 0, units = 0;
+    while (ok && in.get(c, d, ok)) {
+      const bool two = d.tiles == 2;
+      const uint32_t mine = (g - d.x0) & 1;  // two tiles: my tile; one: my first block
+      const uint32_t tile = d.tile0 + (two ? mine : 0);
       const uint32_t tile_nodes = min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes);
       const uint32_t node = tile * p.tile_nodes + q_node;
       const bool row_used = q_node < tile_nodes;
@@ -853,8 +826,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       // which rows of the tree this row sees (none if its node is absent):
       // found at the first block that has some, from parents fetched now
       int2 par = make_int2(-1, -1);
-      if ((w.blk + w.nb) * BN > w.s.ctx) {
-        const int32_t* src = p.parents + (size_t)w.b * p.n_nodes;
+      if ((d.blk + d.nb) * BN > d.ctx) {
+        const int32_t* src = p.parents + (size_t)d.b * p.n_nodes;
         if ((uint32_t)lane < p.n_nodes) par.x = src[lane];
         if ((uint32_t)lane + 32 < p.n_nodes) par.y = src[lane + 32];
       }
@@ -863,17 +836,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       float m = -INFINITY, l = 0.f;
       uint64_t bad = 0;
       const uint32_t step = two ? 1 : 2;
-      uint32_t j = two ? 0 : mine;
-      const uint32_t first_turn = my_turns;
-      for (; j < w.nb; j += step) {
-        const uint32_t turn = my_turns++, buf = turn & 1;
+      const uint32_t first_turn = turn;
+#pragma unroll 1
+      for (uint32_t j = two ? 0 : mine; j < d.nb; j += step, turn++) {
+        const uint32_t buf = turn & 1;
         const uint32_t tmem_s = tmem + (2 * g + buf) * BN + lanes;
-        const uint32_t key0 = (w.blk + j) * BN;
-        const bool tail = key0 + BN > w.s.ctx;
-        if (!warp_wait(bar + 8 * (B_SFULL + 2 * g + buf), (turn >> 1) & 1, abort_flag, err)) {
-          ok = false;
-          break;
-        }
+        const uint32_t key0 = (d.blk + j) * BN;
+        const bool tail = key0 + BN > d.ctx;
+        ok = c.wait(B_SFULL + (int)(2 * g + buf), (turn >> 1) & 1);
+        if (!ok) break;
         tc_fence_after();
         if (warp_used) {
           float s[BN];
@@ -883,20 +854,20 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (tail) {
             if (!have_mask) {
               have_mask = true;
-              const uint64_t all = tree_masks(par, p.n_nodes, node, err);
-              sees = row_used && node < w.s.nodes ? all : 0;
+              const uint64_t all = tree_masks(par, p.n_nodes, node, c.err);
+              sees = row_used && node < d.nodes ? all : 0;
             }
-            // bit c of word i: this row attends cache row key0 + 32 i + c
+            // bit k of word i: this row attends cache row key0 + 32 i + k
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-              const int64_t at = (int64_t)key0 + 32 * i - (int64_t)w.s.ctx;  // in the tree
+              const int64_t at = (int64_t)key0 + 32 * i - (int64_t)d.ctx;  // in the tree
               uint32_t ok32;
               if (at <= -32) ok32 = 0xffffffffu;
               else if (at < 0) ok32 = (uint32_t)(sees << -at) | ((1u << -at) - 1u);
               else ok32 = at < 64 ? (uint32_t)(sees >> at) : 0u;
 #pragma unroll
-              for (int c = 0; c < 32; c++)
-                if (!((ok32 >> c) & 1u)) s[32 * i + c] = -INFINITY;
+              for (int k = 0; k < 32; k++)
+                if (!((ok32 >> k) & 1u)) s[32 * i + k] = -INFINITY;
             }
           }
           // The exponentials are taken against the maximum so far, beside the
@@ -911,14 +882,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             sum = sum1 = make_float2(0.f, 0.f);
             float mv[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 32; c++) {
-              const float2 x = fma2(make_float2(s[2 * c], s[2 * c + 1]), sc, nb2);
+            for (int k = 0; k < 32; k++) {
+              const float2 x = fma2(make_float2(s[2 * k], s[2 * k + 1]), sc, nb2);
               const float2 e = make_float2(ex2f(x.x), ex2f(x.y));
-              mv[c & 3] = fmaxf(mv[c & 3], fmaxf(s[2 * c], s[2 * c + 1]));
-              if (c & 1) sum1 = add2(sum1, e);
+              mv[k & 3] = fmaxf(mv[k & 3], fmaxf(s[2 * k], s[2 * k + 1]));
+              if (k & 1) sum1 = add2(sum1, e);
               else sum = add2(sum, e);
               const __half2 hh = __floats2half2_rn(e.x, e.y);
-              pk[c] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&hh));
+              pk[k] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&hh));
             }
             const float mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * p.scale_log2;
             const bool up = mx > m + RESCALE_LOG2;
@@ -928,20 +899,19 @@ __global__ void __launch_bounds__(THREADS, 1)
               if (turn != first_turn) {
                 // O is rescaled once the P V of the group's last turn is in it
                 const uint32_t last = turn - 1;
-                if (!warp_wait(bar + 8 * (B_PVDONE + 2 * g + (last & 1)), (last >> 1) & 1,
-                               abort_flag, err)) {
+                if (!c.wait(B_PVDONE + (int)(2 * g + (last & 1)), (last >> 1) & 1)) {
                   ok = false;
                   break;
                 }
                 tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < 8; c++) {
+                for (int k = 0; k < 8; k++) {
                   float ov[16];
-                  tmem_ld16(tmem_o + g * HD + c * 16, ov);
+                  tmem_ld16(tmem_o + k * 16, ov);
                   tmem_ld_wait();
 #pragma unroll
                   for (int i = 0; i < 16; i++) ov[i] *= alpha;
-                  tmem_st16(tmem_o + g * HD + c * 16, ov);
+                  tmem_st16(tmem_o + k * 16, ov);
                 }
               }
               l *= alpha;
@@ -953,27 +923,24 @@ __global__ void __launch_bounds__(THREADS, 1)
           l += (sum.x + sum.y) + (sum1.x + sum1.y);
           tmem_st_wait();
         }
-        if (tail && quad == 0) {  // V rows with NaN or infinities, noted by warps 2 and 3
-          const uint32_t n = n0 + j;
-          if (!warp_wait(bar + 8 * (B_VFULL + n % NV), (n / NV) & 1, abort_flag, err)) {
-            ok = false;
-            break;
-          }
-          bad |= vbad[2 * (n % NV)] | vbad[2 * (n % NV) + 1];
+        if (tail && quad == 0) {  // V rows with NaN or infinities, noted by warp 2
+          const uint32_t n = d.n0 + j;
+          ok = c.wait(B_VFULL + (int)(n % NV), (n / NV) & 1);
+          if (!ok) break;
+          bad |= vbad[n % NV];
         }
         tc_fence_before();
-        mbar_arrive(bar + 8 * (B_PFULL + 2 * g + buf));
+        c.arrive(B_PFULL + (int)(2 * g + buf));
       }
       if (!ok) break;
-      n0 += w.nb;
-      x0 += w.nb * un.tiles;
-      if (my_turns != first_turn) {
+      if (turn != first_turn) {
         // (m, l) to the epilogue, once it has read the last ones
-        if (!warp_wait(bar + 8 * (B_OEMPTY + g), (my_units & 1) ^ 1, abort_flag, err)) break;
-        my_units++;
-        ml[g * BM + r] = make_float2(m, l);
+        ok = c.wait(B_OEMPTY + (int)g, (units & 1) ^ 1);
+        if (!ok) break;
+        units++;
+        reinterpret_cast<float2*>(smem + O_ML)[g * BM + r] = make_float2(m, l);
         if (r == 0) gbad[g] = bad;
-        mbar_arrive(bar + 8 * (B_ML + g));
+        c.arrive(B_ML + (int)g);
       }
     }
   } else {
@@ -984,128 +951,62 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t tmem_o = tmem + TMEM_O + (quad * 32u << 16);
     const float2* ml = reinterpret_cast<const float2*>(smem + O_ML);
     const uint32_t q_node = r / p.group, q_head = r % p.group;
-    uint32_t x0 = 0;
-    uint32_t turns[2] = {0, 0}, units[2] = {0, 0};  // of each group
     const bool wide = (reinterpret_cast<uintptr_t>(p.o) & 31u) == 0;  // whole sectors per store
+    uint32_t turns = 0, turns1 = 0, units = 0, units1 = 0;  // of group 0, of group 1
     // group i's part of the piece is complete: its (m, l), and its last P V
     auto complete = [&](uint32_t i) -> bool {
-      const uint32_t last = turns[i] - 1;
-      return warp_wait(bar + 8 * (B_ML + i), units[i] & 1, abort_flag, err) &&
-             warp_wait(bar + 8 * (B_PVDONE + 2 * i + (last & 1)), (last >> 1) & 1, abort_flag, err);
+      const uint32_t last = (i ? turns1 : turns) - 1;
+      return c.wait(B_ML + (int)i, (i ? units1 : units) & 1) &&
+             c.wait(B_PVDONE + (int)(2 * i + (last & 1)), (last >> 1) & 1);
     };
-    auto release = [&](uint32_t i) {
-      mbar_arrive(bar + 8 * (B_OEMPTY + i));
-      units[i]++;
-    };
-    bool ok = true;
-    Pieces w;
-    for (bool more = w.begin(p, plan); more && ok; more = w.next(p)) {
-      const Unit un = w.un;
-      const bool two = un.tiles == 2;
-      const bool direct = w.blk == 0 && w.nb == w.nblk;
-      // a row's outputs, from column `col`: 32 columns
-      auto put = [&](uint32_t t, uint32_t col, float* ov, float inv, uint64_t bad) {
-        const uint32_t tile = un.tile0 + t;
-        const uint32_t node = tile * p.tile_nodes + q_node;
-        if (q_node >= min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes)) return;
-        const bool absent = node >= w.s.nodes;
-        if (bad && !absent) {
-          // what was taken out of the V rows that this row sees
-          const uint64_t sees =
-              nwd::tree_mask(p.parents + (size_t)w.b * p.n_nodes, (int)node, nullptr);
-          const __half* v = p.v + (((size_t)w.s.row0 + w.s.ctx) * p.n_kv + un.hkv) * HD + col;
-          for (uint64_t x = bad & sees; x; x &= x - 1) {
-            const __half* src = v + (size_t)(__ffsll((long long)x) - 1) * p.n_kv * HD;
-#pragma unroll
-            for (int i = 0; i < 32; i++) {
-              const float e = __half2float(src[i]);
-              if (!isfinite(e)) ov[i] += e;
-            }
-          }
-        }
-        if (direct) {
-          __half* dst = p.o + (((size_t)w.b * p.n_nodes + node) * p.n_heads + un.hkv * p.group +
-                               q_head) * HD + col;
-          uint32_t h[16];
-#pragma unroll
-          for (int k = 0; k < 16; k++) {
-            const __half2 x = __floats2half2_rn(ov[2 * k] * inv, ov[2 * k + 1] * inv);
-            h[k] = absent ? 0u : *reinterpret_cast<const uint32_t*>(&x);
-          }
-          if (wide) {
-            store32(dst, h);
-            store32(dst + 16, h + 8);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              reinterpret_cast<uint4*>(dst)[i] =
-                  make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-          }
-        } else {
-          float* slot = reinterpret_cast<float*>(p.ws + ws_o(gridDim.x, p.unit_tiles)) +
-                        (size_t)((blockIdx.x * 2 + (w.blk > 0 ? 0 : 1)) * p.unit_tiles + t) * BM * HD;
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) store_part(slot, r, col + i, ov + i);
-        }
-      };
-      auto put_ml = [&](uint32_t t, float m, float l) {
-        if (!direct)
-          reinterpret_cast<float2*>(p.ws + WS_ML)[((blockIdx.x * 2 + (w.blk > 0 ? 0 : 1)) *
-                                                       p.unit_tiles + t) * BM + r] =
-              make_float2(m, l);
-      };
-      if (two) {
-        turns[0] += w.nb;
-        turns[1] += w.nb;
+    while (ok && in.get(c, d, ok)) {
+      const bool two = d.tiles == 2;
+      const uint32_t lead = d.x0 & 1;  // one tile: the group of the first block
+      const uint32_t of_lead = two ? d.nb : (d.nb + 1) / 2, of_other = two ? d.nb : d.nb / 2;
+      turns += lead ? of_other : of_lead;
+      turns1 += lead ? of_lead : of_other;
+      // two tiles: group 0's, then group 1's; one: both groups' halves of it
 #pragma unroll 1
-        for (uint32_t i = 0; i < 2 && ok; i++) {
-          if (!complete(i)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t t = (i - x0) & 1;  // the group's tile
-          const float2 a = ml[i * BM + r];
-          const uint64_t bad = gbad[i];
-          const float inv = a.y != 0.f ? 1.f / a.y : 0.f;
-#pragma unroll 1
-          for (uint32_t c = 0; c < HD; c += 32) {
-            float ov[32];
-            tmem_ld32(tmem_o + i * HD + c, ov);
-            tmem_ld_wait();
-            put(t, c, ov, inv, bad);
-          }
-          put_ml(t, a.x, a.y);
-          tc_fence_before();
-          release(i);
-        }
-      } else {
-        const uint32_t lead = x0 & 1;  // the group of the first block
-        turns[lead] += (w.nb + 1) / 2;
-        turns[lead ^ 1] += w.nb / 2;
-        const bool both = w.nb > 1;
-        ok = complete(lead) && (!both || complete(lead ^ 1));
+      for (uint32_t part = 0; part < d.tiles; part++) {
+        const uint32_t g0 = two ? part : lead;
+        const bool both = !two && d.nb > 1;
+        ok = complete(g0) && (!both || complete(g0 ^ 1));
         if (!ok) break;
         tc_fence_after();
-        const float2 a = ml[lead * BM + r];
-        const float2 b = both ? ml[(lead ^ 1) * BM + r] : make_float2(-INFINITY, 0.f);
-        const uint64_t bad = gbad[lead] | (both ? gbad[lead ^ 1] : 0);
+        const float2 a = ml[g0 * BM + r];
+        const float2 b = both ? ml[(g0 ^ 1) * BM + r] : make_float2(-INFINITY, 0.f);
         // a group without weights counts for nothing (l may be NaN)
         const float M = fmaxf(a.x, b.x);
         const float wa = a.y != 0.f ? ex2f(a.x - M) : 0.f, wb = b.y != 0.f ? ex2f(b.x - M) : 0.f;
         const float L = (a.y != 0.f ? a.y * wa : 0.f) + (b.y != 0.f ? b.y * wb : 0.f);
-        const float inv = L != 0.f ? 1.f / L : 0.f;
+        const uint32_t t = two ? (g0 - d.x0) & 1 : 0;
+        const uint32_t tile = d.tile0 + t, node = tile * p.tile_nodes + q_node;
+        const bool row_used = q_node < min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes);
+        const bool absent = node >= d.nodes;
+        const float inv = L != 0.f && !absent ? 1.f / L : 0.f;
+        // what was taken out of the V rows that this row sees
+        uint64_t lost = gbad[g0] | (both ? gbad[g0 ^ 1] : 0);
+        if (lost)
+          lost &= absent || !row_used ? 0
+                                      : nwd::tree_mask(p.parents + (size_t)d.b * p.n_nodes,
+                                                       (int)node, nullptr);
+        const size_t slot = (size_t)((blockIdx.x * 2 + (d.blk > 0 ? 0 : 1)) * p.unit_tiles + t) * BM;
+        __half* dst = p.o + (((size_t)d.b * p.n_nodes + node) * p.n_heads + d.hkv * p.group +
+                             q_head) * HD;
+        float* part_o =
+            reinterpret_cast<float*>(p.ws + ws_o(gridDim.x, p.unit_tiles)) + slot * HD + r * 4;
 #pragma unroll 1
-        for (uint32_t c = 0; c < HD; c += 32) {
-          float ov[32], o1[16];
-          tmem_ld32(tmem_o + lead * HD + c, ov);
+        for (uint32_t col = 0; col < HD; col += 32) {
+          float ov[32];
+          tmem_ld32(tmem_o + g0 * HD + col, ov);
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 32; i++) ov[i] = a.y != 0.f ? ov[i] * wa : 0.f;
           if (both) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-              tmem_ld16(tmem_o + (lead ^ 1) * HD + c + 16 * h, o1);
+              float o1[16];
+              tmem_ld16(tmem_o + (g0 ^ 1) * HD + col + 16 * h, o1);
               tmem_ld_wait();
               if (b.y != 0.f) {
 #pragma unroll
@@ -1113,14 +1014,49 @@ __global__ void __launch_bounds__(THREADS, 1)
               }
             }
           }
-          put(0, c, ov, inv, bad);
+          if (row_used) {
+            for (uint64_t x = lost; x; x &= x - 1) {
+              const size_t row = (size_t)d.row0 + d.ctx + (uint32_t)__ffsll((long long)x) - 1;
+              const __half* src = p.v + (row * p.n_kv + d.hkv) * HD + col;
+#pragma unroll
+              for (int i = 0; i < 32; i++) {
+                const float e = __half2float(src[i]);
+                if (!isfinite(e)) ov[i] += e;
+              }
+            }
+            if (d.whole) {
+              uint32_t h[16];
+#pragma unroll
+              for (int k = 0; k < 16; k++) {
+                const __half2 x = __floats2half2_rn(ov[2 * k] * inv, ov[2 * k + 1] * inv);
+                h[k] = absent ? 0u : *reinterpret_cast<const uint32_t*>(&x);
+              }
+              if (wide) {
+                store32(dst + col, h);
+                store32(dst + col + 16, h + 8);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                  reinterpret_cast<uint4*>(dst + col)[i] =
+                      make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4*>(part_o + (size_t)(col + i) * BM) =
+                    make_float4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+            }
+          }
         }
-        put_ml(0, M, L);
+        if (!d.whole && row_used)
+          reinterpret_cast<float2*>(p.ws + WS_ML)[slot + r] = make_float2(M, L);
         tc_fence_before();
-        release(lead);
-        if (both) release(lead ^ 1);
+        // the groups' accumulators, and their (m, l), have been read
+        c.arrive(B_OEMPTY + (int)g0);
+        if (both) c.arrive(B_OEMPTY + (int)(g0 ^ 1));
+        units += both || g0 == 0;
+        units1 += both || g0 == 1;
       }
-      x0 += w.nb * un.tiles;
     }
   }
   tc_fence_before();

@@ -138,6 +138,19 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
         while not b.passed(parity):
             yield
 
+    NP, USERS = 4, 13
+    for i in range(NP):
+        bar("PCE", i, USERS)
+
+    def planner():
+        for n in range(len(plan) + 1):  # the last one says that there are no more
+            yield from wait(bar("PCE", n % NP), (n // NP & 1) ^ 1)
+            bar("PCF", n % NP).arrive()
+
+    def get(n):
+        yield from wait(bar("PCF", n % NP), n // NP & 1)
+        bar("PCE", n % NP).arrive()
+
     flying = []  # copies land in any order
 
     def copy(store, i, item, full):
@@ -153,13 +166,17 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
             yield
 
     def load(kind, slots, store, items):
-        i, ph = 0, 0
+        i, ph, piece = 0, 0, -1
         for item in items:
+            if item[0] != piece:
+                piece = item[0]
+                yield from get(piece)
             yield from wait(bar(kind + "E", i), ph ^ 1)
             copy(store, i, item, bar(kind + "F", i))
             i += 1
             if i == slots:
                 i, ph = 0, ph ^ 1
+        yield from get(len(plan))
 
     def turns_of(g):
         """(piece, block, tile, first, last, Q tile index, block index) of the group's turns."""
@@ -189,9 +206,12 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
                     bar(name + "E", i).arrive()
                 seen[name] += 1
 
-        ou = 0
+        ou, got = 0, 0
         for x, (n, j, t, first, last, qn, kn) in enumerate(turns):
             buf = 2 * g + (x & 1)
+            while got <= n:
+                yield from get(got)
+                got += 1
             if kind == "S":
                 qi, ki = qn % NQ, kn % NK
                 if first:
@@ -228,12 +248,16 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
                 mma.append(bar("PV", buf).arrive)
                 mma.append(bar("VE", vi).arrive)
                 ou += last
+        while got <= len(plan):
+            yield from get(got)
+            got += 1
 
     read, handed = {}, [[None, None], [None, None]]  # [group][thread]
 
     def softmax(g, th):
         x0, turn, units = 0, 0, 0
         for n, (nb, tiles) in enumerate(plan):
+            yield from get(n)
             mine, first = (g - x0) & 1, turn
             for j in range(nb) if tiles == 2 else range(mine, nb, 2):
                 x, buf = turn, 2 * g + (turn & 1)
@@ -254,6 +278,7 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
                 assert handed[g][th] is None
                 handed[g][th] = n
                 bar("ML", g).arrive()
+        yield from get(len(plan))
 
     def epilogue(th):
         x0, turns, units = 0, [0, 0], [0, 0]
@@ -264,6 +289,7 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
             yield from wait(bar("PV", 2 * i + (last & 1)), last >> 1 & 1)
 
         for n, (nb, tiles) in enumerate(plan):
+            yield from get(n)
             lead = x0 & 1
             own = {0: nb, 1: nb} if tiles == 2 else {lead: (nb + 1) // 2, lead ^ 1: nb // 2}
             groups = [i for i in (own if tiles == 2 else (lead, lead ^ 1)) if own[i]]
@@ -285,6 +311,7 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
                     bar("OE", i).arrive()
                     units[i] += 1
             x0 += nb * tiles
+        yield from get(len(plan))
 
     def tensor_core():
         while True:
@@ -309,9 +336,11 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
                 copy(q, i, qs[0].pop(0), bar("QF", i))
                 state["q"] += 1
 
+        yield from get(0)
         yield from load_q()
         qs.pop(0)
         for n, (nb, _) in enumerate(plan):
+            yield from get(n + 1)
             for j in range(nb):
                 i = state["v"] % NV
                 yield from wait(bar("VE", i), (state["v"] // NV & 1) ^ 1)
@@ -326,6 +355,7 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
     def tails():
         phases, i = [0] * NV, 0
         for n, (nb, _) in enumerate(plan):
+            yield from get(n)
             for j in range(nb):
                 if j + 2 >= nb:
                     yield from wait(bar("VT", i), phases[i])
@@ -333,9 +363,10 @@ def protocol(plan, seed, NQ=2, NK=5, NV=5, in_order=True):
                     yield
                     bar("VF", i).arrive()
                 i = (i + 1) % NV
+        yield from get(len(plan))
 
     roles = [issuer(g, kind) for g in range(2) for kind in ("S", "PV")]
-    roles += [load("K", NK, k, kv), v_and_q(), tails()] + [epilogue(th) for th in range(2)]
+    roles += [load("K", NK, k, kv), v_and_q(), tails(), planner()] + [epilogue(th) for th in range(2)]
     roles += [softmax(g, th) for g in range(2) for th in range(2)]
     tc, cp = tensor_core(), copies()
     idle = 0
