@@ -21,7 +21,19 @@
 // part in 10^7, enough to change a drawn token now and then with the order of
 // summation; in f64 the borders hold to 10^-15.
 //
-// One CTA per sequence; a pass over a row gives each warp a contiguous part.
+// A sequence has a cluster of up to 16 CTAs, each with a contiguous part of the
+// vocabulary, its warps with contiguous parts of that.  Every CTA walks the
+// tree for itself, on the same numbers: the entries at the drafted tokens,
+// fetched for all nodes at once, decide while nothing is rejected.  A rejection
+// takes one pass over the row (p and q): each CTA's sum goes to all of them
+// through distributed shared memory, one cluster barrier a pass, and is added
+// in CTA order, so they agree to the bit.  The last pass at the last node also
+// serves the draw.  Without draft rows a node's rejections share one pass: the
+// sum over all tokens but its children's, to which the entries of those not
+// rejected are added.
+//
+// Bound by the rows' bytes where there are many sequences, by the latency of
+// launch, gathers and one pass where there are few.
 #include "nwd_common.h"
 #include "tree.cuh"
 
@@ -29,6 +41,9 @@ namespace {
 
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
+constexpr int CTAS_PER_SM = 2;  // 64 registers per thread
+constexpr uint32_t MAX_CLUSTER = 16;
+constexpr uint32_t MIN_PART = 1024;  // tokens per CTA that make a larger cluster worth its barriers
 
 struct VerifyParams {
   const int32_t* tokens;
@@ -42,37 +57,21 @@ struct VerifyParams {
   int32_t* n_accepted;
   int32_t* next_token;
   uint32_t* err;
-  uint32_t n_nodes, vocab;
+  uint32_t n_nodes, vocab, cluster;
 };
 
 // A probability as it counts: what is not above zero (NaN too) is zero.
 __device__ __forceinline__ double prob(float x) { return x > 0.f ? (double)x : 0.0; }
 
 struct Walk {
-  int32_t parent[nwd::TREE_MAX_NODES];
-  int32_t token[nwd::TREE_MAX_NODES];  // -1: outside the vocabulary, never accepted
   float u[nwd::TREE_MAX_NODES];
   float p[nwd::TREE_MAX_NODES];  // target and draft row of the parent at the token
   float q[nwd::TREE_MAX_NODES];
-  double sum[nwd::TREE_MAX_NODES];       // S before each rejection at the current node
-  int32_t gone[nwd::TREE_MAX_NODES];     // tokens rejected at the current node
-  double part[WARPS];
-  int32_t found;
+  int32_t token[nwd::TREE_MAX_NODES];   // -1: outside the vocabulary, never accepted
+  double sum[nwd::TREE_MAX_NODES];      // S before each rejection at the current node
+  double from[2][MAX_CLUSTER];          // the CTAs' sums of a pass, by its parity
+  double part[WARPS];                   // the warps' sums of the last pass
 };
-
-// r~ at token x after k rejections at the current node.
-template <bool DRAFT>
-__device__ __forceinline__ double rest_at(const Walk& s, int k, uint32_t x, float p, float q) {
-  double r = prob(p);
-  if (DRAFT) {
-    const double qd = prob(q);
-    for (int i = 0; i < k; i++) r = fmax(r - s.sum[i] * qd, 0.0);
-  } else {
-    for (int i = 0; i < k; i++)
-      if (s.gone[i] == (int32_t)x) r = 0.0;
-  }
-  return r;
-}
 
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
@@ -80,127 +79,359 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// The sum of r~ over the vocabulary; s.part holds the warps' shares of it.
+// r~ of an entry after k rejections at the current node (with draft rows).
+__device__ __forceinline__ double rest(const Walk& s, int k, float p, float q) {
+  double r = prob(p);
+  const double qd = prob(q);
+  for (int i = 0; i < k; i++) r = fmax(r - s.sum[i] * qd, 0.0);
+  return r;
+}
+
+// A row of the vocabulary in groups of four entries from a 16-byte boundary at
+// or before its start; entries outside the row read as zero.
+struct Row {
+  const float* p;
+  const float* q;      // nullptr without draft rows
+  uint32_t lead, size;  // entries before the row in its first group; entries
+  bool vec;            // p and q lie alike: whole groups are single loads
+  __device__ __forceinline__ Row(const float* p_, const float* q_, uint32_t size_)
+      : p(p_), q(q_), size(size_) {
+    lead = (uint32_t)(reinterpret_cast<uintptr_t>(p) >> 2) & 3u;
+    vec = !q || ((reinterpret_cast<uintptr_t>(q) >> 2) & 3u) == lead;
+  }
+  __device__ __forceinline__ uint32_t groups() const { return (size + lead + 3) / 4; }
+  __device__ __forceinline__ uint32_t first(uint32_t g) const { return 4 * g - lead; }  // may wrap
+  __device__ __forceinline__ float4 load(const float* row, uint32_t g) const {
+    const uint32_t x = first(g);
+    if (vec && x < size && size - x >= 4)
+      return __ldg(reinterpret_cast<const float4*>(row + x));
+    float4 v;
+    v.x = x < size ? row[x] : 0.f;
+    v.y = x + 1 < size ? row[x + 1] : 0.f;
+    v.z = x + 2 < size ? row[x + 2] : 0.f;
+    v.w = x + 3 < size ? row[x + 3] : 0.f;
+    return v;
+  }
+};
+
+// The tokens taken out of a row (without draft rows): lane l holds those of
+// nodes l and l + 32, -1 where there is none.
+struct Gone {
+  int32_t a, b;
+  // Zeroes the ones among the entries v, which are tokens x .. x + 3 of this
+  // lane and x0 .. x0 + 127 of the warp (x0 may have wrapped below zero).
+  __device__ __forceinline__ void clear(double (&v)[4], uint32_t x, uint32_t x0) const {
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      const int32_t mine = half ? b : a;
+      uint32_t in = __ballot_sync(0xffffffffu, mine >= 0 && (uint32_t)mine - x0 < 128u);
+      for (; in; in &= in - 1) {
+        const uint32_t at = (uint32_t)__shfl_sync(0xffffffffu, mine, __ffs(in) - 1) - x;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++)
+          if (at == i) v[i] = 0.0;
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void cluster_put(double* slot, uint32_t rank, double v) {
+  uint32_t at = (uint32_t)__cvta_generic_to_shared(slot);
+  asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(rank));
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(v) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The warp's groups [lo, hi) of a row, in steps of 32.
+struct Part {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ Part warp_part(uint32_t groups, uint32_t rank, uint32_t cluster) {
+  const uint32_t piece = rank * WARPS + (threadIdx.x >> 5), pieces = cluster * WARPS;
+  return Part{(uint32_t)((uint64_t)groups * piece / pieces),
+              (uint32_t)((uint64_t)groups * (piece + 1) / pieces)};
+}
+
+// r~ of the warp's groups g0 .. g0 + 31, this lane's.
 template <bool DRAFT>
-__device__ double row_sum(Walk& s, int k, const float* p, const float* q, uint32_t lo, uint32_t hi) {
+__device__ __forceinline__ void entries(const Walk& s, int k, const Gone& gone, const Row& row,
+                                        uint32_t g0, float4 p, float4 q, double (&v)[4]) {
+  if (DRAFT) {
+    v[0] = rest(s, k, p.x, q.x);
+    v[1] = rest(s, k, p.y, q.y);
+    v[2] = rest(s, k, p.z, q.z);
+    v[3] = rest(s, k, p.w, q.w);
+  } else {
+    v[0] = prob(p.x);
+    v[1] = prob(p.y);
+    v[2] = prob(p.z);
+    v[3] = prob(p.w);
+    gone.clear(v, row.first(g0 + (threadIdx.x & 31)), row.first(g0));
+  }
+}
+
+// One pass: the sum of r~ over the vocabulary, the same in every thread of the
+// cluster; s.part holds this CTA's warps' shares, s.from[parity] the CTAs'.
+template <bool DRAFT>
+__device__ double row_sum(Walk& s, int k, const Gone& gone, const Row& row, uint32_t rank,
+                          uint32_t cluster, uint32_t parity) {
+  constexpr uint32_t AHEAD = 4;  // groups of a row in flight per thread
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Part w = warp_part(row.groups(), rank, cluster);
   double v = 0.0;
-  for (uint32_t x = lo + lane; x < hi; x += 32)
-    v += rest_at<DRAFT>(s, k, x, p[x], DRAFT ? q[x] : 0.f);
+  for (uint32_t g0 = w.lo; g0 < w.hi; g0 += 32 * AHEAD) {
+    float4 p[AHEAD], q[AHEAD];
+#pragma unroll
+    for (uint32_t i = 0; i < AHEAD; i++) {
+      const uint32_t g = g0 + 32 * i + lane;
+      p[i] = q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (g < w.hi) {
+        p[i] = row.load(row.p, g);
+        if (DRAFT) q[i] = row.load(row.q, g);
+      }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < AHEAD; i++) {
+      double e[4];
+      entries<DRAFT>(s, k, gone, row, g0 + 32 * i, p[i], q[i], e);
+      v += (e[0] + e[1]) + (e[2] + e[3]);
+    }
+  }
   v = warp_sum(v);
-  __syncthreads();
+  __syncthreads();  // the last pass's s.part has been read
   if (lane == 0) s.part[warp] = v;
   __syncthreads();
   double t = 0.0;
   for (int i = 0; i < WARPS; i++) t += s.part[i];
+  if (cluster == 1) return t;
+  if (threadIdx.x < cluster) cluster_put(&s.from[parity][rank], threadIdx.x, t);
+  cluster_arrive();
+  cluster_wait();
+  t = 0.0;
+  for (uint32_t i = 0; i < cluster; i++) t += s.from[parity][i];
   return t;
 }
 
 template <bool DRAFT>
-__global__ void __launch_bounds__(THREADS) verify_tree_kernel(const VerifyParams a) {
+__global__ void __launch_bounds__(THREADS, CTAS_PER_SM) verify_tree_kernel(const VerifyParams a) {
   __shared__ Walk s;
-  const uint32_t b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t b = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster;
   const uint32_t V = a.vocab, N = a.n_nodes;
   const uint64_t node0 = (uint64_t)b * N;
+  nwd::pdl_trigger();
+  cluster_arrive();  // this CTA has started: its shared memory may be written
+  nwd::pdl_wait();
   const uint32_t n = nwd::tree_nodes(a.tree_len, b, N, a.err);
-  if (tid < N) a.path[node0 + tid] = -1;
+  // every warp has the nodes' parents and tokens, lane l those of l and l + 32
+  int par[2] = {-1, -1}, tok[2] = {-1, -1};
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const uint32_t c = lane + 32 * i;
+    if (c > 0 && c < n) {
+      par[i] = nwd::tree_parent(a.parents + node0, (int)c, a.err);
+      tok[i] = a.tokens[node0 + c];
+      if (tok[i] < 0 || (uint32_t)tok[i] >= V) {
+        if (a.err) atomicOr(a.err, NWD_DEVERR_TREE);
+        tok[i] = -1;
+      }
+    }
+  }
+  if (warp < 2) {  // warp i: the entries at the tokens of nodes 32 i ..
+    const uint32_t c = tid;
+    if (c < N) {
+      s.token[c] = tok[warp];
+      s.u[c] = c < n ? a.u[node0 + c] : 0.f;
+      s.p[c] = s.q[c] = 0.f;
+      if (par[warp] >= 0 && tok[warp] >= 0) {
+        const uint64_t at = (node0 + (uint32_t)par[warp]) * V + (uint32_t)tok[warp];
+        s.p[c] = a.target[at];
+        s.q[c] = DRAFT ? a.draft[at] : 1.f;
+      }
+      if (rank == 0) a.path[node0 + c] = -1;
+    }
+  }
+  cluster_wait();  // every CTA of the cluster has
+  __syncthreads();
   if (n == 0) {
-    if (tid == 0) {
+    if (rank == 0 && tid == 0) {
       a.n_accepted[b] = 0;
       a.next_token[b] = -1;
     }
-    return;
+    return;  // the whole cluster
   }
-  if (tid < n) {
-    const int par = nwd::tree_parent(a.parents + node0, (int)tid, a.err);
-    int tok = a.tokens[node0 + tid];
-    if (tid > 0 && (tok < 0 || (uint32_t)tok >= V)) {
-      if (a.err) atomicOr(a.err, NWD_DEVERR_TREE);
-      tok = -1;
+  const bool scribe = rank == 0 && tid == 0;
+  if (scribe) a.path[node0] = 0;
+  uint32_t cur = 0, count = 1, parity = 0;
+  double total = 1.0;   // S: 1 for p itself, else the sum of r~
+  Gone gone{-1, -1};
+  bool summed = false;  // the last pass was over r~ as it now is
+  for (;;) {
+    const Row row(a.target + (node0 + cur) * V, DRAFT ? a.draft + (node0 + cur) * V : nullptr, V);
+    const uint64_t children = (uint64_t)__ballot_sync(0xffffffffu, par[1] == (int)cur) << 32 |
+                              __ballot_sync(0xffffffffu, par[0] == (int)cur);
+    int k = 0;  // rejections that r~ has taken in (since it was last the whole row)
+    int next = -1;
+    bool have_base = false;
+    double base = 0.0;  // without draft rows: the sum but for the children's tokens
+    total = 1.0;
+    gone.a = gone.b = -1;
+    summed = false;
+    for (uint64_t left = children; left; left &= left - 1) {
+      const int c = __ffsll((long long)left) - 1;
+      const int t = s.token[c];
+      double r = 0.0;
+      if (t >= 0) {
+        if (DRAFT) r = rest(s, k, s.p[c], s.q[c]);
+        else r = __any_sync(0xffffffffu, gone.a == t || gone.b == t) ? 0.0 : prob(s.p[c]);
+        if ((double)s.u[c] * prob(s.q[c]) * total < r) {
+          next = c;
+          break;
+        }
+      }
+      if (DRAFT) {
+        __syncthreads();
+        if (tid == 0) s.sum[k] = total;
+        __syncthreads();
+        total = row_sum<true>(s, ++k, gone, row, rank, a.cluster, parity);
+        parity ^= 1;
+        summed = true;
+      } else {
+        if (!have_base) {  // the children's tokens left out, all at once
+          const Gone all{par[0] == (int)cur ? tok[0] : -1, par[1] == (int)cur ? tok[1] : -1};
+          base = row_sum<false>(s, 0, all, row, rank, a.cluster, parity);
+          parity ^= 1;
+          have_base = true;
+        }
+        if ((int)lane == (c & 31)) {
+          if (c < 32) gone.a = t;
+          else gone.b = t;
+        }
+        // the entries of the children's tokens that are still in, each token once
+        total = base;
+        uint64_t seen = 0;
+        for (uint64_t x = children; x; x &= x - 1) {
+          const int e = __ffsll((long long)x) - 1, te = s.token[e];
+          if (te < 0 || __any_sync(0xffffffffu, gone.a == te || gone.b == te)) continue;
+          bool twice = false;
+          for (uint64_t y = seen; y; y &= y - 1) twice |= s.token[__ffsll((long long)y) - 1] == te;
+          if (!twice) total += prob(s.p[e]);
+          seen |= 1ull << e;
+        }
+        // the pass left out all of them: its parts serve the draw if that is so
+        summed = seen == 0;
+      }
+      if (!(total > 0.0)) {  // nothing left: the whole row again
+        k = 0;
+        total = 1.0;
+        gone.a = gone.b = -1;
+        summed = false;
+      }
     }
-    s.parent[tid] = par;
-    s.token[tid] = tok;
-    s.u[tid] = a.u[node0 + tid];
-    if (par >= 0 && tok >= 0) {
-      const uint64_t at = (node0 + (uint32_t)par) * V + (uint32_t)tok;
-      s.p[tid] = a.target[at];
-      s.q[tid] = DRAFT ? a.draft[at] : 1.f;
-    }
-  }
-  __syncthreads();
-  const uint32_t lo = (uint32_t)((uint64_t)V * warp / WARPS);
-  const uint32_t hi = (uint32_t)((uint64_t)V * (warp + 1) / WARPS);
-  uint32_t cur = 0, count = 1;
-  int k = 0;          // rejections that r~ has taken in at `cur`
-  double total = 1.0; // S: 1 for p itself, else the sum of r~
-  if (tid == 0) a.path[node0] = 0;
-  for (uint32_t c = 1; c < n; c++) {
-    if (s.parent[c] != (int32_t)cur) continue;
-    const float* p = a.target + (node0 + cur) * V;
-    const float* q = DRAFT ? a.draft + (node0 + cur) * V : nullptr;
-    const int tok = s.token[c];
-    const double r = tok < 0 ? 0.0 : rest_at<DRAFT>(s, k, (uint32_t)tok, s.p[c], s.q[c]);
-    if (tok >= 0 && (double)s.u[c] * prob(s.q[c]) * total < r) {
-      if (tid == 0) a.path[node0 + count] = (int32_t)c;
-      count++;
-      cur = c;
-      k = 0;
-      total = 1.0;
-      continue;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      s.sum[k] = total;
-      s.gone[k] = tok;
-    }
-    __syncthreads();
-    total = row_sum<DRAFT>(s, ++k, p, q, lo, hi);
-    if (!(total > 0.0)) {
-      k = 0;
-      total = 1.0;
-    }
-  }
-  const float* p = a.target + (node0 + cur) * V;
-  const float* q = DRAFT ? a.draft + (node0 + cur) * V : nullptr;
-  total = row_sum<DRAFT>(s, k, p, q, lo, hi);
-  // the warp whose part holds the border, then its rows of 32
-  const double goal = (double)a.w[b] * total;
-  double before = 0.0, mine = 0.0;
-  int owner = -1;
-  for (int i = 0; i < WARPS; i++) {
-    const double v = s.part[i];
-    if (v > 0.0) {
-      owner = i;
-      before = mine;
-      if (mine + v > goal) break;
-    }
-    mine += v;
-  }
-  if (tid == 0) {
-    a.n_accepted[b] = (int32_t)count;
-    if (owner < 0) a.next_token[b] = -1;
-  }
-  if ((int)warp != owner) return;
-  int32_t last = -1;  // the last token with a probability, should rounding leave the border behind
-  for (uint32_t x0 = lo; x0 < hi; x0 += 32) {
-    const uint32_t x = x0 + lane;
-    const double v = x < hi ? rest_at<DRAFT>(s, k, x, p[x], DRAFT ? q[x] : 0.f) : 0.0;
-    double cum = v;
+    if (next < 0) {
+      if (!summed) {
+        total = row_sum<DRAFT>(s, k, gone, row, rank, a.cluster, parity);
+        parity ^= 1;
+      }
+      // ---- the draw: the CTA whose part holds the border, then its warp
+      const double goal = (double)a.w[b] * total;
+      if (scribe) a.n_accepted[b] = (int32_t)count;
+      double before = 0.0, mine = 0.0;
+      int owner = -1;
+      if (a.cluster > 1) {
+        for (uint32_t i = 0; i < a.cluster; i++) {
+          const double v = s.from[parity ^ 1][i];
+          if (v > 0.0) {
+            owner = (int)i;
+            before = mine;
+            if (mine + v > goal) break;
+          }
+          mine += v;
+        }
+        if (owner < 0 && scribe) a.next_token[b] = -1;
+        if (owner != (int)rank) return;
+      }
+      owner = -1;
+      mine = before;
+      for (int i = 0; i < WARPS; i++) {
+        const double v = s.part[i];
+        if (v > 0.0) {
+          owner = i;
+          before = mine;
+          if (mine + v > goal) break;
+        }
+        mine += v;
+      }
+      if (owner < 0 && tid == 0) a.next_token[b] = -1;  // (a cluster of one: no mass at all)
+      if ((int)warp != owner) return;
+      const Part w = warp_part(row.groups(), rank, a.cluster);
+      int32_t last = -1;  // the last token with mass, should rounding leave the border behind
+      for (uint32_t g0 = w.lo; g0 < w.hi; g0 += 32) {
+        const uint32_t g = g0 + lane, x = row.first(g);
+        float4 p = make_float4(0.f, 0.f, 0.f, 0.f), q = p;
+        if (g < w.hi) {
+          p = row.load(row.p, g);
+          if (DRAFT) q = row.load(row.q, g);
+        }
+        double v[4];
+        entries<DRAFT>(s, k, gone, row, g0, p, q, v);
+        const double own = ((v[0] + v[1]) + v[2]) + v[3];
+        double cum = own;
 #pragma unroll
-    for (int i = 1; i < 32; i <<= 1) {
-      const double y = __shfl_up_sync(0xffffffffu, cum, i);
-      if ((int)lane >= i) cum += y;
+        for (int i = 1; i < 32; i <<= 1) {
+          const double y = __shfl_up_sync(0xffffffffu, cum, i);
+          if ((int)lane >= i) cum += y;
+        }
+        // within the lane: the first entry that takes the sum past the goal
+        double at = before + cum - own;
+        int32_t hit = -1, some = -1;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          at += v[i];
+          if (v[i] > 0.0) {
+            some = (int32_t)(x + i);
+            if (hit < 0 && at > goal) hit = some;
+          }
+        }
+        const uint32_t hits = __ballot_sync(0xffffffffu, hit >= 0);
+        const uint32_t somes = __ballot_sync(0xffffffffu, some >= 0);
+        if (somes) last = __shfl_sync(0xffffffffu, some, 31 - __clz(somes));
+        if (hits) {
+          last = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, cum, 31);
+      }
+      if (lane == 0) a.next_token[b] = last;
+      return;
     }
-    const uint32_t some = __ballot_sync(0xffffffffu, v > 0.0);
-    const uint32_t over = __ballot_sync(0xffffffffu, v > 0.0 && before + cum > goal);
-    if (some) last = (int32_t)(x0 + 31 - __clz(some));
-    if (over) {
-      last = (int32_t)(x0 + __ffs(over) - 1);
-      break;
-    }
-    before += __shfl_sync(0xffffffffu, cum, 31);
+    if (scribe) a.path[node0 + count] = next;
+    count++;
+    cur = (uint32_t)next;
   }
-  if (lane == 0) a.next_token[b] = last;
+}
+
+template <bool DRAFT>
+cudaError_t launch_verify(const VerifyParams& a, uint32_t batch, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(batch * a.cluster);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, verify_tree_kernel<DRAFT>, a);
 }
 
 }  // namespace
@@ -222,13 +453,29 @@ extern "C" int nwd_verify_tree(const int32_t* tokens, const int32_t* parents,
   if (vocab > 0x7fffffffu) return fail(NWD_ERR_UNSUPPORTED, "%s: vocabulary %u", who, vocab);
   if (batch > 65535u) return fail(NWD_ERR_UNSUPPORTED, "%s: batch > 65535", who);
   if (batch == 0) return ok();
-  VerifyParams a{tokens, parents,    tree_len,   target_probs, draft_probs, u,     w, path,
-                 n_accepted, next_token, err, n_nodes, vocab};
-  if (draft_probs)
-    verify_tree_kernel<true><<<batch, THREADS, 0, (cudaStream_t)stream>>>(a);
-  else
-    verify_tree_kernel<false><<<batch, THREADS, 0, (cudaStream_t)stream>>>(a);
-  cudaError_t e = cudaGetLastError();
+  DeviceInfo di;
+  int st = current_device_info(&di);
+  if (st) return st;
+  static bool wide_set[64] = {};  // clusters of 16 allowed, per device
+  if (!wide_set[di.device]) {
+    cudaError_t e = cudaFuncSetAttribute(verify_tree_kernel<true>,
+                                         cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(verify_tree_kernel<false>,
+                               cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(verify_tree_kernel)");
+    wide_set[di.device] = true;
+  }
+  // The largest cluster that leaves all CTAs resident at once and each a part
+  // of the vocabulary worth a barrier.
+  uint32_t cluster = 1;
+  while (cluster < MAX_CLUSTER && (uint64_t)batch * cluster * 2 <= (uint64_t)di.sm_count * CTAS_PER_SM &&
+         vocab / (cluster * 2) >= MIN_PART)
+    cluster *= 2;
+  const VerifyParams a{tokens, parents,    tree_len,   target_probs, draft_probs, u,       w,
+                       path,   n_accepted, next_token, err,          n_nodes,     vocab,   cluster};
+  cudaError_t e = draft_probs ? launch_verify<true>(a, batch, (cudaStream_t)stream)
+                              : launch_verify<false>(a, batch, (cudaStream_t)stream);
   if (e != cudaSuccess) return cuda_fail(e, who);
   return ok();
 }
