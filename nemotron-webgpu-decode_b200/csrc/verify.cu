@@ -39,9 +39,9 @@
 
 namespace {
 
-constexpr int THREADS = 512;
+constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int CTAS_PER_SM = 2;  // 64 registers per thread
+constexpr int CTAS_PER_SM = 4;  // 64 registers per thread
 constexpr uint32_t MAX_CLUSTER = 16;
 constexpr uint32_t MIN_PART = 1024;  // tokens per CTA that make a larger cluster worth its barriers
 
@@ -78,13 +78,49 @@ __device__ __forceinline__ double warp_sum(double v) {
   for (int i = 16; i; i >>= 1) v += __shfl_xor_sync(0xffffffffu, v, i);
   return v;
 }
+// Lane i holds part i of a sum: the part that takes it past `goal` (the last
+// one with mass, should rounding leave the border behind; -1: none has any),
+// and the sum before it.  The same in all lanes, and wherever the parts are.
+__device__ __forceinline__ int find_part(double mine, double goal, double* before) {
+  const uint32_t lane = threadIdx.x & 31;
+  double upto = mine;
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) {
+    const double v = __shfl_up_sync(0xffffffffu, upto, i);
+    if ((int)lane >= i) upto += v;
+  }
+  const double ahead = *before + upto;
+  const uint32_t mass = __ballot_sync(0xffffffffu, mine > 0.0);
+  const uint32_t over = __ballot_sync(0xffffffffu, mine > 0.0 && ahead > goal);
+  if (!mass) return -1;
+  const int at = over ? __ffs(over) - 1 : 31 - __clz(mass);
+  const double up = __shfl_up_sync(0xffffffffu, upto, 1);
+  *before += __shfl_sync(0xffffffffu, lane ? up : 0.0, at);
+  return at;
+}
 
-// r~ of an entry after k rejections at the current node (with draft rows).
-__device__ __forceinline__ double rest(const Walk& s, int k, float p, float q) {
-  double r = prob(p);
-  const double qd = prob(q);
-  for (int i = 0; i < k; i++) r = fmax(r - s.sum[i] * qd, 0.0);
-  return r;
+// max(p - q, 0): r~ of an entry after one rejection (S was 1), with the
+// comparison in f32, which is exact, so that the f64 pipe has one difference.
+__device__ __forceinline__ double rest1(float p, float q) {
+  p = fmaxf(p, 0.f);  // (NaN gives 0)
+  q = fmaxf(q, 0.f);
+  const bool in = p > q;
+  return (double)(in ? p : 0.f) - (double)(in ? q : 0.f);
+}
+// r~ of N entries after k rejections at the current node (with draft rows).
+template <int N>
+__device__ __forceinline__ void rest(const Walk& s, int k, const float* p, const float* q, double* r) {
+#pragma unroll
+  for (int e = 0; e < N; e++) r[e] = k ? rest1(p[e], q[e]) : prob(p[e]);
+#pragma unroll 1
+  for (int i = 1; i < k; i++) {
+    const double sum = s.sum[i];
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const double t = r[e] - sum * prob(q[e]);
+      r[e] = t > 0.0 ? t : 0.0;
+    }
+  }
 }
 
 // A row of the vocabulary in groups of four entries from a 16-byte boundary at
@@ -151,38 +187,25 @@ __device__ __forceinline__ void cluster_wait() {
 struct Part {
   uint32_t lo, hi;
 };
+__device__ __forceinline__ Part piece(uint32_t groups, uint32_t i, uint32_t pieces) {
+  return Part{(uint32_t)((uint64_t)groups * i / pieces),
+              (uint32_t)((uint64_t)groups * (i + 1) / pieces)};
+}
 __device__ __forceinline__ Part warp_part(uint32_t groups, uint32_t rank, uint32_t cluster) {
-  const uint32_t piece = rank * WARPS + (threadIdx.x >> 5), pieces = cluster * WARPS;
-  return Part{(uint32_t)((uint64_t)groups * piece / pieces),
-              (uint32_t)((uint64_t)groups * (piece + 1) / pieces)};
+  return piece(groups, rank * WARPS + (threadIdx.x >> 5), cluster * WARPS);
 }
 
-// r~ of the warp's groups g0 .. g0 + 31, this lane's.
-template <bool DRAFT>
-__device__ __forceinline__ void entries(const Walk& s, int k, const Gone& gone, const Row& row,
-                                        uint32_t g0, float4 p, float4 q, double (&v)[4]) {
-  if (DRAFT) {
-    v[0] = rest(s, k, p.x, q.x);
-    v[1] = rest(s, k, p.y, q.y);
-    v[2] = rest(s, k, p.z, q.z);
-    v[3] = rest(s, k, p.w, q.w);
-  } else {
-    v[0] = prob(p.x);
-    v[1] = prob(p.y);
-    v[2] = prob(p.z);
-    v[3] = prob(p.w);
-    gone.clear(v, row.first(g0 + (threadIdx.x & 31)), row.first(g0));
-  }
-}
+// What r~ is made of: the row alone, p - q once, or the node's rejections one
+// after the other.
+enum Rest { WHOLE, ONCE, CHAIN };
 
-// One pass: the sum of r~ over the vocabulary, the same in every thread of the
-// cluster; s.part holds this CTA's warps' shares, s.from[parity] the CTAs'.
-template <bool DRAFT>
-__device__ double row_sum(Walk& s, int k, const Gone& gone, const Row& row, uint32_t rank,
-                          uint32_t cluster, uint32_t parity) {
-  constexpr uint32_t AHEAD = 4;  // groups of a row in flight per thread
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Part w = warp_part(row.groups(), rank, cluster);
+// The sum of r~ over the warp's groups [lo, hi) of a row, this lane's share;
+// AHEAD groups per lane in flight.
+template <bool DRAFT, int REST>
+__device__ __forceinline__ double part_sum(const Walk& s, int k, const Gone& gone, const Row& row,
+                                           Part w) {
+  constexpr uint32_t AHEAD = REST == WHOLE ? 8 : REST == ONCE ? 4 : 2;
+  const uint32_t lane = threadIdx.x & 31;
   double v = 0.0;
   for (uint32_t g0 = w.lo; g0 < w.hi; g0 += 32 * AHEAD) {
     float4 p[AHEAD], q[AHEAD];
@@ -192,29 +215,61 @@ __device__ double row_sum(Walk& s, int k, const Gone& gone, const Row& row, uint
       p[i] = q[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (g < w.hi) {
         p[i] = row.load(row.p, g);
-        if (DRAFT) q[i] = row.load(row.q, g);
+        if (REST != WHOLE) q[i] = row.load(row.q, g);
       }
     }
+    const float* pe = &p[0].x;
+    const float* qe = &q[0].x;
+    if (REST == CHAIN) {
+      double r[4 * AHEAD];
+      rest<4 * AHEAD>(s, k, pe, qe, r);
 #pragma unroll
-    for (uint32_t i = 0; i < AHEAD; i++) {
-      double e[4];
-      entries<DRAFT>(s, k, gone, row, g0 + 32 * i, p[i], q[i], e);
-      v += (e[0] + e[1]) + (e[2] + e[3]);
+      for (uint32_t i = 0; i < 4 * AHEAD; i++) v += r[i];
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < AHEAD; i++) {
+        double e[4];
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++)
+          e[c] = REST == ONCE ? rest1(pe[4 * i + c], qe[4 * i + c]) : prob(pe[4 * i + c]);
+        if (!DRAFT) gone.clear(e, row.first(g0 + 32 * i + lane), row.first(g0 + 32 * i));
+        v += (e[0] + e[1]) + (e[2] + e[3]);
+      }
     }
   }
+  return v;
+}
+template <bool DRAFT>
+__device__ __forceinline__ double any_part_sum(const Walk& s, int k, const Gone& gone,
+                                               const Row& row, Part w) {
+  if (!DRAFT || k == 0) return part_sum<DRAFT, WHOLE>(s, k, gone, row, w);
+  if (k == 1) return part_sum<DRAFT, ONCE>(s, k, gone, row, w);
+  return part_sum<DRAFT, CHAIN>(s, k, gone, row, w);
+}
+
+// The warps' sums, in s.part, added up: the same in every thread of the CTA.
+__device__ __forceinline__ double block_sum(Walk& s, double v) {
+  const uint32_t lane = threadIdx.x & 31;
   v = warp_sum(v);
   __syncthreads();  // the last pass's s.part has been read
-  if (lane == 0) s.part[warp] = v;
+  if (lane == 0) s.part[threadIdx.x >> 5] = v;
   __syncthreads();
-  double t = 0.0;
-  for (int i = 0; i < WARPS; i++) t += s.part[i];
+  return warp_sum(lane < WARPS ? s.part[lane] : 0.0);
+}
+
+// One pass: the sum of r~ over the vocabulary, the same in every thread of the
+// cluster; s.part holds this CTA's warps' shares, s.from[parity] the CTAs'.
+template <bool DRAFT>
+__device__ double row_sum(Walk& s, int k, const Gone& gone, const Row& row, uint32_t rank,
+                          uint32_t cluster, uint32_t parity) {
+  const uint32_t lane = threadIdx.x & 31;
+  const Part w = warp_part(row.groups(), rank, cluster);
+  const double t = block_sum(s, any_part_sum<DRAFT>(s, k, gone, row, w));
   if (cluster == 1) return t;
   if (threadIdx.x < cluster) cluster_put(&s.from[parity][rank], threadIdx.x, t);
   cluster_arrive();
   cluster_wait();
-  t = 0.0;
-  for (uint32_t i = 0; i < cluster; i++) t += s.from[parity][i];
-  return t;
+  return warp_sum(lane < cluster ? s.from[parity][lane] : 0.0);
 }
 
 template <bool DRAFT>
@@ -285,9 +340,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) verify_tree_kernel(const
     for (uint64_t left = children; left; left &= left - 1) {
       const int c = __ffsll((long long)left) - 1;
       const int t = s.token[c];
-      double r = 0.0;
       if (t >= 0) {
-        if (DRAFT) r = rest(s, k, s.p[c], s.q[c]);
+        double r;
+        if (DRAFT) rest<1>(s, k, &s.p[c], &s.q[c], &r);
         else r = __any_sync(0xffffffffu, gone.a == t || gone.b == t) ? 0.0 : prob(s.p[c]);
         if ((double)s.u[c] * prob(s.q[c]) * total < r) {
           next = c;
@@ -302,29 +357,39 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) verify_tree_kernel(const
         parity ^= 1;
         summed = true;
       } else {
+        const Gone mine{par[0] == (int)cur ? tok[0] : -1, par[1] == (int)cur ? tok[1] : -1};
         if (!have_base) {  // the children's tokens left out, all at once
-          const Gone all{par[0] == (int)cur ? tok[0] : -1, par[1] == (int)cur ? tok[1] : -1};
-          base = row_sum<false>(s, 0, all, row, rank, a.cluster, parity);
+          base = row_sum<false>(s, 0, mine, row, rank, a.cluster, parity);
           parity ^= 1;
           have_base = true;
         }
-        if ((int)lane == (c & 31)) {
-          if (c < 32) gone.a = t;
-          else gone.b = t;
+        if (t >= 0) {
+          if (mine.a == t) gone.a = t;
+          if (mine.b == t) gone.b = t;
         }
-        // the entries of the children's tokens that are still in, each token once
-        total = base;
-        uint64_t seen = 0;
-        for (uint64_t x = children; x; x &= x - 1) {
-          const int e = __ffsll((long long)x) - 1, te = s.token[e];
-          if (te < 0 || __any_sync(0xffffffffu, gone.a == te || gone.b == te)) continue;
-          bool twice = false;
-          for (uint64_t y = seen; y; y &= y - 1) twice |= s.token[__ffsll((long long)y) - 1] == te;
-          if (!twice) total += prob(s.p[e]);
-          seen |= 1ull << e;
+        // the entries of the children's tokens that are still in, each token
+        // once: at its first node
+        bool in[2] = {mine.a >= 0 && gone.a < 0, mine.b >= 0 && gone.b < 0};
+        const uint32_t ina = __ballot_sync(0xffffffffu, in[0]);
+        uint32_t inb = __ballot_sync(0xffffffffu, in[1]);
+        summed = !(ina | inb);  // the pass left out just those: its parts serve the draw
+        if (!summed) {
+          const uint32_t same = __match_any_sync(0xffffffffu, in[0] ? mine.a : -1 - (int)lane);
+          if (in[0] && (same & ((1u << lane) - 1u))) in[0] = false;
+          for (; inb; inb &= inb - 1) {  // (trees of more than 32 nodes)
+            const int l = __ffs(inb) - 1, tb = __shfl_sync(0xffffffffu, mine.b, l);
+            const uint32_t ahead = __ballot_sync(0xffffffffu, in[1] && mine.b == tb);
+            const bool twice = __any_sync(0xffffffffu, in[0] && mine.a == tb) ||
+                               (ahead & ((1u << l) - 1u));
+            if ((int)lane == l && twice) in[1] = false;
+          }
+          double more = 0.0;
+          if (in[0]) more += prob(s.p[lane]);
+          if (in[1]) more += prob(s.p[lane + 32]);
+          total = base + warp_sum(more);
+        } else {
+          total = base;
         }
-        // the pass left out all of them: its parts serve the draw if that is so
-        summed = seen == 0;
       }
       if (!(total > 0.0)) {  // nothing left: the whole row again
         k = 0;
@@ -341,35 +406,27 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) verify_tree_kernel(const
       // ---- the draw: the CTA whose part holds the border, then its warp
       const double goal = (double)a.w[b] * total;
       if (scribe) a.n_accepted[b] = (int32_t)count;
-      double before = 0.0, mine = 0.0;
-      int owner = -1;
+      double before = 0.0;
       if (a.cluster > 1) {
-        for (uint32_t i = 0; i < a.cluster; i++) {
-          const double v = s.from[parity ^ 1][i];
-          if (v > 0.0) {
-            owner = (int)i;
-            before = mine;
-            if (mine + v > goal) break;
-          }
-          mine += v;
-        }
-        if (owner < 0 && scribe) a.next_token[b] = -1;
-        if (owner != (int)rank) return;
+        const int cta = find_part(lane < a.cluster ? s.from[parity ^ 1][lane] : 0.0, goal, &before);
+        if (cta < 0 && scribe) a.next_token[b] = -1;
+        if (cta != (int)rank) return;
       }
-      owner = -1;
-      mine = before;
-      for (int i = 0; i < WARPS; i++) {
-        const double v = s.part[i];
-        if (v > 0.0) {
-          owner = i;
-          before = mine;
-          if (mine + v > goal) break;
-        }
-        mine += v;
+      int owner = find_part(lane < WARPS ? s.part[lane] : 0.0, goal, &before);
+      if (owner < 0) {  // (a cluster of one: no mass at all)
+        if (tid == 0) a.next_token[b] = -1;
+        return;
       }
-      if (owner < 0 && tid == 0) a.next_token[b] = -1;  // (a cluster of one: no mass at all)
+      Part w = piece(row.groups(), rank * WARPS + owner, a.cluster * WARPS);
+      if (w.hi - w.lo > 64) {  // all warps on the owner's part
+        const Part all = w;
+        w = piece(all.hi - all.lo, warp, WARPS);
+        w.lo += all.lo;
+        w.hi += all.lo;
+        block_sum(s, any_part_sum<DRAFT>(s, k, gone, row, w));
+        owner = find_part(lane < WARPS ? s.part[lane] : 0.0, goal, &before);
+      }
       if ((int)warp != owner) return;
-      const Part w = warp_part(row.groups(), rank, a.cluster);
       int32_t last = -1;  // the last token with mass, should rounding leave the border behind
       for (uint32_t g0 = w.lo; g0 < w.hi; g0 += 32) {
         const uint32_t g = g0 + lane, x = row.first(g);
@@ -379,7 +436,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) verify_tree_kernel(const
           if (DRAFT) q = row.load(row.q, g);
         }
         double v[4];
-        entries<DRAFT>(s, k, gone, row, g0, p, q, v);
+        rest<4>(s, k, &p.x, &q.x, v);
+        if (!DRAFT) gone.clear(v, x, row.first(g0));
         const double own = ((v[0] + v[1]) + v[2]) + v[3];
         double cum = own;
 #pragma unroll
