@@ -11,6 +11,7 @@ import re
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG_DIR, "libnwd.so")
+BINDING_PATH = os.path.join(PKG_DIR, "_nwd_torch.so")
 HEADER_PATH = os.path.join(os.path.dirname(PKG_DIR), "include", "nwd.h")
 
 NWD_OK = 0
@@ -143,6 +144,30 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_torch = None
+
+
+def torch_calls():
+    """The extension module with the speculative-decoding calls (binding/nwd_torch.cc).  Raises
+    if it is missing: there is no fallback."""
+    global _torch
+    if _torch is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries are the module's)
+        load()
+        if not os.path.exists(BINDING_PATH):
+            raise ImportError(f"{BINDING_PATH} is missing: build it with __graft_entry__.build()")
+        loader = importlib.machinery.ExtensionFileLoader("_nwd_torch", BINDING_PATH)
+        spec = importlib.util.spec_from_file_location("_nwd_torch", BINDING_PATH, loader=loader)
+        mod = importlib.util.module_from_spec(spec)
+        loader.exec_module(mod)
+        mod.set_error(NwdError)
+        _torch = mod
+    return _torch
 
 
 def check(status: int) -> None:

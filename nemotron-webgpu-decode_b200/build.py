@@ -22,6 +22,8 @@ BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libnwd.so")
 HOST_SRC = os.path.join(PKG_DIR, "host", "nwd_host.cc")
 HOST_PATH = os.path.join(PKG_DIR, "nwd_host")
+BINDING_SRC = os.path.join(PKG_DIR, "binding", "nwd_torch.cc")
+BINDING_PATH = os.path.join(PKG_DIR, "_nwd_torch.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
@@ -73,7 +75,33 @@ def build(verbose: bool = False, ptxas_info: bool = False) -> str:
         subprocess.run(cmd, check=True)
         os.replace(tmp, LIB_PATH)
     build_host(verbose)
+    build_binding(verbose)
     return LIB_PATH
+
+
+def build_binding(verbose: bool = False) -> str:
+    """The extension module of the speculative-decoding calls (binding/nwd_torch.cc): links
+    libnwd.so, found next to it, and the installed PyTorch."""
+    if _stale(BINDING_PATH, [BINDING_SRC, LIB_PATH, os.path.join(INCLUDE, "nwd.h")]):
+        import sysconfig
+
+        import torch
+        root = os.path.dirname(torch.__file__)
+        cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+        inc = [INCLUDE, os.path.join(root, "include"),
+               os.path.join(root, "include", "torch", "csrc", "api", "include"), cuda,
+               sysconfig.get_paths()["include"]]
+        tmp = BINDING_PATH + ".tmp"
+        cmd = [os.environ.get("CXX_HOST", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               *[f for d in inc for f in ("-isystem", d)], BINDING_SRC, "-o", tmp, "-L", PKG_DIR,
+               "-lnwd", "-Wl,-rpath,$ORIGIN", "-L", os.path.join(root, "lib"), "-ltorch_python",
+               "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+        os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
 
 
 def build_host(verbose: bool = False) -> str:

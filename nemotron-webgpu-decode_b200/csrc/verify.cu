@@ -112,12 +112,15 @@ template <int N>
 __device__ __forceinline__ void rest(const Walk& s, int k, const float* p, const float* q, double* r) {
 #pragma unroll
   for (int e = 0; e < N; e++) r[e] = k ? rest1(p[e], q[e]) : prob(p[e]);
+  double qd[N];
+#pragma unroll
+  for (int e = 0; e < N; e++) qd[e] = prob(q[e]);
 #pragma unroll 1
   for (int i = 1; i < k; i++) {
     const double sum = s.sum[i];
 #pragma unroll
     for (int e = 0; e < N; e++) {
-      const double t = r[e] - sum * prob(q[e]);
+      const double t = r[e] - sum * qd[e];
       r[e] = t > 0.0 ? t : 0.0;
     }
   }

@@ -237,10 +237,9 @@ def commit_layers(layers, path, n_accepted, stream=None) -> None:
     first = layers[0]
     pools = [p for layer in layers for p in (layer.k_pool, layer.v_pool)]
 
-    def run(raw):
-        ops.kv_commit(pools, first.row_offset, first.lengths, path, n_accepted,
-                      scratch=first.scratch)
-        for layer in layers:
-            layer.lengths += n_accepted
-
-    ops._on(first.lengths.device, stream, run)
+    if stream is not None:
+        with ops._on(stream, first.lengths.device):
+            return commit_layers(layers, path, n_accepted)
+    ops.kv_commit(pools, first.row_offset, first.lengths, path, n_accepted, scratch=first.scratch)
+    for layer in layers:
+        layer.lengths += n_accepted

@@ -373,20 +373,6 @@ def q4_qkv_append(h: torch.Tensor, wq: Q4Weights, wk: Q4Weights, wv: Q4Weights,
 
 # ---------------------------------------------------------------- speculative decoding
 
-def _dev_ptr(t, dtype, shape, device, name) -> int:
-    """The pointer of a contiguous tensor of this type, shape and (CUDA) device."""
-    try:
-        if (t.dtype is dtype and t.shape == shape and t.device == device
-                and device.type == "cuda" and t.is_contiguous()):
-            return t.data_ptr()
-    except AttributeError:
-        pass
-    _ptr(t, dtype, name)
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-
-
 class TreeWorkspace:
     """Partials of the tree-attention calls of one shape.  Needs no initialisation and
     keeps nothing between calls; calls that may overlap need one each (without one, a
@@ -403,70 +389,32 @@ class TreeWorkspace:
         self.ptr = self._buf.data_ptr()
 
 
-_tree_ws_sizes: dict = {}
-
-
 def _tree_ws_bytes(device: int, *shape) -> int:
-    """nwd_attn_tree_workspace_size of a shape (a pure function of shape and device)."""
-    key = (device,) + shape
-    n = _tree_ws_sizes.get(key)
-    if n is None:
-        v = ctypes.c_size_t(0)
-        with torch.cuda.device(device):
-            call("nwd_attn_tree_workspace_size", *shape, ctypes.byref(v))
-        n = _tree_ws_sizes[key] = int(v.value)
-    return n
+    v = ctypes.c_size_t(0)
+    with torch.cuda.device(device):
+        call("nwd_attn_tree_workspace_size", *shape, ctypes.byref(v))
+    return int(v.value)
 
 
-def _on(device, stream, fn, *args):
-    """fn(raw stream, *args) with `device` current and, for a given stream, PyTorch's
-    allocations on it: what the call allocates belongs to the stream that uses it."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _on(device, stream, fn, *args)
-    if stream is None:
-        return fn(torch._C._cuda_getCurrentRawStream(device.index), *args)
+def _on(stream, device):
+    """A context in which `stream` (a torch stream or a raw handle) is PyTorch's current one:
+    the speculative calls run on the current stream of their tensors' device, and what they
+    allocate belongs to it."""
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
-    with torch.cuda.stream(stream):
-        return fn(stream.cuda_stream, *args)
+    return torch.cuda.stream(stream)
 
 
-def _run_tree(raw, name, args, shape, workspace, scratch, device):
-    err = None if scratch is None else scratch.ptr
-    if workspace is not None:
-        call(name, *args, workspace.ptr, workspace.nbytes, err, raw)
-        return
-    nbytes = _tree_ws_bytes(device.index, *shape)
-    buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    call(name, *args, buf.data_ptr(), nbytes, err, raw)
-
-
-def _attention_tree(name, q, new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads,
-                    n_kv_heads, head_dim, tree_len, scale, workspace, scratch, stream):
-    dev, f16, i32 = q.device, torch.float16, torch.int32
-    if parents.dim() != 2:
-        raise ValueError(f"parents must be [batch, n_nodes], got {tuple(parents.shape)}")
-    bn = parents.shape
-    batch, n = bn
-    row, qo, b1 = n_kv_heads * head_dim, (batch, n, n_heads, head_dim), (batch,)
-    args = [_dev_ptr(q, f16, qo, dev, "q")]
-    if new is not None:
-        kv = (batch, n, n_kv_heads, head_dim)
-        args += [_dev_ptr(new[0], f16, kv, dev, "k_new"), _dev_ptr(new[1], f16, kv, dev, "v_new")]
-    pool = k_pool.shape
-    rows = k_pool.numel() // row if row else 0
-    if rows * row != k_pool.numel() or v_pool.numel() != rows * row:
-        raise ValueError("k_pool and v_pool must hold the same whole number of rows")
-    args += [_dev_ptr(k_pool, f16, pool, dev, "k_pool"),
-             _dev_ptr(v_pool, f16, v_pool.shape, dev, "v_pool"), rows,
-             _dev_ptr(row_offset, torch.int64, b1, dev, "row_offset"),
-             _dev_ptr(seq_len, i32, b1, dev, "seq_len" if new is None else "pos"),
-             _dev_ptr(parents, i32, bn, dev, "parents"),
-             None if tree_len is None else _dev_ptr(tree_len, i32, b1, dev, "tree_len"),
-             _dev_ptr(o, f16, qo, dev, "o"), batch, n, n_heads, n_kv_heads, head_dim, scale]
-    _on(dev, stream, _run_tree, name, args, (batch, n, n_heads, n_kv_heads, head_dim), workspace,
-        scratch, dev)
+def _tree(q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads, n_kv_heads,
+          head_dim, tree_len, scale, workspace, scratch, stream):
+    if stream is not None:
+        with _on(stream, q.device):
+            return _tree(q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads,
+                         n_kv_heads, head_dim, tree_len, scale, workspace, scratch, None)
+    ptr, nbytes = (0, 0) if workspace is None else (workspace.ptr, workspace.nbytes)
+    (_lib._torch or _lib.torch_calls()).tree(
+        q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads, n_kv_heads,
+        head_dim, tree_len, scale, ptr, nbytes, 0 if scratch is None else scratch.ptr)
     return o
 
 
@@ -481,9 +429,8 @@ def attention_tree(q, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads: 
     parents [B, N] int32: parents[b, i] < i, -1 for a root; N <= 64.  tree_len [B] int32:
     nodes at or past it are absent (their o is zero).  Device errors (a parent or length out
     of range, rows outside the pool) go to `scratch` (:meth:`Scratch.check`) when given."""
-    return _attention_tree("nwd_attn_tree", q, None, k_pool, v_pool, row_offset, seq_len, parents,
-                           o, n_heads, n_kv_heads, head_dim, tree_len, scale, workspace, scratch,
-                           stream)
+    return _tree(q, None, None, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads,
+                 n_kv_heads, head_dim, tree_len, scale, workspace, scratch, stream)
 
 
 def kv_append_attention_tree(q, k_new, v_new, k_pool, v_pool, row_offset, pos, parents, o,
@@ -492,9 +439,8 @@ def kv_append_attention_tree(q, k_new, v_new, k_pool, v_pool, row_offset, pos, p
                              scratch: Scratch | None = None, stream=None) -> torch.Tensor:
     """:func:`attention_tree` after writing the present nodes' rows k_new / v_new
     [B, N, n_kv, hd] to pool rows row_offset[b] + pos[b] + i (pos: rows before the tree)."""
-    return _attention_tree("nwd_kv_append_attn_tree", q, (k_new, v_new), k_pool, v_pool,
-                           row_offset, pos, parents, o, n_heads, n_kv_heads, head_dim, tree_len,
-                           scale, workspace, scratch, stream)
+    return _tree(q, k_new, v_new, k_pool, v_pool, row_offset, pos, parents, o, n_heads,
+                 n_kv_heads, head_dim, tree_len, scale, workspace, scratch, stream)
 
 
 def verify_tree(tokens, parents, target_probs, u, w, draft_probs=None, tree_len=None, out=None,
@@ -507,33 +453,14 @@ def verify_tree(tokens, parents, target_probs, u, w, draft_probs=None, tree_len=
     i: the target behind node i); draft_probs of the same shape (row i: what node i's
     children were drawn from) or None for drafts without probabilities; u [B, N], w [B] f32
     uniforms in [0, 1).  `out`: the three outputs, to be written in place."""
-    dev, i32, f32 = target_probs.device, torch.int32, torch.float32
-    if target_probs.dim() != 3:
-        raise ValueError("target_probs must be [batch, n_nodes, vocab], got "
-                         f"{tuple(target_probs.shape)}")
-    shape = target_probs.shape
-    batch, n, vocab = shape
-    bn, b1 = (batch, n), (batch,)
-    args = (_dev_ptr(tokens, i32, bn, dev, "tokens"), _dev_ptr(parents, i32, bn, dev, "parents"),
-            None if tree_len is None else _dev_ptr(tree_len, i32, b1, dev, "tree_len"),
-            _dev_ptr(target_probs, f32, shape, dev, "target_probs"),
-            None if draft_probs is None else _dev_ptr(draft_probs, f32, shape, dev, "draft_probs"),
-            _dev_ptr(u, f32, bn, dev, "u"), _dev_ptr(w, f32, b1, dev, "w"))
-    if out is not None:
-        path, n_accepted, next_token = out
-        _dev_ptr(path, i32, bn, dev, "path")
-        _dev_ptr(n_accepted, i32, b1, dev, "n_accepted")
-        _dev_ptr(next_token, i32, b1, dev, "next_token")
-        out = (path, n_accepted, next_token)
-    return _on(dev, stream, _run_verify, args, bn, vocab, out, scratch, tokens)
-
-
-def _run_verify(raw, args, bn, vocab, out, scratch, tokens):
-    if out is None:
-        out = tokens.new_empty(bn), tokens.new_empty(bn[0]), tokens.new_empty(bn[0])
-    call("nwd_verify_tree", *args, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), *bn,
-         vocab, None if scratch is None else scratch.ptr, raw)
-    return out
+    if stream is not None:
+        with _on(stream, target_probs.device):
+            return verify_tree(tokens, parents, target_probs, u, w, draft_probs, tree_len, out,
+                               scratch)
+    path, n_accepted, next_token = (None, None, None) if out is None else out
+    return (_lib._torch or _lib.torch_calls()).verify(
+        tokens, parents, tree_len, target_probs, draft_probs, u, w, path, n_accepted, next_token,
+        0 if scratch is None else scratch.ptr)
 
 
 def kv_commit(pools, row_offset, pos, path, n_accepted, scratch: Scratch | None = None,
@@ -543,31 +470,12 @@ def kv_commit(pools, row_offset, pos, path, n_accepted, scratch: Scratch | None 
     n_accepted[b], in every pool of `pools` (K and V of several layers, each [rows, n_kv, hd]
     fp16, 16 per launch).  path / n_accepted as :func:`verify_tree` returns them; the
     caller's lengths grow by n_accepted."""
-    if path.dim() != 2:
-        raise ValueError(f"path must be [batch, n_nodes], got {tuple(path.shape)}")
-    bn = path.shape
-    dev, i32, b1 = path.device, torch.int32, (bn[0],)
-    args = (_dev_ptr(row_offset, torch.int64, b1, dev, "row_offset"),
-            _dev_ptr(pos, i32, b1, dev, "pos"), _dev_ptr(path, i32, bn, dev, "path"),
-            _dev_ptr(n_accepted, i32, b1, dev, "n_accepted"), *bn)
-    pools = list(pools)
-    if not pools:
-        return
-    shape = pools[0].shape
-    if len(shape) != 3:
-        raise ValueError(f"pools must be [rows, n_kv, hd], got {tuple(shape)}")
-    ptrs = [_dev_ptr(t, torch.float16, shape, dev, "pool") for t in pools]
-    if len(set(ptrs)) != len(ptrs):
-        raise ValueError("pools must differ from one another")
-    _on(dev, stream, _run_commit, ptrs, shape, args, scratch)
-
-
-def _run_commit(raw, ptrs, shape, args, scratch):
-    err = None if scratch is None else scratch.ptr
-    for i in range(0, len(ptrs), 16):
-        part = ptrs[i:i + 16]
-        call("nwd_kv_commit", (ctypes.c_void_p * len(part))(*part), len(part), shape[0], *args,
-             shape[1], shape[2], err, raw)
+    if stream is not None:
+        with _on(stream, path.device):
+            return kv_commit(pools, row_offset, pos, path, n_accepted, scratch)
+    (_lib._torch or _lib.torch_calls()).commit(
+        pools if type(pools) is list else list(pools), row_offset, pos, path, n_accepted,
+        0 if scratch is None else scratch.ptr)
 
 
 def selftest_wait_timeout(workspace: "Workspace", stream=None) -> int:
