@@ -22,8 +22,15 @@ own = False
 HD = 128  # the head size of this framework's attention
 
 
+_package = None
+
+
 def _ops():
-    return importlib.import_module("nemotron-webgpu-decode_b200.ops")
+    """The package's operators, imported once, as a user's program does."""
+    global _package
+    if _package is None:
+        _package = importlib.import_module("nemotron-webgpu-decode_b200.ops")
+    return _package
 
 
 # ------------------------------------------------------------------ cases
