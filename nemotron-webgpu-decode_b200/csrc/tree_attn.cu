@@ -56,8 +56,9 @@
 // (0 x NaN would be NaN), and NaN or infinities in the V rows of the tree are
 // zeroed there too and added at the end to the nodes that see them.
 //
-// All waits are bounded: on expiry the kernel records NWD_DEVERR_PIPE_TIMEOUT,
-// lets its copies and MMAs land, frees its tensor memory and returns.
+// All waits are bounded: the planner gives the CTA up after 2 s without
+// progress, records NWD_DEVERR_PIPE_TIMEOUT, and every role lets its copies and
+// MMAs land and returns; the tensor memory is freed.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -87,8 +88,11 @@ constexpr uint32_t TILE = 2 * CHUNK;    // a K or V block: 16 KiB
 constexpr uint32_t NQ = 2, NK = 5, NV = 5;  // stages
 constexpr uint32_t NP = 4;              // piece descriptors
 constexpr uint32_t PIECE_USERS = 19;    // warps that read them: all but the planner
-// what a block costs in a unit of one tile, of two (in the same unit of time)
-constexpr uint32_t COST1 = 1, COST2 = 2;
+// what a block costs in a unit of one tile, of two (in the same unit of time),
+// and how many blocks' time a unit's beginning and end take
+constexpr uint32_t COST1 = 3, COST2 = 5;
+constexpr uint32_t UNIT_BLOCKS = 6;
+constexpr uint32_t MIN_BLOCKS = 4;  // least part of a unit, of a single sequence
 
 constexpr uint32_t O_Q = 0;
 constexpr uint32_t O_K = O_Q + NQ * Q_TILE;
@@ -102,11 +106,13 @@ constexpr int B_QFULL = 0, B_QEMPTY = B_QFULL + NQ, B_KFULL = B_QEMPTY + NQ,
     B_SFULL = B_VTMA + NV, B_PFULL = B_SFULL + 4, B_PVDONE = B_PFULL + 4,
               // by softmax group
     B_OEMPTY = B_PVDONE + 4, B_ML = B_OEMPTY + 2, B_DRAIN = B_ML + 2,
-              B_PCFULL = B_DRAIN + 1, B_PCEMPTY = B_PCFULL + NP, NBAR = B_PCEMPTY + NP;
+              B_PCFULL = B_DRAIN + 1, B_PCEMPTY = B_PCFULL + NP, B_DONE = B_PCEMPTY + NP,
+              NBAR = B_DONE + 1;
 constexpr uint32_t O_PIECE = (O_BAR + NBAR * 8 + 15) / 16 * 16;  // [NP] Piece
 constexpr uint32_t O_VBAD = O_PIECE + NP * 64;    // [NV] u64: tree rows with NaN or inf in V
 constexpr uint32_t O_GBAD = O_VBAD + NV * 8;      // [2] u64: the same, gathered per group
 constexpr uint32_t O_MISC = O_GBAD + 16;          // tensor memory base, abort flag
+constexpr uint32_t O_DONE = O_MISC + 8;           // [2] u32: K blocks issued, pieces finished
 constexpr uint32_t SMEM_USED = O_MISC + 16;
 // dynamic shared memory starts 1024-byte aligned (there is no static shared
 // memory in this kernel); the kernel checks it
@@ -132,7 +138,8 @@ struct TParams {
   uint64_t pool_rows;
   uint32_t batch, n_nodes, n_heads, n_kv, group;
   uint32_t tile_nodes, n_tiles, unit_tiles, n_units;  // n_units: per sequence
-  uint32_t min_cost;                 // least cost of a CTA's range
+  // one sequence: CTAs per kv head, and of those per unit of two tiles, of one; head_ctas 0: a batch
+  uint32_t head_ctas, pair_ctas, single_ctas;
   uint32_t cost1, cost2, head_cost;  // of a block of a unit of one tile, of two, of all of a head's
   float scale_log2;
 };
@@ -222,8 +229,13 @@ struct Ctx {
   uint32_t sb, bar;  // shared memory, its barriers
   volatile int32_t* abort_flag;
   uint32_t* err;
+  // Waits, the whole warp, until the phase is complete or the CTA gives up:
+  // the planner watches over the others' progress (watch), so that the many
+  // waits are a few instructions each.
   __device__ __forceinline__ bool wait(int b, uint32_t parity) const {
-    return warp_wait(bar + 8 * b, parity, abort_flag, err);
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar + 8 * b, parity)))
+      if (*abort_flag) return false;
+    return true;
   }
   __device__ __forceinline__ void arrive(int b) const { mbar_arrive(bar + 8 * b); }
 };
@@ -286,88 +298,147 @@ __device__ __forceinline__ uint64_t div_small(uint64_t a, uint64_t b) {
   return q;
 }
 
+// The planner's wait: gives the CTA up, with NWD_DEVERR_PIPE_TIMEOUT, after
+// WAIT_LIMIT_NS without a K block issued or a piece finished.
+__device__ __forceinline__ bool watch(const Ctx& c, int b, uint32_t parity) {
+  const volatile uint32_t* done = reinterpret_cast<const uint32_t*>(c.smem + O_DONE);
+  uint32_t last = 0;
+  uint64_t since = 0;
+  while (!__all_sync(0xffffffffu, mbar_try_wait(c.bar + 8 * b, parity))) {
+    if (*c.abort_flag) return false;
+    const uint32_t now = done[0] + done[1];
+    const uint64_t t = globaltimer();
+    if (since == 0 || now != last) {
+      last = now;
+      since = t;
+    }
+    if (__any_sync(0xffffffffu, t - since > WAIT_LIMIT_NS)) {
+      if ((threadIdx.x & 31) == 0) {
+        *c.abort_flag = 1;
+        atomicOr(c.err, NWD_DEVERR_PIPE_TIMEOUT);
+      }
+      return false;
+    }
+  }
+  return true;
+}
+
 // The planner (one warp): this CTA's range, its join, and its pieces.
 //
-// The line that is cut into equal ranges is as long as the blocks' costs; a
-// cut inside a block gives the block to the CTA before the cut.
+// One sequence: its units get CTAs in proportion to their costs (the host's
+// split), each a part of one unit's blocks, so that no CTA has two units'
+// beginnings and ends to wait for.
+//
+// A batch: the units make a line, each as long as its blocks' costs and
+// UNIT_BLOCKS more for its beginning and end, which is cut into equal ranges.
+// A cut inside a block gives the block to the CTA before the cut.
 __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
   const uint32_t lane = threadIdx.x & 31;
-  const uint32_t groups = (p.batch + 31) / 32, per_head = p.n_units / p.n_kv;
-  const uint32_t seq_cost = p.n_kv * p.head_cost;  // of a sequence per block of its length
+  const uint32_t per_head = p.n_units / p.n_kv;
   auto cost_of = [&](uint32_t tiles) { return tiles == 2 ? p.cost2 : p.cost1; };
-  // blocks of 32 sequences at a time; lane l keeps group l's
-  auto group_blocks = [&](uint32_t g, uint32_t* err) -> uint32_t {
-    const uint32_t i = g * 32 + lane;
-    return i < p.batch ? seq_blocks(load_seq(p, i, err)) : 0u;
-  };
-  uint32_t kept = 0;
-  uint64_t total = 0;
-#pragma unroll 2
-  for (uint32_t g = 0; g < groups; g++) {
-    const uint32_t sum = __reduce_add_sync(0xffffffffu, group_blocks(g, p.err));
-    if (lane == g) kept = sum;
-    total += sum;
-  }
-  total *= seq_cost;
-  const uint64_t per = max(div_small(total + gridDim.x - 1, gridDim.x), (uint64_t)p.min_cost);
-  const uint64_t x0 = min(total, (uint64_t)blockIdx.x * per), x1 = min(total, x0 + per);
   MergeDesc join{0, 0, 0, 0};
   int64_t left = 0;
-  uint32_t b = 0, u = 0, blk = 0;
+  uint32_t b = 0, u = 0, blk = 0, nblk = 0;
   TreeSeq s{};
-  uint32_t nblk = 0;
-  if (x1 > x0) {
-    // the sequence that x0 falls into: its group, then its lane
-    const uint64_t y = div_small(x0, seq_cost);  // in blocks of sequence length
-    uint64_t base = 0, upto64 = kept;
-#pragma unroll
-    for (int i = 1; i < 32; i <<= 1) {
-      const uint64_t v = __shfl_up_sync(0xffffffffu, upto64, i);
-      if ((int)lane >= i) upto64 += v;
+  if (p.head_ctas) {
+    s = load_seq(p, 0, p.err);
+    nblk = seq_blocks(s);
+    const uint32_t head = blockIdx.x / p.head_ctas, i = blockIdx.x % p.head_ctas;
+    const uint32_t pairs = p.n_tiles / 2;
+    uint32_t k = p.pair_ctas, unit = pairs ? i / k : 0, at = pairs ? i % k : i;
+    if (unit >= pairs) {
+      unit = pairs;
+      at = i - pairs * k;
+      k = p.single_ctas;
     }
-    uint32_t group;
-    const uint32_t hit = __ballot_sync(0xffffffffu, y < upto64);
-    if (hit) {
-      group = (uint32_t)__ffs(hit) - 1;
-      base = __shfl_sync(0xffffffffu, upto64 - kept, (int)group);
-    } else {  // past the first 1024 sequences
-      base = __shfl_sync(0xffffffffu, upto64, 31);
-      for (group = 32;; group++) {
-        const uint32_t sum = __reduce_add_sync(0xffffffffu, group_blocks(group, nullptr));
-        if (y < base + sum) break;
-        base += sum;
+    if (head < p.n_kv && unit < per_head && at < k) {
+      k = max(1u, min(k, nblk / MIN_BLOCKS));  // parts of at least MIN_BLOCKS
+      u = head * per_head + unit;
+      if (at < k) {
+        blk = (uint32_t)((uint64_t)nblk * at / k);
+        const uint32_t end = (uint32_t)((uint64_t)nblk * (at + 1) / k);
+        left = (int64_t)(end - blk) * cost_of(unit < pairs ? 2 : 1);
+        if (at > 0 && at + 1 == k) join = MergeDesc{1, 0, u, blockIdx.x - at};
       }
     }
-    b = group * 32 + lane;
-    if (b < p.batch) s = load_seq(p, b, nullptr);
-    nblk = b < p.batch ? seq_blocks(s) : 0u;
-    uint32_t upto = nblk;
-#pragma unroll
-    for (int i = 1; i < 32; i <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, upto, i);
-      if ((int)lane >= i) upto += v;
+  } else {
+    const uint32_t groups = (p.batch + 31) / 32;
+    const uint32_t seq_cost = p.n_kv * p.head_cost;  // of a sequence per block of its length
+    // lengths on the line of 32 sequences at a time; lane l keeps group l's
+    auto group_blocks = [&](uint32_t g, uint32_t* err) -> uint32_t {
+      const uint32_t i = g * 32 + lane;
+      return i < p.batch ? seq_blocks(load_seq(p, i, err)) + UNIT_BLOCKS : 0u;
+    };
+    uint32_t kept = 0;
+    uint64_t total = 0;
+#pragma unroll 2
+    for (uint32_t g = 0; g < groups; g++) {
+      const uint32_t sum = __reduce_add_sync(0xffffffffu, group_blocks(g, p.err));
+      if (lane == g) kept = sum;
+      total += sum;
     }
-    const int at = __ffs(__ballot_sync(0xffffffffu, y < base + upto)) - 1;
-    base += __shfl_sync(0xffffffffu, upto - nblk, at);
-    b = group * 32 + (uint32_t)at;
-    nblk = __shfl_sync(0xffffffffu, nblk, at);
-    s.row0 = __shfl_sync(0xffffffffu, s.row0, at);
-    s.ctx = __shfl_sync(0xffffffffu, s.ctx, at);
-    s.nodes = __shfl_sync(0xffffffffu, s.nodes, at);
-    // the unit of this sequence that x0 falls into, and where it starts
-    const uint64_t of_head = (uint64_t)nblk * p.head_cost, of_pair = (uint64_t)nblk * p.cost2;
-    uint64_t r = x0 - base * seq_cost;
-    const uint32_t head = (uint32_t)div_small(r, of_head);
-    r -= head * of_head;
-    const uint32_t k = min((uint32_t)div_small(r, of_pair), per_head - 1);
-    r -= k * of_pair;
-    const uint64_t start = x0 - r;  // of the unit, on the line
-    u = head * per_head + k;
-    const uint32_t cost = cost_of(unit_of(p, u).tiles);
-    blk = (uint32_t)div_small(r + cost - 1, cost);
-    left = (int64_t)(x1 - start) - (int64_t)((uint64_t)blk * cost);
-    if (blk > 0 && blk < nblk && left > 0 && blk + div_small(left + cost - 1, cost) >= nblk)
-      join = MergeDesc{1, b, u, (uint32_t)div_small(start, per)};
+    total *= seq_cost;
+    const uint64_t per = max(div_small(total + gridDim.x - 1, gridDim.x), (uint64_t)p.cost2);
+    const uint64_t x0 = min(total, (uint64_t)blockIdx.x * per), x1 = min(total, x0 + per);
+    if (x1 > x0) {
+      // the sequence that x0 falls into: its group, then its lane
+      const uint64_t y = div_small(x0, seq_cost);  // in blocks of sequence length
+      uint64_t base = 0, upto64 = kept;
+#pragma unroll
+      for (int i = 1; i < 32; i <<= 1) {
+        const uint64_t v = __shfl_up_sync(0xffffffffu, upto64, i);
+        if ((int)lane >= i) upto64 += v;
+      }
+      uint32_t group;
+      const uint32_t hit = __ballot_sync(0xffffffffu, y < upto64);
+      if (hit) {
+        group = (uint32_t)__ffs(hit) - 1;
+        base = __shfl_sync(0xffffffffu, upto64 - kept, (int)group);
+      } else {  // past the first 1024 sequences
+        base = __shfl_sync(0xffffffffu, upto64, 31);
+        for (group = 32;; group++) {
+          const uint32_t sum = __reduce_add_sync(0xffffffffu, group_blocks(group, nullptr));
+          if (y < base + sum) break;
+          base += sum;
+        }
+      }
+      b = group * 32 + lane;
+      if (b < p.batch) s = load_seq(p, b, nullptr);
+      const uint32_t len = b < p.batch ? seq_blocks(s) + UNIT_BLOCKS : 0u;
+      uint32_t upto = len;
+#pragma unroll
+      for (int i = 1; i < 32; i <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, i);
+        if ((int)lane >= i) upto += v;
+      }
+      const int at = __ffs(__ballot_sync(0xffffffffu, y < base + upto)) - 1;
+      base += __shfl_sync(0xffffffffu, upto - len, at);
+      b = group * 32 + (uint32_t)at;
+      s.row0 = __shfl_sync(0xffffffffu, s.row0, at);
+      s.ctx = __shfl_sync(0xffffffffu, s.ctx, at);
+      s.nodes = __shfl_sync(0xffffffffu, s.nodes, at);
+      nblk = seq_blocks(s);
+      // the unit of this sequence that x0 falls into, and where it starts
+      const uint64_t of_head = (uint64_t)(nblk + UNIT_BLOCKS) * p.head_cost;
+      const uint64_t of_pair = (uint64_t)(nblk + UNIT_BLOCKS) * p.cost2;
+      uint64_t r = x0 - base * seq_cost;
+      const uint32_t head = (uint32_t)div_small(r, of_head);
+      r -= head * of_head;
+      const uint32_t k = min((uint32_t)div_small(r, of_pair), per_head - 1);
+      r -= k * of_pair;
+      const uint64_t start = x0 - r;  // of the unit, on the line
+      u = head * per_head + k;
+      const uint32_t cost = cost_of(unit_of(p, u).tiles);
+      blk = (uint32_t)div_small(r + cost - 1, cost);
+      if (blk < nblk) {
+        left = (int64_t)(x1 - start) - (int64_t)((uint64_t)blk * cost);
+        if (blk > 0 && left > 0 && blk + div_small(left + cost - 1, cost) >= nblk)
+          join = MergeDesc{1, b, u, (uint32_t)div_small(start, per)};
+      } else {  // the unit's last block is the CTA's before
+        left = (int64_t)(x1 - start) - (int64_t)((uint64_t)(nblk + UNIT_BLOCKS) * cost);
+        blk = nblk;
+      }
+    }
   }
   if (lane == 0) reinterpret_cast<MergeDesc*>(p.ws + WS_DESC)[blockIdx.x] = join;
 
@@ -378,8 +449,8 @@ __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
     ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, b + 1, p.n_nodes);
   for (;;) {
     Piece d{};
-    if (left > 0 && blk == nblk) {  // on to the next unit (at the start: its last block is the
-      blk = 0;                      // CTA's before)
+    if (left > 0 && blk == nblk) {  // on to the next unit
+      blk = 0;
       if (++u == p.n_units) {
         u = 0;
         b++;
@@ -409,10 +480,10 @@ __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
       turns += d.nb * un.tiles;
       blocks += d.nb;
       tiles += un.tiles;
-      left -= (int64_t)d.nb * cost;
       blk += d.nb;
+      left -= (int64_t)(d.nb + (blk == nblk ? UNIT_BLOCKS : 0)) * cost;
     }
-    if (!c.wait(B_PCEMPTY + (int)r.i, r.phase ^ 1u)) break;
+    if (!watch(c, B_PCEMPTY + (int)r.i, r.phase ^ 1u)) break;
     if (lane == 0) {
       reinterpret_cast<Piece*>(c.smem + O_PIECE)[r.i] = d;
       c.arrive(B_PCFULL + (int)r.i);
@@ -421,6 +492,7 @@ __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
     r.next();
     if (d.tiles == 0) break;
   }
+  watch(c, B_DONE, 0);
 }
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -509,13 +581,17 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + O_MISC);
   volatile uint64_t* vbad = reinterpret_cast<uint64_t*>(smem + O_VBAD);
   volatile uint64_t* gbad = reinterpret_cast<uint64_t*>(smem + O_GBAD);
+  volatile uint32_t* done = reinterpret_cast<uint32_t*>(smem + O_DONE);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Ctx c{smem, smem_u32(smem), smem_u32(smem) + O_BAR,
               reinterpret_cast<int32_t*>(smem + O_MISC + 4), p.err};
 
   nwd::pdl_trigger();
   if (warp == 1) {
-    if (lane == 0) *c.abort_flag = 0;
+    if (lane == 0) {
+      *c.abort_flag = 0;
+      reinterpret_cast<uint2*>(smem + O_DONE)[0] = make_uint2(0u, 0u);
+    }
     for (int i = lane; i < NBAR; i += 32) {
       uint32_t count = 1;
       // a stage is released by both groups' issuers
@@ -524,7 +600,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         count = 2;
       if ((i >= B_PFULL && i < B_PVDONE) || (i >= B_OEMPTY && i < B_DRAIN)) count = BM;
       if (i == B_DRAIN) count = 4;
-      if (i >= B_PCEMPTY) count = PIECE_USERS;
+      if (i >= B_PCEMPTY) count = PIECE_USERS;  // and B_DONE: the same warps
       mbar_init(c.bar + 8 * i, count);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -580,6 +656,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           __syncwarp();
           r.next();
           issued++;
+          if (lane == 0) done[0] = issued;
         }
       }
       if (!ok) land<NK>(c, B_KFULL, issued);
@@ -871,8 +948,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
           // The exponentials are taken against the maximum so far, beside the
-          // search for this block's: only where that lies 2^8 above it (the
-          // first blocks, as a rule) is O rescaled and are they taken again.
+          // search for this block's: only where that lies 2^8 above it is O
+          // rescaled and are they taken again.
+          if (turn == first_turn) {
+            float mv[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int k = 4; k < (int)BN; k++) mv[k & 3] = fmaxf(mv[k & 3], s[k]);
+            m = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * p.scale_log2;
+          }
           float pk[32];
           float2 sum, sum1;
           bool again;
@@ -1056,9 +1139,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (both) c.arrive(B_OEMPTY + (int)(g0 ^ 1));
         units += both || g0 == 0;
         units1 += both || g0 == 1;
+        if (tid == 512) done[1] = units + units1;
       }
     }
   }
+  if (warp != 3 && lane == 0) c.arrive(B_DONE);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1309,7 +1394,13 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
   p.cost1 = COST1;
   p.cost2 = COST2;
   p.head_cost = t.n_tiles / 2 * p.cost2 + (t.n_tiles & 1) * p.cost1;
-  p.min_cost = p.cost2;
+  if (batch == 1 && (uint32_t)di.sm_count / n_kv >= p.n_units / n_kv) {
+    const uint32_t pairs = t.n_tiles / 2, single = t.n_tiles & 1;
+    p.head_ctas = (uint32_t)di.sm_count / n_kv;
+    if (single) p.single_ctas = std::max(1u, p.head_ctas * p.cost1 / p.head_cost);
+    if (pairs) p.pair_ctas = (p.head_ctas - p.single_ctas) / pairs;
+    if (single) p.single_ctas = p.head_ctas - pairs * p.pair_ctas;
+  }
   p.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f;
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e = cudaSuccess;
