@@ -1158,16 +1158,17 @@ __global__ void __launch_bounds__(THREADS, 1)
 //
 // A work item is 8 rows of a tile of such a unit.  Every block finds the units
 // (all CTAs' descriptors in one round of loads) and takes its share of the
-// items, 256 threads to an item: a thread has one row's column quad.  The
-// rows' (m, l) of all pieces are fetched at once and become weights in shared
-// memory; the O terms are then independent loads, 8 in flight per thread.
-// (One block per item and CTA, most of them for nothing, took 12 us where this
-// takes 5: 26 nodes over 4 070 rows.)
+// items; a thread has one row's column quad, and fetches 8 pieces' (m, l) and
+// O terms at a time, all in flight together, with no word to the other
+// threads.  (A first form with a block per item and CTA, and the weights in
+// shared memory, took 5 us of 26 nodes over 4 070 rows, where this takes 3, and
+// 24 us of 16 x 61 nodes, where this takes 7.)  One wave of blocks: six blocks
+// per SM where three are resident cost 16 x 61 nodes 3 us more.
 constexpr uint32_t MERGE_ROWS = 8;
 constexpr uint32_t MERGE_THREADS = 256;
+constexpr uint32_t MERGE_AHEAD = 8;
 __global__ void __launch_bounds__(MERGE_THREADS)
     tree_merge_kernel(const __grid_constant__ TParams p, uint32_t ctas) {
-  __shared__ float2 w[(MAX_CTAS + 1) * MERGE_ROWS];  // (m, l), then (weight, weighted l); last 1 / L
   __shared__ MergeDesc units[MAX_CTAS];
   __shared__ uint32_t owner[MAX_CTAS];  // the CTA that a unit ends in
   __shared__ uint32_t counts[MERGE_THREADS / 32];
@@ -1196,59 +1197,51 @@ __global__ void __launch_bounds__(MERGE_THREADS)
   const uint32_t per_unit = p.unit_tiles * chunks;
   const float2* ml = reinterpret_cast<const float2*>(p.ws + WS_ML);
   const float4* po = reinterpret_cast<const float4*>(p.ws + ws_o(ctas, p.unit_tiles));
+  const uint32_t r = tid & 7, quad = tid >> 3;
+#pragma unroll 1
   for (uint32_t item = blockIdx.x; item < n_units * per_unit; item += gridDim.x) {
     d = units[item / per_unit];
     const uint32_t first = d.first, n = owner[item / per_unit] - first + 1;
-    const uint32_t t = item % per_unit / chunks, row0 = item % chunks * MERGE_ROWS;
+    const uint32_t t = item % per_unit / chunks, row = item % chunks * MERGE_ROWS + r;
     const Unit un = unit_of(p, d.u);
     const uint32_t tile = un.tile0 + t;
     if (t >= un.tiles) continue;
-    const uint32_t rows = min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes) * p.group;
-    if (row0 >= rows) continue;
-    // the unit's first piece is the one its CTA ended with, the others begin theirs
-    auto slot = [&](uint32_t i) {
-      return (((first + i) * 2 + (i == 0 ? 1 : 0)) * p.unit_tiles + t) * BM;
-    };
-    const uint32_t r = tid & 7, row = row0 + r, quad = tid >> 3;
+    if (row >= min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes) * p.group) continue;
     const uint32_t node = tile * p.tile_nodes + row / p.group;
     const nwd::TreeRaw raw =
         nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, d.b, p.n_nodes);
-    float4 x[8];  // the first terms, on their way while the weights are found
-#pragma unroll
-    for (uint32_t k = 0; k < 8; k++)
-      if (k < n) x[k] = __ldcg(po + (size_t)slot(k) * (HD / 4) + quad * BM + row);
-    for (uint32_t i = tid; i < n * MERGE_ROWS; i += MERGE_THREADS)
-      w[i] = __ldcg(ml + slot(i / MERGE_ROWS) + row0 + i % MERGE_ROWS);
-    __syncthreads();
-    {  // a warp per row
-      float M = -INFINITY, L = 0.f;
-      for (uint32_t i = lane; i < n; i += 32) M = fmaxf(M, w[i * MERGE_ROWS + warp].x);
-#pragma unroll
-      for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-      for (uint32_t i = lane; i < n; i += 32) {
-        const float2 a = w[i * MERGE_ROWS + warp];
-        // a piece without weights counts for nothing (l may be NaN)
-        const float e = a.y != 0.f ? ex2f(a.x - M) : 0.f;
-        const float l = a.y != 0.f ? a.y * e : 0.f;
-        w[i * MERGE_ROWS + warp] = make_float2(e, l);
-        L += l;
-      }
-#pragma unroll
-      for (int k = 16; k; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
-      if (lane == 0) w[n * MERGE_ROWS + warp].x = L != 0.f ? 1.f / L : 0.f;
-    }
-    __syncthreads();
+    float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t i0 = 0; i0 < n; i0 += 8) {
-      if (i0) {
+#pragma unroll 1
+    for (uint32_t i0 = 0; i0 < n; i0 += MERGE_AHEAD) {
+      float4 x[MERGE_AHEAD];
+      float2 a[MERGE_AHEAD];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++)
-          if (i0 + k < n) x[k] = __ldcg(po + (size_t)slot(i0 + k) * (HD / 4) + quad * BM + row);
+      for (uint32_t k = 0; k < MERGE_AHEAD; k++) {
+        // the unit's first piece is the one its CTA ended with, the others begin theirs
+        const uint32_t i = i0 + k;
+        const uint32_t slot = (((first + i) * 2 + (i == 0 ? 1 : 0)) * p.unit_tiles + t) * BM;
+        a[k] = make_float2(-INFINITY, 0.f);
+        if (i < n) {
+          a[k] = __ldcg(ml + slot + row);
+          x[k] = __ldcg(po + (size_t)slot * (HD / 4) + quad * BM + row);
+        }
       }
+      float top = M;
 #pragma unroll
-      for (uint32_t k = 0; k < 8; k++) {
-        const float e = i0 + k < n ? w[(i0 + k) * MERGE_ROWS + r].x : 0.f;
-        if (e != 0.f) {
+      for (uint32_t k = 0; k < MERGE_AHEAD; k++) top = fmaxf(top, a[k].x);
+      const float alpha = L != 0.f ? ex2f(M - top) : 0.f;
+      L = L != 0.f ? L * alpha : 0.f;
+      o.x *= alpha;
+      o.y *= alpha;
+      o.z *= alpha;
+      o.w *= alpha;
+      M = top;
+#pragma unroll
+      for (uint32_t k = 0; k < MERGE_AHEAD; k++) {
+        if (a[k].y != 0.f) {  // a piece without weights counts for nothing (l may be NaN)
+          const float e = ex2f(a[k].x - top);
+          L += a[k].y * e;
           o.x += x[k].x * e;
           o.y += x[k].y * e;
           o.z += x[k].z * e;
@@ -1256,16 +1249,13 @@ __global__ void __launch_bounds__(MERGE_THREADS)
         }
       }
     }
-    if (row < rows) {
-      const bool none = node >= nwd::tree_seq(raw, p.pool_rows, p.n_nodes, nullptr).nodes;
-      const float inv = w[n * MERGE_ROWS + r].x;
-      const __half2 h[2] = {__floats2half2_rn(none ? 0.f : o.x * inv, none ? 0.f : o.y * inv),
-                            __floats2half2_rn(none ? 0.f : o.z * inv, none ? 0.f : o.w * inv)};
-      *reinterpret_cast<uint2*>(p.o + (((size_t)d.b * p.n_nodes + node) * p.n_heads +
-                                       un.hkv * p.group + row % p.group) * HD + quad * 4) =
-          *reinterpret_cast<const uint2*>(h);
-    }
-    __syncthreads();  // w is free for the next item
+    const bool none = node >= nwd::tree_seq(raw, p.pool_rows, p.n_nodes, nullptr).nodes;
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+    const __half2 h[2] = {__floats2half2_rn(none ? 0.f : o.x * inv, none ? 0.f : o.y * inv),
+                          __floats2half2_rn(none ? 0.f : o.z * inv, none ? 0.f : o.w * inv)};
+    *reinterpret_cast<uint2*>(p.o + (((size_t)d.b * p.n_nodes + node) * p.n_heads +
+                                     un.hkv * p.group + row % p.group) * HD + quad * 4) =
+        *reinterpret_cast<const uint2*>(h);
   }
 }
 
@@ -1416,7 +1406,7 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
   const uint32_t ctas = (uint32_t)di.sm_count;
   e = launch_pdl(tree_kernel, dim3(ctas), dim3(THREADS), SMEM_BYTES, s, tq, tk, tv, p);
   if (e == cudaSuccess)
-    e = launch_pdl(tree_merge_kernel, dim3(ctas * 6), dim3(MERGE_THREADS), 0, s, p, ctas);
+    e = launch_pdl(tree_merge_kernel, dim3(ctas * 3), dim3(MERGE_THREADS), 0, s, p, ctas);
   if (e != cudaSuccess) return cuda_fail(e, who);
   return ok();
 }
