@@ -453,8 +453,9 @@ int nwd_attn_tree_workspace_size(uint32_t batch, uint32_t n_nodes, uint32_t n_he
  *   q, o          : [batch, n_nodes, n_heads, head_dim]; absent nodes' o = 0
  *   k_pool, v_pool: [pool_rows, n_kv_heads, head_dim], the nodes' rows in place
  *   row_offset    : device int64[batch]; seq_len: device int32[batch]
- * head_dim 128, group 1..8, batch <= 4096.  Rows that a node does not attend
- * never reach its output, whatever they hold. */
+ * head_dim 128, group 1..8, batch <= 4096; tensors 16-byte aligned, o apart from
+ * the others.  Rows that a node does not attend never reach its output, whatever
+ * they hold. */
 int nwd_attn_tree(const uint16_t* q, const uint16_t* k_pool, const uint16_t* v_pool,
                   uint64_t pool_rows, const int64_t* row_offset, const int32_t* seq_len,
                   const int32_t* parents, const int32_t* tree_len, uint16_t* o, uint32_t batch,
@@ -463,7 +464,7 @@ int nwd_attn_tree(const uint16_t* q, const uint16_t* k_pool, const uint16_t* v_p
 
 /* The same after writing the present nodes' rows k_new / v_new ([batch, n_nodes,
  * n_kv_heads, head_dim]) into the pools (bit-exact).  Sequences of one call must
- * not share the rows that they write. */
+ * not share the rows that they write, and the pools must be two. */
 int nwd_kv_append_attn_tree(const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
                             uint16_t* k_pool, uint16_t* v_pool, uint64_t pool_rows,
                             const int64_t* row_offset, const int32_t* pos, const int32_t* parents,

@@ -204,14 +204,17 @@ class BatchedDecodeAttention:
         """A speculative step: the trees' K/V rows go behind every sequence's rows and each
         node attends the rows, its ancestors and itself.  q [B, N, heads, hd], k_new / v_new
         [B, N, kv_heads, hd], parents [B, N] (:func:`ops.attention_tree`).  The lengths stay
-        until :meth:`commit`."""
+        until :meth:`commit`.  A sequence's capacity has to hold its tree too."""
+        if stream is not None:
+            with ops._on(stream, self.device):
+                return self.tree_step(q, k_new, v_new, parents, tree_len, out)
         if out is None:
             out = torch.empty(q.shape, dtype=torch.float16, device=self.device)
         return ops.kv_append_attention_tree(q, k_new, v_new, self.k_pool, self.v_pool,
                                             self.row_offset, self.lengths, parents, out,
                                             self.heads, self.kv_heads, self.head_dim,
                                             tree_len=tree_len, scale=self.scale,
-                                            scratch=self.scratch, stream=stream)
+                                            scratch=self.scratch)
 
     def commit(self, path, n_accepted, stream=None) -> None:
         """Keeps the accepted nodes of the last :meth:`tree_step` (:func:`ops.verify_tree`'s
@@ -241,5 +244,5 @@ def commit_layers(layers, path, n_accepted, stream=None) -> None:
         with ops._on(stream, first.lengths.device):
             return commit_layers(layers, path, n_accepted)
     ops.kv_commit(pools, first.row_offset, first.lengths, path, n_accepted, scratch=first.scratch)
-    for layer in layers:
-        layer.lengths += n_accepted
+    for lengths in {layer.lengths.data_ptr(): layer.lengths for layer in layers}.values():
+        lengths += n_accepted  # (layers may share one tensor)

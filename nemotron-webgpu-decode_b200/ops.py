@@ -411,7 +411,11 @@ def _tree(q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_he
         with _on(stream, q.device):
             return _tree(q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads,
                          n_kv_heads, head_dim, tree_len, scale, workspace, scratch, None)
-    ptr, nbytes = (0, 0) if workspace is None else (workspace.ptr, workspace.nbytes)
+    ptr, nbytes = 0, 0
+    if workspace is not None:
+        if workspace.device != q.device:
+            raise ValueError(f"the workspace is on {workspace.device}, q on {q.device}")
+        ptr, nbytes = workspace.ptr, workspace.nbytes
     (_lib._torch or _lib.torch_calls()).tree(
         q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads, n_kv_heads,
         head_dim, tree_len, scale, ptr, nbytes, 0 if scratch is None else scratch.ptr)

@@ -181,3 +181,37 @@ def test_speculative_steps_as_used(ops, engine_mod):
                                            np.array([-1]), 1, nkv, HD ** -0.5)
             assert (np.abs(got[i] - ref[0]) <=
                     attention_bound(ref, mag, amp, len(kk), HD ** -0.5, 6.0)[0]).all()
+
+
+def test_layers_that_share_their_lengths(ops, engine_mod):
+    layers = [engine_mod.BatchedDecodeAttention([20, 20], 4, 2) for _ in range(2)]
+    layers[1].lengths = layers[0].lengths
+    path = torch.tensor([[0, 2, -1], [0, -1, -1]], dtype=torch.int32, device="cuda")
+    count = torch.tensor([2, 1], dtype=torch.int32, device="cuda")
+    engine_mod.commit_layers(layers, path, count)
+    assert layers[0].lengths.tolist() == [2, 1]
+    with pytest.raises(ValueError, match="differ"):
+        engine_mod.commit_layers([layers[0], layers[0]], path, count)
+
+
+def test_tree_step_on_a_stream(ops, engine_mod):
+    """A step on a stream that is not the current one, which still has work to do."""
+    rng = np.random.default_rng(5)
+    layer = engine_mod.BatchedDecodeAttention([64], 8, 2)
+    t = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float16)).cuda()  # noqa: E731
+    layer.k_pool.copy_(t(64, 2, HD))
+    layer.v_pool.copy_(t(64, 2, HD))
+    layer.lengths.fill_(20)
+    q, k, v = t(1, 5, 8, HD), t(1, 5, 2, HD), t(1, 5, 2, HD)
+    parents = torch.tensor([[-1, 0, 0, 1, 2]], dtype=torch.int32, device="cuda")
+    want = layer.tree_step(q, k, v, parents).clone()
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    busy = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(10):
+        trash = torch.mm(busy, busy)
+        del trash
+    got = layer.tree_step(q, k, v, parents, stream=s)
+    s.synchronize()
+    assert torch.equal(got, want)

@@ -14,9 +14,10 @@ def L(nwd):
 
 
 P = ctypes.c_void_p(256)
+O = ctypes.c_void_p(512)  # an output apart from P  # noqa: E741
 
 
-def _tree(lib, q=P, k=P, rows=100, off=P, parents=P, o=P, b=1, n=4, nh=8, nkv=2, hd=128, scale=0.0,
+def _tree(lib, q=P, k=O, rows=100, off=P, parents=P, o=O, b=1, n=4, nh=8, nkv=2, hd=128, scale=0.0,
           ws=P, ws_bytes=1 << 40, new=None):
     f = ctypes.c_float(scale)
     if new is None:
@@ -42,7 +43,7 @@ def test_tree_attention_refusals(L, new):
         (dict(scale=float("inf")), L.NWD_ERR_INVALID), (dict(rows=0), L.NWD_ERR_INVALID),
         (dict(rows=2 ** 31 + 1), L.NWD_ERR_INVALID),
         (dict(ws=None), L.NWD_ERR_WORKSPACE), (dict(ws=odd), L.NWD_ERR_WORKSPACE),
-        (dict(ws_bytes=0), L.NWD_ERR_WORKSPACE),
+        (dict(ws_bytes=0), L.NWD_ERR_WORKSPACE), (dict(o=P), L.NWD_ERR_INVALID),
     ]:
         assert _tree(lib, new=new, **kw) == status, kw
         assert lib.nwd_last_error()
@@ -50,6 +51,7 @@ def test_tree_attention_refusals(L, new):
     assert _tree(lib, new=new, n=0) == L.NWD_OK
     if new is not None:
         assert _tree(lib, new=odd) == L.NWD_ERR_INVALID
+        assert _tree(lib, new=new, k=P) == L.NWD_ERR_INVALID  # K and V in one pool
 
 
 def test_workspace_size_refusals(L):

@@ -322,3 +322,102 @@ def test_given_workspace(ops):
     ws = ops.TreeWorkspace(2, 12, 40, 8)
     ws._buf.fill_(255)  # whatever it held
     c.check(_attend(ops, d, 40, 8, workspace=ws))
+
+
+@pytest.mark.parametrize("ctx,n,nh,nkv,tree_len", [
+    ([300, 0, 1000, 64, 63, 2000, 5], 61, 40, 8, [61, 1, 25, 26, 0, 50, 51]),  # 25 nodes per tile
+    ([700, 20, 90, 333, 128], 64, 8, 1, [17, 64, 0, 16, 48]),                  # 16 per tile, 4 tiles
+    ([4000], 61, 40, 8, [25]), ([4000], 61, 40, 8, [26]), ([4000], 61, 40, 8, [61]),
+    ([4000], 64, 16, 2, [33]), ([900], 64, 16, 2, [0]), ([0], 61, 40, 8, [7]),
+    ([500] * 40, 60, 5, 1, [0] * 38 + [60, 1]),
+])
+def test_short_trees_of_several_tiles(ops, ctx, n, nh, nkv, tree_len):
+    """Tiles without a present node: no work, zero outputs."""
+    c = Case(ctx, n, nh, nkv, seed=sum(tree_len) + n, tree_len=tree_len)
+    sc = ops.Scratch()
+    c.check(_attend(ops, c.dev(), nh, nkv, scratch=sc))
+    assert sc.check() == 0
+
+
+@pytest.mark.parametrize("n,tree_len", [(2, None), (34, 3)])
+def test_more_than_a_thousand_sequences(ops, n, tree_len):
+    rng = np.random.default_rng(21)
+    ctx = rng.integers(0, 90, 1100).tolist()
+    lens = None if tree_len is None else rng.integers(0, tree_len + 1, 1100).tolist()
+    if lens:
+        lens[1050] = n
+    c = Case(ctx, n, 4, 1, seed=22, tree_len=lens)
+    c.check(_attend(ops, c.dev(), 4, 1))
+
+
+def test_more_heads_than_processors(ops):
+    c = Case([150], 3, 200, 200, seed=23)
+    c.check(_attend(ops, c.dev(), 200, 200))
+
+
+def test_output_aligned_to_16_bytes(ops):
+    c = Case([90, 300], 11, 16, 4, seed=24)
+    d = c.dev()
+    buf = torch.full((c.q.size + 16,), 9.0, dtype=torch.float16, device="cuda")
+    o = buf[8:-8].view(c.q.shape)
+    assert o.data_ptr() % 32 == 16
+    ops.attention_tree(d["q"], d["k_pool"], d["v_pool"], d["row_offset"], d["seq_len"],
+                       d["parents"], o, 16, 4, HD)
+    c.check(o)
+    assert (buf[:8] == 9).all() and (buf[-8:] == 9).all()
+
+
+@pytest.mark.parametrize("b", [1, 6])
+@pytest.mark.parametrize("n", [5, 40])
+def test_scores_that_keep_rising(ops, b, n):
+    """Every block's largest score lies more than 2^8 above the block's before."""
+    c = Case([700] * b, n, 16, 2, seed=25)
+    c.q = np.abs(c.q)
+    c.k = (np.sign(c.k) * 0.25).astype(np.float16)
+    for i in range(b):
+        c.k[c.off[i]:c.off[i] + 700] += (np.arange(700) // 64 * 1.5).astype(np.float16)[:, None, None]
+    c.check(_attend(ops, c.dev(), 16, 2))
+
+
+def test_nothing_to_do(ops):
+    """No sequence, or no node: the output stays as it is."""
+    k = torch.zeros(4, 2, HD, dtype=torch.float16, device="cuda")
+    for b, n in ((0, 4), (2, 0)):
+        q = torch.zeros(b, n, 8, HD, dtype=torch.float16, device="cuda")
+        one = torch.zeros(b, dtype=torch.int32, device="cuda")
+        par = torch.zeros(b, n, dtype=torch.int32, device="cuda")
+        o = torch.empty_like(q)
+        assert ops.attention_tree(q, k, k, one.long(), one, par, o, 8, 2) is o
+
+
+def test_refusals_of_tensors(ops):
+    c = Case([30, 50], 6, 8, 2, seed=26)
+    d = c.dev()
+    o = torch.empty_like(d["q"])
+
+    def call(**kw):
+        a = dict(d, o=o)
+        ws = kw.pop("workspace", None)
+        a.update(kw)
+        ops.attention_tree(a["q"], a["k_pool"], a["v_pool"], a["row_offset"], a["seq_len"],
+                           a["parents"], a["o"], 8, 2, HD, tree_len=a["tree_len"], workspace=ws)
+
+    call()
+    for kw in (dict(q=d["q"].float()), dict(row_offset=d["row_offset"].int()),
+               dict(seq_len=d["seq_len"].long()), dict(parents=d["parents"].long()),
+               dict(o=o.bfloat16()), dict(tree_len=d["seq_len"].float()), dict(q=None)):
+        with pytest.raises(TypeError):
+            call(**kw)
+    for kw in (dict(q=d["q"][:, :5].contiguous()), dict(q=d["q"].transpose(0, 1).contiguous()),
+               dict(o=o.transpose(0, 1)), dict(seq_len=d["seq_len"][:1]),
+               dict(k_pool=d["k_pool"][:-1]), dict(k_pool=d["k_pool"].transpose(0, 1)),
+               dict(parents=d["parents"][0]), dict(q=d["q"].cpu()), dict(parents=d["parents"].cpu()),
+               dict(q=torch.empty(2, 6, 8, 2 * HD, dtype=torch.float16, device="cuda")[..., ::2])):
+        with pytest.raises(ValueError):
+            call(**kw)
+    with pytest.raises(ops.NwdError):
+        call(o=d["q"])
+    small = ops.TreeWorkspace(2, 6, 8, 2)
+    small.nbytes = 4096
+    with pytest.raises(ops.NwdError):
+        call(workspace=small)

@@ -51,18 +51,18 @@ def one_sequence(nblk, n_kv, n_tiles, ctas, cost1, cost2):
     return out, joins, n_kv * per_head
 
 
-def pieces(blocks, n_kv, n_tiles, ctas, cost1, cost2):
-    """Per CTA the list of (b, u, blk, nb) and its join (b, u, first), as the kernel finds them."""
+def pieces(blocks, n_kv, tiles, ctas, cost1, cost2):
+    """Per CTA the list of (b, u, blk, nb) and its join (b, u, first), as the kernel finds them;
+    `tiles`: those of each sequence's present nodes."""
     if len(blocks) == 1:
-        split = one_sequence(blocks[0], n_kv, n_tiles, ctas, cost1, cost2)
+        split = one_sequence(blocks[0], n_kv, tiles[0], ctas, cost1, cost2)
         if split:
             return split
-    per_head = -(-n_tiles // 2)
-    n_units, head_cost = n_kv * per_head, n_tiles // 2 * cost2 + n_tiles % 2 * cost1
-    seq_cost = n_kv * head_cost
-    total = sum(n + UNIT_BLOCKS for n in blocks) * seq_cost
+    head_cost = [t // 2 * cost2 + t % 2 * cost1 for t in tiles]
+    length = [(n + UNIT_BLOCKS) * h for n, h in zip(blocks, head_cost)]
+    total = sum(length) * n_kv
     per = max(-(-total // ctas), cost2)
-    cost_of = lambda u: cost2 if unit_tiles(u, n_tiles) == 2 else cost1  # noqa: E731
+    cost_of = lambda b, u: cost2 if unit_tiles(u, tiles[b]) == 2 else cost1  # noqa: E731
     out, joins = [], {}
     for c in range(ctas):
         x0, x1 = min(total, c * per), min(total, c * per + per)
@@ -70,17 +70,17 @@ def pieces(blocks, n_kv, n_tiles, ctas, cost1, cost2):
         out.append(mine)
         if x0 >= x1:
             continue
-        y, lo, b = x0 // seq_cost, 0, 0
-        while not lo <= y < lo + blocks[b] + UNIT_BLOCKS:
-            lo += blocks[b] + UNIT_BLOCKS
+        y, lo, b = x0 // n_kv, 0, 0
+        while not lo <= y < lo + length[b]:
+            lo += length[b]
             b += 1
-        n = blocks[b]
-        r = x0 - lo * seq_cost
-        head, r = divmod(r, (n + UNIT_BLOCKS) * head_cost)
+        n, per_head = blocks[b], -(-tiles[b] // 2)
+        r = x0 - lo * n_kv
+        head, r = divmod(r, length[b])
         k = min(r // ((n + UNIT_BLOCKS) * cost2), per_head - 1)
         r -= k * (n + UNIT_BLOCKS) * cost2
         start, u = x0 - r, head * per_head + k
-        cost = cost_of(u)
+        cost = cost_of(b, u)
         blk = -(-r // cost)
         if blk < n:
             left = x1 - start - blk * cost
@@ -92,15 +92,15 @@ def pieces(blocks, n_kv, n_tiles, ctas, cost1, cost2):
         while left > 0:
             if blk == n:
                 blk, u = 0, u + 1
-                if u == n_units:
+                if u == n_kv * -(-tiles[b] // 2):
                     u, b = 0, b + 1
                 n = blocks[b]
-            cost = cost_of(u)
+            cost = cost_of(b, u)
             nb = n - blk if left >= (n - blk) * cost else -(-left // cost)
             mine.append((b, u, blk, nb))
             blk += nb
             left -= (nb + (UNIT_BLOCKS if blk == n else 0)) * cost
-    return out, joins, n_units
+    return out, joins, n_kv * sum(-(-t // 2) for t in tiles)
 
 
 @pytest.mark.parametrize("seed", range(120))
@@ -108,8 +108,10 @@ def test_split_covers_every_unit(seed):
     r = random.Random(seed)
     blocks = [r.choice([1, 1, 2, 5, 33, r.randint(1, 400)]) for _ in range(r.choice([1, 1, 2, 7, 64]))]
     cost1 = r.choice([1, 1, 2, 3])
-    got, joins, n_units = pieces(blocks, r.choice([1, 2, 8]), r.choice([1, 2, 3, 4]),
-                                 r.choice([1, 7, 148]), cost1, r.randint(cost1, 2 * cost1))
+    n_tiles = r.choice([1, 2, 3, 4])
+    tiles = [r.choice([n_tiles, r.randint(1, n_tiles)]) for _ in blocks]
+    got, joins, n_units = pieces(blocks, r.choice([1, 2, 8]), tiles, r.choice([1, 7, 148]), cost1,
+                                 r.randint(cost1, 2 * cost1))
     seen, slots = {}, set()
     for c, mine in enumerate(got):
         for b, u, blk, nb in mine:
@@ -134,7 +136,7 @@ def test_split_covers_every_unit(seed):
             cs = [c for _, _, c in parts]
             assert cs == list(range(first, joining[0] + 1))
             assert parts[0][0] == 0 and all(blk > 0 for blk, _, _ in parts[1:])
-    assert len(seen) == len(blocks) * n_units
+    assert len(seen) == n_units
 
 
 class Bar:
