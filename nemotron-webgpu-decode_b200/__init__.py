@@ -5,9 +5,10 @@ C ABI of ``include/nwd.h``).  This package is the host-side mirror of the
 reference's operator interface for that path:
 
 * :mod:`.ops`    — ``kv_append`` / ``attention`` with the WGSL ``Params``
-  fields, plus batched, fused and shard-partial variants;
+  fields, plus batched, fused and shard-partial variants, and the
+  speculative-decoding calls (``attention_tree``, ``verify_tree``, ``kv_commit``);
 * :mod:`.engine` — the attention-layer slice of ``DecodeEngine`` (caches,
-  ``seq``, step, reset);
+  ``seq``, step, reset; ``tree_step`` / ``commit`` of a batch);
 * :mod:`.mgpu`   — the long-context decode sharded over GPUs.
 
 Import with ``importlib.import_module("nemotron-webgpu-decode_b200")``.

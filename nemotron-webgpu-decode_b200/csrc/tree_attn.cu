@@ -57,6 +57,18 @@
 // (0 x NaN would be NaN), and NaN or infinities in the V rows of the tree are
 // zeroed there too and added at the end to the nodes that see them.
 //
+// Bound by: the cache's bytes while the query rows of a kv head fill one tile in
+// part (256 chains of 5 nodes, group 4: 4.7 GB in 751 us, 6.25 TB/s); with two
+// tiles by the latency of a turn's chain S -> softmax -> P V, about 1.1 us per
+// block and pair of tiles: no unit of the SM is more than 45 % busy then
+// (sixteen trees of up to 61 nodes, group 5: 137 us; tensor pipe 39 %, exponentials
+// 42 %, DRAM 45 %).  Shared memory and tensor memory are full with two groups, so
+// a third turn in flight would need smaller blocks.  Built, measured and not
+// kept (60 nodes over 32 700 rows, 66 us): scores in registers at once with the
+// weights in buffers of their own 69.5; one arrival per warp on the barriers
+// 68.4; a quarter of the exponentials by polynomial 66.4; one issuer per group
+// instead of two cost the 256 chains a third.
+//
 // All waits are bounded: the planner gives the CTA up after 2 s without
 // progress, records NWD_DEVERR_PIPE_TIMEOUT, and every role lets its copies and
 // MMAs land and returns; the tensor memory is freed.
@@ -89,11 +101,16 @@ constexpr uint32_t TILE = 2 * CHUNK;    // a K or V block: 16 KiB
 constexpr uint32_t NQ = 2, NK = 5, NV = 5;  // stages
 constexpr uint32_t NP = 4;              // piece descriptors
 constexpr uint32_t PIECE_USERS = 19;    // warps that read them: all but the planner
-// what a block costs in a unit of one tile, of two (in the same unit of time),
-// and how many blocks' time a unit's beginning and end take
-constexpr uint32_t COST1 = 3, COST2 = 5;
+// What a block costs in a unit of one tile, of two (in the same unit of time):
+// 60 nodes over 32 700 rows, three tiles, 65.2 us; as 3 to 5 65.6, 3 to 4 69.0.
+constexpr uint32_t COST1 = 1, COST2 = 2;
+// How many blocks' time a unit's beginning and end take: sixteen trees of 16
+// nodes over 8 192 to 32 768 rows 222 us; with none 230, with twelve 222.
 constexpr uint32_t UNIT_BLOCKS = 6;
-constexpr uint32_t MIN_BLOCKS = 4;  // least part of a unit, of a single sequence
+// Least part of a unit, of a single sequence: more parts are more partials to
+// join.  8 nodes over 150 rows (three blocks, so one part) 11.9 us, 26 nodes
+// over 4 070 rows 19.5; with 1 block 13.0 and 20.3, with 8 11.9 and 23.0.
+constexpr uint32_t MIN_BLOCKS = 4;
 
 constexpr uint32_t O_Q = 0;
 constexpr uint32_t O_K = O_Q + NQ * Q_TILE;
@@ -341,7 +358,8 @@ __device__ __forceinline__ bool watch(const Ctx& c, int b, uint32_t parity) {
 //
 // One sequence: its units get CTAs in proportion to their costs, each a part of
 // one unit's blocks, so that no CTA has two units' beginnings and ends to wait
-// for.
+// for (8 nodes over 150 rows 11.9 us, 26 over 4 070 19.5, 60 over 32 700 65.5;
+// cut as a batch 15.0, 21.7, 68.3).
 //
 // A batch: the units make a line, each as long as its blocks' costs and
 // UNIT_BLOCKS more for its beginning and end, which is cut into equal ranges.
@@ -1303,7 +1321,9 @@ __global__ void __launch_bounds__(MERGE_THREADS)
 }
 
 // The nodes' K / V rows [batch, n_nodes, n_kv, hd] into pool rows
-// row_offset[b] + pos[b] + i, 16 bytes per thread (kv_append for a tree).
+// row_offset[b] + pos[b] + i, 16 bytes per thread (kv_append for a tree).  A
+// launch of its own, because any CTA of the attention may meet any tree's rows;
+// its time (2 to 3 us) lies mostly under the attention kernel's own start.
 __global__ void tree_append_kernel(const uint4* __restrict__ k_new, const uint4* __restrict__ v_new,
                                    uint4* __restrict__ k_pool, uint4* __restrict__ v_pool,
                                    const int64_t* row_offset, const int32_t* pos,
