@@ -64,7 +64,7 @@
 // (sixteen trees of up to 61 nodes, group 5: 137 us; tensor pipe 39 %, exponentials
 // 42 %, DRAM 45 %).  Shared memory and tensor memory are full with two groups, so
 // a third turn in flight would need smaller blocks.  Built, measured and not
-// kept (60 nodes over 32 700 rows, 66 us): scores in registers at once with the
+// kept (64 nodes over 32 768 rows, 66 us): scores in registers at once with the
 // weights in buffers of their own 69.5; one arrival per warp on the barriers
 // 68.4; a quarter of the exponentials by polynomial 66.4; one issuer per group
 // instead of two cost the 256 chains a third.
@@ -102,10 +102,10 @@ constexpr uint32_t NQ = 2, NK = 5, NV = 5;  // stages
 constexpr uint32_t NP = 4;              // piece descriptors
 constexpr uint32_t PIECE_USERS = 19;    // warps that read them: all but the planner
 // What a block costs in a unit of one tile, of two (in the same unit of time):
-// 60 nodes over 32 700 rows, three tiles, 65.2 us; as 3 to 5 65.6, 3 to 4 69.0.
+// 64 nodes over 32 768 rows, three tiles, 65.2 us; as 3 to 5 65.6, 3 to 4 69.0.
 constexpr uint32_t COST1 = 1, COST2 = 2;
-// How many blocks' time a unit's beginning and end take: sixteen trees of 16
-// nodes over 8 192 to 32 768 rows 222 us; with none 230, with twelve 222.
+// How many blocks' time a unit's beginning and end take: 64 trees of 16 nodes
+// over 512 to 8 192 rows 222 us; with none 230, with twelve 222.
 constexpr uint32_t UNIT_BLOCKS = 6;
 // Least part of a unit, of a single sequence: more parts are more partials to
 // join.  8 nodes over 150 rows (three blocks, so one part) 11.9 us, 26 nodes
@@ -358,7 +358,7 @@ __device__ __forceinline__ bool watch(const Ctx& c, int b, uint32_t parity) {
 //
 // One sequence: its units get CTAs in proportion to their costs, each a part of
 // one unit's blocks, so that no CTA has two units' beginnings and ends to wait
-// for (8 nodes over 150 rows 11.9 us, 26 over 4 070 19.5, 60 over 32 700 65.5;
+// for (8 nodes over 150 rows 11.9 us, 26 over 4 070 19.5, 64 over 32 768 65.5;
 // cut as a batch 15.0, 21.7, 68.3).
 //
 // A batch: the units make a line, each as long as its blocks' costs and
@@ -1371,7 +1371,7 @@ int check_tree(const char* who, const void* q, const void* k_pool, const void* v
 // How a shape's query rows are tiled, in as few tiles of whole nodes as hold
 // them.  Trees of different lengths: as many nodes per tile as fit, so that the
 // short ones need few (16 trees of up to 61 nodes, group 5: 140 us, evenly 156).
-// Trees that are all present: evenly (60 nodes, group 5, 32 700 rows: 66 us,
+// Trees that are all present: evenly (64 nodes, group 5, 32 768 rows: 66 us,
 // filled up 68.6; 26 nodes, 4 070 rows: 19.6 and 19.3).
 struct Tiling {
   uint32_t tile_nodes, n_tiles, unit_tiles;
