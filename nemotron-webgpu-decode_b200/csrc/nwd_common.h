@@ -54,6 +54,23 @@ int launch_decode_short(const uint16_t* q, const uint16_t* k_new, const uint16_t
                         uint32_t n_kv, uint32_t group, float scale_log2, bool append,
                         uint32_t cta_rows, void* stream, const char* who);
 
+// ---- attention for the tree of one short sequence (tree_short.cu) ----
+constexpr uint64_t TREE_SHORT_ROWS = 2048;  // of the pool: the most that the sequence can have
+// Whether a call of this shape (rows: query rows per kv head) runs there.
+bool tree_short_fits(uint64_t pool_rows, uint32_t batch, uint32_t rows);
+struct TreeShortArgs {
+  const uint16_t *q, *k_new, *v_new;  // k_new, v_new: nullptr, or to be appended
+  uint16_t *k_pool, *v_pool, *o;
+  uint64_t pool_rows;
+  const int64_t* row_offset;
+  const int32_t *seq_len, *parents, *tree_len;
+  uint32_t n_nodes, n_heads, n_kv;
+  float scale_log2;
+  uint32_t* err;
+  void* stream;
+};
+int launch_tree_short(const TreeShortArgs& a, const char* who);
+
 // ---- programmatic dependent launch ----
 // A kernel launched with launch_pdl() may start while the kernel before it in
 // the stream is still running.  Such a kernel calls pdl_trigger() at entry (so

@@ -29,6 +29,44 @@ static __device__ __forceinline__ uint64_t tree_mask(const int32_t* parents, int
   return m;
 }
 
+// The rows that each node sees, for a warp whose lane i has the parents of nodes
+// i and i + 32 (-1 for those past n): seen[0] is node i's, seen[1] node i + 32's.
+// The lanes walk up in doubling steps, so a chain takes as many as the logarithm
+// of its depth.
+static __device__ __forceinline__ void tree_closure(int2 par, uint32_t n, uint32_t* err,
+                                                    uint64_t (&seen)[2]) {
+  const int lane = (int)(threadIdx.x & 31);
+  int up[2] = {par.x, par.y};
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const int i = lane + 32 * k;
+    if (up[k] < -1 || up[k] >= i) {
+      if (i < (int)n && err) atomicOr(err, NWD_DEVERR_TREE);
+      up[k] = -1;
+    }
+    seen[k] = 1ull << i;
+  }
+  while (__any_sync(0xffffffffu, up[0] >= 0 || up[1] >= 0)) {
+    uint64_t more[2];
+    int far[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int from = up[k] & 31;
+      const uint64_t lo = __shfl_sync(0xffffffffu, seen[0], from);
+      const uint64_t hi = __shfl_sync(0xffffffffu, seen[1], from);
+      const int flo = __shfl_sync(0xffffffffu, up[0], from);
+      const int fhi = __shfl_sync(0xffffffffu, up[1], from);
+      more[k] = up[k] < 0 ? 0 : up[k] < 32 ? lo : hi;
+      far[k] = up[k] < 0 ? -1 : up[k] < 32 ? flo : fhi;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      seen[k] |= more[k];
+      up[k] = far[k];
+    }
+  }
+}
+
 // Present nodes of sequence b: tree_len[b] (nullptr: all), held to [0, n].
 static __device__ __forceinline__ uint32_t tree_nodes(const int32_t* tree_len, uint32_t b,
                                                       uint32_t n, uint32_t* err) {

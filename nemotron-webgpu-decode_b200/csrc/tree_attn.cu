@@ -574,40 +574,10 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 // The rows of the tree that `node` sees (its ancestors and itself), from the
-// parents of all nodes: lane i has those of nodes i and i + 32.  The lanes walk
-// up in doubling steps, so a chain takes as many as the logarithm of its depth.
+// parents of all nodes: lane i has those of nodes i and i + 32.
 __device__ uint64_t tree_masks(int2 par, uint32_t n, uint32_t node, uint32_t* err) {
-  const int lane = (int)(threadIdx.x & 31);
   uint64_t seen[2];
-  int up[2] = {par.x, par.y};
-#pragma unroll
-  for (int k = 0; k < 2; k++) {
-    const int i = lane + 32 * k;
-    if (up[k] < -1 || up[k] >= i) {
-      if (i < (int)n) atomicOr(err, NWD_DEVERR_TREE);
-      up[k] = -1;
-    }
-    seen[k] = 1ull << i;
-  }
-  while (__any_sync(0xffffffffu, up[0] >= 0 || up[1] >= 0)) {
-    uint64_t more[2];
-    int far[2];
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-      const int from = up[k] & 31;
-      const uint64_t lo = __shfl_sync(0xffffffffu, seen[0], from);
-      const uint64_t hi = __shfl_sync(0xffffffffu, seen[1], from);
-      const int flo = __shfl_sync(0xffffffffu, up[0], from);
-      const int fhi = __shfl_sync(0xffffffffu, up[1], from);
-      more[k] = up[k] < 0 ? 0 : up[k] < 32 ? lo : hi;
-      far[k] = up[k] < 0 ? -1 : up[k] < 32 ? flo : fhi;
-    }
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-      seen[k] |= more[k];
-      up[k] = far[k];
-    }
-  }
+  nwd::tree_closure(par, n, err, seen);
   const uint64_t lo = __shfl_sync(0xffffffffu, seen[0], (int)(node & 31));
   const uint64_t hi = __shfl_sync(0xffffffffu, seen[1], (int)(node & 31));
   return node < 32 ? lo : hi;
@@ -1409,6 +1379,14 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
   if (ws_bytes < need)
     return fail(NWD_ERR_WORKSPACE, "%s: needs a workspace of >= %zu bytes, got %zu", who, need,
                 ws_bytes);
+  const float scale_log2 =
+      (scale != 0.f ? scale : 1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f;
+  if (tree_short_fits(pool_rows, batch, n_nodes * group))
+    return launch_tree_short({q, k_new, v_new, const_cast<uint16_t*>(k_pool),
+                              const_cast<uint16_t*>(v_pool), o, pool_rows, row_offset, seq_len,
+                              parents, tree_len, n_nodes, n_heads, n_kv, scale_log2,
+                              err ? err : reinterpret_cast<uint32_t*>(workspace), stream},
+                             who);
   static bool smem_set[64] = {};
   if (!smem_set[di.device]) {
     cudaError_t e = cudaFuncSetAttribute(tree_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1449,7 +1427,7 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
   p.unit_tiles = t.unit_tiles;
   const uint32_t of_head = (uint32_t)di.sm_count / n_kv;
   p.head_ctas = batch == 1 && of_head >= (t.n_tiles + 1) / 2 ? of_head : 0;
-  p.scale_log2 = (scale != 0.f ? scale : 1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e = cudaSuccess;
   if (k_new) {

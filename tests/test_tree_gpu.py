@@ -421,3 +421,115 @@ def test_refusals_of_tensors(ops):
     small.nbytes = 4096
     with pytest.raises(ops.NwdError):
         call(workspace=small)
+
+
+# ---- one sequence in a small pool: csrc/tree_short.cu up to 2 048 rows and 64 query rows a head
+
+@pytest.mark.parametrize("ctx,n,nh,nkv,tree_len", [
+    (0, 1, 5, 1, None), (0, 8, 8, 1, None), (1, 64, 2, 2, None), (15, 1, 1, 1, None),
+    (200, 8, 40, 8, None), (31, 16, 4, 1, [9]), (150, 8, 40, 8, [0]), (150, 8, 40, 8, [3]),
+    (245, 8, 40, 8, None),   # a pool of 256 rows
+    (246, 8, 40, 8, None),   # 257: a cluster
+    (300, 1, 8, 1, None), (500, 33, 3, 3, None), (640, 12, 20, 4, [5]), (0, 12, 10, 2, None),
+    (900, 64, 2, 2, None), (1500, 12, 40, 8, None), (2, 7, 9, 1, None),
+    (2037, 8, 40, 8, None),  # 2 048
+    (2038, 8, 40, 8, None),  # 2 049: the general kernel
+    (150, 13, 40, 8, None),  # 65 query rows: the general kernel
+])
+@pytest.mark.parametrize("chain", [False, True])
+def test_small_pool(ops, ctx, n, nh, nkv, tree_len, chain):
+    guard = 260 if (ctx, n) in ((0, 12), (2, 7)) else 3  # few rows in many CTAs
+    if nh == 9:
+        nh, nkv = 8, 1
+    c = Case([ctx], n, nh, nkv, seed=ctx + n, tree_len=tree_len, chain=chain, guard=guard)
+    d = c.dev()
+    end = c.ctx[0] + c.m[0]
+    d["k_pool"][end:] = float("nan")
+    d["v_pool"][end:] = float("inf")
+    sc = ops.Scratch()
+    c.check(_attend(ops, d, nh, nkv, scratch=sc))
+    assert sc.check() == 0
+
+
+@pytest.mark.parametrize("ctx", [70, 1100])
+@pytest.mark.parametrize("append", [False, True])
+def test_small_pool_infinite_rows(ops, ctx, append):
+    """Tree rows with NaN and infinities in V (and one in K) reach their descendants alone."""
+    c = Case([ctx], 9, 10, 2, seed=31)
+    v = c.v.copy()
+    v[ctx + 3, 0, 5], v[ctx + 3, 1, 127] = np.inf, -np.inf
+    v[ctx + 6, 1, 0], v[ctx + 6, 1, 64] = np.nan, 65504
+    k = c.k.copy()
+    k[ctx + 8] = np.nan
+    d = c.dev()
+    o = torch.full(d["q"].shape, 9.0, dtype=torch.float16, device="cuda")
+    t = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    if append:
+        kp, vp = d["k_pool"].clone(), d["v_pool"].clone()
+        kp[ctx:], vp[ctx:] = float("nan"), float("nan")
+        ops.kv_append_attention_tree(d["q"], t(k[None, ctx:ctx + 9]), t(v[None, ctx:ctx + 9]), kp, vp,
+                                     d["row_offset"], d["seq_len"], d["parents"], o, 10, 2)
+        assert np.array_equal(bits(kp[:ctx + 9]), k[:ctx + 9].view(np.uint16))
+        assert np.array_equal(bits(vp[:ctx + 9]), v[:ctx + 9].view(np.uint16))
+    else:
+        ops.attention_tree(d["q"], t(k), t(v), d["row_offset"], d["seq_len"], d["parents"], o, 10, 2)
+    got = vals(o)[0]
+    kk, vv = np.nan_to_num(k[:ctx + 9].astype(np.float64)), v[:ctx + 9].astype(np.float64)
+    clean = np.where(np.isfinite(vv), vv, 0)
+    ref, mag, amp = tree_attention(c.q[0].astype(np.float64), kk, clean, ctx, c.parents[0], 9, 2,
+                                   HD ** -0.5)
+    tol = attention_bound(ref, mag, amp, ctx + 9, HD ** -0.5, 65504.0)
+    for i in range(9):
+        line, j = [], i
+        while j >= 0:
+            line.append(j)
+            j = int(c.parents[0, j])
+        if 8 in line:
+            assert np.isnan(got[i]).all()
+            continue
+        for h in range(10):
+            extra = vv[[ctx + a for a in line], h // 5]
+            extra = np.where(np.isfinite(extra), 0, extra).sum(0)
+            ok = np.isfinite(extra)
+            assert np.array_equal(got[i, h][~ok], extra[~ok], equal_nan=True)
+            assert (np.abs(got[i, h] - ref[i, h])[ok] <= tol[i, h][ok]).all()
+
+
+def test_small_pool_lengths_that_grow(ops):
+    """One captured call, replayed as the sequence grows on the device."""
+    for rows in (256, 700):
+        c = Case([rows - 9], 6, 40, 8, seed=rows)
+        d = c.dev()
+        o = torch.zeros_like(d["q"])
+        args = (d["q"], d["k_pool"], d["v_pool"], d["row_offset"], d["seq_len"], d["parents"], o, 40, 8)
+        ops.attention_tree(*args)
+        s = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            ops.attention_tree(*args)
+        for ctx in (0, 1, 17, 63, 64, 65, 128, 200, 247, rows - 9):
+            d["seq_len"].fill_(ctx)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            c.ctx = [ctx]
+            c.check(o)
+
+
+def test_small_pool_rows_outside(ops):
+    """A sequence that leaves the pool has no rows and no nodes."""
+    for ctx in (100, 1000):
+        c = Case([ctx], 6, 8, 2, seed=33, guard=0)
+        d = c.dev()
+        new = torch.ones(1, 6, 2, HD, dtype=torch.float16, device="cuda")
+        for off, length in ((1, ctx), (-1, ctx), (0, ctx + 1), (0, -1), (2 ** 40, 3)):
+            d["row_offset"].fill_(off)
+            d["seq_len"].fill_(length)
+            o = torch.full(d["q"].shape, 9.0, dtype=torch.float16, device="cuda")
+            sc = ops.Scratch()
+            ops.kv_append_attention_tree(d["q"], new, new, d["k_pool"], d["v_pool"], d["row_offset"],
+                                         d["seq_len"], d["parents"], o, 8, 2, scratch=sc)
+            assert (o == 0).all() and sc.check() != 0
+        assert np.array_equal(bits(d["k_pool"]), c.k.view(np.uint16))
+        assert np.array_equal(bits(d["v_pool"]), c.v.view(np.uint16))
