@@ -1381,7 +1381,7 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
                 ws_bytes);
   const float scale_log2 =
       (scale != 0.f ? scale : 1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f;
-  if (tree_short_fits(pool_rows, batch, n_nodes * group))
+  if (tree_short_fits(pool_rows, batch, n_nodes * group))  // one launch, no partials
     return launch_tree_short({q, k_new, v_new, const_cast<uint16_t*>(k_pool),
                               const_cast<uint16_t*>(v_pool), o, pool_rows, row_offset, seq_len,
                               parents, tree_len, n_nodes, n_heads, n_kv, scale_log2,

@@ -2,14 +2,15 @@
 // the masks and the roundings): the engine's own case, a cache of 256 rows.
 //
 // There the general kernel's append, plan, pipeline fill and join are nearly
-// all of its time.  Here a kv head is one CTA of 16 warps, or past 256 pool
+// all of its time.  Here a kv head is one CTA of 16 warps, or past 128 pool
 // rows a thread-block cluster of up to 8, each with an equal part of the
 // context and tree rows in shared memory, and one launch does it all:
 //   S    a warp has 16 cache rows and all query rows (up to 64, as 16-row
 //        tiles): mma.sync m16n8k16, Q and K through ldmatrix;
 //   P    against the CTA's maximum per row, as fp16 into shared memory, its
 //        largest 2^15;
-//   O    a warp has 8 output columns and all rows: P and V through ldmatrix;
+//   O    a warp has 16 output columns and every other row tile, so that P, which
+//        all warps read, crosses shared memory half as often;
 //   out  normalised, or joined over the cluster through distributed shared
 //        memory, each CTA a share of the rows.
 // With the append, tree rows come from k_new / v_new and are written to the
@@ -17,6 +18,12 @@
 //
 // mma.sync: tcgen05 would need its tensor memory, descriptors and barriers set
 // up for 40 rows x 158 keys of work.
+//
+// Bound by latency: launch, lengths, rows, then S, P and O with a barrier after
+// each (about 1 us a stage at 40 query rows, most of it shared-memory reads).
+// 40/8 heads, with the append, and the general kernel's time: 8 nodes over 150
+// rows 7.0 us (11.7), over 1 000 8.9 (14.1), over 2 000 11.5 (15.4); 12 nodes
+// over 2 000 12.8 (15.6); one node over 150 4.9 (11.2).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -31,9 +38,12 @@ constexpr uint32_t THREADS = 512, WARPS = THREADS / 32;
 constexpr uint32_t MAX_ROWS = 64;      // query rows per kv head
 constexpr uint32_t MAX_KEYS = 256;     // cache rows per CTA
 constexpr uint32_t MAX_CLUSTER = 8;    // portable cluster size
-constexpr uint32_t CLUSTER_KEYS = 64;  // cache rows per CTA that a cluster aims at
+// Up to ONE_KEYS pool rows are one CTA's, more are shared out by CLUSTER_KEYS.  A
+// cluster's launch and barriers cost what 64 rows do: 8 nodes over 120 rows 6.3
+// us in one CTA, 7.0 in a cluster; over 240 8.8 and 7.1; by 32 rows 7.3, by 128 8.7.
+constexpr uint32_t ONE_KEYS = 128, CLUSTER_KEYS = 64;
 constexpr float P_BIAS = 15.f;
-static_assert(MAX_KEYS == WARPS * 16 && HD == WARPS / 2 * 16 && MAX_ROWS * 8 == THREADS, "the warps' shares");
+static_assert(ONE_KEYS <= MAX_KEYS && MAX_KEYS == WARPS * 16 && HD == WARPS / 2 * 16 && MAX_ROWS * 8 == THREADS, "the warps' shares");
 
 struct Params {
   const __half* q;
@@ -512,7 +522,7 @@ int launch_tree_short(const TreeShortArgs& a, const char* who) {
   p.group = group;
   p.scale_log2 = a.scale_log2;
   const uint32_t most = (uint32_t)a.pool_rows;
-  p.cluster = most <= MAX_KEYS ? 1 : std::min(MAX_CLUSTER, (most + CLUSTER_KEYS - 1) / CLUSTER_KEYS);
+  p.cluster = most <= ONE_KEYS ? 1 : std::min(MAX_CLUSTER, (most + CLUSTER_KEYS - 1) / CLUSTER_KEYS);
   p.keys = ((most + p.cluster - 1) / p.cluster + 31) / 32 * 32;
   const uint32_t mt = (rows + 15) / 16, smem = smem_bytes(p.keys, mt * 16);
   cudaStream_t s = (cudaStream_t)a.stream;

@@ -428,8 +428,9 @@ def test_refusals_of_tensors(ops):
 @pytest.mark.parametrize("ctx,n,nh,nkv,tree_len", [
     (0, 1, 5, 1, None), (0, 8, 8, 1, None), (1, 64, 2, 2, None), (15, 1, 1, 1, None),
     (200, 8, 40, 8, None), (31, 16, 4, 1, [9]), (150, 8, 40, 8, [0]), (150, 8, 40, 8, [3]),
-    (245, 8, 40, 8, None),   # a pool of 256 rows
-    (246, 8, 40, 8, None),   # 257: a cluster
+    (117, 8, 40, 8, None),   # a pool of 128 rows
+    (118, 8, 40, 8, None),   # 129: a cluster
+    (245, 8, 40, 8, None), (246, 8, 40, 8, None),
     (300, 1, 8, 1, None), (500, 33, 3, 3, None), (640, 12, 20, 4, [5]), (0, 12, 10, 2, None),
     (900, 64, 2, 2, None), (1500, 12, 40, 8, None), (2, 7, 9, 1, None),
     (2037, 8, 40, 8, None),  # 2 048
