@@ -114,11 +114,14 @@ __device__ __forceinline__ double rest1(float p, float q) {
 // r~ of N entries after k rejections at the current node (with draft rows).
 template <int N>
 __device__ __forceinline__ void rest(const Walk& s, int k, const float* p, const float* q, double* r) {
+  double qd[N];  // (two conversions per entry: they bound a pass)
 #pragma unroll
-  for (int e = 0; e < N; e++) r[e] = k ? rest1(p[e], q[e]) : prob(p[e]);
-  double qd[N];
-#pragma unroll
-  for (int e = 0; e < N; e++) qd[e] = prob(q[e]);
+  for (int e = 0; e < N; e++) {
+    r[e] = prob(p[e]);
+    qd[e] = prob(q[e]);
+    const double t = r[e] - qd[e];
+    if (k) r[e] = t > 0.0 ? t : 0.0;
+  }
 #pragma unroll 1
   for (int i = 1; i < k; i++) {
     const double sum = s.sum[i];
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) verify_tree_kernel(const
                               __ballot_sync(0xffffffffu, par[0] == (int)cur);
     int k = 0;  // rejections that r~ has taken in (since it was last the whole row)
     int next = -1;
-    bool have_base = false;
+    bool have_base = false, first[2] = {false, false};
     double base = 0.0;  // without draft rows: the sum but for the children's tokens
     total = 1.0;
     gone.a = gone.b = -1;
@@ -369,6 +372,16 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) verify_tree_kernel(const
           base = row_sum<false>(s, 0, mine, row, rank, a.cluster, parity);
           parity ^= 1;
           have_base = true;
+          first[0] = mine.a >= 0;
+          first[1] = mine.b >= 0;
+          const uint32_t same = __match_any_sync(0xffffffffu, first[0] ? mine.a : -1 - (int)lane);
+          if (same & ((1u << lane) - 1u)) first[0] = false;
+          for (uint32_t left_b = __ballot_sync(0xffffffffu, first[1]); left_b; left_b &= left_b - 1) {
+            const int l = __ffs(left_b) - 1, tb = __shfl_sync(0xffffffffu, mine.b, l);
+            const uint32_t ahead = __ballot_sync(0xffffffffu, mine.a == tb);
+            const uint32_t ahead_b = __ballot_sync(0xffffffffu, mine.b == tb) & ((1u << l) - 1u);
+            if ((int)lane == l && (ahead | ahead_b)) first[1] = false;
+          }
         }
         if (t >= 0) {
           if (mine.a == t) gone.a = t;
@@ -376,27 +389,12 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) verify_tree_kernel(const
         }
         // the entries of the children's tokens that are still in, each token
         // once: at its first node
-        bool in[2] = {mine.a >= 0 && gone.a < 0, mine.b >= 0 && gone.b < 0};
-        const uint32_t ina = __ballot_sync(0xffffffffu, in[0]);
-        uint32_t inb = __ballot_sync(0xffffffffu, in[1]);
-        summed = !(ina | inb);  // the pass left out just those: its parts serve the draw
-        if (!summed) {
-          const uint32_t same = __match_any_sync(0xffffffffu, in[0] ? mine.a : -1 - (int)lane);
-          if (in[0] && (same & ((1u << lane) - 1u))) in[0] = false;
-          for (; inb; inb &= inb - 1) {  // (trees of more than 32 nodes)
-            const int l = __ffs(inb) - 1, tb = __shfl_sync(0xffffffffu, mine.b, l);
-            const uint32_t ahead = __ballot_sync(0xffffffffu, in[1] && mine.b == tb);
-            const bool twice = __any_sync(0xffffffffu, in[0] && mine.a == tb) ||
-                               (ahead & ((1u << l) - 1u));
-            if ((int)lane == l && twice) in[1] = false;
-          }
-          double more = 0.0;
-          if (in[0]) more += prob(s.p[lane]);
-          if (in[1]) more += prob(s.p[lane + 32]);
-          total = base + warp_sum(more);
-        } else {
-          total = base;
-        }
+        const bool in[2] = {first[0] && gone.a < 0, first[1] && gone.b < 0};
+        summed = !__any_sync(0xffffffffu, in[0] || in[1]);  // the pass left out just those: its
+        double more = 0.0;                                   // parts serve the draw
+        if (in[0]) more += prob(s.p[lane]);
+        if (in[1]) more += prob(s.p[lane + 32]);
+        total = base + (summed ? 0.0 : warp_sum(more));
       }
       if (!(total > 0.0)) {  // nothing left: the whole row again
         k = 0;
@@ -425,15 +423,19 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) verify_tree_kernel(const
         return;
       }
       Part w = piece(row.groups(), rank * WARPS + owner, a.cluster * WARPS);
-      if (w.hi - w.lo > 64) {  // all warps on the owner's part
-        const Part all = w;
-        w = piece(all.hi - all.lo, warp, WARPS);
-        w.lo += all.lo;
-        w.hi += all.lo;
+      while (w.hi - w.lo > 64) {  // all warps on the owner's part
+        const uint32_t lo = w.lo, n_all = w.hi - w.lo;
+        w = piece(n_all, warp, WARPS);
+        w.lo += lo;
+        w.hi += lo;
         block_sum(s, any_part_sum<DRAFT>(s, k, gone, row, w));
         owner = find_part(lane < WARPS ? s.part[lane] : 0.0, goal, &before);
+        if (owner < 0) break;  // (cannot be: the part has mass)
+        w = piece(n_all, (uint32_t)owner, WARPS);
+        w.lo += lo;
+        w.hi += lo;
       }
-      if ((int)warp != owner) return;
+      if (warp != 0) return;
       int32_t last = -1;  // the last token with mass, should rounding leave the border behind
       for (uint32_t g0 = w.lo; g0 < w.hi; g0 += 32) {
         const uint32_t g = g0 + lane, x = row.first(g);
