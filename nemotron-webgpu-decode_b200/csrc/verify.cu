@@ -111,6 +111,11 @@ __device__ __forceinline__ double rest1(float p, float q) {
   const bool in = p > q;
   return (double)(in ? p : 0.f) - (double)(in ? q : 0.f);
 }
+// max(t, 0) by the sign bit: a comparison in f64 would take the pipe that the
+// differences need
+__device__ __forceinline__ double positive(double t) {
+  return __double2hiint(t) < 0 ? 0.0 : t;
+}
 // r~ of N entries after k rejections at the current node (with draft rows).
 template <int N>
 __device__ __forceinline__ void rest(const Walk& s, int k, const float* p, const float* q, double* r) {
@@ -120,15 +125,14 @@ __device__ __forceinline__ void rest(const Walk& s, int k, const float* p, const
     r[e] = prob(p[e]);
     qd[e] = prob(q[e]);
     const double t = r[e] - qd[e];
-    if (k) r[e] = t > 0.0 ? t : 0.0;
+    if (k) r[e] = positive(t);
   }
 #pragma unroll 1
   for (int i = 1; i < k; i++) {
     const double sum = s.sum[i];
 #pragma unroll
     for (int e = 0; e < N; e++) {
-      const double t = r[e] - sum * qd[e];
-      r[e] = t > 0.0 ? t : 0.0;
+      r[e] = positive(r[e] - sum * qd[e]);
     }
   }
 }
