@@ -33,11 +33,12 @@
 // rejected are added.
 //
 // Bound by the rows' bytes where there are many sequences: 256 chains of 5 nodes
-// over 131 072 tokens read 248 MB in 52 us (4.8 TB/s).  Else by the longest
-// walk, a pass of which is 4 to 6 us (fetching the row's part, its conversions
-// to f64 on a pipe of 16 per clock, two barriers): 32 trees of 26 nodes 42 to
-// 51 us, with 3.1 passes on average and 7 in one; one chain 8 us with its
-// launch.
+// over 131 072 tokens read 248 MB in 51 us (4.9 TB/s; the pass itself runs at
+// 7, gathers before it and the draw behind it read little).  Else by the
+// longest walk, a pass of which is 3 to 5 us (fetching the row's part, its
+// conversions to f64 on a pipe of 16 per clock, the differences on one of 64,
+// two barriers): 32 trees of 26 nodes 43 us, with 3.1 passes on average and 7
+// in one; one chain 8 us with its launch.
 #include "nwd_common.h"
 #include "tree.cuh"
 
@@ -214,7 +215,8 @@ __device__ __forceinline__ Part warp_part(uint32_t groups, uint32_t rank, uint32
 enum Rest { WHOLE, ONCE, CHAIN };
 
 // The sum of r~ over the warp's groups [lo, hi) of a row, this lane's share;
-// AHEAD groups per lane in flight.
+// AHEAD groups per lane in flight, as many as 64 registers hold (CHAIN with 1: 32
+// trees of 26 nodes 48 us, with 3 46, with 2 43).
 template <bool DRAFT, int REST>
 __device__ __forceinline__ double part_sum(const Walk& s, int k, const Gone& gone, const Row& row,
                                            Part w) {
@@ -539,8 +541,8 @@ extern "C" int nwd_verify_tree(const int32_t* tokens, const int32_t* parents,
   }
   // The largest cluster that leaves all CTAs resident at once and each a part
   // of the vocabulary worth a barrier.  Up to 16, 8, 4 and 1 CTAs: one chain
-  // over 131 072 tokens 8.0, 10.1, 14.5 and 34 us, 32 trees 51, 78, 129 and 446;
-  // 256 chains, which get two, 52 and with one 69.
+  // over 131 072 tokens 8.0, 10.0, 13.8 and 34 us, 32 trees 43, 65, 99 and 334;
+  // 256 chains, which get two, 51 and with one 67.
   uint32_t cluster = 1;
   while (cluster < MAX_CLUSTER && (uint64_t)batch * cluster * 2 <= (uint64_t)di.sm_count * CTAS_PER_SM &&
          vocab / (cluster * 2) >= MIN_PART)
