@@ -176,7 +176,7 @@ static_assert(sizeof(Piece) == 64, "piece");
 // with, the piece it ends with) of unit_tiles tiles: (m, l) [tile][128], then
 // O [tile][32 column quads][128 rows][4] f32.
 struct MergeDesc {
-  uint32_t valid, b, u, first;  // the unit's pieces are CTAs first .. this one
+  uint32_t valid, b, u, first;  // 1 + the sequence's nodes; the unit's pieces are CTAs first .. this one
 };
 constexpr uint32_t MAX_CTAS = 240;
 constexpr size_t WS_DESC = 256;
@@ -390,10 +390,12 @@ __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
       k = max(1u, min(k, nblk / MIN_BLOCKS));  // parts of at least MIN_BLOCKS
       u = head * ((nt + 1) / 2) + unit;
       if (at < k) {
-        blk = (uint32_t)((uint64_t)nblk * at / k);
-        const uint32_t end = (uint32_t)((uint64_t)nblk * (at + 1) / k);
+        // nblk * at / k, in 32 bits
+        const uint32_t each = nblk / k, rest = nblk - each * k;
+        blk = each * at + rest * at / k;
+        const uint32_t end = each * (at + 1) + rest * (at + 1) / k;
         left = (int64_t)(end - blk) * cost_of(unit < pairs ? 2 : 1);
-        if (at > 0 && at + 1 == k) join = MergeDesc{1, 0, u, blockIdx.x - at};
+        if (at > 0 && at + 1 == k) join = MergeDesc{1 + s.nodes, 0, u, blockIdx.x - at};
       }
     }
   } else {
@@ -402,10 +404,13 @@ __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
     auto length = [&](const TreeSeq& q) {
       return (seq_blocks(q) + UNIT_BLOCKS) * head_cost(seq_tiles(p, q.nodes));
     };
-    // of 32 sequences at a time; lane l keeps group l's
+    // of 32 sequences at a time; lane l keeps group l's, s is group `loaded`'s
+    uint32_t loaded = 0;
     auto group_length = [&](uint32_t g, uint32_t* err) -> uint64_t {
       const uint32_t i = g * 32 + lane;
-      return warp_sum64(i < p.batch ? length(load_seq(p, i, err)) : 0u);
+      loaded = g;
+      if (i < p.batch) s = load_seq(p, i, err);
+      return warp_sum64(i < p.batch ? length(s) : 0u);
     };
     uint64_t kept = 0, total = 0;
 #pragma unroll 1
@@ -440,7 +445,7 @@ __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
         }
       }
       b = group * 32 + lane;
-      if (b < p.batch) s = load_seq(p, b, nullptr);
+      if (b < p.batch && loaded != group) s = load_seq(p, b, nullptr);
       const uint64_t len = b < p.batch ? length(s) : 0u;
       upto = len;
 #pragma unroll
@@ -471,7 +476,7 @@ __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
       if (blk < nblk) {
         left = (int64_t)(x1 - start) - (int64_t)((uint64_t)blk * cost);
         if (blk > 0 && left > 0 && blk + div_small(left + cost - 1, cost) >= nblk)
-          join = MergeDesc{1, b, u, (uint32_t)div_small(start, per)};
+          join = MergeDesc{1 + s.nodes, b, u, (uint32_t)div_small(start, per)};
       } else {  // the unit's last block is the CTA's before
         left = (int64_t)(x1 - start) - (int64_t)((uint64_t)(nblk + UNIT_BLOCKS) * cost);
         blk = nblk;
@@ -1129,7 +1134,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               }
             }
           }
-          if (row_used) {
+          if (row_used && (d.whole || !absent)) {  // (absent nodes have no partials)
             for (uint64_t x = lost; x; x &= x - 1) {
               const size_t row = (size_t)d.row0 + d.ctx + (uint32_t)__ffsll((long long)x) - 1;
               const __half* src = p.v + (row * p.n_kv + d.hkv) * HD + col;
@@ -1163,7 +1168,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           }
         }
-        if (!d.whole && row_used)
+        if (!d.whole && row_used && !absent)
           reinterpret_cast<float2*>(p.ws + WS_ML)[slot + r] = make_float2(M, L);
         tc_fence_before();
         // the groups' accumulators, and their (m, l), have been read
@@ -1233,14 +1238,15 @@ __global__ void __launch_bounds__(MERGE_THREADS)
 #pragma unroll 1
   for (uint32_t item = blockIdx.x; item < n_units * per_unit; item += gridDim.x) {
     d = units[item / per_unit];
-    const uint32_t first = d.first, n = owner[item / per_unit] - first + 1;
+    const uint32_t first = d.first;
     const uint32_t t = item % per_unit / chunks, row = item % chunks * MERGE_ROWS + r;
-    const uint32_t nodes = load_seq(p, d.b, nullptr).nodes;
+    const uint32_t nodes = d.valid - 1;
     const Unit un = unit_of(seq_tiles(p, nodes), d.u);
     const uint32_t tile = un.tile0 + t;
     if (t >= un.tiles) continue;
     if (row >= min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes) * p.group) continue;
     const uint32_t node = tile * p.tile_nodes + row / p.group;
+    const uint32_t n = node < nodes ? owner[item / per_unit] - first + 1 : 0;  // none: zeros
     float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
@@ -1280,10 +1286,9 @@ __global__ void __launch_bounds__(MERGE_THREADS)
         }
       }
     }
-    const bool none = node >= nodes;
     const float inv = L != 0.f ? 1.f / L : 0.f;
-    const __half2 h[2] = {__floats2half2_rn(none ? 0.f : o.x * inv, none ? 0.f : o.y * inv),
-                          __floats2half2_rn(none ? 0.f : o.z * inv, none ? 0.f : o.w * inv)};
+    const __half2 h[2] = {__floats2half2_rn(o.x * inv, o.y * inv),
+                          __floats2half2_rn(o.z * inv, o.w * inv)};
     *reinterpret_cast<uint2*>(p.o + (((size_t)d.b * p.n_nodes + node) * p.n_heads +
                                      un.hkv * p.group + row % p.group) * HD + quad * 4) =
         *reinterpret_cast<const uint2*>(h);
