@@ -1194,20 +1194,26 @@ __global__ void __launch_bounds__(THREADS, 1)
 // (deterministic): M = max m, O = sum O_c 2^(m_c - M) / sum l_c 2^(m_c - M).
 //
 // A work item is 8 rows of a tile of such a unit.  Every block finds the units
-// (all CTAs' descriptors in one round of loads) and takes its share of the
-// items; a thread has one row's column quad, and fetches 8 pieces' (m, l) and
-// O terms at a time, all in flight together, with no word to the other
-// threads.  (A first form with a block per item and CTA, and the weights in
-// shared memory, took 5 us of 26 nodes over 4 070 rows, where this takes 3, and
-// 24 us of 16 x 61 nodes, where this takes 7.)  One wave of blocks: six blocks
-// per SM where three are resident cost 16 x 61 nodes 3 us more.
+// (all CTAs' descriptors in one round of loads), works out where each one's rows
+// are, once, and takes its share of the items; a thread has one row's column
+// quad, and fetches 8 pieces' (m, l) and O terms at a time, all in flight
+// together, with no word to the other threads.  26 nodes over 4 070 rows, 8.5 MB
+// of partials: 3 us after its launch; sixteen trees of up to 61 nodes, some 22
+// MB: 9 to 17 us.  (Divisions for every item cost the first 1 us; a form with a
+// block per item and piece, the weights in shared memory, took 5 and 24.)
 constexpr uint32_t MERGE_ROWS = 8;
 constexpr uint32_t MERGE_THREADS = 256;
 constexpr uint32_t MERGE_AHEAD = 8;
+constexpr uint32_t MERGE_PER_SM = 2;  // resident blocks (98 registers): one wave
+struct Join {
+  uint32_t first, n;    // its pieces: CTAs first .. first + n - 1
+  uint32_t rows[2];     // per tile: query rows
+  uint32_t present[2];  // ... of present nodes
+  size_t out;           // its first row in o
+};
 __global__ void __launch_bounds__(MERGE_THREADS)
     tree_merge_kernel(const __grid_constant__ TParams p, uint32_t ctas) {
-  __shared__ MergeDesc units[MAX_CTAS];
-  __shared__ uint32_t owner[MAX_CTAS];  // the CTA that a unit ends in
+  __shared__ Join joins[MAX_CTAS];
   __shared__ uint32_t counts[MERGE_THREADS / 32];
   static_assert(MAX_CTAS <= MERGE_THREADS, "one descriptor per thread");
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1218,35 +1224,40 @@ __global__ void __launch_bounds__(MERGE_THREADS)
   const uint32_t some = __ballot_sync(0xffffffffu, d.valid != 0);
   if (lane == 0) counts[warp] = (uint32_t)__popc(some);
   __syncthreads();
-  uint32_t n_units = 0, before = 0;
+  uint32_t n_joins = 0, before = 0;
 #pragma unroll
   for (uint32_t i = 0; i < MERGE_THREADS / 32; i++) {
     if (i < warp) before += counts[i];
-    n_units += counts[i];
+    n_joins += counts[i];
   }
-  if (d.valid) {
-    const uint32_t at = before + (uint32_t)__popc(some & ((1u << lane) - 1u));
-    units[at] = d;
-    owner[at] = tid;
+  if (d.valid) {  // what the items need of it, found once
+    const uint32_t nodes = d.valid - 1;
+    const Unit un = unit_of(seq_tiles(p, nodes), d.u);
+    Join j;
+    j.first = d.first;
+    j.n = tid - d.first + 1;
+#pragma unroll
+    for (uint32_t t = 0; t < 2; t++) {
+      const uint32_t node0 = (un.tile0 + t) * p.tile_nodes;
+      j.rows[t] = t < un.tiles ? min(p.tile_nodes, p.n_nodes - node0) * p.group : 0;
+      j.present[t] = nodes > node0 ? min((nodes - node0) * p.group, j.rows[t]) : 0;
+    }
+    j.out = (((size_t)d.b * p.n_nodes + un.tile0 * p.tile_nodes) * p.n_heads + un.hkv * p.group) * HD;
+    joins[before + (uint32_t)__popc(some & ((1u << lane) - 1u))] = j;
   }
   __syncthreads();
-  const uint32_t chunks = (p.tile_nodes * p.group + MERGE_ROWS - 1) / MERGE_ROWS;
-  const uint32_t per_unit = p.unit_tiles * chunks;
   const float2* ml = reinterpret_cast<const float2*>(p.ws + WS_ML);
   const float4* po = reinterpret_cast<const float4*>(p.ws + ws_o(ctas, p.unit_tiles));
   const uint32_t r = tid & 7, quad = tid >> 3;
+  const uint32_t per_group = (65536u + p.group - 1) / p.group;  // row / group, as a product
+  constexpr uint32_t CHUNKS = BM / MERGE_ROWS;
 #pragma unroll 1
-  for (uint32_t item = blockIdx.x; item < n_units * per_unit; item += gridDim.x) {
-    d = units[item / per_unit];
-    const uint32_t first = d.first;
-    const uint32_t t = item % per_unit / chunks, row = item % chunks * MERGE_ROWS + r;
-    const uint32_t nodes = d.valid - 1;
-    const Unit un = unit_of(seq_tiles(p, nodes), d.u);
-    const uint32_t tile = un.tile0 + t;
-    if (t >= un.tiles) continue;
-    if (row >= min(p.tile_nodes, p.n_nodes - tile * p.tile_nodes) * p.group) continue;
-    const uint32_t node = tile * p.tile_nodes + row / p.group;
-    const uint32_t n = node < nodes ? owner[item / per_unit] - first + 1 : 0;  // none: zeros
+  for (uint32_t item = blockIdx.x; item < n_joins * p.unit_tiles * CHUNKS; item += gridDim.x) {
+    const uint32_t row = item % CHUNKS * MERGE_ROWS + r;
+    const uint32_t t = p.unit_tiles == 2 ? item / CHUNKS & 1 : 0;
+    const Join& join = joins[p.unit_tiles == 2 ? item / (2 * CHUNKS) : item / CHUNKS];
+    if (row >= join.rows[t]) continue;
+    const uint32_t first = join.first, n = row < join.present[t] ? join.n : 0;  // none: zeros
     float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
@@ -1289,9 +1300,10 @@ __global__ void __launch_bounds__(MERGE_THREADS)
     const float inv = L != 0.f ? 1.f / L : 0.f;
     const __half2 h[2] = {__floats2half2_rn(o.x * inv, o.y * inv),
                           __floats2half2_rn(o.z * inv, o.w * inv)};
-    *reinterpret_cast<uint2*>(p.o + (((size_t)d.b * p.n_nodes + node) * p.n_heads +
-                                     un.hkv * p.group + row % p.group) * HD + quad * 4) =
-        *reinterpret_cast<const uint2*>(h);
+    const uint32_t node = row * per_group >> 16;  // within the tile
+    *reinterpret_cast<uint2*>(p.o + join.out +
+                              ((size_t)(t * p.tile_nodes + node) * p.n_heads + row - node * p.group) * HD +
+                              quad * 4) = *reinterpret_cast<const uint2*>(h);
   }
 }
 
@@ -1447,7 +1459,7 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
   const uint32_t ctas = (uint32_t)di.sm_count;
   e = launch_pdl(tree_kernel, dim3(ctas), dim3(THREADS), SMEM_BYTES, s, tq, tk, tv, p);
   if (e == cudaSuccess)
-    e = launch_pdl(tree_merge_kernel, dim3(ctas * 3), dim3(MERGE_THREADS), 0, s, p, ctas);
+    e = launch_pdl(tree_merge_kernel, dim3(ctas * MERGE_PER_SM), dim3(MERGE_THREADS), 0, s, p, ctas);
   if (e != cudaSuccess) return cuda_fail(e, who);
   return ok();
 }
