@@ -536,8 +536,9 @@ __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
     r.next();
     if (d.tiles == 0) break;
   }
-  if (p.tree_len && p.n_tiles > 1) {
+  if (p.n_tiles > 1) {
     // all sequences' rows of zeros, dealt out to the CTAs one after the other
+    // (without tree_len those of sequences that leave the pool)
     const uint32_t row_vec = p.n_heads * (HD / 8);
     uint32_t turn = 0;  // the CTA whose row comes next
 #pragma unroll 1

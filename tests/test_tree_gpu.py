@@ -432,7 +432,7 @@ def test_refusals_of_tensors(ops):
     (118, 8, 40, 8, None),   # 129: a cluster
     (245, 8, 40, 8, None), (246, 8, 40, 8, None),
     (300, 1, 8, 1, None), (500, 33, 3, 3, None), (640, 12, 20, 4, [5]), (0, 12, 10, 2, None),
-    (900, 64, 2, 2, None), (1500, 12, 40, 8, None), (2, 7, 9, 1, None),
+    (900, 64, 2, 2, None), (1500, 12, 40, 8, None), (2, 7, 8, 1, None),
     (2037, 8, 40, 8, None),  # 2 048
     (2038, 8, 40, 8, None),  # 2 049: the general kernel
     (150, 13, 40, 8, None),  # 65 query rows: the general kernel
@@ -440,8 +440,6 @@ def test_refusals_of_tensors(ops):
 @pytest.mark.parametrize("chain", [False, True])
 def test_small_pool(ops, ctx, n, nh, nkv, tree_len, chain):
     guard = 260 if (ctx, n) in ((0, 12), (2, 7)) else 3  # few rows in many CTAs
-    if nh == 9:
-        nh, nkv = 8, 1
     c = Case([ctx], n, nh, nkv, seed=ctx + n, tree_len=tree_len, chain=chain, guard=guard)
     d = c.dev()
     end = c.ctx[0] + c.m[0]
@@ -534,3 +532,15 @@ def test_small_pool_rows_outside(ops):
             assert (o == 0).all() and sc.check() != 0
         assert np.array_equal(bits(d["k_pool"]), c.k.view(np.uint16))
         assert np.array_equal(bits(d["v_pool"]), c.v.view(np.uint16))
+
+
+@pytest.mark.parametrize("b", [1, 3])
+def test_rows_outside_the_pool_with_several_tiles(ops, b):
+    """All of such a sequence's nodes are absent, in every tile, without tree lengths too."""
+    c = Case([900, 2000, 64][:b], 61, 40, 8, seed=40)
+    d = c.dev()
+    d["row_offset"][0] = c.off[-1] - 5
+    sc = ops.Scratch()
+    o = _attend(ops, d, 40, 8, scratch=sc)
+    assert (o[0] == 0).all() and sc.check() == 2
+    c.check(o, only=range(1, b))
