@@ -22,15 +22,8 @@ own = False
 HD = 128  # the head size of this framework's attention
 
 
-_package = None
-
-
 def _ops():
-    """The package's operators, imported once, as a user's program does."""
-    global _package
-    if _package is None:
-        _package = importlib.import_module("nemotron-webgpu-decode_b200.ops")
-    return _package
+    return importlib.import_module("nemotron-webgpu-decode_b200.ops")
 
 
 # ------------------------------------------------------------------ cases
