@@ -45,12 +45,16 @@
 //                 at the next unit.
 //
 // Softmax in the log2 domain with a lazily moved maximum (O is rescaled in
-// tensor memory only when a row's maximum grows by more than 2^8).  P is
-// rounded to fp16 once, as P V's operand: 2^-11 of a weight, at random over
-// the rows, so about the size of the output's own rounding; its largest value
-// is put near 2^15 (P_BIAS) so that weights down to 2^-29 of the largest keep
-// all their bits, which a long flat tail behind one large score needs.  Sums
-// and accumulators are f32.
+// tensor memory only when a row's maximum grows by more than 2^8).  P goes to
+// P V as an fp16 head and an fp16 remainder, two MMAs over the same V, as in the
+// decode and prefill kernels: one rounding to fp16, 2^-11 of a weight, puts
+// outputs that average out to nearly nothing up to 7 % off, where the decode
+// path keeps 1 %.  Its price, with the remainder's conversions: 64 nodes over
+// 32 768 rows 78 us (one rounding 66), 64 trees of 16 nodes 256 (219), 256
+// chains of 5 1 080 (900, both at the power cap).  A row's largest P lies
+// between 2^7 (P_BIAS) and 2^15, and an fp16 step below the normal range is
+// 2^-24: a weight is off by 2^-22 of itself, or by 2^-32 of the largest where
+// that is more.  Sums and accumulators are f32.
 //
 // Rows a node does not attend never reach its output: scores are selected to
 // -inf before the maximum, V rows behind the tree are zeroed in shared memory
@@ -892,17 +896,17 @@ __global__ void __launch_bounds__(THREADS, 1)
             ok = v.reach(c, n0 + j, B_VFULL, B_VEMPTY) && c.wait(B_PFULL + (int)(2 * g + buf), phase);
             if (!ok) break;
             tc_fence_after();
-            // P: key pairs in the buffer's first 32 columns; V MN-major
-            // (head_dim contiguous), its 64-column chunks 8 KiB apart, 16
-            // keys 2 KiB
+            // P: key pairs, the heads in the buffer's first 32 columns, the
+            // remainders in the other 32; V MN-major (head_dim contiguous),
+            // its 64-column chunks 8 KiB apart, 16 keys 2 KiB
             const uint32_t dv = (c.sb + O_V + v.r.i * TILE) >> 4;
             constexpr uint64_t top = sdesc(0, CHUNK, 1024);
             if (leader) {
               umma_ts(tmem_o, tmem_s + buf * BN, top | dv, IDESC_O, add);
 #pragma unroll
-              for (uint32_t kk = 1; kk < BN / 16; kk++)
-                umma_ts(tmem_o, tmem_s + buf * BN + kk * 8u, top | (dv + ((kk * 16 * 128) >> 4)),
-                        IDESC_O, 1u);
+              for (uint32_t kk = 1; kk < 2 * BN / 16; kk++)
+                umma_ts(tmem_o, tmem_s + buf * BN + kk * 8u,
+                        top | (dv + ((kk % (BN / 16) * 16 * 128) >> 4)), IDESC_O, 1u);
               umma_commit(c.bar + 8 * (B_PVDONE + 2 * g + buf));
               umma_commit(c.bar + 8 * (B_VEMPTY + v.r.i));
             }
@@ -962,42 +966,42 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!ok) break;
         tc_fence_after();
         if (warp_used) {
-          float s[BN];
-          tmem_ld32(tmem_s, s);
-          tmem_ld32(tmem_s + 32, s + 32);
-          tmem_ld_wait();
-          if (tail) {
-            if (!have_mask) {
-              have_mask = true;
-              const uint64_t all = tree_masks(par, p.n_nodes, node, c.err);
-              sees = row_used && node < d.nodes ? all : 0;
-            }
-            // bit k of word i: this row attends cache row key0 + 32 i + k
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-              const int64_t at = (int64_t)key0 + 32 * i - (int64_t)d.ctx;  // in the tree
-              uint32_t ok32;
-              if (at <= -32) ok32 = 0xffffffffu;
-              else if (at < 0) ok32 = (uint32_t)(sees << -at) | ((1u << -at) - 1u);
-              else ok32 = at < 64 ? (uint32_t)(sees >> at) : 0u;
-#pragma unroll
-              for (int k = 0; k < 32; k++)
-                if (!((ok32 >> k) & 1u)) s[32 * i + k] = -INFINITY;
-            }
+          if (tail && !have_mask) {
+            have_mask = true;
+            const uint64_t all = tree_masks(par, p.n_nodes, node, c.err);
+            sees = row_used && node < d.nodes ? all : 0;
           }
           // The exponentials are taken against the maximum so far, beside the
           // search for this block's: only where that lies 2^8 above it is O
-          // rescaled and are they taken again.
-          if (turn == first_turn) {
-            float mv[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int k = 4; k < (int)BN; k++) mv[k & 3] = fmaxf(mv[k & 3], s[k]);
-            m = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * p.scale_log2;
-          }
-          float pk[32];
+          // rescaled and are they taken again, from the scores, which are
+          // still in the buffer.
+          float s[BN];
           float2 sum, sum1;
           bool again;
           do {
+            tmem_ld32(tmem_s, s);
+            tmem_ld32(tmem_s + 32, s + 32);
+            tmem_ld_wait();
+            if (tail) {
+              // bit k of word i: this row attends cache row key0 + 32 i + k
+#pragma unroll
+              for (int i = 0; i < 2; i++) {
+                const int64_t at = (int64_t)key0 + 32 * i - (int64_t)d.ctx;  // in the tree
+                uint32_t ok32;
+                if (at <= -32) ok32 = 0xffffffffu;
+                else if (at < 0) ok32 = (uint32_t)(sees << -at) | ((1u << -at) - 1u);
+                else ok32 = at < 64 ? (uint32_t)(sees >> at) : 0u;
+#pragma unroll
+                for (int k = 0; k < 32; k++)
+                  if (!((ok32 >> k) & 1u)) s[32 * i + k] = -INFINITY;
+              }
+            }
+            if (turn == first_turn) {
+              float mv[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+              for (int k = 4; k < (int)BN; k++) mv[k & 3] = fmaxf(mv[k & 3], s[k]);
+              m = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * p.scale_log2;
+            }
             const float nb = m == -INFINITY ? 0.f : P_BIAS - m;
             const float2 sc = make_float2(p.scale_log2, p.scale_log2), nb2 = make_float2(nb, nb);
             sum = sum1 = make_float2(0.f, 0.f);
@@ -1009,8 +1013,8 @@ __global__ void __launch_bounds__(THREADS, 1)
               mv[k & 3] = fmaxf(mv[k & 3], fmaxf(s[2 * k], s[2 * k + 1]));
               if (k & 1) sum1 = add2(sum1, e);
               else sum = add2(sum, e);
-              const __half2 hh = __floats2half2_rn(e.x, e.y);
-              pk[k] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&hh));
+              s[2 * k] = e.x;
+              s[2 * k + 1] = e.y;
             }
             const float mx = fmaxf(fmaxf(mv[0], mv[1]), fmaxf(mv[2], mv[3])) * p.scale_log2;
             const bool up = mx > m + RESCALE_LOG2;
@@ -1040,7 +1044,21 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
           } while (again);
           if (!ok) break;
-          tmem_st32(tmem_s, pk);
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            float head[16], rem[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+              const float e0 = s[32 * h + 2 * k], e1 = s[32 * h + 2 * k + 1];
+              const __half2 hh = __floats2half2_rn(e0, e1);
+              const float2 taken = __half22float2(hh);
+              const __half2 rr = __floats2half2_rn(e0 - taken.x, e1 - taken.y);
+              head[k] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&hh));
+              rem[k] = __uint_as_float(*reinterpret_cast<const uint32_t*>(&rr));
+            }
+            tmem_st16(tmem_s + 16 * h, head);
+            tmem_st16(tmem_s + 32 + 16 * h, rem);
+          }
           l += (sum.x + sum.y) + (sum1.x + sum1.y);
           tmem_st_wait();
         }

@@ -7,8 +7,8 @@
 // context and tree rows in shared memory, and one launch does it all:
 //   S    a warp has 16 cache rows and all query rows (up to 64, as 16-row
 //        tiles): mma.sync m16n8k16, Q and K through ldmatrix;
-//   P    against the CTA's maximum per row, as fp16 into shared memory, its
-//        largest 2^15;
+//   P    against the CTA's maximum per row, as fp16 head and fp16 remainder
+//        into shared memory, its largest 2^15;
 //   O    a warp has 16 output columns and every other row tile, so that P, which
 //        all warps read, crosses shared memory half as often;
 //   out  normalised, or joined over the cluster through distributed shared
@@ -111,7 +111,7 @@ __device__ __forceinline__ uint32_t cluster_at(const void* local, uint32_t rank)
   return at;
 }
 
-// Shared memory: K (later the CTA's O, f32), V, Q, P, then what follows.
+// Shared memory: K (later the CTA's O, f32), V, Q, P's heads and remainders, then what follows.
 struct Tail {
   uint64_t sees[nwd::TREE_MAX_NODES];  // the rows of the tree that a node sees
   float2 ml[MAX_ROWS];
@@ -124,10 +124,10 @@ __host__ __device__ inline uint32_t k_bytes(uint32_t keys, uint32_t rows) {
   return keys * 256u > rows * HD * 4u ? keys * 256u : rows * HD * 4u;
 }
 __host__ __device__ inline uint32_t p_bytes(uint32_t keys, uint32_t rows) {
-  return (keys + 127u) / 128u * rows * 256u;  // [128 keys][rows][256 B]
+  return (keys + 127u) / 128u * rows * 256u;  // [128 keys][rows][256 B], of heads or remainders
 }
 inline uint32_t smem_bytes(uint32_t keys, uint32_t rows) {
-  return k_bytes(keys, rows) + keys * 256u + rows * 256u + p_bytes(keys, rows) + (uint32_t)sizeof(Tail);
+  return k_bytes(keys, rows) + keys * 256u + rows * 256u + 2 * p_bytes(keys, rows) + (uint32_t)sizeof(Tail);
 }
 
 template <int MT, bool CLUSTER>
@@ -142,7 +142,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_short_kernel(const __grid_con
   uint8_t* vs = ks + k_bytes(p.keys, ROWS);
   uint8_t* qs = vs + p.keys * 256u;
   uint8_t* ps = qs + ROWS * 256u;
-  Tail& s = *reinterpret_cast<Tail*>(ps + p_bytes(p.keys, ROWS));
+  const uint32_t rem = p_bytes(p.keys, ROWS);  // from a head to its remainder
+  Tail& s = *reinterpret_cast<Tail*>(ps + 2 * rem);
   const uint32_t rows = p.n_nodes * p.group;  // of MT * 16
 
   nwd::pdl_trigger();
@@ -277,10 +278,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_short_kernel(const __grid_con
         for (uint32_t h = 0; h < 2; h++) {
           const float e0 = ex2(sc[m][h][half * 2] + nb), e1 = ex2(sc[m][h][half * 2 + 1] + nb);
           sum += e0 + e1;
-          const __half2 e = __floats2half2_rn(e0, e1);
+          const __half2 head = __floats2half2_rn(e0, e1);
+          const float2 taken = __half22float2(head);
           const uint32_t key = key0 + h * 8;
-          *reinterpret_cast<__half2*>(ps + (key >> 7) * (ROWS * 256u) +
-                                      sw_off(row, (key & 127u) >> 3) + t * 4) = e;
+          uint8_t* at = ps + (key >> 7) * (ROWS * 256u) + sw_off(row, (key & 127u) >> 3) + t * 4;
+          *reinterpret_cast<__half2*>(at) = head;
+          *reinterpret_cast<__half2*>(at + rem) = __floats2half2_rn(e0 - taken.x, e1 - taken.y);
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -342,12 +345,16 @@ __global__ void __launch_bounds__(THREADS, 1) tree_short_kernel(const __grid_con
 #pragma unroll
       for (uint32_t m = 0; m < OT; m++) {
         if (tile0 + 2 * m < (uint32_t)MT) {
-          uint32_t a[4];
-          ldsm_x4(pb + (key >> 7) * (ROWS * 256u) +
-                      sw_off((tile0 + 2 * m) * 16 + (lane & 15), ((key & 127u) >> 3) + (lane >> 4)),
-                  a);
+          const uint32_t at =
+              pb + (key >> 7) * (ROWS * 256u) +
+              sw_off((tile0 + 2 * m) * 16 + (lane & 15), ((key & 127u) >> 3) + (lane >> 4));
+          uint32_t a[4], a1[4];
+          ldsm_x4(at, a);
+          ldsm_x4(at + rem, a1);
           mma16816(acc[m][0], a, b[0], b[1]);
           mma16816(acc[m][1], a, b[2], b[3]);
+          mma16816(acc[m][0], a1, b[0], b[1]);
+          mma16816(acc[m][1], a1, b[2], b[3]);
         }
       }
     }
