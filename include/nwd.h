@@ -472,6 +472,19 @@ int nwd_kv_append_attn_tree(const uint16_t* q, const uint16_t* k_new, const uint
                             uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,
                             void* workspace, size_t ws_bytes, uint32_t* err, void* stream);
 
+/* The same for sequences that share a pool: capacity (device int32[batch], may be
+ * NULL) holds the rows of each sequence's region, from row_offset[b] on.  A tree
+ * that would pass its end (pos[b] + its nodes > capacity[b]) is treated like one
+ * that leaves the pool, so it cannot overwrite the region behind. */
+int nwd_kv_append_attn_tree_bounded(const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
+                                    uint16_t* k_pool, uint16_t* v_pool, uint64_t pool_rows,
+                                    const int64_t* row_offset, const int32_t* pos,
+                                    const int32_t* capacity, const int32_t* parents,
+                                    const int32_t* tree_len, uint16_t* o, uint32_t batch,
+                                    uint32_t n_nodes, uint32_t n_heads, uint32_t n_kv_heads,
+                                    uint32_t head_dim, float scale, void* workspace,
+                                    size_t ws_bytes, uint32_t* err, void* stream);
+
 /* Which drafted tokens stand, and the next token, from given uniform numbers
  * (multi-round rejection sampling; the reference's counterpart is the argmax of
  * one row, kernels/argmax_partial.wgsl).

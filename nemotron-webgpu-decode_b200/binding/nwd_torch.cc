@@ -111,9 +111,9 @@ bool expect(Py_ssize_t got, Py_ssize_t want) {
 }
 
 // tree(q, k_new | None, v_new | None, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads,
-//      n_kv_heads, head_dim, tree_len | None, scale, workspace, ws_bytes, err)
+//      n_kv_heads, head_dim, tree_len | None, scale, workspace, ws_bytes, err, capacity | None)
 PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-  if (!expect(n_args, 17)) return nullptr;
+  if (!expect(n_args, 18)) return nullptr;
   return guarded([&]() -> PyObject* {
     const at::Tensor& q = tensor(a[0], "q");
     const int dev = q.get_device();
@@ -146,6 +146,8 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     auto* op = pointer<uint16_t>(a[8], "o", F16, qo, dev);
     const auto* tl =
         a[12] == Py_None ? nullptr : pointer<int32_t>(a[12], "tree_len", I32, one, dev);
+    const auto* cap =
+        a[17] == Py_None ? nullptr : pointer<int32_t>(a[17], "capacity", I32, one, dev);
     void* ws = reinterpret_cast<void*>(number(a[14], "workspace"));
     size_t ws_bytes = number(a[15], "ws_bytes");
     auto* err = reinterpret_cast<uint32_t*>(number(a[16], "err"));
@@ -160,9 +162,9 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     }
     void* stream = c10::cuda::getCurrentCUDAStream(dev).stream();
     if (append)
-      check(nwd_kv_append_attn_tree(qp, kn, vn, k, v, rows, off, len, pr, tl, op, (uint32_t)batch,
-                                    (uint32_t)n, n_heads, n_kv, hd, (float)scale, ws, ws_bytes, err,
-                                    stream));
+      check(nwd_kv_append_attn_tree_bounded(qp, kn, vn, k, v, rows, off, len, cap, pr, tl, op,
+                                            (uint32_t)batch, (uint32_t)n, n_heads, n_kv, hd,
+                                            (float)scale, ws, ws_bytes, err, stream));
     else
       check(nwd_attn_tree(qp, k, v, rows, off, len, pr, tl, op, (uint32_t)batch, (uint32_t)n,
                           n_heads, n_kv, hd, (float)scale, ws, ws_bytes, err, stream));

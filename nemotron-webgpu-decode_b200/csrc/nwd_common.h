@@ -63,7 +63,7 @@ struct TreeShortArgs {
   uint16_t *k_pool, *v_pool, *o;
   uint64_t pool_rows;
   const int64_t* row_offset;
-  const int32_t *seq_len, *parents, *tree_len;
+  const int32_t *seq_len, *parents, *tree_len, *capacity;  // capacity: or nullptr
   uint32_t n_nodes, n_heads, n_kv;
   float scale_log2;
   uint32_t* err;

@@ -78,20 +78,23 @@ static __device__ __forceinline__ uint32_t tree_nodes(const int32_t* tree_len, u
 }
 
 // The rows of a sequence: ctx context rows from pool row row0, then its nodes'.
-// A sequence whose rows leave the pool is recorded as NWD_DEVERR_ROW_RANGE and
-// has no rows and no nodes.
+// A sequence whose rows leave the pool, or its region of `capacity` rows where
+// those are given, is recorded as NWD_DEVERR_ROW_RANGE and has no rows and no
+// nodes.
 struct TreeSeq {
   int64_t row0;
   uint32_t ctx, nodes;
 };
 struct TreeRaw {
   int64_t row_offset;
-  int32_t seq_len, tree_len;
+  int32_t seq_len, tree_len, capacity;
 };
 static __device__ __forceinline__ TreeRaw tree_raw(const int64_t* row_offset,
                                                    const int32_t* seq_len, const int32_t* tree_len,
-                                                   uint32_t b, uint32_t n) {
-  return TreeRaw{row_offset[b], seq_len[b], tree_len ? tree_len[b] : (int32_t)n};
+                                                   const int32_t* capacity, uint32_t b,
+                                                   uint32_t n) {
+  return TreeRaw{row_offset[b], seq_len[b], tree_len ? tree_len[b] : (int32_t)n,
+                 capacity ? capacity[b] : 0x7fffffff};
 }
 static __device__ __forceinline__ TreeSeq tree_seq(const TreeRaw& raw, uint64_t pool_rows,
                                                    uint32_t n, uint32_t* err) {
@@ -101,7 +104,8 @@ static __device__ __forceinline__ TreeSeq tree_seq(const TreeRaw& raw, uint64_t 
   s.nodes = min((uint32_t)max(raw.tree_len, 0), n);
   if ((uint32_t)raw.tree_len > n && err) atomicOr(err, NWD_DEVERR_TREE);
   if (s.row0 < 0 || raw.seq_len < 0 || (uint64_t)s.row0 > pool_rows ||
-      (uint64_t)s.ctx + s.nodes > pool_rows - (uint64_t)s.row0) {
+      (uint64_t)s.ctx + s.nodes > pool_rows - (uint64_t)s.row0 ||
+      (int64_t)s.ctx + s.nodes > raw.capacity) {
     if (err) atomicOr(err, NWD_DEVERR_ROW_RANGE);
     s.row0 = 0;
     s.ctx = s.nodes = 0;
@@ -110,9 +114,9 @@ static __device__ __forceinline__ TreeSeq tree_seq(const TreeRaw& raw, uint64_t 
 }
 static __device__ __forceinline__ TreeSeq tree_seq(const int64_t* row_offset,
                                                    const int32_t* seq_len, const int32_t* tree_len,
-                                                   uint64_t pool_rows, uint32_t b, uint32_t n,
-                                                   uint32_t* err) {
-  return tree_seq(tree_raw(row_offset, seq_len, tree_len, b, n), pool_rows, n, err);
+                                                   const int32_t* capacity, uint64_t pool_rows,
+                                                   uint32_t b, uint32_t n, uint32_t* err) {
+  return tree_seq(tree_raw(row_offset, seq_len, tree_len, capacity, b, n), pool_rows, n, err);
 }
 
 }  // namespace nwd

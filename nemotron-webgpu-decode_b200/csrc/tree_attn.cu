@@ -155,6 +155,7 @@ struct TParams {
   const int32_t* seq_len;
   const int32_t* parents;
   const int32_t* tree_len;
+  const int32_t* capacity;  // rows of the sequences' regions, or nullptr
   uint32_t* err;      // the caller's error word, or the workspace's
   uint8_t* ws;
   uint64_t pool_rows;
@@ -194,7 +195,8 @@ __host__ __device__ inline size_t ws_total(uint32_t ctas, uint32_t unit_tiles) {
 static_assert(WS_ML % 256 == 0, "alignment");
 
 __device__ __forceinline__ TreeSeq load_seq(const TParams& p, uint32_t b, uint32_t* err) {
-  return nwd::tree_seq(p.row_offset, p.seq_len, p.tree_len, p.pool_rows, b, p.n_nodes, err);
+  return nwd::tree_seq(p.row_offset, p.seq_len, p.tree_len, p.capacity, p.pool_rows, b, p.n_nodes,
+                       err);
 }
 // A unit has at least one block, so that its output rows are written; without
 // nodes there is nothing to read.
@@ -493,7 +495,7 @@ __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
   uint32_t turns = 0, blocks = 0, tiles = 0;
   nwd::TreeRaw ahead{};
   if (left > 0 && b + 1 < p.batch)
-    ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, b + 1, p.n_nodes);
+    ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, p.capacity, b + 1, p.n_nodes);
   for (;;) {
     Piece d{};
     if (left > 0 && blk == nblk) {  // on to the next unit
@@ -505,7 +507,7 @@ __device__ __forceinline__ void plan(const TParams& p, const Ctx& c) {
         nblk = seq_blocks(s);
         nt = seq_tiles(p, s.nodes);
         if (b + 1 < p.batch)
-          ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, b + 1, p.n_nodes);
+          ahead = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, p.capacity, b + 1, p.n_nodes);
       }
     }
     if (left > 0) {
@@ -1333,12 +1335,13 @@ __global__ void __launch_bounds__(MERGE_THREADS)
 __global__ void tree_append_kernel(const uint4* __restrict__ k_new, const uint4* __restrict__ v_new,
                                    uint4* __restrict__ k_pool, uint4* __restrict__ v_pool,
                                    const int64_t* row_offset, const int32_t* pos,
-                                   const int32_t* tree_len, uint64_t pool_rows, uint32_t n_nodes,
-                                   uint32_t row_vec, uint32_t* err) {
+                                   const int32_t* tree_len, const int32_t* capacity,
+                                   uint64_t pool_rows, uint32_t n_nodes, uint32_t row_vec,
+                                   uint32_t* err) {
   nwd::pdl_trigger();
   nwd::pdl_wait();
   const uint32_t b = blockIdx.y;
-  const TreeSeq s = nwd::tree_seq(row_offset, pos, tree_len, pool_rows, b, n_nodes, err);
+  const TreeSeq s = nwd::tree_seq(row_offset, pos, tree_len, capacity, pool_rows, b, n_nodes, err);
   const uint64_t dst = ((uint64_t)s.row0 + s.ctx) * row_vec, src = (uint64_t)b * n_nodes * row_vec;
   for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < s.nodes * row_vec;
        i += gridDim.x * blockDim.x) {
@@ -1398,7 +1401,8 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
              const int32_t* parents, const int32_t* tree_len, uint16_t* o, uint32_t batch,
              uint32_t n_nodes, uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, float scale,
              void* workspace, size_t ws_bytes, uint32_t* err, void* stream,
-             const uint16_t* k_new = nullptr, const uint16_t* v_new = nullptr) {
+             const uint16_t* k_new = nullptr, const uint16_t* v_new = nullptr,
+             const int32_t* capacity = nullptr) {
   using namespace nwd;
   const uint32_t group = n_heads / n_kv;
   const Tiling t = tiling(n_nodes, group, tree_len != nullptr);
@@ -1420,7 +1424,7 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
   if (tree_short_fits(pool_rows, batch, n_nodes * group))  // one launch, no partials
     return launch_tree_short({q, k_new, v_new, const_cast<uint16_t*>(k_pool),
                               const_cast<uint16_t*>(v_pool), o, pool_rows, row_offset, seq_len,
-                              parents, tree_len, n_nodes, n_heads, n_kv, scale_log2,
+                              parents, tree_len, capacity, n_nodes, n_heads, n_kv, scale_log2,
                               err ? err : reinterpret_cast<uint32_t*>(workspace), stream},
                              who);
   static bool smem_set[64] = {};
@@ -1450,6 +1454,7 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
   p.seq_len = seq_len;
   p.parents = parents;
   p.tree_len = tree_len;
+  p.capacity = capacity;
   p.ws = reinterpret_cast<uint8_t*>(workspace);
   p.err = err ? err : reinterpret_cast<uint32_t*>(workspace);
   p.pool_rows = pool_rows;
@@ -1472,7 +1477,7 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
                    reinterpret_cast<const uint4*>(k_new), reinterpret_cast<const uint4*>(v_new),
                    reinterpret_cast<uint4*>(const_cast<uint16_t*>(k_pool)),
                    reinterpret_cast<uint4*>(const_cast<uint16_t*>(v_pool)), row_offset, seq_len,
-                   tree_len, pool_rows, n_nodes, row_vec, p.err);
+                   tree_len, capacity, pool_rows, n_nodes, row_vec, p.err);
     if (e != cudaSuccess) return cuda_fail(e, who);
   }
   const uint32_t ctas = (uint32_t)di.sm_count;
@@ -1526,6 +1531,20 @@ int nwd_kv_append_attn_tree(const uint16_t* q, const uint16_t* k_new, const uint
                             const int32_t* tree_len, uint16_t* o, uint32_t batch, uint32_t n_nodes,
                             uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,
                             void* workspace, size_t ws_bytes, uint32_t* err, void* stream) {
+  return nwd_kv_append_attn_tree_bounded(q, k_new, v_new, k_pool, v_pool, pool_rows, row_offset,
+                                         pos, nullptr, parents, tree_len, o, batch, n_nodes,
+                                         n_heads, n_kv_heads, head_dim, scale, workspace, ws_bytes,
+                                         err, stream);
+}
+
+int nwd_kv_append_attn_tree_bounded(const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
+                                    uint16_t* k_pool, uint16_t* v_pool, uint64_t pool_rows,
+                                    const int64_t* row_offset, const int32_t* pos,
+                                    const int32_t* capacity, const int32_t* parents,
+                                    const int32_t* tree_len, uint16_t* o, uint32_t batch,
+                                    uint32_t n_nodes, uint32_t n_heads, uint32_t n_kv_heads,
+                                    uint32_t head_dim, float scale, void* workspace,
+                                    size_t ws_bytes, uint32_t* err, void* stream) {
   const char* who = "nwd_kv_append_attn_tree";
   int st = check_tree(who, q, k_pool, v_pool, row_offset, pos, parents, o, pool_rows, batch,
                       n_nodes, n_heads, n_kv_heads, head_dim, scale);
@@ -1538,7 +1557,7 @@ int nwd_kv_append_attn_tree(const uint16_t* q, const uint16_t* k_new, const uint
     return fail(NWD_ERR_INVALID, "%s: k_pool and v_pool must not overlap", who);
   return run_tree(who, q, k_pool, v_pool, pool_rows, row_offset, pos, parents, tree_len, o, batch,
                   n_nodes, n_heads, n_kv_heads, head_dim, scale, workspace, ws_bytes, err, stream,
-                  k_new, v_new);
+                  k_new, v_new, capacity);
 }
 
 }  // extern "C"

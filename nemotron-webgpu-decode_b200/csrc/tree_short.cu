@@ -56,6 +56,7 @@ struct Params {
   const int32_t* seq_len;
   const int32_t* parents;
   const int32_t* tree_len;
+  const int32_t* capacity;
   uint32_t* err;
   uint64_t pool_rows;
   uint32_t n_nodes, n_heads, n_kv, group, cluster, keys;  // keys: a CTA's room, a multiple of 32
@@ -153,7 +154,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_short_kernel(const __grid_con
     if (lane < p.n_nodes) par.x = p.parents[lane];
     if (lane + 32 < p.n_nodes) par.y = p.parents[lane + 32];
   }
-  const nwd::TreeRaw raw = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, 0, p.n_nodes);
+  const nwd::TreeRaw raw = nwd::tree_raw(p.row_offset, p.seq_len, p.tree_len, p.capacity, 0,
+                                         p.n_nodes);
   const uint32_t kb = s_u32(ks), vb = s_u32(vs), qb = s_u32(qs), pb = s_u32(ps);
 
   // ---- Q and K, then V, into shared memory ----
@@ -521,6 +523,7 @@ int launch_tree_short(const TreeShortArgs& a, const char* who) {
   p.seq_len = a.seq_len;
   p.parents = a.parents;
   p.tree_len = a.tree_len;
+  p.capacity = a.capacity;
   p.err = a.err;
   p.pool_rows = a.pool_rows;
   p.n_nodes = a.n_nodes;

@@ -184,6 +184,8 @@ class BatchedDecodeAttention:
         self.v_pool = torch.zeros_like(self.k_pool)
         self.row_offset = offs.to(self.device)
         self.lengths = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
+        # the regions' ends as the speculative calls watch them
+        self.region_rows = caps.clamp(max=2**31 - 1).to(torch.int32).to(self.device)
         self.workspace = ops.Workspace(self.batch, heads, kv_heads, head_dim, self.device)
         self.scratch = ops.Scratch(self.device)  # device errors of the speculative calls
 
@@ -204,7 +206,8 @@ class BatchedDecodeAttention:
         """A speculative step: the trees' K/V rows go behind every sequence's rows and each
         node attends the rows, its ancestors and itself.  q [B, N, heads, hd], k_new / v_new
         [B, N, kv_heads, hd], parents [B, N] (:func:`ops.attention_tree`).  The lengths stay
-        until :meth:`commit`.  A sequence's capacity has to hold its tree too."""
+        until :meth:`commit`.  A sequence's capacity has to hold its tree too: one whose does
+        not writes nothing, gets zeros, and is recorded in ``scratch`` (a device error)."""
         if stream is not None:
             with ops._on(stream, self.device):
                 return self.tree_step(q, k_new, v_new, parents, tree_len, out)
@@ -214,7 +217,7 @@ class BatchedDecodeAttention:
                                             self.row_offset, self.lengths, parents, out,
                                             self.heads, self.kv_heads, self.head_dim,
                                             tree_len=tree_len, scale=self.scale,
-                                            scratch=self.scratch)
+                                            scratch=self.scratch, capacity=self.region_rows)
 
     def commit(self, path, n_accepted, stream=None) -> None:
         """Keeps the accepted nodes of the last :meth:`tree_step` (:func:`ops.verify_tree`'s

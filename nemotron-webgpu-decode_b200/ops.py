@@ -406,11 +406,11 @@ def _on(stream, device):
 
 
 def _tree(q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads, n_kv_heads,
-          head_dim, tree_len, scale, workspace, scratch, stream):
+          head_dim, tree_len, scale, workspace, scratch, stream, capacity=None):
     if stream is not None:
         with _on(stream, q.device):
             return _tree(q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads,
-                         n_kv_heads, head_dim, tree_len, scale, workspace, scratch, None)
+                         n_kv_heads, head_dim, tree_len, scale, workspace, scratch, None, capacity)
     ptr, nbytes = 0, 0
     if workspace is not None:
         if workspace.device != q.device:
@@ -418,7 +418,7 @@ def _tree(q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_he
         ptr, nbytes = workspace.ptr, workspace.nbytes
     (_lib._torch or _lib.torch_calls()).tree(
         q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads, n_kv_heads,
-        head_dim, tree_len, scale, ptr, nbytes, 0 if scratch is None else scratch.ptr)
+        head_dim, tree_len, scale, ptr, nbytes, 0 if scratch is None else scratch.ptr, capacity)
     return o
 
 
@@ -440,11 +440,14 @@ def attention_tree(q, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads: 
 def kv_append_attention_tree(q, k_new, v_new, k_pool, v_pool, row_offset, pos, parents, o,
                              n_heads: int, n_kv_heads: int, head_dim: int = 128, tree_len=None,
                              scale: float = 0.0, workspace: TreeWorkspace | None = None,
-                             scratch: Scratch | None = None, stream=None) -> torch.Tensor:
+                             scratch: Scratch | None = None, stream=None,
+                             capacity=None) -> torch.Tensor:
     """:func:`attention_tree` after writing the present nodes' rows k_new / v_new
-    [B, N, n_kv, hd] to pool rows row_offset[b] + pos[b] + i (pos: rows before the tree)."""
+    [B, N, n_kv, hd] to pool rows row_offset[b] + pos[b] + i (pos: rows before the tree).
+    capacity [B] int32: the rows of each sequence's region; a tree that would pass its end
+    is refused like one that leaves the pool (zero outputs, no row written, a device error)."""
     return _tree(q, k_new, v_new, k_pool, v_pool, row_offset, pos, parents, o, n_heads,
-                 n_kv_heads, head_dim, tree_len, scale, workspace, scratch, stream)
+                 n_kv_heads, head_dim, tree_len, scale, workspace, scratch, stream, capacity)
 
 
 def verify_tree(tokens, parents, target_probs, u, w, draft_probs=None, tree_len=None, out=None,

@@ -1,0 +1,100 @@
+"""Speculative steps at the end of a sequence's region, and steps that are refused: the
+neighbours' rows, the lengths and the layers' own places (engine.BatchedDecodeAttention)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from devutil import bits, vals
+from spec_ref import attention_bound, random_parents, tree_attention
+
+pytestmark = pytest.mark.gpu
+HD = 128
+
+
+def _t(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def _i(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _layer(engine_mod, rng, caps, lengths, nh=8, nkv=2):
+    layer = engine_mod.BatchedDecodeAttention(caps, nh, nkv)
+    layer.k_pool.copy_(_t(rng.standard_normal(layer.k_pool.shape).astype(np.float16)))
+    layer.v_pool.copy_(_t(rng.standard_normal(layer.v_pool.shape).astype(np.float16)))
+    layer.lengths.copy_(_i(lengths))
+    return layer
+
+
+def _trees(rng, b, n, nh=8, nkv=2):
+    h = lambda *s: rng.standard_normal(s).astype(np.float16)  # noqa: E731
+    parents = np.stack([random_parents(rng, n) for _ in range(b)])
+    return h(b, n, nh, HD), h(b, n, nkv, HD), h(b, n, nkv, HD), parents
+
+
+def _check_output(got, q, k_rows, v_rows, ctx, parents, m, nkv):
+    ref, mag, amp = tree_attention(q.astype(np.float64), k_rows.astype(np.float64),
+                                   v_rows.astype(np.float64), ctx, parents, m, nkv, HD ** -0.5)
+    tol = attention_bound(ref, mag, amp, len(k_rows), HD ** -0.5, 6.0)
+    assert (np.abs(got - ref) <= tol).all()
+    assert (got[m:] == 0).all()
+
+
+@pytest.mark.parametrize("caps,lengths,n,tree_len", [
+    ([40, 40, 40], [36, 10, 40], 6, None),
+    ([40, 40, 40], [36, 10, 35], 6, [4, 6, 6]),     # the first one fits, the last does not
+    ([100, 70, 300], [90, 69, 200], 61, [10, 2, 61]),
+    ([64, 64, 64], [64, 0, 1], 64, None),
+])
+def test_a_tree_past_its_region_leaves_the_neighbour(ops, engine_mod, caps, lengths, n, tree_len):
+    rng = np.random.default_rng(n)
+    layer = _layer(engine_mod, rng, caps, lengths)
+    q, k, v, parents = _trees(rng, len(caps), n)
+    kp, vp = bits(layer.k_pool).copy(), bits(layer.v_pool).copy()
+    got = vals(layer.tree_step(_t(q), _t(k), _t(v), _t(parents),
+                               tree_len=None if tree_len is None else _i(tree_len)))
+    assert layer.scratch.check() == 2
+    off = np.cumsum([0] + caps)
+    for b, ctx in enumerate(lengths):
+        m = n if tree_len is None else tree_len[b]
+        if ctx + m > caps[b]:
+            assert (got[b] == 0).all()
+            continue
+        lo = off[b]
+        kp[lo + ctx:lo + ctx + m] = k[b, :m].view(np.uint16)
+        vp[lo + ctx:lo + ctx + m] = v[b, :m].view(np.uint16)
+        f = lambda x: x[lo:lo + ctx + m].view(np.float16)  # noqa: E731
+        _check_output(got[b], q[b], f(kp), f(vp), ctx, parents[b], m, 2)
+    assert np.array_equal(bits(layer.k_pool), kp)
+    assert np.array_equal(bits(layer.v_pool), vp)
+
+
+@pytest.mark.parametrize("room,fits", [(37, True), (36, False), (0, False), (-5, False), (1000, True)])
+@pytest.mark.parametrize("b", [1, 2])
+def test_given_capacities(ops, b, room, fits):
+    """The operator itself, in a pool that has room behind the sequence (both kernels)."""
+    rng = np.random.default_rng(9)
+    n, ctx, rows = 7, 30, 80
+    q, k, v, parents = _trees(rng, b, n)
+    pools = [_t(rng.standard_normal((rows, 2, HD)).astype(np.float16)) for _ in range(2)]
+    old = [bits(p).copy() for p in pools]
+    o = torch.full(q.shape, 9.0, dtype=torch.float16, device="cuda")
+    sc = ops.Scratch()
+    ops.kv_append_attention_tree(_t(q), _t(k), _t(v), *pools,
+                                 torch.tensor([0, 40][:b], device="cuda"), _i([ctx] * b),
+                                 _t(parents), o, 8, 2, capacity=_i([room] + [40] * (b - 1)),
+                                 scratch=sc)
+    got = vals(o)
+    assert sc.check() == (0 if fits else 2)
+    for x in range(b):
+        if x == 0 and not fits:
+            assert (got[0] == 0).all()
+            continue
+        lo = 40 * x + ctx
+        old[0][lo:lo + n], old[1][lo:lo + n] = k[x].view(np.uint16), v[x].view(np.uint16)
+        f = lambda a: a[40 * x:lo + n].view(np.float16)  # noqa: E731
+        _check_output(got[x], q[x], f(old[0]), f(old[1]), ctx, parents[x], n, 2)
+    assert np.array_equal(bits(pools[0]), old[0]) and np.array_equal(bits(pools[1]), old[1])
