@@ -528,6 +528,16 @@ int nwd_kv_commit(uint16_t* const* pools, uint32_t n_pools, uint64_t pool_rows,
                   const int32_t* n_accepted, uint32_t batch, uint32_t n_nodes, uint32_t n_kv,
                   uint32_t hd, uint32_t* err, void* stream);
 
+/* The same for the layers of a model (at most 32), each with its own place: layer
+ * i's K and V are pools[2 i] and pools[2 i + 1], its sequences stand at
+ * row_offset[i] and pos[i] (host arrays of device pointers; layers may share
+ * them).  A sequence that one layer refuses is left as it is in all of them. */
+int nwd_kv_commit_layers(uint16_t* const* pools, uint32_t n_layers, uint64_t pool_rows,
+                         const int64_t* const* row_offset, const int32_t* const* pos,
+                         const int32_t* path, const int32_t* n_accepted, uint32_t batch,
+                         uint32_t n_nodes, uint32_t n_kv, uint32_t hd, uint32_t* err,
+                         void* stream);
+
 /* ------------------------------------------------------------------ */
 /* Synthetic inputs                                                    */
 /* ------------------------------------------------------------------ */

@@ -55,7 +55,7 @@ std::string text(at::IntArrayRef shape) {
 }
 
 // The pointer of a contiguous tensor of this type, shape and device.
-template <typename T>
+template <typename T>  // (may be const)
 T* pointer(PyObject* o, const char* name, at::ScalarType type, at::IntArrayRef shape, int device) {
   const at::Tensor& t = tensor(o, name);
   if (t.scalar_type() != type)
@@ -229,6 +229,27 @@ PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// The pools of a list, all of the first one's shape and on `dev`; that shape.
+std::vector<uint16_t*> pool_pointers(PyObject* list, int dev, at::IntArrayRef* shape) {
+  if (!PyList_Check(list)) refuse(PyExc_TypeError, "pools must be a list");
+  const Py_ssize_t count = PyList_GET_SIZE(list);
+  std::vector<uint16_t*> ptrs((size_t)count);
+  if (count == 0) return ptrs;
+  const at::Tensor& first = tensor(PyList_GET_ITEM(list, 0), "pool");
+  if (first.dim() != 3)
+    refuse(PyExc_ValueError, "pools must be [rows, n_kv, hd], got " + text(first.sizes()));
+  for (Py_ssize_t i = 0; i < count; i++) {
+    ptrs[i] = pointer<uint16_t>(PyList_GET_ITEM(list, i), "pool", F16, first.sizes(), dev);
+    for (Py_ssize_t j = 0; j < i; j++)
+      if (ptrs[j] == ptrs[i] && first.numel())
+        refuse(PyExc_ValueError, "pools must differ from one another");
+  }
+  *shape = first.sizes();
+  if (first.size(1) > 0xffffffffll || first.size(2) > 0xffffffffll)
+    refuse(PyExc_ValueError, "pools are too large");
+  return ptrs;
+}
+
 // commit(pools (a list), row_offset, pos, path, n_accepted, err): 16 pools per launch
 PyObject* commit(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   if (!expect(n_args, 6)) return nullptr;
@@ -244,29 +265,62 @@ PyObject* commit(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const auto* pp = pointer<int32_t>(a[3], "path", I32, path.sizes(), dev);
     const auto* na = pointer<int32_t>(a[4], "n_accepted", I32, one, dev);
     auto* err = reinterpret_cast<uint32_t*>(number(a[5], "err"));
-    if (!PyList_Check(a[0])) refuse(PyExc_TypeError, "pools must be a list");
-    const Py_ssize_t count = PyList_GET_SIZE(a[0]);
-    if (count == 0) Py_RETURN_NONE;
-    const at::Tensor& first = tensor(PyList_GET_ITEM(a[0], 0), "pool");
-    if (first.dim() != 3)
-      refuse(PyExc_ValueError, "pools must be [rows, n_kv, hd], got " + text(first.sizes()));
-    std::vector<uint16_t*> ptrs((size_t)count);
-    for (Py_ssize_t i = 0; i < count; i++) {
-      ptrs[i] = pointer<uint16_t>(PyList_GET_ITEM(a[0], i), "pool", F16, first.sizes(), dev);
-      for (Py_ssize_t j = 0; j < i; j++)
-        if (ptrs[j] == ptrs[i] && first.numel())
-          refuse(PyExc_ValueError, "pools must differ from one another");
-    }
-    if (batch > 0xffffffffll || n > 0xffffffffll || first.size(1) > 0xffffffffll ||
-        first.size(2) > 0xffffffffll)
-      refuse(PyExc_ValueError, "path or pools are too large");
-    if (batch == 0 || n == 0 || first.numel() == 0) Py_RETURN_NONE;
+    at::IntArrayRef shape;
+    const std::vector<uint16_t*> ptrs = pool_pointers(a[0], dev, &shape);
+    const Py_ssize_t count = (Py_ssize_t)ptrs.size();
+    if (batch > 0xffffffffll || n > 0xffffffffll) refuse(PyExc_ValueError, "path is too large");
+    if (batch == 0 || n == 0 || count == 0 || !ptrs[0]) Py_RETURN_NONE;
     const c10::cuda::CUDAGuard on(dev);
     void* stream = c10::cuda::getCurrentCUDAStream(dev).stream();
     for (Py_ssize_t i = 0; i < count; i += 16)
       check(nwd_kv_commit(ptrs.data() + i, (uint32_t)std::min<Py_ssize_t>(16, count - i),
-                          (uint64_t)first.size(0), off, pos, pp, na, (uint32_t)batch, (uint32_t)n,
-                          (uint32_t)first.size(1), (uint32_t)first.size(2), err, stream));
+                          (uint64_t)shape[0], off, pos, pp, na, (uint32_t)batch, (uint32_t)n,
+                          (uint32_t)shape[1], (uint32_t)shape[2], err, stream));
+    Py_RETURN_NONE;
+  });
+}
+
+// The pointers of a list of tensors of one type and shape.
+template <typename T>
+std::vector<T*> pointers(PyObject* list, const char* name, at::ScalarType type, size_t count,
+                         at::IntArrayRef shape, int dev) {
+  if (!PyList_Check(list) || (size_t)PyList_GET_SIZE(list) != count)
+    refuse(PyExc_TypeError, std::string(name) + " must be a list with an entry per layer");
+  std::vector<T*> ptrs(count);
+  for (size_t i = 0; i < count; i++)
+    ptrs[i] = pointer<T>(PyList_GET_ITEM(list, (Py_ssize_t)i), name, type, shape, dev);
+  return ptrs;
+}
+
+// commit_layers(pools (K, V, K, V ..), row_offsets, lengths (lists, an entry per layer), path,
+//               n_accepted, err): 32 layers per launch
+PyObject* commit_layers(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  if (!expect(n_args, 6)) return nullptr;
+  return guarded([&]() -> PyObject* {
+    const at::Tensor& path = tensor(a[3], "path");
+    if (path.dim() != 2)
+      refuse(PyExc_ValueError, "path must be [batch, n_nodes], got " + text(path.sizes()));
+    const int dev = path.get_device();
+    const int64_t batch = path.size(0), n = path.size(1);
+    const int64_t one[1] = {batch};
+    at::IntArrayRef shape;
+    const std::vector<uint16_t*> ptrs = pool_pointers(a[0], dev, &shape);
+    if (ptrs.size() % 2) refuse(PyExc_ValueError, "a layer has two pools");
+    const size_t layers = ptrs.size() / 2;
+    const auto off = pointers<const int64_t>(a[1], "row_offset", I64, layers, one, dev);
+    const auto len = pointers<int32_t>(a[2], "lengths", I32, layers, one, dev);
+    const auto* pp = pointer<int32_t>(a[3], "path", I32, path.sizes(), dev);
+    const auto* na = pointer<int32_t>(a[4], "n_accepted", I32, one, dev);
+    auto* err = reinterpret_cast<uint32_t*>(number(a[5], "err"));
+    if (batch > 0xffffffffll || n > 0xffffffffll) refuse(PyExc_ValueError, "path is too large");
+    if (batch == 0 || n == 0 || layers == 0 || !ptrs[0]) Py_RETURN_NONE;
+    const c10::cuda::CUDAGuard on(dev);
+    void* stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+    for (size_t i = 0; i < layers; i += 32)
+      check(nwd_kv_commit_layers(ptrs.data() + 2 * i, (uint32_t)std::min<size_t>(32, layers - i),
+                                 (uint64_t)shape[0], off.data() + i, len.data() + i, pp, na,
+                                 (uint32_t)batch, (uint32_t)n, (uint32_t)shape[1],
+                                 (uint32_t)shape[2], err, stream));
     Py_RETURN_NONE;
   });
 }
@@ -281,6 +335,8 @@ PyMethodDef methods[] = {
     {"tree", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(tree)), METH_FASTCALL, nullptr},
     {"verify", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(verify)), METH_FASTCALL, nullptr},
     {"commit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(commit)), METH_FASTCALL, nullptr},
+    {"commit_layers", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(commit_layers)),
+     METH_FASTCALL, nullptr},
     {"set_error", set_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

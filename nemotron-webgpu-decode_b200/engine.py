@@ -234,18 +234,15 @@ class BatchedDecodeAttention:
 
 
 def commit_layers(layers, path, n_accepted, stream=None) -> None:
-    """:meth:`BatchedDecodeAttention.commit` for the layers of one model: the same sequences
-    and lengths in each (every layer has run the step's trees), all their pools moved in one
-    launch per eight layers."""
+    """:meth:`BatchedDecodeAttention.commit` for the layers of one model (every layer has run
+    the step's trees): the rows of all of them move in one launch per 32 layers, each layer's
+    at its own offsets and lengths."""
     layers = list(layers)
     if not layers:
         return
-    first = layers[0]
-    pools = [p for layer in layers for p in (layer.k_pool, layer.v_pool)]
-
     if stream is not None:
-        with ops._on(stream, first.lengths.device):
+        with ops._on(stream, layers[0].lengths.device):
             return commit_layers(layers, path, n_accepted)
-    ops.kv_commit(pools, first.row_offset, first.lengths, path, n_accepted, scratch=first.scratch)
+    ops._kv_commit_layers(layers, path, n_accepted, layers[0].scratch)
     for lengths in {layer.lengths.data_ptr(): layer.lengths for layer in layers}.values():
         lengths += n_accepted  # (layers may share one tensor)

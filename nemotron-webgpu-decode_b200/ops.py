@@ -485,6 +485,15 @@ def kv_commit(pools, row_offset, pos, path, n_accepted, scratch: Scratch | None 
         0 if scratch is None else scratch.ptr)
 
 
+def _kv_commit_layers(layers, path, n_accepted, scratch):
+    """:func:`kv_commit` for K and V of several layers, each at its own offsets and lengths
+    (:func:`engine.commit_layers`), 32 layers per launch."""
+    _lib.torch_calls().commit_layers(
+        [p for layer in layers for p in (layer.k_pool, layer.v_pool)],
+        [layer.row_offset for layer in layers], [layer.lengths for layer in layers], path,
+        n_accepted, scratch.ptr)
+
+
 def selftest_wait_timeout(workspace: "Workspace", stream=None) -> int:
     """Make one of the library's bounded device waits run out (about 2 s) and return the
     workspace's device error word afterwards (NWD_DEVERR_PIPE_TIMEOUT expected); the

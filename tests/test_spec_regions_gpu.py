@@ -72,6 +72,27 @@ def test_a_tree_past_its_region_leaves_the_neighbour(ops, engine_mod, caps, leng
     assert np.array_equal(bits(layer.v_pool), vp)
 
 
+@pytest.mark.parametrize("n_layers", [2, 3, 33])
+def test_layers_keep_their_own_places(engine_mod, n_layers):
+    """Layers of different lengths, and of different regions in pools of one size."""
+    rng = np.random.default_rng(6)
+    caps = [[20, 30], [30, 20], [25, 25]]
+    lens = [[5, 9], [7, 3], [0, 19]]
+    layers = [_layer(engine_mod, rng, caps[i % 3], lens[i % 3]) for i in range(n_layers)]
+    path, count = [[0, 2, 5, -1, -1, -1], [0, 1, 3, 4, -1, -1]], [3, 4]
+    before = [[bits(p).copy() for p in (layer.k_pool, layer.v_pool)] for layer in layers]
+    engine_mod.commit_layers(layers, _i(path), _i(count))
+    for i, (layer, pools) in enumerate(zip(layers, before)):
+        off = [0, caps[i % 3][0]]
+        for pool, want in zip((layer.k_pool, layer.v_pool), pools):
+            for b in range(2):
+                base = off[b] + lens[i % 3][b]
+                want[base:base + count[b]] = want[[base + x for x in path[b][:count[b]]]]
+            assert np.array_equal(bits(pool), want)
+        assert layer.lengths.tolist() == [lens[i % 3][b] + count[b] for b in range(2)]
+    assert layers[0].scratch.check() == 0
+
+
 @pytest.mark.parametrize("room,fits", [(37, True), (36, False), (0, False), (-5, False), (1000, True)])
 @pytest.mark.parametrize("b", [1, 2])
 def test_given_capacities(ops, b, room, fits):
