@@ -528,12 +528,18 @@ int nwd_kv_commit(uint16_t* const* pools, uint32_t n_pools, uint64_t pool_rows,
                   const int32_t* n_accepted, uint32_t batch, uint32_t n_nodes, uint32_t n_kv,
                   uint32_t hd, uint32_t* err, void* stream);
 
-/* The same for the layers of a model (at most 32), each with its own place: layer
- * i's K and V are pools[2 i] and pools[2 i + 1], its sequences stand at
- * row_offset[i] and pos[i] (host arrays of device pointers; layers may share
- * them).  A sequence that one layer refuses is left as it is in all of them. */
+/* The same for the layers of a model (at most 32), each with its own place, and
+ * with the lengths: layer i's K and V are pools[2 i] and pools[2 i + 1], its
+ * sequences have lengths[i] rows from row_offset[i] on, in regions of capacity[i]
+ * rows, and trees of tree_len[i] nodes (host arrays of device pointers; capacity
+ * and tree_len, or entries of theirs, may be NULL; layers may share tensors).  The
+ * lengths grow by n_accepted (a shared tensor once).  A sequence is refused, its
+ * rows and lengths left as they are in all layers, if one layer refuses it: its
+ * path holds an absent node, or its whole tree does not fit the region or the pool
+ * (the rule by which nwd_kv_append_attn_tree_bounded wrote no rows). */
 int nwd_kv_commit_layers(uint16_t* const* pools, uint32_t n_layers, uint64_t pool_rows,
-                         const int64_t* const* row_offset, const int32_t* const* pos,
+                         const int64_t* const* row_offset, int32_t* const* lengths,
+                         const int32_t* const* capacity, const int32_t* const* tree_len,
                          const int32_t* path, const int32_t* n_accepted, uint32_t batch,
                          uint32_t n_nodes, uint32_t n_kv, uint32_t hd, uint32_t* err,
                          void* stream);

@@ -94,8 +94,8 @@ SIGNATURES = {
                                                        _P, _P, _u32, _u32, _u32, _u32, _u32, _f32,
                                                        _P, _sz, _P, _P]),
     "nwd_verify_tree": (ctypes.c_int, [_P] * 10 + [_u32] * 3 + [_P, _P]),
-    "nwd_kv_commit_layers": (ctypes.c_int, [_P, _u32, _u64, _P, _P, _P, _P, _u32, _u32, _u32, _u32,
-                                            _P, _P]),
+    "nwd_kv_commit_layers": (ctypes.c_int, [_P, _u32, _u64, _P, _P, _P, _P, _P, _P, _u32, _u32,
+                                            _u32, _u32, _P, _P]),
     "nwd_kv_commit": (ctypes.c_int, [_P, _u32, _u64, _P, _P, _P, _P, _u32, _u32, _u32, _u32, _P,
                                      _P]),
     "nwd_mgpu_unique_id": (ctypes.c_int, [_P]),

@@ -280,24 +280,27 @@ PyObject* commit(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
-// The pointers of a list of tensors of one type and shape.
+// The pointers of a list of tensors of one type and shape; nullptr for None where
+// that is allowed.
 template <typename T>
 std::vector<T*> pointers(PyObject* list, const char* name, at::ScalarType type, size_t count,
-                         at::IntArrayRef shape, int dev) {
+                         at::IntArrayRef shape, int dev, bool optional = false) {
   if (!PyList_Check(list) || (size_t)PyList_GET_SIZE(list) != count)
     refuse(PyExc_TypeError, std::string(name) + " must be a list with an entry per layer");
   std::vector<T*> ptrs(count);
-  for (size_t i = 0; i < count; i++)
-    ptrs[i] = pointer<T>(PyList_GET_ITEM(list, (Py_ssize_t)i), name, type, shape, dev);
+  for (size_t i = 0; i < count; i++) {
+    PyObject* o = PyList_GET_ITEM(list, (Py_ssize_t)i);
+    ptrs[i] = optional && o == Py_None ? nullptr : pointer<T>(o, name, type, shape, dev);
+  }
   return ptrs;
 }
 
-// commit_layers(pools (K, V, K, V ..), row_offsets, lengths (lists, an entry per layer), path,
-//               n_accepted, err): 32 layers per launch
+// commit_layers(pools (K, V, K, V ..), row_offsets, lengths, capacities, tree_lens (or None; lists,
+//               an entry per layer), path, n_accepted, err): 32 layers per launch
 PyObject* commit_layers(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-  if (!expect(n_args, 6)) return nullptr;
+  if (!expect(n_args, 8)) return nullptr;
   return guarded([&]() -> PyObject* {
-    const at::Tensor& path = tensor(a[3], "path");
+    const at::Tensor& path = tensor(a[5], "path");
     if (path.dim() != 2)
       refuse(PyExc_ValueError, "path must be [batch, n_nodes], got " + text(path.sizes()));
     const int dev = path.get_device();
@@ -309,18 +312,20 @@ PyObject* commit_layers(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const size_t layers = ptrs.size() / 2;
     const auto off = pointers<const int64_t>(a[1], "row_offset", I64, layers, one, dev);
     const auto len = pointers<int32_t>(a[2], "lengths", I32, layers, one, dev);
-    const auto* pp = pointer<int32_t>(a[3], "path", I32, path.sizes(), dev);
-    const auto* na = pointer<int32_t>(a[4], "n_accepted", I32, one, dev);
-    auto* err = reinterpret_cast<uint32_t*>(number(a[5], "err"));
+    const auto cap = pointers<const int32_t>(a[3], "capacity", I32, layers, one, dev);
+    const auto tree = pointers<const int32_t>(a[4], "tree_len", I32, layers, one, dev, true);
+    const auto* pp = pointer<int32_t>(a[5], "path", I32, path.sizes(), dev);
+    const auto* na = pointer<int32_t>(a[6], "n_accepted", I32, one, dev);
+    auto* err = reinterpret_cast<uint32_t*>(number(a[7], "err"));
     if (batch > 0xffffffffll || n > 0xffffffffll) refuse(PyExc_ValueError, "path is too large");
     if (batch == 0 || n == 0 || layers == 0 || !ptrs[0]) Py_RETURN_NONE;
     const c10::cuda::CUDAGuard on(dev);
     void* stream = c10::cuda::getCurrentCUDAStream(dev).stream();
     for (size_t i = 0; i < layers; i += 32)
       check(nwd_kv_commit_layers(ptrs.data() + 2 * i, (uint32_t)std::min<size_t>(32, layers - i),
-                                 (uint64_t)shape[0], off.data() + i, len.data() + i, pp, na,
-                                 (uint32_t)batch, (uint32_t)n, (uint32_t)shape[1],
-                                 (uint32_t)shape[2], err, stream));
+                                 (uint64_t)shape[0], off.data() + i, len.data() + i,
+                                 cap.data() + i, tree.data() + i, pp, na, (uint32_t)batch,
+                                 (uint32_t)n, (uint32_t)shape[1], (uint32_t)shape[2], err, stream));
     Py_RETURN_NONE;
   });
 }

@@ -28,10 +28,14 @@ struct Args {
   uint4* pools[POOLS];
   const int64_t* row_offset[LAYERS];
   const int32_t* pos[LAYERS];
+  const int32_t* capacity[LAYERS];  // or nullptr: the pool alone bounds a region
+  const int32_t* tree_len[LAYERS];  // or nullptr: all nodes are present
+  int32_t* lengths[LAYERS];         // what grows: pos, once where layers share it
   const int32_t* path;
   const int32_t* n_accepted;
   uint64_t pool_rows;
   uint32_t n_layers, pools_per_layer, batch, n_nodes, row_vec;
+  bool whole_tree;  // the region has to hold the whole tree, not just the path
   uint32_t* err;
 };
 using OnePlace = Args<MAX_POOLS, 1>;
@@ -40,26 +44,30 @@ using OwnPlaces = Args<2 * MAX_LAYERS, MAX_LAYERS>;
 // A sequence's move, as a warp has it: lane l holds nodes l and l + 32 of the
 // path, and layer l's place.
 struct Move {
-  int32_t n, lo, hi, pos;
+  int32_t n, lo, hi, pos, capacity, tree_len;
   int64_t off;
 };
 template <typename A>
 __device__ __forceinline__ Move load_move(const A& a, uint32_t b) {
   const uint32_t lane = threadIdx.x & 31;
   const int32_t* path = a.path + (uint64_t)b * a.n_nodes;
-  Move m{a.n_accepted[b], -1, -1, 0, 0};
+  Move m{a.n_accepted[b], -1, -1, 0, 0x7fffffff, (int32_t)a.n_nodes, 0};
   if (lane < a.n_nodes) m.lo = path[lane];
   if (lane + 32 < a.n_nodes) m.hi = path[lane + 32];
   if (lane < a.n_layers) {
     m.pos = a.pos[lane][b];
     m.off = a.row_offset[lane][b];
+    if (a.capacity[lane]) m.capacity = a.capacity[lane][b];
+    if (a.tree_len[lane]) m.tree_len = a.tree_len[lane][b];
   }
   return m;
 }
 
 // What speaks against a move, for the whole warp (error bits; 0:
 // nothing): a path that does not ascend or leaves the tree, or rows outside the
-// pool in any of the layers, which a lane each looks at.
+// pool or the region in any of the layers, which a lane each looks at.  With
+// whole_tree the rows are those that the attention asked for, so a tree that it
+// refused, and whose rows it did not write, is refused here too.
 template <typename A>
 __device__ __forceinline__ uint32_t refusal(const A& a, const Move& p) {
   const uint32_t all = 0xffffffffu, lane = threadIdx.x & 31;
@@ -73,10 +81,16 @@ __device__ __forceinline__ uint32_t refusal(const A& a, const Move& p) {
   if (__any_sync(all, bad)) return NWD_DEVERR_TREE;
   if (p.n == 0) return 0;
   const uint32_t at = (uint32_t)p.n - 1;
-  const uint64_t rows = (uint64_t)__shfl_sync(all, at < 32 ? p.lo : p.hi, (int)(at & 31)) + 1;
+  uint32_t rows = (uint32_t)__shfl_sync(all, at < 32 ? p.lo : p.hi, (int)(at & 31)) + 1;
+  if (a.whole_tree) {
+    const uint32_t nodes = min((uint32_t)max(p.tree_len, 0), a.n_nodes);
+    if (__any_sync(all, lane < a.n_layers && rows > nodes)) return NWD_DEVERR_TREE;
+    rows = nodes;
+  }
   const bool out = lane < a.n_layers &&
                    (p.off < 0 || p.pos < 0 || (uint64_t)p.off > a.pool_rows ||
-                    (uint64_t)p.pos + rows > a.pool_rows - (uint64_t)p.off);
+                    (uint64_t)p.pos + rows > a.pool_rows - (uint64_t)p.off ||
+                    (int64_t)p.pos + rows > p.capacity);
   return __any_sync(all, out) ? NWD_DEVERR_ROW_RANGE : 0u;
 }
 
@@ -106,6 +120,20 @@ __global__ void __launch_bounds__(THREADS) kv_commit_kernel(const __grid_constan
     for (int i = 0; i < AHEAD; i++)
       if (mine && j0 + i < p.n && from[i] != j0 + i) col[(uint64_t)(j0 + i) * a.row_vec] = x[i];
   }
+}
+
+// The lengths that grow by what was accepted, behind the moves: a warp per
+// sequence, a lane per layer.  A launch of its own, because every block of the
+// moves reads the lengths.
+constexpr uint32_t GROW_THREADS = 128;
+__global__ void __launch_bounds__(GROW_THREADS)
+    kv_commit_lengths_kernel(const __grid_constant__ OwnPlaces a) {
+  nwd::pdl_wait();
+  const uint32_t b = (blockIdx.x * GROW_THREADS + threadIdx.x) / 32, lane = threadIdx.x & 31;
+  if (b >= a.batch) return;
+  const Move p = load_move(a, b);
+  if (refusal(a, p)) return;
+  if (lane < a.n_layers && a.lengths[lane]) a.lengths[lane][b] = p.pos + p.n;
 }
 
 // The arguments that both calls have, checked in the order that their errors have.
@@ -173,15 +201,16 @@ extern "C" int nwd_kv_commit(uint16_t* const* pools, uint32_t n_pools, uint64_t 
 }
 
 extern "C" int nwd_kv_commit_layers(uint16_t* const* pools, uint32_t n_layers, uint64_t pool_rows,
-                                    const int64_t* const* row_offset, const int32_t* const* pos,
+                                    const int64_t* const* row_offset, int32_t* const* lengths,
+                                    const int32_t* const* capacity, const int32_t* const* tree_len,
                                     const int32_t* path, const int32_t* n_accepted, uint32_t batch,
                                     uint32_t n_nodes, uint32_t n_kv, uint32_t hd, uint32_t* err,
                                     void* stream) {
   const char* who = "nwd_kv_commit_layers";
   if (n_layers > MAX_LAYERS)
     return fail(NWD_ERR_INVALID, "%s: %u layers (at most %u)", who, n_layers, MAX_LAYERS);
-  bool null = !path || !n_accepted || (n_layers && (!row_offset || !pos));
-  for (uint32_t i = 0; !null && i < n_layers; i++) null = !row_offset[i] || !pos[i];
+  bool null = !path || !n_accepted || (n_layers && (!row_offset || !lengths));
+  for (uint32_t i = 0; !null && i < n_layers; i++) null = !row_offset[i] || !lengths[i];
   int st = check_commit(who, null, pools, 2 * n_layers, 2 * MAX_LAYERS, batch, n_nodes, n_kv, hd);
   if (st) return st;
   if (batch == 0 || n_layers == 0 || n_nodes == 0) return ok();
@@ -190,8 +219,13 @@ extern "C" int nwd_kv_commit_layers(uint16_t* const* pools, uint32_t n_layers, u
     a.pools[2 * i] = reinterpret_cast<uint4*>(pools[2 * i]);
     a.pools[2 * i + 1] = reinterpret_cast<uint4*>(pools[2 * i + 1]);
     a.row_offset[i] = row_offset[i];
-    a.pos[i] = pos[i];
+    a.pos[i] = a.lengths[i] = lengths[i];
+    for (uint32_t j = 0; j < i; j++)
+      if (lengths[j] == lengths[i]) a.lengths[i] = nullptr;
+    a.capacity[i] = capacity ? capacity[i] : nullptr;
+    a.tree_len[i] = tree_len ? tree_len[i] : nullptr;
   }
+  a.whole_tree = true;
   a.path = path;
   a.n_accepted = n_accepted;
   a.pool_rows = pool_rows;
@@ -201,5 +235,11 @@ extern "C" int nwd_kv_commit_layers(uint16_t* const* pools, uint32_t n_layers, u
   a.n_nodes = n_nodes;
   a.row_vec = (uint32_t)((uint64_t)n_kv * hd / 8);
   a.err = err;
-  return launch_commit(who, a, 2 * n_layers, (cudaStream_t)stream);
+  st = launch_commit(who, a, 2 * n_layers, (cudaStream_t)stream);
+  if (st) return st;
+  const cudaError_t e =
+      launch_pdl(kv_commit_lengths_kernel, dim3((batch + GROW_THREADS / 32 - 1) / (GROW_THREADS / 32)),
+                 dim3(GROW_THREADS), 0, (cudaStream_t)stream, a);
+  if (e != cudaSuccess) return cuda_fail(e, who);
+  return ok();
 }

@@ -188,6 +188,7 @@ class BatchedDecodeAttention:
         self.region_rows = caps.clamp(max=2**31 - 1).to(torch.int32).to(self.device)
         self.workspace = ops.Workspace(self.batch, heads, kv_heads, head_dim, self.device)
         self.scratch = ops.Scratch(self.device)  # device errors of the speculative calls
+        self.tree_len = None  # the last tree_step's, until it is committed
 
     def step(self, q, k_new, v_new, out=None, stream=None) -> torch.Tensor:
         """Every sequence appends one row and attends over its rows (fused launch)."""
@@ -206,22 +207,26 @@ class BatchedDecodeAttention:
         """A speculative step: the trees' K/V rows go behind every sequence's rows and each
         node attends the rows, its ancestors and itself.  q [B, N, heads, hd], k_new / v_new
         [B, N, kv_heads, hd], parents [B, N] (:func:`ops.attention_tree`).  The lengths stay
-        until :meth:`commit`.  A sequence's capacity has to hold its tree too: one whose does
-        not writes nothing, gets zeros, and is recorded in ``scratch`` (a device error)."""
+        until :meth:`commit`, which reads tree_len again.  A sequence's capacity has to hold its
+        tree too: one whose does not writes nothing, gets zeros, and is recorded in ``scratch``
+        (a device error)."""
         if stream is not None:
             with ops._on(stream, self.device):
                 return self.tree_step(q, k_new, v_new, parents, tree_len, out)
         if out is None:
             out = torch.empty(q.shape, dtype=torch.float16, device=self.device)
-        return ops.kv_append_attention_tree(q, k_new, v_new, self.k_pool, self.v_pool,
-                                            self.row_offset, self.lengths, parents, out,
-                                            self.heads, self.kv_heads, self.head_dim,
-                                            tree_len=tree_len, scale=self.scale,
-                                            scratch=self.scratch, capacity=self.region_rows)
+        ops.kv_append_attention_tree(q, k_new, v_new, self.k_pool, self.v_pool, self.row_offset,
+                                     self.lengths, parents, out, self.heads, self.kv_heads,
+                                     self.head_dim, tree_len=tree_len, scale=self.scale,
+                                     scratch=self.scratch, capacity=self.region_rows)
+        self.tree_len = tree_len
+        return out
 
     def commit(self, path, n_accepted, stream=None) -> None:
         """Keeps the accepted nodes of the last :meth:`tree_step` (:func:`ops.verify_tree`'s
-        path and n_accepted): their rows follow the context and the lengths grow by them."""
+        path and n_accepted): their rows follow the context and the lengths grow by them.
+        A sequence whose tree did not fit, or whose path is not one of its tree, keeps its
+        rows and its length; ``scratch`` records it."""
         commit_layers([self], path, n_accepted, stream=stream)
 
     def attend(self, q, out=None, stream=None) -> torch.Tensor:
@@ -236,7 +241,8 @@ class BatchedDecodeAttention:
 def commit_layers(layers, path, n_accepted, stream=None) -> None:
     """:meth:`BatchedDecodeAttention.commit` for the layers of one model (every layer has run
     the step's trees): the rows of all of them move in one launch per 32 layers, each layer's
-    at its own offsets and lengths."""
+    at its own offsets and lengths, and a second one lets the lengths grow.  A sequence that
+    one layer refuses stays as it is in all of them; the first layer's ``scratch`` records it."""
     layers = list(layers)
     if not layers:
         return
@@ -244,5 +250,5 @@ def commit_layers(layers, path, n_accepted, stream=None) -> None:
         with ops._on(stream, layers[0].lengths.device):
             return commit_layers(layers, path, n_accepted)
     ops._kv_commit_layers(layers, path, n_accepted, layers[0].scratch)
-    for lengths in {layer.lengths.data_ptr(): layer.lengths for layer in layers}.values():
-        lengths += n_accepted  # (layers may share one tensor)
+    for layer in layers:
+        layer.tree_len = None

@@ -486,11 +486,12 @@ def kv_commit(pools, row_offset, pos, path, n_accepted, scratch: Scratch | None 
 
 
 def _kv_commit_layers(layers, path, n_accepted, scratch):
-    """:func:`kv_commit` for K and V of several layers, each at its own offsets and lengths
-    (:func:`engine.commit_layers`), 32 layers per launch."""
+    """:func:`kv_commit` for K and V of several layers, each at its own offsets and lengths,
+    which grow (:func:`engine.commit_layers`), 32 layers per launch."""
     _lib.torch_calls().commit_layers(
         [p for layer in layers for p in (layer.k_pool, layer.v_pool)],
-        [layer.row_offset for layer in layers], [layer.lengths for layer in layers], path,
+        [layer.row_offset for layer in layers], [layer.lengths for layer in layers],
+        [layer.region_rows for layer in layers], [layer.tree_len for layer in layers], path,
         n_accepted, scratch.ptr)
 
 

@@ -19,12 +19,12 @@ Q = ctypes.c_void_p(512)
 def test_commit_layers_refusals(L):
     lib = L.load()
 
-    def call(pools=(256, 512, 768, 1024), n_layers=None, off=(256, 256), pos=(256, 256), path=P,
-             acc=P, b=1, n=4, nkv=2, hd=128):
+    def call(pools=(256, 512, 768, 1024), n_layers=None, off=(256, 256), pos=(256, 256), cap=None,
+             tree=None, path=P, acc=P, b=1, n=4, nkv=2, hd=128):
         arr = lambda x: None if x is None else (ctypes.c_void_p * max(1, len(x)))(*x)  # noqa: E731
         layers = len(pools) // 2 if n_layers is None else n_layers
-        return lib.nwd_kv_commit_layers(arr(pools), layers, 100, arr(off), arr(pos), path, acc, b,
-                                        n, nkv, hd, None, None)
+        return lib.nwd_kv_commit_layers(arr(pools), layers, 100, arr(off), arr(pos), arr(cap),
+                                        arr(tree), path, acc, b, n, nkv, hd, None, None)
 
     for kw in (dict(off=None), dict(pos=None), dict(path=None), dict(acc=None), dict(pools=None, n_layers=2),
                dict(off=(256, None)), dict(pos=(None, 256)), dict(pools=(256, 512, None, 768)),
@@ -34,7 +34,8 @@ def test_commit_layers_refusals(L):
         assert lib.nwd_last_error()
     for kw in (dict(pools=(256, 264, 512, 768)), dict(nkv=1, hd=4), dict(n=65), dict(b=65536)):
         assert call(**kw) == L.NWD_ERR_UNSUPPORTED, kw
-    for kw in (dict(pools=(), off=None, pos=None), dict(b=0), dict(n=0)):
+    for kw in (dict(pools=(), off=None, pos=None), dict(b=0), dict(n=0),
+               dict(b=0, cap=(256, None), tree=(None, 256))):
         assert call(**kw) == L.NWD_OK, kw
 
 
