@@ -433,8 +433,9 @@ int nwd_attn_prefill(const uint16_t* q, const uint16_t* k_pool, const uint16_t* 
  *
  * A tree: parents [batch, n_nodes] (device int32), parents[b, i] < i, -1 for a
  * root; n_nodes at most 64.  tree_len (device int32[batch], may be NULL: all):
- * sequence b has tree_len[b] nodes, the rest are absent.  Node i's K/V row is
- * pool row row_offset[b] + seq_len[b] + i: behind the context rows.
+ * sequence b has tree_len[b] nodes, the rest are absent (their parents may be
+ * anything).  Node i's K/V row is pool row row_offset[b] + seq_len[b] + i: behind
+ * the context rows.
  *
  * err: a device word (may be NULL) that receives NWD_DEVERR_* bits; zero it
  * once (any workspace's first word serves: nwd_workspace_check reads it).  A

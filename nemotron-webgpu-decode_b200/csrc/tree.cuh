@@ -29,8 +29,9 @@ static __device__ __forceinline__ uint64_t tree_mask(const int32_t* parents, int
   return m;
 }
 
-// The rows that each node sees, for a warp whose lane i has the parents of nodes
-// i and i + 32 (-1 for those past n): seen[0] is node i's, seen[1] node i + 32's.
+// The rows that each of n nodes sees, for a warp whose lane i has the parents of
+// nodes i and i + 32 (anything for those past n): seen[0] is node i's, seen[1]
+// node i + 32's.
 // The lanes walk up in doubling steps, so a chain takes as many as the logarithm
 // of its depth.
 static __device__ __forceinline__ void tree_closure(int2 par, uint32_t n, uint32_t* err,

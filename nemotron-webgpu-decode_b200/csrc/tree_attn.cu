@@ -586,7 +586,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 // The rows of the tree that `node` sees (its ancestors and itself), from the
-// parents of all nodes: lane i has those of nodes i and i + 32.
+// parents of its n nodes: lane i has those of nodes i and i + 32.
 __device__ uint64_t tree_masks(int2 par, uint32_t n, uint32_t node, uint32_t* err) {
   uint64_t seen[2];
   nwd::tree_closure(par, n, err, seen);
@@ -970,7 +970,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (warp_used) {
           if (tail && !have_mask) {
             have_mask = true;
-            const uint64_t all = tree_masks(par, p.n_nodes, node, c.err);
+            const uint64_t all = tree_masks(par, d.nodes, node, c.err);
             sees = row_used && node < d.nodes ? all : 0;
           }
           // The exponentials are taken against the maximum so far, beside the

@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_short_kernel(const __grid_con
     *reinterpret_cast<uint4*>(vs + sw_off(i >> 4, i & 15)) = make_uint4(0u, 0u, 0u, 0u);
   if (warp == WARPS - 1) {
     uint64_t seen[2];
-    nwd::tree_closure(par, p.n_nodes, blockIdx.x == 0 ? p.err : nullptr, seen);
+    nwd::tree_closure(par, seq.nodes, blockIdx.x == 0 ? p.err : nullptr, seen);
     s.sees[lane] = lane < seq.nodes ? seen[0] : 0;
     s.sees[lane + 32] = lane + 32 < seq.nodes ? seen[1] : 0;
     if (lane < 2) s.bad[lane] = 0;
