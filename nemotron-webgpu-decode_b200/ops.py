@@ -396,12 +396,25 @@ def _tree_ws_bytes(device: int, *shape) -> int:
     return int(v.value)
 
 
+def _on_device(name, thing, device):
+    """Refuses a stream, workspace or scratch of another device than the tensors'."""
+    own = getattr(thing, "device", None)
+    if own is None or not isinstance(device, torch.device):
+        return
+    if device.index is None:
+        device = torch.device(device.type, torch.cuda.current_device())
+    if own != device:
+        raise ValueError(f"the {name} is on {own}, the tensors on {device}")
+
+
 def _on(stream, device):
     """A context in which `stream` (a torch stream or a raw handle) is PyTorch's current one:
     the speculative calls run on the current stream of their tensors' device, and what they
-    allocate belongs to it."""
+    allocate belongs to it.  So a stream of another device is refused: the call would run on
+    whatever stream is current on its own."""
     if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
+    _on_device("stream", stream, device)
     return torch.cuda.stream(stream)
 
 

@@ -1,0 +1,49 @@
+"""Streams and workspaces of another device are refused (runs without a GPU:
+what is asked is the host's check, before any CUDA call)."""
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+ONE = torch.device("cuda", 1)
+
+
+class OnZero:
+    """A tensor of cuda:0, as far as these checks look."""
+    device = torch.device("cuda", 0)
+    lengths = row_offset = k_pool = v_pool = None
+
+
+def calls(ops, engine_mod):
+    t = OnZero()
+    return [
+        lambda **kw: ops.attention_tree(t, t, t, t, t, t, t, 8, 2, **kw),
+        lambda **kw: ops.kv_append_attention_tree(t, t, t, t, t, t, t, t, t, 8, 2, **kw),
+        lambda **kw: ops.verify_tree(t, t, t, t, t, **kw),
+        lambda **kw: ops.kv_commit([t], t, t, t, t, **kw),
+    ]
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_streams_of_another_device(ops, engine_mod, i):
+    other = SimpleNamespace(cuda_stream=1234, device=ONE)
+    with pytest.raises(ValueError, match="stream is on cuda:1"):
+        calls(ops, engine_mod)[i](stream=other)
+
+
+def test_streams_of_another_device_in_the_engine(ops, engine_mod):
+    other = SimpleNamespace(cuda_stream=1234, device=ONE)
+    layer = SimpleNamespace(lengths=OnZero(), device=OnZero.device)
+    with pytest.raises(ValueError, match="stream is on cuda:1"):
+        engine_mod.commit_layers([layer], OnZero(), OnZero(), stream=other)
+    with pytest.raises(ValueError, match="stream is on cuda:1"):
+        engine_mod.BatchedDecodeAttention.tree_step(layer, None, None, None, None, stream=other)
+
+
+@pytest.mark.parametrize("i", range(2))
+def test_workspace_of_another_device(ops, engine_mod, i):
+    ws = SimpleNamespace(ptr=4096, nbytes=1 << 30, device=ONE)
+    with pytest.raises(ValueError, match="workspace is on cuda:1"):
+        calls(ops, engine_mod)[i](workspace=ws)
