@@ -264,6 +264,7 @@ class Scratch:
         device = torch.device(device) if device is not None else torch.device(
             "cuda", torch.cuda.current_device())
         self._buf = torch.zeros(512, dtype=torch.uint8, device=device)
+        self.device = self._buf.device
         self.ptr = (self._buf.data_ptr() + 255) // 256 * 256
         self.nbytes = 256
 
@@ -407,6 +408,14 @@ def _on_device(name, thing, device):
         raise ValueError(f"the {name} is on {own}, the tensors on {device}")
 
 
+def _err(scratch, tensor) -> int:
+    """The error word of a call on `tensor`'s device."""
+    if scratch is None:
+        return 0
+    _on_device("scratch", scratch, getattr(tensor, "device", None))
+    return scratch.ptr
+
+
 def _on(stream, device):
     """A context in which `stream` (a torch stream or a raw handle) is PyTorch's current one:
     the speculative calls run on the current stream of their tensors' device, and what they
@@ -426,12 +435,11 @@ def _tree(q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_he
                          n_kv_heads, head_dim, tree_len, scale, workspace, scratch, None, capacity)
     ptr, nbytes = 0, 0
     if workspace is not None:
-        if workspace.device != q.device:
-            raise ValueError(f"the workspace is on {workspace.device}, q on {q.device}")
+        _on_device("workspace", workspace, getattr(q, "device", None))
         ptr, nbytes = workspace.ptr, workspace.nbytes
     (_lib._torch or _lib.torch_calls()).tree(
         q, k_new, v_new, k_pool, v_pool, row_offset, seq_len, parents, o, n_heads, n_kv_heads,
-        head_dim, tree_len, scale, ptr, nbytes, 0 if scratch is None else scratch.ptr, capacity)
+        head_dim, tree_len, scale, ptr, nbytes, _err(scratch, q), capacity)
     return o
 
 
@@ -480,7 +488,7 @@ def verify_tree(tokens, parents, target_probs, u, w, draft_probs=None, tree_len=
     path, n_accepted, next_token = (None, None, None) if out is None else out
     return (_lib._torch or _lib.torch_calls()).verify(
         tokens, parents, tree_len, target_probs, draft_probs, u, w, path, n_accepted, next_token,
-        0 if scratch is None else scratch.ptr)
+        _err(scratch, target_probs))
 
 
 def kv_commit(pools, row_offset, pos, path, n_accepted, scratch: Scratch | None = None,
@@ -495,7 +503,7 @@ def kv_commit(pools, row_offset, pos, path, n_accepted, scratch: Scratch | None 
             return kv_commit(pools, row_offset, pos, path, n_accepted, scratch)
     (_lib._torch or _lib.torch_calls()).commit(
         pools if type(pools) is list else list(pools), row_offset, pos, path, n_accepted,
-        0 if scratch is None else scratch.ptr)
+        _err(scratch, path))
 
 
 def _kv_commit_layers(layers, path, n_accepted, scratch):
@@ -505,7 +513,7 @@ def _kv_commit_layers(layers, path, n_accepted, scratch):
         [p for layer in layers for p in (layer.k_pool, layer.v_pool)],
         [layer.row_offset for layer in layers], [layer.lengths for layer in layers],
         [layer.region_rows for layer in layers], [layer.tree_len for layer in layers], path,
-        n_accepted, scratch.ptr)
+        n_accepted, _err(scratch, path))
 
 
 def selftest_wait_timeout(workspace: "Workspace", stream=None) -> int:

@@ -1,4 +1,4 @@
-"""Streams and workspaces of another device are refused (runs without a GPU:
+"""Streams, scratch words and workspaces of another device are refused (runs without a GPU:
 what is asked is the host's check, before any CUDA call)."""
 from __future__ import annotations
 
@@ -40,6 +40,13 @@ def test_streams_of_another_device_in_the_engine(ops, engine_mod):
         engine_mod.commit_layers([layer], OnZero(), OnZero(), stream=other)
     with pytest.raises(ValueError, match="stream is on cuda:1"):
         engine_mod.BatchedDecodeAttention.tree_step(layer, None, None, None, None, stream=other)
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_scratch_of_another_device(ops, engine_mod, i):
+    scratch = SimpleNamespace(ptr=4096, nbytes=256, device=ONE)
+    with pytest.raises(ValueError, match="scratch is on cuda:1"):
+        calls(ops, engine_mod)[i](scratch=scratch)
 
 
 @pytest.mark.parametrize("i", range(2))
