@@ -400,8 +400,8 @@ def _tree_ws_bytes(device: int, *shape) -> int:
 def _on_device(name, thing, device):
     """Refuses a stream, workspace or scratch of another device than the tensors'."""
     own = getattr(thing, "device", None)
-    if own is None or not isinstance(device, torch.device):
-        return
+    if own is None or own.index is None or not isinstance(device, torch.device):
+        return  # (a workspace made for "cuda" does not say which)
     if device.index is None:
         device = torch.device(device.type, torch.cuda.current_device())
     if own != device:

@@ -49,6 +49,14 @@ def test_scratch_of_another_device(ops, engine_mod, i):
         calls(ops, engine_mod)[i](scratch=scratch)
 
 
+@pytest.mark.parametrize("i", range(4))
+def test_scratch_that_does_not_say_its_device(ops, engine_mod, i):
+    """A decode workspace made for "cuda" serves as scratch: the call goes on to its tensors."""
+    scratch = SimpleNamespace(ptr=4096, nbytes=256, device=torch.device("cuda"))
+    with pytest.raises(TypeError, match="must be a torch.Tensor"):
+        calls(ops, engine_mod)[i](scratch=scratch)
+
+
 @pytest.mark.parametrize("i", range(2))
 def test_workspace_of_another_device(ops, engine_mod, i):
     ws = SimpleNamespace(ptr=4096, nbytes=1 << 30, device=ONE)
