@@ -507,6 +507,7 @@ int nwd_kv_append_attn_tree_bounded(const uint16_t* q, const uint16_t* k_new, co
  *   path        : int32 [batch, n_nodes], the accepted nodes from node 0 on,
  *                 then -1; n_accepted: int32 [batch] (node 0 counts)
  *   next_token  : int32 [batch]; -1 if the row holds no positive number
+ * The three outputs must not overlap each other or anything that is read.
  * Probabilities that are not above zero (NaN too) count as zero.  A sequence
  * without nodes gets n_accepted 0 and next_token -1.  A token outside
  * [0, vocab) is never accepted (NWD_DEVERR_TREE). */

@@ -39,6 +39,17 @@ int kv_tensor_map(CUtensorMap* out, const void* base, uint64_t rows, uint32_t n_
 int tree_q_tensor_map(CUtensorMap* out, const void* base, uint64_t nodes, uint32_t n_kv,
                       uint32_t group, uint32_t box_nodes);
 
+// Memory that a call reads or writes; none where p is nullptr or bytes 0.
+struct Span {
+  const char* name;
+  const void* p;
+  uint64_t bytes;
+};
+inline bool overlap(const Span& a, const Span& b) {
+  const uint64_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---- decode of one short sequence (decode_short.cu) ----

@@ -526,6 +526,26 @@ extern "C" int nwd_verify_tree(const int32_t* tokens, const int32_t* parents,
   if (vocab > 0x7fffffffu) return fail(NWD_ERR_UNSUPPORTED, "%s: vocabulary %u", who, vocab);
   if (batch > 65535u) return fail(NWD_ERR_UNSUPPORTED, "%s: batch > 65535", who);
   if (batch == 0) return ok();
+  // The CTAs of a cluster walk the tree each for itself, on the same numbers: an
+  // output written over an input that another CTA has yet to read would let them
+  // part ways.
+  const uint64_t each = (uint64_t)batch * 4, nodes = each * n_nodes;
+  const Span span[] = {{"path", path, nodes},
+                       {"n_accepted", n_accepted, each},
+                       {"next_token", next_token, each},
+                       {"tokens", tokens, nodes},
+                       {"parents", parents, nodes},
+                       {"tree_len", tree_len, each},
+                       {"target_probs", target_probs, nodes * vocab},
+                       {"draft_probs", draft_probs, nodes * vocab},
+                       {"u", u, nodes},
+                       {"w", w, each},
+                       {"err", err, 4}};
+  for (uint32_t i = 0; i < 3; i++)
+    for (uint32_t j = i + 1; j < sizeof(span) / sizeof(span[0]); j++)
+      if (overlap(span[i], span[j]))
+        return fail(NWD_ERR_INVALID, "%s: %s and %s must not overlap", who, span[i].name,
+                    span[j].name);
   DeviceInfo di;
   int st = current_device_info(&di);
   if (st) return st;

@@ -480,7 +480,8 @@ def verify_tree(tokens, parents, target_probs, u, w, draft_probs=None, tree_len=
     tokens / parents [B, N] int32, node 0 the pending token; target_probs [B, N, V] f32 (row
     i: the target behind node i); draft_probs of the same shape (row i: what node i's
     children were drawn from) or None for drafts without probabilities; u [B, N], w [B] f32
-    uniforms in [0, 1).  `out`: the three outputs, to be written in place."""
+    uniforms in [0, 1).  `out`: the three outputs, to be written in place (memory of their
+    own: none may overlap another or an input)."""
     if stream is not None:
         with _on(stream, target_probs.device):
             return verify_tree(tokens, parents, target_probs, u, w, draft_probs, tree_len, out,
