@@ -454,9 +454,10 @@ int nwd_attn_tree_workspace_size(uint32_t batch, uint32_t n_nodes, uint32_t n_he
  *   q, o          : [batch, n_nodes, n_heads, head_dim]; absent nodes' o = 0
  *   k_pool, v_pool: [pool_rows, n_kv_heads, head_dim], the nodes' rows in place
  *   row_offset    : device int64[batch]; seq_len: device int32[batch]
- * head_dim 128, group 1..8, batch <= 4096; tensors 16-byte aligned, o apart from
- * the others.  Rows that a node does not attend never reach its output, whatever
- * they hold. */
+ * head_dim 128, group 1..8, batch <= 4096; tensors 16-byte aligned.  Neither o nor
+ * the workspace may overlap anything else (NWD_ERR_INVALID; err may be a word of
+ * the workspace's first 256 bytes).  Rows that a node does not attend never reach
+ * its output, whatever they hold. */
 int nwd_attn_tree(const uint16_t* q, const uint16_t* k_pool, const uint16_t* v_pool,
                   uint64_t pool_rows, const int64_t* row_offset, const int32_t* seq_len,
                   const int32_t* parents, const int32_t* tree_len, uint16_t* o, uint32_t batch,
@@ -464,8 +465,9 @@ int nwd_attn_tree(const uint16_t* q, const uint16_t* k_pool, const uint16_t* v_p
                   float scale, void* workspace, size_t ws_bytes, uint32_t* err, void* stream);
 
 /* The same after writing the present nodes' rows k_new / v_new ([batch, n_nodes,
- * n_kv_heads, head_dim]) into the pools (bit-exact).  Sequences of one call must
- * not share the rows that they write, and the pools must be two. */
+ * n_kv_heads, head_dim], apart from the pools) into the pools (bit-exact).
+ * Sequences of one call must not share the rows that they write, and the pools
+ * must not overlap. */
 int nwd_kv_append_attn_tree(const uint16_t* q, const uint16_t* k_new, const uint16_t* v_new,
                             uint16_t* k_pool, uint16_t* v_pool, uint64_t pool_rows,
                             const int64_t* row_offset, const int32_t* pos, const int32_t* parents,

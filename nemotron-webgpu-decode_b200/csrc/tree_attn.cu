@@ -1394,6 +1394,20 @@ Tiling tiling(uint32_t n_nodes, uint32_t group, bool lengths) {
   return t;
 }
 
+// What a call reads and writes, as it may not overlap: o, and the workspace, with
+// nothing else.  The planners read lengths and offsets while other CTAs write o
+// and partials; a length that changed under them could leave a search for a
+// sequence without an end, a join descriptor that did would send its rows
+// anywhere.
+struct Spans {
+  enum { O, V_POOL, K_POOL, COUNT = 11 };
+  nwd::Span at[COUNT];
+};
+int refuse_overlap(const char* who, const nwd::Span& a, const nwd::Span& b) {
+  if (!nwd::overlap(a, b)) return NWD_OK;
+  return nwd::fail(NWD_ERR_INVALID, "%s: %s and %s must not overlap", who, a.name, b.name);
+}
+
 // Checks the workspace, then launches the append (when there are new rows),
 // the attention and the join of its partials.
 int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const uint16_t* v_pool,
@@ -1410,8 +1424,26 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
     return fail(NWD_ERR_WORKSPACE, "%s: the workspace is NULL or not 256-byte aligned", who);
   if (ws_bytes < ws_total(1, t.unit_tiles))
     return fail(NWD_ERR_WORKSPACE, "%s: a workspace of %zu bytes is too small", who, ws_bytes);
+  const uint64_t nodes = (uint64_t)batch * n_nodes, row = (uint64_t)n_kv * head_dim * 2;
+  const Spans spans = {{{"o", o, nodes * n_heads * head_dim * 2},
+                        {"v_pool", v_pool, pool_rows * row},
+                        {"k_pool", k_pool, pool_rows * row},
+                        {"q", q, nodes * n_heads * head_dim * 2},
+                        {"k_new", k_new, nodes * row},
+                        {"v_new", v_new, nodes * row},
+                        {"row_offset", row_offset, (uint64_t)batch * 8},
+                        {"lengths", seq_len, (uint64_t)batch * 4},
+                        {"parents", parents, nodes * 4},
+                        {"tree_len", tree_len, (uint64_t)batch * 4},
+                        {"capacity", capacity, (uint64_t)batch * 4}}};
+  int st = NWD_OK;
+  for (uint32_t i = 1; i < Spans::COUNT && !st; i++)
+    st = refuse_overlap(who, spans.at[Spans::O], spans.at[i]);
+  if (!st) st = refuse_overlap(who, spans.at[Spans::O], {"err", err, 4});
+  if (!st && k_new) st = refuse_overlap(who, spans.at[Spans::K_POOL], spans.at[Spans::V_POOL]);
+  if (st) return st;
   DeviceInfo di;
-  int st = current_device_info(&di);
+  st = current_device_info(&di);
   if (st) return st;
   if (di.sm_count > (int)MAX_CTAS)
     return fail(NWD_ERR_UNSUPPORTED, "%s: %d SMs (at most %u)", who, di.sm_count, MAX_CTAS);
@@ -1419,6 +1451,9 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
   if (ws_bytes < need)
     return fail(NWD_ERR_WORKSPACE, "%s: needs a workspace of >= %zu bytes, got %zu", who, need,
                 ws_bytes);
+  for (uint32_t i = 0; i < Spans::COUNT && !st; i++)
+    st = refuse_overlap(who, {"the workspace", workspace, need}, spans.at[i]);
+  if (st) return st;
   const float scale_log2 =
       (scale != 0.f ? scale : 1.0f / sqrtf((float)head_dim)) * 1.4426950408889634f;
   if (tree_short_fits(pool_rows, batch, n_nodes * group))  // one launch, no partials
