@@ -211,7 +211,7 @@ class BatchedDecodeAttention:
         tree too: one whose does not writes nothing, gets zeros, and is recorded in ``scratch``
         (a device error)."""
         if stream is not None:
-            with ops._on(stream, self.device):
+            with ops._on(stream, self.lengths.device):
                 return self.tree_step(q, k_new, v_new, parents, tree_len, out)
         if out is None:
             out = torch.empty(q.shape, dtype=torch.float16, device=self.device)

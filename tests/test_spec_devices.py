@@ -42,6 +42,14 @@ def test_streams_of_another_device_in_the_engine(ops, engine_mod):
         engine_mod.BatchedDecodeAttention.tree_step(layer, None, None, None, None, stream=other)
 
 
+def test_an_engine_made_for_the_device_of_its_day(ops, engine_mod):
+    """An engine made for "cuda" is on the device that was current then."""
+    other = SimpleNamespace(cuda_stream=1234, device=ONE)
+    layer = SimpleNamespace(lengths=OnZero(), device=torch.device("cuda"))
+    with pytest.raises(ValueError, match="stream is on cuda:1, the tensors on cuda:0"):
+        engine_mod.BatchedDecodeAttention.tree_step(layer, None, None, None, None, stream=other)
+
+
 @pytest.mark.parametrize("i", range(4))
 def test_scratch_of_another_device(ops, engine_mod, i):
     scratch = SimpleNamespace(ptr=4096, nbytes=256, device=ONE)
