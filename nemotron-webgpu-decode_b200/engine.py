@@ -214,7 +214,7 @@ class BatchedDecodeAttention:
             with ops._on(stream, self.lengths.device):
                 return self.tree_step(q, k_new, v_new, parents, tree_len, out)
         if out is None:
-            out = torch.empty(q.shape, dtype=torch.float16, device=self.device)
+            out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
         ops.kv_append_attention_tree(q, k_new, v_new, self.k_pool, self.v_pool, self.row_offset,
                                      self.lengths, parents, out, self.heads, self.kv_heads,
                                      self.head_dim, tree_len=tree_len, scale=self.scale,

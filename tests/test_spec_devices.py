@@ -50,6 +50,17 @@ def test_an_engine_made_for_the_device_of_its_day(ops, engine_mod):
         engine_mod.BatchedDecodeAttention.tree_step(layer, None, None, None, None, stream=other)
 
 
+def test_the_output_is_where_the_queries_are(engine_mod, monkeypatch):
+    """Not on the device that is current when the step runs (stand-ins: meta and cpu)."""
+    seen = []
+    monkeypatch.setattr(engine_mod.ops, "kv_append_attention_tree", lambda *a, **kw: seen.append(a[8]))
+    names = "k_pool v_pool row_offset lengths heads kv_heads head_dim scale scratch region_rows"
+    layer = SimpleNamespace(device=torch.device("cpu"), **{n: None for n in names.split()})
+    q = torch.empty(1, 2, 8, 128, dtype=torch.float16, device="meta")
+    out = engine_mod.BatchedDecodeAttention.tree_step(layer, q, None, None, None)
+    assert out is seen[0] and out.device == q.device and out.shape == q.shape
+
+
 @pytest.mark.parametrize("i", range(4))
 def test_scratch_of_another_device(ops, engine_mod, i):
     scratch = SimpleNamespace(ptr=4096, nbytes=256, device=ONE)
