@@ -1377,19 +1377,17 @@ int check_tree(const char* who, const void* q, const void* k_pool, const void* v
   return NWD_OK;
 }
 
-// How a shape's query rows are tiled, in as few tiles of whole nodes as hold
-// them.  Trees of different lengths: as many nodes per tile as fit, so that the
-// short ones need few (16 trees of up to 61 nodes, group 5: 140 us, evenly 156).
-// Trees that are all present: evenly (64 nodes, group 5, 32 768 rows: 66 us,
-// filled up 68.6; 26 nodes, 4 070 rows: 19.6 and 19.3).
+// How a shape's query rows are tiled: as many whole nodes per tile as fit, so that
+// the tiles are few and short trees, where lengths differ, need few of them.
+// Group 5, shared out evenly instead: 16 trees of up to 61 nodes 156 us (160), of
+// up to 26 86 (105), of 26 each 138 (152); 64 nodes over 32 768 rows 82 (86).
 struct Tiling {
   uint32_t tile_nodes, n_tiles, unit_tiles;
 };
-Tiling tiling(uint32_t n_nodes, uint32_t group, bool lengths) {
+Tiling tiling(uint32_t n_nodes, uint32_t group) {
   Tiling t;
   t.tile_nodes = std::min(n_nodes, BM / group);
   t.n_tiles = (n_nodes + t.tile_nodes - 1) / t.tile_nodes;
-  if (!lengths) t.tile_nodes = (n_nodes + t.n_tiles - 1) / t.n_tiles;
   t.unit_tiles = t.n_tiles > 1 ? 2 : 1;
   return t;
 }
@@ -1419,7 +1417,7 @@ int run_tree(const char* who, const uint16_t* q, const uint16_t* k_pool, const u
              const int32_t* capacity = nullptr) {
   using namespace nwd;
   const uint32_t group = n_heads / n_kv;
-  const Tiling t = tiling(n_nodes, group, tree_len != nullptr);
+  const Tiling t = tiling(n_nodes, group);
   if (!workspace || ((uintptr_t)workspace & 255u))
     return fail(NWD_ERR_WORKSPACE, "%s: the workspace is NULL or not 256-byte aligned", who);
   if (ws_bytes < ws_total(1, t.unit_tiles))
@@ -1540,7 +1538,7 @@ int nwd_attn_tree_workspace_size(uint32_t batch, uint32_t n_nodes, uint32_t n_he
   DeviceInfo di;
   st = current_device_info(&di);
   if (st) return st;
-  const Tiling t = tiling(n_nodes ? n_nodes : 1, n_heads / n_kv_heads, false);
+  const Tiling t = tiling(n_nodes ? n_nodes : 1, n_heads / n_kv_heads);
   *bytes = ws_total((uint32_t)di.sm_count, t.unit_tiles);
   return ok();
 }
