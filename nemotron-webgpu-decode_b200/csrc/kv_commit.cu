@@ -9,8 +9,11 @@
 // that a later batch reads): columns are independent, so no thread waits for
 // another.
 //
-// Bound by the rows' bytes, read and written once: 128 sequences, 8 pools, 8 of
-// 64 rows each, 33.6 MB in 5.8 us (5.8 TB/s); one sequence by its launch, 2.5 us.
+// Bound by latency, then by the rows' bytes, read and written once.  128 sequences,
+// 8 pools, 8 of 64 rows each, 33.6 MB: 9.0 us with rows that L2 does not hold (3.7
+// TB/s, where the bytes alone take 5.2: the path, the places and the first rows
+// are loads that wait for one another, and the ninth node is a second round of
+// them); 5.4 us in replays, from L2.  One sequence: its launch, 1.9 us.
 #include "nwd_common.h"
 #include "tree.cuh"
 

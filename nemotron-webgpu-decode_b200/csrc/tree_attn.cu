@@ -50,8 +50,8 @@
 // decode and prefill kernels: one rounding to fp16, 2^-11 of a weight, puts
 // outputs that average out to nearly nothing up to 7 % off, where the decode
 // path keeps 1 %.  Its price, with the remainder's conversions: 64 nodes over
-// 32 768 rows 78 us (one rounding 66), 64 trees of 16 nodes 256 (219), 256
-// chains of 5 1 080 (900, both at the power cap).  A row's largest P lies
+// 32 768 rows 78 us (one rounding 66), 64 trees of 16 nodes 256 (219), sixteen of
+// up to 61 185 (138), 256 chains of 5 1 080 (900).  A row's largest P lies
 // between 2^7 (P_BIAS) and 2^15, and an fp16 step below the normal range is
 // 2^-24: a weight is off by 2^-22 of itself, or by 2^-32 of the largest where
 // that is more.  Sums and accumulators are f32.
@@ -61,17 +61,26 @@
 // (0 x NaN would be NaN), and NaN or infinities in the V rows of the tree are
 // zeroed there too and added at the end to the nodes that see them.
 //
-// Bound by: the cache's bytes while the query rows of a kv head fill one tile in
-// part (256 chains of 5 nodes, group 4: 4.7 GB in 751 us, 6.25 TB/s); with two
-// tiles by the latency of a turn's chain S -> softmax -> P V, about 1.1 us per
-// block and pair of tiles: no unit of the SM is more than 45 % busy then
-// (sixteen trees of up to 61 nodes, group 5: 137 us; tensor pipe 39 %, exponentials
-// 42 %, DRAM 45 %).  Shared memory and tensor memory are full with two groups, so
-// a third turn in flight would need smaller blocks.  Built, measured and not
-// kept (64 nodes over 32 768 rows, 66 us): scores in registers at once with the
-// weights in buffers of their own 69.5; one arrival per warp on the barriers
-// 68.4; a quarter of the exponentials by polynomial 66.4; one issuer per group
-// instead of two cost the 256 chains a third.
+// Bound by (figures here and below are replays of one call, inputs as L2 holds
+// them, unless they say otherwise).  Few query rows: the cache's bytes and, in
+// steady use, the 1 kW power cap: 256 chains of 5 nodes, group 4, 4.7 GB, take 995
+// us after a pause and 1 150 at the 1.46 GHz of the cap (4.1 TB/s; the decode
+// kernel reads the same bytes at 6.8).  An MMA has 128 rows of which these use
+// 20, and the remainder doubles P V, so most of what the tensor pipe (active 53 %
+// of the time) multiplies, and the cap pays for, is padding.  Two tiles: a turn's
+// chain S -> softmax -> P V, 1.2 us per block and pair of tiles at 1.9 GHz.
+// Sixteen trees of up to 61 nodes, group 5, 157 us after a pause, 182 at the cap's
+// 1.59 GHz: tensor pipe active 50 %, issue slots 43 %, exponentials 36 %, DRAM
+// 36 %.  S alone reads 6 KB of operands from shared memory per 32 clocks of
+// multiplication (64 cache rows against 128 query rows), 48 clocks at 128 bytes a
+// clock, so part of the pipe's time is waiting for operands.  Shared memory
+// and tensor memory are full with two groups; a third turn in flight would need
+// smaller blocks, fewer operand bytes per turn larger ones.  Built and measured
+// before the remainder, and not kept (64 nodes over 32 768 rows, then 66 us):
+// scores in registers at once with the weights in buffers of their own 69.5; one
+// arrival per warp on the barriers 68.4; a quarter of the exponentials by
+// polynomial 66.4; one issuer per group instead of two cost the 256 chains a
+// third.
 //
 // All waits are bounded: the planner gives the CTA up after 2 s without
 // progress, records NWD_DEVERR_PIPE_TIMEOUT, and every role lets its copies and
@@ -106,14 +115,14 @@ constexpr uint32_t NQ = 2, NK = 5, NV = 5;  // stages
 constexpr uint32_t NP = 4;              // piece descriptors
 constexpr uint32_t PIECE_USERS = 19;    // warps that read them: all but the planner
 // What a block costs in a unit of one tile, of two (in the same unit of time):
-// 64 nodes over 32 768 rows, three tiles, 65.2 us; as 3 to 5 65.6, 3 to 4 69.0.
+// 64 nodes over 32 768 rows, three tiles, 78.4 us; as 3 to 5 78.3, 3 to 4 81.5.
 constexpr uint32_t COST1 = 1, COST2 = 2;
 // How many blocks' time a unit's beginning and end take: 64 trees of 16 nodes
-// over 512 to 8 192 rows 222 us; with none 230, with twelve 222.
+// over 512 to 8 192 rows 256 us; with none 263, with twelve 259.
 constexpr uint32_t UNIT_BLOCKS = 6;
 // Least part of a unit, of a single sequence: more parts are more partials to
-// join.  8 nodes over 150 rows (three blocks, so one part) 11.9 us, 26 nodes
-// over 4 070 rows 19.5; with 1 block 13.0 and 20.3, with 8 11.9 and 23.0.
+// join.  26 nodes over 4 070 rows 19.4 us; with 1 block 20.4, with 8 23.1; 8
+// nodes over 3 000 rows 16.7, 16.7 and 18.0.
 constexpr uint32_t MIN_BLOCKS = 4;
 
 constexpr uint32_t O_Q = 0;
@@ -364,8 +373,8 @@ __device__ __forceinline__ bool watch(const Ctx& c, int b, uint32_t parity) {
 //
 // One sequence: its units get CTAs in proportion to their costs, each a part of
 // one unit's blocks, so that no CTA has two units' beginnings and ends to wait
-// for (8 nodes over 150 rows 11.9 us, 26 over 4 070 19.5, 64 over 32 768 65.5;
-// cut as a batch 15.0, 21.7, 68.3).
+// for (8 nodes over 3 000 rows 16.7 us, 26 over 4 070 19.4, 64 over 32 768 78.4;
+// cut as a batch 17.6, 21.3, 79.0).
 //
 // A batch: the units make a line, each as long as its blocks' costs and
 // UNIT_BLOCKS more for its beginning and end, which is cut into equal ranges.

@@ -1,5 +1,5 @@
 // Attention for the tree of one short sequence (tree_attn.cu has the formula,
-// the masks and the roundings): the engine's own case, a cache of 256 rows.
+// the masks and the roundings), for instance a cache of the engine's 256 rows.
 //
 // There the general kernel's append, plan, pipeline fill and join are nearly
 // all of its time.  Here a kv head is one CTA of 16 warps, or past 128 pool
@@ -22,8 +22,8 @@
 // Bound by latency: launch, lengths, rows, then S, P and O with a barrier after
 // each (about 1 us a stage at 40 query rows, most of it shared-memory reads).
 // 40/8 heads, with the append, and the general kernel's time: 8 nodes over 150
-// rows 7.0 us (11.7), over 1 000 8.9 (14.1), over 2 000 11.5 (15.4); 12 nodes
-// over 2 000 12.8 (15.6); one node over 150 4.9 (11.2).
+// rows 7.5 us (11.7), over 1 000 9.8 (13.8), over 2 000 12.7 (14.7); 12 nodes
+// over 2 000 14.3 (14.7); one node over 150 5.2 (11.7).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -39,8 +39,9 @@ constexpr uint32_t MAX_ROWS = 64;      // query rows per kv head
 constexpr uint32_t MAX_KEYS = 256;     // cache rows per CTA
 constexpr uint32_t MAX_CLUSTER = 8;    // portable cluster size
 // Up to ONE_KEYS pool rows are one CTA's, more are shared out by CLUSTER_KEYS.  A
-// cluster's launch and barriers cost what 64 rows do: 8 nodes over 120 rows 6.3
-// us in one CTA, 7.0 in a cluster; over 240 8.8 and 7.1; by 32 rows 7.3, by 128 8.7.
+// cluster's launch and barriers cost what 64 rows do: 8 nodes over 120 rows 7.2
+// us in one CTA, 7.4 in a cluster; over 150 8.0 and 7.5; over 240 10.2 and 7.6, by
+// 32 rows 7.9, by 128 9.4.
 constexpr uint32_t ONE_KEYS = 128, CLUSTER_KEYS = 64;
 constexpr float P_BIAS = 15.f;
 static_assert(ONE_KEYS <= MAX_KEYS && MAX_KEYS == WARPS * 16 && HD == WARPS / 2 * 16 && MAX_ROWS * 8 == THREADS, "the warps' shares");
