@@ -457,7 +457,8 @@ int nwd_attn_tree_workspace_size(uint32_t batch, uint32_t n_nodes, uint32_t n_he
  * head_dim 128, group 1..8, batch <= 4096; tensors 16-byte aligned.  Neither o nor
  * the workspace may overlap anything else (NWD_ERR_INVALID; err may be a word of
  * the workspace's first 256 bytes).  Rows that a node does not attend never reach
- * its output, whatever they hold. */
+ * its output, whatever they hold; an infinity in a context row of V comes out as an
+ * infinity or NaN, in a tree row as itself for the nodes that see it. */
 int nwd_attn_tree(const uint16_t* q, const uint16_t* k_pool, const uint16_t* v_pool,
                   uint64_t pool_rows, const int64_t* row_offset, const int32_t* seq_len,
                   const int32_t* parents, const int32_t* tree_len, uint16_t* o, uint32_t batch,
@@ -491,7 +492,8 @@ int nwd_kv_append_attn_tree_bounded(const uint16_t* q, const uint16_t* k_new, co
 /* Which drafted tokens stand, and the next token, from given uniform numbers
  * (multi-round rejection sampling; the reference's counterpart is the argmax of
  * one row, kernels/argmax_partial.wgsl).
- *   tokens      : int32 [batch, n_nodes]; node 0 is the pending token, whose
+ *   tokens      : int32 [batch, n_nodes], n_nodes 1 to 64 (a tree without a
+ *                 pending token is refused); node 0 is the pending token, whose
  *                 own token is not read
  *   target_probs: f32 [batch, n_nodes, vocab], row i: the target's distribution
  *                 behind node i
