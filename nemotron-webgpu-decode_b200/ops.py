@@ -498,7 +498,9 @@ def kv_commit(pools, row_offset, pos, path, n_accepted, scratch: Scratch | None 
     row_offset[b] + pos[b] + path[b, j] moves to row_offset[b] + pos[b] + j for j <
     n_accepted[b], in every pool of `pools` (K and V of several layers, each [rows, n_kv, hd]
     fp16, 16 per launch).  path / n_accepted as :func:`verify_tree` returns them; the
-    caller's lengths grow by n_accepted."""
+    caller's lengths grow by n_accepted, but for a sequence that is refused (its path does
+    not ascend, its rows leave the pool: recorded in `scratch`), whose rows stay.
+    :func:`engine.commit_layers` does both."""
     if stream is not None:
         with _on(stream, path.device):
             return kv_commit(pools, row_offset, pos, path, n_accepted, scratch)
